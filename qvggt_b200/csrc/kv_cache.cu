@@ -1,0 +1,423 @@
+// A paged K/V cache in 8 bits: block tables and slot maps, the quantising
+// write, and the read-back.
+//
+// Layout: codes int8 [blocks][kv heads][block_size][head_dim] (one tensor for
+// K, one for V) and one fp32 scale per (block, kv head): a (block, head) tile
+// is contiguous, so attention fetches it with one bulk copy.  Token j of
+// request b is at offset j % block_size of block table[b][j / block_size].
+#include "host.hpp"
+#include "kv_cache.cuh"
+
+namespace qv {
+namespace {
+
+// ------------------------------------------------------------ block tables
+constexpr int PLAN_THREADS = 512;
+constexpr int PLAN_MAX_REQUESTS = 8192;   // 4 prefix arrays of it fit shared memory
+
+enum : int32_t { PLAN_OK = 0, PLAN_NO_BLOCKS = 1, PLAN_TABLE_FULL = 2, PLAN_BAD_LENGTH = 3, PLAN_MORE_TOKENS = 4 };
+
+struct PlanArgs {
+  const int32_t *cached, *target;
+  int32_t* table;
+  int32_t* ring;
+  const long long* free_range;
+  int32_t *slots, *cu_new, *cu_blocks, *lens, *status;
+  long long* free_out;
+  int B, wide, bs, num_blocks, most;
+};
+
+struct Quad {
+  int new_tok, grow, drop, touched;
+  __device__ Quad operator+(const Quad& o) const {
+    return {new_tok + o.new_tok, grow + o.grow, drop + o.drop, touched + o.touched};
+  }
+};
+__device__ __forceinline__ Quad shfl_up(const Quad& v, int d) {
+  return {__shfl_up_sync(~0u, v.new_tok, d), __shfl_up_sync(~0u, v.grow, d), __shfl_up_sync(~0u, v.drop, d),
+          __shfl_up_sync(~0u, v.touched, d)};
+}
+
+// What request i contributes when it goes from `c` to `t` tokens.
+__device__ __forceinline__ Quad plan_counts(int c, int t, int bs) {
+  const int have = (int)(((long long)c + bs - 1) / bs), need = (int)(((long long)t + bs - 1) / bs);
+  return {max(t - c, 0), max(need - have, 0), max(have - need, 0), t > c ? (t - 1) / bs - c / bs + 1 : 0};
+}
+
+// Largest i in [0, n) with a[i] <= x (a[0] = 0 <= x, a non-decreasing).
+__device__ __forceinline__ int last_le(const int* a, int n, int x) {
+  int lo = 0;
+  while (n > 1) {
+    const int half = n / 2;
+    if (a[lo + half] <= x) lo += half;
+    n -= half;
+  }
+  return lo;
+}
+
+// One launch, no CTA waits for another: every CTA repeats the scan over the
+// requests (a few KB out of L2) and then writes its share of the slots and
+// table entries.  The call changes all requests or, when it cannot serve one
+// of them, none.
+__global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(PlanArgs a) {
+  extern __shared__ int sm[];
+  int* cu_new = sm;                          // [B + 1] exclusive prefix sums
+  int* first = cu_new + a.B + 1;             // blocks taken by the requests before
+  int* freed = first + a.B + 1;              // blocks given back by the requests before
+  int* cu_blk = freed + a.B + 1;             // blocks written by the requests before
+  __shared__ Quad warp_sum_[PLAN_THREADS / 32];
+  __shared__ int bad;
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int per = (a.B + PLAN_THREADS - 1) / PLAN_THREADS;
+  const int i0 = min(a.B, tid * per), i1 = min(a.B, i0 + per);
+  if (tid == 0) bad = 0;
+  __syncthreads();
+  Quad sum{0, 0, 0, 0};
+  int my_bad = 0;
+  unsigned long long tokens = 0;
+  for (int i = i0; i < i1; ++i) {
+    const int c = a.cached[i], t = a.target[i];
+    if (c < 0 || t < 0) {
+      my_bad |= 1 << PLAN_BAD_LENGTH;
+      continue;
+    }
+    if (((long long)t + a.bs - 1) / a.bs > a.wide || ((long long)c + a.bs - 1) / a.bs > a.wide)
+      my_bad |= 1 << PLAN_TABLE_FULL;
+    tokens += t > c ? t - c : 0;
+    if (tokens > (unsigned long long)a.most) my_bad |= 1 << PLAN_MORE_TOKENS;
+    sum = sum + plan_counts(c, t, a.bs);
+  }
+  if (my_bad) atomicOr(&bad, my_bad);
+  Quad inc = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const Quad o = shfl_up(inc, d);
+    if (lane >= d) inc = inc + o;
+  }
+  if (lane == 31) warp_sum_[warp] = inc;
+  __syncthreads();
+  Quad base{0, 0, 0, 0}, total{0, 0, 0, 0};
+  for (int w = 0; w < PLAN_THREADS / 32; ++w) {
+    if (w == warp) base = total;
+    total = total + warp_sum_[w];
+  }
+  const long long head = a.free_range[0], tail = a.free_range[1];
+  int flags = bad;
+  if (total.new_tok > a.most || total.new_tok < 0) flags |= 1 << PLAN_MORE_TOKENS;
+  if (total.grow > tail - head || total.grow < 0) flags |= 1 << PLAN_NO_BLOCKS;
+  // the first reason in this order is reported
+  const int status = flags & (1 << PLAN_BAD_LENGTH)    ? PLAN_BAD_LENGTH
+                     : flags & (1 << PLAN_TABLE_FULL)  ? PLAN_TABLE_FULL
+                     : flags & (1 << PLAN_MORE_TOKENS) ? PLAN_MORE_TOKENS
+                     : flags & (1 << PLAN_NO_BLOCKS)   ? PLAN_NO_BLOCKS
+                                                       : PLAN_OK;
+  const bool ok = status == PLAN_OK;
+  if (!ok) total = Quad{0, 0, 0, 0};
+  Quad run = base + Quad{inc.new_tok - sum.new_tok, inc.grow - sum.grow, inc.drop - sum.drop,
+                         inc.touched - sum.touched};
+  for (int i = i0; i < i1; ++i) {
+    cu_new[i] = ok ? run.new_tok : 0;
+    first[i] = run.grow;
+    freed[i] = run.drop;
+    cu_blk[i] = ok ? run.touched : 0;
+    const int c = a.cached[i], t = a.target[i];
+    if (blockIdx.x == 0) a.lens[i] = ok ? t : c;
+    if (ok) run = run + plan_counts(c, t, a.bs);
+  }
+  if (tid == 0) {
+    cu_new[a.B] = total.new_tok;
+    first[a.B] = total.grow;
+    freed[a.B] = total.drop;
+    cu_blk[a.B] = total.touched;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int i = tid; i <= a.B; i += PLAN_THREADS) {
+      a.cu_new[i] = cu_new[i];
+      a.cu_blocks[i] = cu_blk[i];
+    }
+    if (tid == 0) {
+      a.free_out[0] = head + total.grow;
+      a.free_out[1] = tail + total.drop;
+      a.status[0] = status;
+    }
+  }
+  const int gtid = blockIdx.x * PLAN_THREADS + tid, gsize = gridDim.x * PLAN_THREADS;
+  const int head_m = (int)(head % a.num_blocks), tail_m = (int)(tail % a.num_blocks);
+  auto ring_at = [&](int from, int off) {    // off < num_blocks
+    const int x = from + off;
+    return x >= a.num_blocks ? x - a.num_blocks : x;
+  };
+  for (int n = gtid; n < a.most; n += gsize) {
+    int slot = -1;
+    if (n < total.new_tok) {
+      const int b = last_le(cu_new, a.B, n);
+      const int c = a.cached[b], pos = c + n - cu_new[b];
+      const int have = (c + a.bs - 1) / a.bs, j = pos / a.bs;
+      const int blk = j < have ? a.table[(long long)b * a.wide + j] : a.ring[ring_at(head_m, first[b] + j - have)];
+      slot = blk * a.bs + pos - j * a.bs;
+    }
+    a.slots[n] = slot;
+  }
+  for (int n = gtid; n < total.grow; n += gsize) {
+    const int b = last_le(first, a.B, n);
+    const int have = (a.cached[b] + a.bs - 1) / a.bs;
+    a.table[(long long)b * a.wide + have + n - first[b]] = a.ring[ring_at(head_m, n)];
+  }
+  for (int n = gtid; n < total.drop; n += gsize) {
+    const int b = last_le(freed, a.B, n);
+    const int need = (a.target[b] + a.bs - 1) / a.bs;
+    a.ring[ring_at(tail_m, n)] = a.table[(long long)b * a.wide + need + n - freed[b]];
+  }
+}
+
+// ------------------------------------------------------------------ append
+constexpr int APPEND_THREADS = 128;
+
+struct AppendArgs {
+  const uint16_t* x[2];                  // K, V: [tokens][heads][D], unit stride in D
+  long long tok_stride[2], head_stride[2];
+  int8_t* codes[2];
+  float* scales[2];
+  const int32_t *table, *cached, *cu_new, *cu_blocks;
+  long long block_stride;                // codes between blocks
+  long long tokens;
+  int B, wide, bs, num_blocks, heads, D;
+  Ctl ctl;
+};
+
+// One CTA per (written block, head, K or V): the new rows' largest magnitude,
+// the block's scale, the codes.
+template <bool BF16>
+__global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(AppendArgs a) {
+  __shared__ float red[APPEND_THREADS / 32];
+  pdl_wait();
+  pdl_trigger();
+  const int unit = blockIdx.x, h = blockIdx.y, side = blockIdx.z;
+  if (unit >= a.cu_blocks[a.B]) return;
+  const int b = last_le(a.cu_blocks, a.B, unit);
+  const int c = a.cached[b], n0 = a.cu_new[b], end = c + a.cu_new[b + 1] - n0;
+  const int j = c / a.bs + unit - a.cu_blocks[b];
+  const int lo = max(c, j * a.bs), hi = min(end, (j + 1) * a.bs);      // new tokens of the block
+  const int blk = j < a.wide ? a.table[(long long)b * a.wide + j] : -1;
+  if (c < 0 || n0 < 0 || hi <= lo || (long long)n0 + end - c > a.tokens || blk < 0 || blk >= a.num_blocks) {
+    if (threadIdx.x == 0) report_status(a.ctl, c < 0 || hi <= lo ? ST_BAD_LENGTH : ST_BAD_BLOCK);
+    return;
+  }
+  const int older = lo - j * a.bs;                                     // earlier tokens of the block
+  const uint16_t* x = a.x[side] + (n0 + lo - c) * a.tok_stride[side] + h * a.head_stride[side];
+  int8_t* codes = a.codes[side] + blk * a.block_stride + (long long)h * a.bs * a.D;
+  float* scale = a.scales[side] + (long long)blk * a.heads + h;
+  const int total = (hi - lo) * a.D;
+  float m = 0.f;
+  for (int i = threadIdx.x; i < total; i += APPEND_THREADS) {
+    const float v = fabsf(half_bits_to_f32<BF16>(x[(i / a.D) * a.tok_stride[side] + i % a.D]));
+    if (v <= 3.4028235e38f) m = fmaxf(m, v);                           // finite values only
+  }
+  m = warp_max(m);
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float before = older > 0 ? *scale : 0.f;
+  const float s = fmaxf(fmaxf(before, __fdiv_rn(m, 127.f)), KV_SCALE_MIN);
+  const float inv = __frcp_rn(s);
+  __syncthreads();                                                     // everyone has read the old scale
+  if (threadIdx.x == 0) *scale = s;
+  if (older > 0 && s != before) {
+    const float r = before * inv;
+    for (int i = threadIdx.x; i < older * a.D; i += APPEND_THREADS) codes[i] = kv_code((float)codes[i] * r);
+  }
+  for (int i = threadIdx.x; i < total; i += APPEND_THREADS)
+    codes[older * a.D + i] = kv_code(half_bits_to_f32<BF16>(x[(i / a.D) * a.tok_stride[side] + i % a.D]) * inv);
+}
+
+// ------------------------------------------------------------------ gather
+constexpr int GATHER_THREADS = 256;
+
+struct GatherArgs {
+  const int8_t* codes[2];
+  const float* scales[2];
+  const int32_t* slots;
+  uint16_t* out;                         // [n][2][heads][D], rows of out_stride
+  long long out_stride, block_stride, n;
+  int bs, num_blocks, heads, D;
+  Ctl ctl;
+};
+
+// 16 codes per thread; a slot of -1 gives a row of zeros.
+template <bool BF16>
+__global__ void __launch_bounds__(GATHER_THREADS) kv_gather_kernel(GatherArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const int per_head = a.D / 16, per_side = a.heads * per_head, per_row = 2 * per_side;
+  const long long total = a.n * per_row;
+  for (long long i = (long long)blockIdx.x * GATHER_THREADS + threadIdx.x; i < total;
+       i += (long long)gridDim.x * GATHER_THREADS) {
+    const long long row = i / per_row;
+    const int rem = (int)(i - row * per_row);
+    const int side = rem >= per_side, hp = rem - side * per_side, h = hp / per_head, part = hp - h * per_head;
+    const int slot = a.slots[row];
+    uint4 o[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    if (slot >= 0) {
+      const int blk = slot / a.bs;
+      if (blk < a.num_blocks) {
+        const int8_t* src = a.codes[side] + blk * a.block_stride +
+                            ((long long)h * a.bs + (slot - blk * a.bs)) * a.D + part * 16;
+        const uint4 c = *reinterpret_cast<const uint4*>(src);
+        const float s = a.scales[side][(long long)blk * a.heads + h];
+        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+        uint32_t r[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t u = w[k / 2] >> (16 * (k & 1));
+          const float x0 = (float)(int8_t)u * s, x1 = (float)(int8_t)(u >> 8) * s;
+          r[k] = BF16 ? pack_bf162(x0, x1) : pack_half2(x0, x1);
+        }
+        o[0] = make_uint4(r[0], r[1], r[2], r[3]);
+        o[1] = make_uint4(r[4], r[5], r[6], r[7]);
+      } else if (rem == 0) {
+        report_bad_block(a.ctl);
+      }
+    }
+    uint4* dst = reinterpret_cast<uint4*>(a.out + row * a.out_stride + (long long)side * a.heads * a.D + h * a.D +
+                                          part * 16);
+    dst[0] = o[0];
+    dst[1] = o[1];
+  }
+}
+
+}  // namespace
+
+int check_cache(const char* name, const void* kc, const void* vc, const void* ks, const void* vs, int64_t block_stride,
+                int32_t num_blocks, int32_t heads, int32_t block_size, int32_t head_dim) {
+  if (num_blocks <= 0 || heads <= 0) return set_error(QVGGT_ERR_INVALID, "%s: empty cache", name);
+  if (block_size != 32 && block_size != 64 && block_size != 128)
+    return set_error(QVGGT_ERR_UNSUPPORTED, "%s: block_size must be 32, 64 or 128", name);
+  if (head_dim != 64 && head_dim != 128)
+    return set_error(QVGGT_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128", name);
+  if (!kc || !vc || !ks || !vs) return set_error(QVGGT_ERR_INVALID, "%s: null cache tensor", name);
+  if (!aligned16(kc) || !aligned16(vc) || block_stride % 16)
+    return set_error(QVGGT_ERR_ALIGN, "%s: cache codes and their block stride must be 16-byte aligned", name);
+  if (block_stride < (int64_t)heads * block_size * head_dim)
+    return set_error(QVGGT_ERR_INVALID, "%s: block stride smaller than a block", name);
+  if ((int64_t)num_blocks * block_size > 2147483647LL)
+    return set_error(QVGGT_ERR_UNSUPPORTED, "%s: more than 2^31 slots", name);
+  return QVGGT_OK;
+}
+
+}  // namespace qv
+
+using namespace qv;
+
+extern "C" int qvggt_block_plan(const int32_t* cached_lens, const int32_t* target_lens, int32_t requests,
+                                int32_t* block_tables, int32_t max_blocks, int32_t* free_ring, int32_t num_blocks,
+                                const int64_t* free_range, int32_t block_size, int32_t max_new, int32_t* slots,
+                                int32_t* cu_new, int32_t* cu_blocks, int32_t* lens_out, int64_t* free_range_out,
+                                int32_t* status, void* stream) {
+  if (requests < 0 || max_blocks < 0 || num_blocks <= 0 || max_new < 0)
+    return set_error(QVGGT_ERR_INVALID, "block_plan: bad shape");
+  if (requests > PLAN_MAX_REQUESTS)
+    return set_error(QVGGT_ERR_UNSUPPORTED, "block_plan: at most %d requests", PLAN_MAX_REQUESTS);
+  if (block_size <= 0 || (block_size & (block_size - 1)))
+    return set_error(QVGGT_ERR_INVALID, "block_plan: block_size must be a power of two");
+  if ((int64_t)num_blocks * block_size > 2147483647LL)
+    return set_error(QVGGT_ERR_UNSUPPORTED, "block_plan: more than 2^31 slots");
+  if (!free_ring || !free_range || !cu_new || !cu_blocks || !free_range_out || !status || (max_new && !slots) ||
+      (requests && (!cached_lens || !target_lens || !lens_out)) || (requests && max_blocks && !block_tables))
+    return set_error(QVGGT_ERR_INVALID, "block_plan: null tensor");
+  if (lens_out == cached_lens || lens_out == target_lens || free_range_out == free_range)
+    return set_error(QVGGT_ERR_INVALID, "block_plan: the outputs must not be the inputs");
+  PlanArgs a{cached_lens, target_lens, block_tables, free_ring, reinterpret_cast<const long long*>(free_range),
+             slots, cu_new, cu_blocks, lens_out, status, reinterpret_cast<long long*>(free_range_out),
+             requests, max_blocks, block_size, num_blocks, max_new};
+  const int smem = 4 * (requests + 1) * (int)sizeof(int);
+  static DeviceFlags attr;
+  if (int rc = ensure_smem(attr, block_plan_kernel, 4 * (PLAN_MAX_REQUESTS + 1) * (int)sizeof(int),
+                           "cudaFuncSetAttribute(block_plan)"))
+    return rc;
+  const int sms = device_info().num_sms;
+  const int grid = (int)std::min<int64_t>(sms, std::max<int64_t>(1, ((int64_t)max_new + PLAN_THREADS - 1) / PLAN_THREADS));
+  int rc = check_cuda(launch_pdl(block_plan_kernel, dim3(grid), dim3(PLAN_THREADS), (size_t)smem,
+                                 static_cast<cudaStream_t>(stream), 1u, a),
+                      "block_plan launch");
+  if (!rc) count_launch(1);
+  return rc;
+}
+
+extern "C" int qvggt_kv_append(const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok,
+                               int64_t v_head, int64_t tokens, int32_t dtype, int8_t* k_cache, int8_t* v_cache, int64_t block_stride,
+                               float* k_scale, float* v_scale, int32_t num_blocks, int32_t kv_heads,
+                               int32_t block_size, int32_t head_dim, const int32_t* block_tables, int32_t max_blocks,
+                               const int32_t* cached_lens, const int32_t* cu_new, const int32_t* cu_blocks,
+                               int32_t requests, int32_t max_units, void* stream) {
+  if (int rc = check_cache("kv_append", k_cache, v_cache, k_scale, v_scale, block_stride, num_blocks, kv_heads,
+                           block_size, head_dim))
+    return rc;
+  if (dtype != QVGGT_DTYPE_F16 && dtype != QVGGT_DTYPE_BF16)
+    return set_error(QVGGT_ERR_UNSUPPORTED, "kv_append: dtype must be fp16 or bf16");
+  if (tokens < 0 || requests < 0 || max_blocks < 0 || max_units < 0) return set_error(QVGGT_ERR_INVALID, "kv_append: bad shape");
+  if (tokens == 0 || requests == 0 || max_units == 0) return QVGGT_OK;
+  if (!k || !v || !block_tables || !cached_lens || !cu_new || !cu_blocks)
+    return set_error(QVGGT_ERR_INVALID, "kv_append: null tensor");
+  if (!aligned16(k) || !aligned16(v) || k_tok % 8 || k_head % 8 || v_tok % 8 || v_head % 8)
+    return set_error(QVGGT_ERR_ALIGN, "kv_append: k and v rows must be 16-byte aligned");
+  if (kv_heads > 65535) return set_error(QVGGT_ERR_UNSUPPORTED, "kv_append: too many heads");
+  AppendArgs a{};
+  a.x[0] = static_cast<const uint16_t*>(k);
+  a.x[1] = static_cast<const uint16_t*>(v);
+  a.tok_stride[0] = k_tok;
+  a.tok_stride[1] = v_tok;
+  a.head_stride[0] = k_head;
+  a.head_stride[1] = v_head;
+  a.codes[0] = k_cache;
+  a.codes[1] = v_cache;
+  a.scales[0] = k_scale;
+  a.scales[1] = v_scale;
+  a.table = block_tables;
+  a.cached = cached_lens;
+  a.cu_new = cu_new;
+  a.cu_blocks = cu_blocks;
+  a.block_stride = block_stride;
+  a.tokens = tokens;
+  a.B = requests;
+  a.wide = max_blocks;
+  a.bs = block_size;
+  a.num_blocks = num_blocks;
+  a.heads = kv_heads;
+  a.D = head_dim;
+  a.ctl = make_ctl();
+  const auto fn = dtype == QVGGT_DTYPE_BF16 ? kv_append_kernel<true> : kv_append_kernel<false>;
+  int rc = check_cuda(launch_pdl(fn, dim3(max_units, kv_heads, 2), dim3(APPEND_THREADS), 0,
+                                 static_cast<cudaStream_t>(stream), 1u, a),
+                      "kv_append launch");
+  if (!rc) count_launch(1);
+  return rc;
+}
+
+extern "C" int qvggt_kv_gather(const int8_t* k_cache, const int8_t* v_cache, int64_t block_stride,
+                               const float* k_scale, const float* v_scale, int32_t num_blocks, int32_t kv_heads,
+                               int32_t block_size, int32_t head_dim, const int32_t* slots, int64_t n, void* out,
+                               int64_t out_stride, int32_t dtype, void* stream) {
+  if (int rc = check_cache("kv_gather", k_cache, v_cache, k_scale, v_scale, block_stride, num_blocks, kv_heads,
+                           block_size, head_dim))
+    return rc;
+  if (dtype != QVGGT_DTYPE_F16 && dtype != QVGGT_DTYPE_BF16)
+    return set_error(QVGGT_ERR_UNSUPPORTED, "kv_gather: dtype must be fp16 or bf16");
+  if (n < 0) return set_error(QVGGT_ERR_INVALID, "kv_gather: bad shape");
+  if (n == 0) return QVGGT_OK;
+  if (!slots || !out) return set_error(QVGGT_ERR_INVALID, "kv_gather: null tensor");
+  if (!aligned16(out) || out_stride % 8 || out_stride < 2LL * kv_heads * head_dim)
+    return set_error(QVGGT_ERR_ALIGN, "kv_gather: out rows must be 16-byte aligned and hold K and V");
+  GatherArgs a{{k_cache, v_cache}, {k_scale, v_scale}, slots, static_cast<uint16_t*>(out), out_stride, block_stride,
+               n, block_size, num_blocks, kv_heads, head_dim, make_ctl()};
+  const long long work = (n * 2 * kv_heads * (head_dim / 16) + GATHER_THREADS - 1) / GATHER_THREADS;
+  const long long grid = std::min<long long>(work, 16LL * device_info().num_sms);
+  const auto fn = dtype == QVGGT_DTYPE_BF16 ? kv_gather_kernel<true> : kv_gather_kernel<false>;
+  int rc = check_cuda(launch_pdl(fn, dim3((unsigned)grid), dim3(GATHER_THREADS), 0,
+                                 static_cast<cudaStream_t>(stream), 1u, a),
+                      "kv_gather launch");
+  if (!rc) count_launch(1);
+  return rc;
+}

@@ -1,0 +1,238 @@
+// Rotary positions with several axes (time, height, width): q and k rotated in
+// one pass, positions and frequencies given.
+//
+// Pair j of a head (j < R/2) is rotated by the angle t_j = pos[axis_j] * f_j:
+//   y[lo] = x[lo] cos t - x[hi] sin t,   y[hi] = x[hi] cos t + x[lo] sin t
+// (the inverse, which is also the gradient, turns by -t); dims >= R pass
+// through.  A token's angles are shared by all its heads, so a CTA first
+// computes the sines and cosines of its tokens into shared memory and then
+// streams the heads through registers: 2 bytes in and 2 out per element, HBM
+// bound.
+#include "host.hpp"
+
+namespace qv {
+namespace {
+
+constexpr int ROPE_THREADS = 256;
+constexpr int ROPE_MAX_PAIRS = 128;     // head_dim <= 256
+constexpr int ROPE_MAX_TOK = 16;        // tokens of one CTA
+constexpr int ROPE_AXES = 4;
+
+enum RopeLayout : int32_t { ROPE_AXIAL = 0, ROPE_SPLIT = 1, ROPE_INTERLEAVED = 2 };
+
+struct RopeSide {                        // q or k: element strides of tokens and heads
+  const uint16_t* in;
+  uint16_t* out;
+  long long in_ts, in_hs, out_ts, out_hs;
+  int heads;
+};
+
+struct RopeArgs {
+  RopeSide s[2];
+  const int32_t* pos;                    // [axes][T], row stride pos_stride
+  const float* inv_freq;                 // [pairs]
+  long long pos_stride, T;
+  int D, pairs, tok, layout;
+  int sect_end[ROPE_AXES];               // pair index one past each axis' last (unused axes: pairs)
+  float sign;
+};
+
+template <int V>
+struct VecBits;
+template <> struct VecBits<8> { using T = uint4; };
+template <> struct VecBits<4> { using T = uint2; };
+template <> struct VecBits<2> { using T = uint32_t; };
+template <> struct VecBits<1> { using T = uint16_t; };
+
+template <bool BF16>
+__device__ __forceinline__ float to_f32(uint16_t u) {
+  if (BF16) return __uint_as_float((uint32_t)u << 16);
+  return __half2float(__ushort_as_half(u));
+}
+template <bool BF16>
+__device__ __forceinline__ uint16_t from_f32(float x) {
+  if (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(x));
+  return __half_as_ushort(__float2half_rn(x));
+}
+
+// V pairs per item: two V-element vectors in, two out.
+template <bool BF16, int V>
+__global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(RopeArgs a) {
+  using Vec = typename VecBits<V>::T;
+  union Pack {
+    Vec v;
+    uint16_t e[V];
+  };
+  extern __shared__ float2 cs[];         // [tok][pairs] (cos, sin)
+  pdl_wait();
+  pdl_trigger();
+  const long long t0 = (long long)blockIdx.x * a.tok;
+  const int nt = (int)min((long long)a.tok, a.T - t0);
+  // The angle is reduced modulo 2 pi in double: a float product of a large
+  // position and its frequency would already be off by the angle's ulp.
+  for (int i = threadIdx.x; i < nt * a.pairs; i += ROPE_THREADS) {
+    const int tt = i / a.pairs, j = i - tt * a.pairs;
+    int ax = 0;
+#pragma unroll
+    for (int x = 0; x < ROPE_AXES - 1; ++x) ax += j >= a.sect_end[x];
+    const double t = (double)a.pos[ax * a.pos_stride + t0 + tt] * (double)a.inv_freq[j];
+    const double r = t - rint(t * 0.15915494309189533577) * 6.28318530717958647693;
+    float sn, cn;
+    sincosf((float)r, &sn, &cn);
+    cs[i] = make_float2(cn, sn * a.sign);
+  }
+  __syncthreads();
+  const int rot = a.pairs / V;                            // rotation items of a head
+  const int copy = (a.D - 2 * a.pairs) / V;               // pass-through items
+  const int per_head = rot + copy;
+  const int heads = a.s[0].heads + a.s[1].heads;
+  const int per_tok = heads * per_head;
+  for (int i = threadIdx.x; i < nt * per_tok; i += ROPE_THREADS) {
+    const int tt = i / per_tok, rem = i - tt * per_tok;
+    int h = rem / per_head;
+    const int item = rem - h * per_head;
+    const int side = h >= a.s[0].heads;
+    if (side) h -= a.s[0].heads;
+    const RopeSide& s = a.s[side];
+    const uint16_t* in = s.in + (t0 + tt) * s.in_ts + h * s.in_hs;
+    uint16_t* out = s.out + (t0 + tt) * s.out_ts + h * s.out_hs;
+    if (item >= rot) {
+      const int d = 2 * a.pairs + (item - rot) * V;
+      *reinterpret_cast<Vec*>(out + d) = *reinterpret_cast<const Vec*>(in + d);
+      continue;
+    }
+    const int j = item * V;
+    int lo, hi;
+    if (a.layout == ROPE_SPLIT) {
+      lo = j;
+      hi = j + a.pairs;
+    } else if (a.layout == ROPE_INTERLEAVED) {
+      lo = 2 * j;
+      hi = lo + V;
+    } else {
+      int base = 0, end = a.sect_end[0];
+#pragma unroll
+      for (int x = 0; x < ROPE_AXES - 1; ++x)
+        if (j >= a.sect_end[x]) {
+          base = a.sect_end[x];
+          end = a.sect_end[x + 1];
+        }
+      lo = base + j;
+      hi = lo + (end - base);
+    }
+    Pack x, y;
+    x.v = *reinterpret_cast<const Vec*>(in + lo);
+    y.v = *reinterpret_cast<const Vec*>(in + hi);
+    const float2* c = cs + tt * a.pairs + j;
+    if (a.layout == ROPE_INTERLEAVED) {
+      // the 2V consecutive elements are (x | y): pair e is elements 2e, 2e + 1
+      uint16_t z[2 * V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        z[e] = x.e[e];
+        z[V + e] = y.e[e];
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float p = to_f32<BF16>(z[2 * e]), q = to_f32<BF16>(z[2 * e + 1]);
+        z[2 * e] = from_f32<BF16>(p * c[e].x - q * c[e].y);
+        z[2 * e + 1] = from_f32<BF16>(q * c[e].x + p * c[e].y);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        x.e[e] = z[e];
+        y.e[e] = z[V + e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float p = to_f32<BF16>(x.e[e]), q = to_f32<BF16>(y.e[e]);
+        x.e[e] = from_f32<BF16>(p * c[e].x - q * c[e].y);
+        y.e[e] = from_f32<BF16>(q * c[e].x + p * c[e].y);
+      }
+    }
+    *reinterpret_cast<Vec*>(out + lo) = x.v;
+    *reinterpret_cast<Vec*>(out + hi) = y.v;
+  }
+}
+
+}  // namespace
+}  // namespace qv
+
+using namespace qv;
+
+extern "C" int qvggt_rope_axes(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok,
+                               int64_t qo_head, int32_t q_heads, const void* k, int64_t k_tok, int64_t k_head,
+                               void* k_out, int64_t ko_tok, int64_t ko_head, int32_t k_heads, int64_t T,
+                               int32_t head_dim, const int32_t* positions, int64_t pos_stride, const float* inv_freq,
+                               const int32_t* sections, int32_t n_axes, int32_t layout, int32_t inverse,
+                               int32_t dtype, void* stream) {
+  if (T < 0 || q_heads < 0 || k_heads < 0 || q_heads + k_heads == 0)
+    return set_error(QVGGT_ERR_INVALID, "rope_axes: bad shape");
+  if (dtype != QVGGT_DTYPE_F16 && dtype != QVGGT_DTYPE_BF16)
+    return set_error(QVGGT_ERR_UNSUPPORTED, "rope_axes: dtype must be fp16 or bf16");
+  if (layout < 0 || layout > 2) return set_error(QVGGT_ERR_INVALID, "rope_axes: layout must be 0, 1 or 2");
+  if (n_axes < 1 || n_axes > ROPE_AXES || sections == nullptr)
+    return set_error(QVGGT_ERR_INVALID, "rope_axes: 1 to %d axes", ROPE_AXES);
+  if (T == 0) return QVGGT_OK;
+  if (!positions || !inv_freq || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out)))
+    return set_error(QVGGT_ERR_INVALID, "rope_axes: null tensor");
+  RopeArgs a{};
+  int pairs = 0;
+  for (int x = 0; x < n_axes; ++x) {
+    if (sections[x] <= 0) return set_error(QVGGT_ERR_INVALID, "rope_axes: section sizes must be positive");
+    pairs += sections[x] > ROPE_MAX_PAIRS ? ROPE_MAX_PAIRS + 1 : sections[x];
+    a.sect_end[x] = pairs;
+  }
+  for (int x = n_axes; x < ROPE_AXES; ++x) a.sect_end[x] = pairs;
+  if (pairs > ROPE_MAX_PAIRS || head_dim > 2 * ROPE_MAX_PAIRS)
+    return set_error(QVGGT_ERR_UNSUPPORTED, "rope_axes: head_dim up to %d", 2 * ROPE_MAX_PAIRS);
+  if (2 * pairs > head_dim)
+    return set_error(QVGGT_ERR_INVALID, "rope_axes: %d rotated pairs do not fit head_dim %d", pairs, head_dim);
+  a.s[0] = {static_cast<const uint16_t*>(q), static_cast<uint16_t*>(q_out), q_tok, q_head, qo_tok, qo_head, q_heads};
+  a.s[1] = {static_cast<const uint16_t*>(k), static_cast<uint16_t*>(k_out), k_tok, k_head, ko_tok, ko_head, k_heads};
+  a.pos = positions;
+  a.inv_freq = inv_freq;
+  a.pos_stride = pos_stride;
+  a.T = T;
+  a.D = head_dim;
+  a.pairs = pairs;
+  a.layout = layout;
+  a.sign = inverse ? -1.f : 1.f;
+  // Widest vector that divides every run of pairs, the pass-through tail, the
+  // strides and the addresses.
+  long long align = 8;
+  auto limit = [&](long long v) {
+    while (v % align) align /= 2;
+  };
+  if (layout == ROPE_AXIAL)
+    for (int x = 0; x < n_axes; ++x) limit(sections[x]);
+  limit(pairs);
+  limit(head_dim - 2 * pairs);
+  for (const RopeSide& s : a.s) {
+    if (!s.heads) continue;
+    const long long strides[4] = {s.in_ts, s.in_hs, s.out_ts, s.out_hs};
+    for (long long v : strides) limit(v < 0 ? -v : v);
+    if ((reinterpret_cast<uintptr_t>(s.in) | reinterpret_cast<uintptr_t>(s.out)) & 1)
+      return set_error(QVGGT_ERR_ALIGN, "rope_axes: tensors must be aligned to their element");
+    limit((long long)(reinterpret_cast<uintptr_t>(s.in) / 2 % 8));
+    limit((long long)(reinterpret_cast<uintptr_t>(s.out) / 2 % 8));
+  }
+  // Tokens per CTA: few enough that every SM has several CTAs, up to 16 so
+  // that the per-CTA start-up is paid for many rows.
+  const long long want = 8LL * device_info().num_sms;
+  a.tok = 1;
+  while (a.tok < ROPE_MAX_TOK && T / (2 * a.tok) >= want) a.tok *= 2;
+  const long long grid = (T + a.tok - 1) / a.tok;
+  if (grid > 2147483647LL) return set_error(QVGGT_ERR_UNSUPPORTED, "rope_axes: too many tokens");
+  using Kfn = void (*)(RopeArgs);
+  static const Kfn fns[2][4] = {
+      {rope_axes_kernel<false, 1>, rope_axes_kernel<false, 2>, rope_axes_kernel<false, 4>, rope_axes_kernel<false, 8>},
+      {rope_axes_kernel<true, 1>, rope_axes_kernel<true, 2>, rope_axes_kernel<true, 4>, rope_axes_kernel<true, 8>}};
+  const int vi = align == 8 ? 3 : align == 4 ? 2 : align == 2 ? 1 : 0;
+  int rc = check_cuda(launch_pdl(fns[dtype == QVGGT_DTYPE_BF16][vi], dim3((unsigned)grid), dim3(ROPE_THREADS),
+                                 (size_t)a.tok * pairs * sizeof(float2), static_cast<cudaStream_t>(stream), 1u, a),
+                      "rope_axes launch");
+  if (!rc) count_launch(1);
+  return rc;
+}
