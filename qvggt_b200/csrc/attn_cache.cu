@@ -1,15 +1,8 @@
-// Attention over a paged K/V cache in 8 bits, few query rows.
-//
-// With code c of a key's element and the scales ks_B, vs_B of its (block,
-// head), the row's result is
-//   out = sum_j w_j vs_B(j) c_v[j] / sum_j w_j,   w_j = exp(scale ks_B(j) q.c_k[j]).
-// Neither scale is multiplied into the rows.  With
-//   x_j = (scale log2e ks_B) (q.c_k[j]) + log2 vs_B,   P_j = 2^(x_j - m),
-// the products q.c_k and P.c_v have the codes themselves as operands (exact in
-// fp16 and bf16), m = max x_j keeps every P_j (which now holds the V scale) in
-// fp16's range, and the denominator is sum_B (1 / vs_B) sum_{j in B} P_j.
+// Attention over a paged K/V cache in 8 bits, few query rows
+// (the mathematics is in attn_cache.cuh).
+#include "attn_cache.cuh"
+#include "attn_common.cuh"
 #include "host.hpp"
-#include "kv_cache.cuh"
 
 namespace qv {
 namespace {
@@ -18,35 +11,6 @@ constexpr int TOK_WARPS = 4;
 constexpr int TOK_ROWS = 16;             // (query, head) rows of a tile: the M of mma.m16n8k16
 constexpr int UNIT = 32;                 // keys a warp takes at a time: never across two blocks
 constexpr int MAX_SPLITS = 64;
-
-struct CacheAttnArgs {
-  const uint16_t* q;
-  uint16_t* out;
-  float* lse;                            // [heads][Tq] or null
-  const int8_t *kc, *vc;
-  const float *ks, *vs;
-  const int32_t *table, *cu_q, *kv_lens;
-  float *part_o, *part_lse;              // [splits][Tq * hq][D], [splits][Tq * hq] (splits > 1)
-  long long q_tok, q_head, o_tok, o_head, block_stride, Tq;
-  int B, hq, hk, group, wide, num_blocks, bs_log2, chunk, max_q, splits;
-  float scale_log2;
-  Ctl ctl;
-};
-
-// Keys that query i (of ql) of a request with n keys sees.
-__device__ __forceinline__ int key_limit(int i, int ql, int n, int chunk) {
-  if (!chunk) return n;
-  const int pos = n - ql + i;
-  if (pos < 0) return 0;
-  const long long lim = ((long long)(pos / chunk) + 1) * chunk;
-  return lim < n ? (int)lim : n;
-}
-
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -58,30 +22,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Two codes (bytes 0 and 1, or 2 and 3 with HI, of w) as a pair of fp16 / bf16.
-// fp16: the byte with its sign bit flipped (c + 128) placed under the exponent
-// of 1024 reads 1024 + c + 128; subtracting 1152 is exact.
-template <bool HI>
-__device__ __forceinline__ uint32_t codes_f16(uint32_t flipped) {
-  const uint32_t u = __byte_perm(flipped, 0x64646464u, HI ? 0x4342 : 0x4140);
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __float2half2_rn(1152.f));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-// bf16 holds 7 fraction bits, one short of that: 128 + (c & 127) minus 128, or
-// minus 256 where c is negative; both have the form 0x4300 | bits of c.
-template <bool HI>
-__device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
-  const uint32_t u = __byte_perm(w, 0u, HI ? 0x4342 : 0x4140);
-  const uint32_t x = (u & 0x007f007fu) | 0x43004300u, y = (u & 0x00800080u) | 0x43004300u;
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x),
-                                   *reinterpret_cast<const __nv_bfloat162*>(&y));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-template <bool BF16, bool HI>
-__device__ __forceinline__ uint32_t codes2(uint32_t w) {
-  return BF16 ? codes_bf16<HI>(w) : codes_f16<HI>(w ^ 0x80808080u);
 }
 
 // One CTA per (16 rows, kv head, request, split of the keys); its warps take
@@ -183,7 +123,7 @@ __global__ void __launch_bounds__(TOK_WARPS * 32) attn_cache_rows_kernel(CacheAt
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(~0u, mx[r], 2));
       const float mn = fmaxf(m[r], mx[r]);
       base[r] = mn == -INFINITY ? 0.f : mn;
-      const float alpha = ex2f(m[r] - base[r]);        // 0 while the row has seen no key
+      const float alpha = ex2(m[r] - base[r]);        // 0 while the row has seen no key
       m[r] = mn;
       l[r] *= alpha;
 #pragma unroll
@@ -197,7 +137,7 @@ __global__ void __launch_bounds__(TOK_WARPS * 32) attn_cache_rows_kernel(CacheAt
     for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[nt][e] = ex2f(s[nt][e] - base[e >> 1]);
+        s[nt][e] = ex2(s[nt][e] - base[e >> 1]);
         ps[e >> 1] += s[nt][e];
       }
     // (a row that sees none of these keys takes nothing from their scale either)
@@ -256,7 +196,7 @@ __global__ void __launch_bounds__(TOK_WARPS * 32) attn_cache_rows_kernel(CacheAt
     float lt = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
     for (int w = 0; w < TOK_WARPS; ++w) {
-      const float f = ex2f(sm_m[w][r] - base);
+      const float f = ex2(sm_m[w][r] - base);
       lt += f * sm_l[w][r];
       x += f * sm_o[w][r][d];
       y += f * sm_o[w][r][d + 1];
@@ -293,7 +233,7 @@ __global__ void __launch_bounds__(256) attn_cache_join_kernel(CacheAttnArgs a) {
 #pragma unroll
   for (int e = 0; e < D / 32; ++e) acc[e] = 0.f;
   for (int s = 0; s < a.splits; ++s) {
-    const float w = ex2f(a.part_lse[s * rows + row] - base);
+    const float w = ex2(a.part_lse[s * rows + row] - base);
     if (w == 0.f) continue;
     l += w;
     const float* p = a.part_o + (s * rows + row) * D + lane * (D / 32);
@@ -310,9 +250,15 @@ __global__ void __launch_bounds__(256) attn_cache_join_kernel(CacheAttnArgs a) {
   if (lane == 0 && a.lse) a.lse[h * a.Tq + tok] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
 }
 
-// Splits of the keys so that the grid covers the SMs a few times over, each
-// split keeping at least 8 units for each warp to hide its start.
-int plan_splits(long long tiles, long long max_kv) {
+// How a call is laid out, by its sizes alone.
+struct Plan {
+  bool tiles;                            // attn_cache_sm100.cu's kernel
+  int row_blocks, splits;                // 16-row tiles or Q blocks of a request, parts of the keys
+};
+
+// Few rows: splits so that the grid covers the SMs a few times over, each
+// split keeping at least 4 units for each warp.
+int row_splits(long long tiles, long long max_kv) {
   const long long sms = device_info().num_sms;
   const long long units = (max_kv + UNIT - 1) / UNIT;
   long long s = (4 * sms + tiles - 1) / std::max<long long>(1, tiles);
@@ -320,13 +266,38 @@ int plan_splits(long long tiles, long long max_kv) {
   return (int)std::max<long long>(1, std::min<long long>(s, MAX_SPLITS));
 }
 
-int plan(int64_t Tq, int32_t q_heads, int32_t kv_heads, int32_t requests, int32_t max_q, int64_t max_kv,
-         int32_t head_dim, int32_t* splits, int64_t* scratch_bytes) {
-  const long long group = q_heads / kv_heads;
-  const long long tiles = (max_q * group + TOK_ROWS - 1) / TOK_ROWS * kv_heads * requests;
-  *splits = plan_splits(tiles, max_kv);
-  *scratch_bytes = *splits > 1 ? (int64_t)*splits * Tq * q_heads * (head_dim + 1) * 4 : 0;
-  return QVGGT_OK;
+// Q tiles: the splits that end soonest when `items` CTAs of nt key tiles each
+// run one to an SM, counting two tiles' time of start and end (three with a
+// join); taken when they win more than 3 %.
+int tile_splits(long long items, long long nt) {
+  const long long sms = std::max(1, device_info().num_sms);
+  auto cost = [&](long long s) {
+    return (double)((items * s + sms - 1) / sms) * ((double)nt / s + (s > 1 ? 3.0 : 2.0));
+  };
+  int best = 1;
+  for (int s = 2; s <= MAX_SPLITS && nt / s >= 4; ++s)
+    if (cost(s) < 0.97 * cost(best)) best = s;
+  return best;
+}
+
+Plan make_plan(int group, int kv_heads, int requests, int max_q, long long max_kv, int head_dim) {
+  Plan p{};
+  const long long rows = (long long)max_q * group;
+  p.tiles = rows > TOK_ROWS && group <= 128;
+  if (p.tiles) {
+    const int tokens = 2 * (128 / group);
+    p.row_blocks = (int)(((long long)max_q + tokens - 1) / tokens);
+    const int kt = head_dim == 64 ? 128 : 64;
+    p.splits = tile_splits((long long)p.row_blocks * kv_heads * requests, (max_kv + kt - 1) / kt);
+  } else {
+    p.row_blocks = (int)((rows + TOK_ROWS - 1) / TOK_ROWS);
+    p.splits = row_splits((long long)p.row_blocks * kv_heads * requests, max_kv);
+  }
+  return p;
+}
+
+int64_t plan_scratch(const Plan& p, int64_t Tq, int q_heads, int head_dim) {
+  return p.splits > 1 ? (int64_t)p.splits * Tq * q_heads * (head_dim + 1) * 4 : 0;
 }
 
 int check_shape(const char* name, int64_t Tq, int32_t q_heads, int32_t kv_heads, int32_t requests, int32_t max_q,
@@ -352,8 +323,9 @@ extern "C" int qvggt_cached_attention_scratch(int64_t Tq, int32_t q_heads, int32
   if (int rc = check_shape("cached_attention_scratch", Tq, q_heads, kv_heads, requests, max_q, max_kv, head_dim))
     return rc;
   if (!bytes) return set_error(QVGGT_ERR_INVALID, "cached_attention_scratch: null pointer");
-  int32_t splits;
-  return plan(Tq, q_heads, kv_heads, requests, max_q, max_kv, head_dim, &splits, bytes);
+  *bytes = plan_scratch(make_plan(q_heads / kv_heads, kv_heads, requests, max_q, max_kv, head_dim), Tq, q_heads,
+                        head_dim);
+  return QVGGT_OK;
 }
 
 extern "C" int qvggt_cached_attention(const void* q, int64_t q_tok, int64_t q_head, void* out, int64_t o_tok,
@@ -381,12 +353,6 @@ extern "C" int qvggt_cached_attention(const void* q, int64_t q_tok, int64_t q_he
     return set_error(QVGGT_ERR_INVALID, "%s: null tensor", name);
   if (!aligned16(q) || !aligned16(out) || q_tok % 8 || q_head % 8 || o_tok % 8 || o_head % 8)
     return set_error(QVGGT_ERR_ALIGN, "%s: q and out rows must be 16-byte aligned", name);
-  int32_t splits;
-  int64_t need;
-  plan(Tq, q_heads, kv_heads, requests, max_q, max_kv, head_dim, &splits, &need);
-  if (need && (!scratch || scratch_bytes < need || !aligned16(scratch)))
-    return set_error(QVGGT_ERR_INVALID, "%s: needs %lld bytes of 16-byte aligned scratch, got %lld", name,
-                     (long long)need, (long long)scratch_bytes);
   CacheAttnArgs a{};
   a.q = static_cast<const uint16_t*>(q);
   a.out = static_cast<uint16_t*>(out);
@@ -398,8 +364,6 @@ extern "C" int qvggt_cached_attention(const void* q, int64_t q_tok, int64_t q_he
   a.table = block_tables;
   a.cu_q = cu_q;
   a.kv_lens = kv_lens;
-  a.part_o = static_cast<float*>(scratch);
-  a.part_lse = a.part_o ? a.part_o + (long long)splits * Tq * q_heads * head_dim : nullptr;
   a.q_tok = q_tok;
   a.q_head = q_head;
   a.o_tok = o_tok;
@@ -415,24 +379,39 @@ extern "C" int qvggt_cached_attention(const void* q, int64_t q_tok, int64_t q_he
   a.bs_log2 = block_size == 32 ? 5 : block_size == 64 ? 6 : 7;
   a.chunk = causal_chunk;
   a.max_q = max_q;
-  a.splits = splits;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.ctl = make_ctl();
+  Plan p = make_plan(a.group, kv_heads, requests, max_q, max_kv, head_dim);
+  if (p.tiles && !tiles_can_read(a)) {
+    // strides no TMA map takes (a broadcast or reversed query): the row kernel, unsplit
+    p.tiles = false;
+    p.row_blocks = (int)(((long long)max_q * a.group + TOK_ROWS - 1) / TOK_ROWS);
+    p.splits = 1;
+  }
+  const int64_t need = plan_scratch(p, Tq, q_heads, head_dim);
+  if (need && (!scratch || scratch_bytes < need || !aligned16(scratch)))
+    return set_error(QVGGT_ERR_INVALID, "%s: needs %lld bytes of 16-byte aligned scratch, got %lld", name,
+                     (long long)need, (long long)scratch_bytes);
+  a.row_blocks = p.row_blocks;
+  a.splits = p.splits;
+  a.part_o = static_cast<float*>(scratch);
+  a.part_lse = need ? a.part_o + (long long)p.splits * Tq * q_heads * head_dim : nullptr;
   const bool bf16 = dtype == QVGGT_DTYPE_BF16;
-  const long long tiles = ((long long)max_q * a.group + TOK_ROWS - 1) / TOK_ROWS;
   using Kfn = void (*)(CacheAttnArgs);
   static const Kfn rows_fns[2][2] = {{attn_cache_rows_kernel<false, 64>, attn_cache_rows_kernel<false, 128>},
                                      {attn_cache_rows_kernel<true, 64>, attn_cache_rows_kernel<true, 128>}};
   static const Kfn join_fns[2][2] = {{attn_cache_join_kernel<false, 64>, attn_cache_join_kernel<false, 128>},
                                      {attn_cache_join_kernel<true, 64>, attn_cache_join_kernel<true, 128>}};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int rc = check_cuda(launch_pdl(rows_fns[bf16][head_dim == 128],
-                                     dim3((unsigned)tiles, (unsigned)(kv_heads * requests), (unsigned)splits),
-                                     dim3(TOK_WARPS * 32), 0, st, 1u, a),
-                          "cached_attention launch"))
-    return rc;
+  const int rc = p.tiles ? launch_tiles(a, head_dim, bf16, st)
+                         : check_cuda(launch_pdl(rows_fns[bf16][head_dim == 128],
+                                                 dim3((unsigned)p.row_blocks, (unsigned)(kv_heads * requests),
+                                                      (unsigned)p.splits),
+                                                 dim3(TOK_WARPS * 32), 0, st, 1u, a),
+                                      "cached_attention launch");
+  if (rc) return rc;
   count_launch(1);
-  if (splits > 1) {
+  if (p.splits > 1) {
     if (int rc = check_cuda(launch_pdl(join_fns[bf16][head_dim == 128], dim3((unsigned)((Tq * q_heads + 7) / 8)),
                                        dim3(256), 0, st, 1u, a),
                             "cached_attention join launch"))
