@@ -253,7 +253,8 @@ __global__ void __launch_bounds__(256) attn_cache_join_kernel(CacheAttnArgs a) {
 // How a call is laid out, by its sizes alone.
 struct Plan {
   bool tiles;                            // attn_cache_sm100.cu's kernel
-  int row_blocks, splits;                // 16-row tiles or Q blocks of a request, parts of the keys
+  int row_blocks, splits;                // 16-row tiles or Q blocks of a request, parts of the keys (row kernel)
+  int64_t scratch;
 };
 
 // Few rows: splits so that the grid covers the SMs a few times over, each
@@ -266,38 +267,21 @@ int row_splits(long long tiles, long long max_kv) {
   return (int)std::max<long long>(1, std::min<long long>(s, MAX_SPLITS));
 }
 
-// Q tiles: the splits that end soonest when `items` CTAs of nt key tiles each
-// run one to an SM, counting two tiles' time of start and end (three with a
-// join); taken when they win more than 3 %.
-int tile_splits(long long items, long long nt) {
-  const long long sms = std::max(1, device_info().num_sms);
-  auto cost = [&](long long s) {
-    return (double)((items * s + sms - 1) / sms) * ((double)nt / s + (s > 1 ? 3.0 : 2.0));
-  };
-  int best = 1;
-  for (int s = 2; s <= MAX_SPLITS && nt / s >= 4; ++s)
-    if (cost(s) < 0.97 * cost(best)) best = s;
-  return best;
-}
-
-Plan make_plan(int group, int kv_heads, int requests, int max_q, long long max_kv, int head_dim) {
+Plan make_plan(long long Tq, int group, int kv_heads, int requests, int max_q, long long max_kv, int head_dim) {
   Plan p{};
   const long long rows = (long long)max_q * group;
   p.tiles = rows > TOK_ROWS && group <= 128;
   if (p.tiles) {
     const int tokens = 2 * (128 / group);
     p.row_blocks = (int)(((long long)max_q + tokens - 1) / tokens);
-    const int kt = head_dim == 64 ? 128 : 64;
-    p.splits = tile_splits((long long)p.row_blocks * kv_heads * requests, (max_kv + kt - 1) / kt);
+    p.splits = 1;
+    p.scratch = tiles_scratch((long long)p.row_blocks * kv_heads * requests, max_kv, head_dim);
   } else {
     p.row_blocks = (int)((rows + TOK_ROWS - 1) / TOK_ROWS);
     p.splits = row_splits((long long)p.row_blocks * kv_heads * requests, max_kv);
+    p.scratch = p.splits > 1 ? (int64_t)p.splits * Tq * kv_heads * group * (head_dim + 1) * 4 : 0;
   }
   return p;
-}
-
-int64_t plan_scratch(const Plan& p, int64_t Tq, int q_heads, int head_dim) {
-  return p.splits > 1 ? (int64_t)p.splits * Tq * q_heads * (head_dim + 1) * 4 : 0;
 }
 
 int check_shape(const char* name, int64_t Tq, int32_t q_heads, int32_t kv_heads, int32_t requests, int32_t max_q,
@@ -323,8 +307,7 @@ extern "C" int qvggt_cached_attention_scratch(int64_t Tq, int32_t q_heads, int32
   if (int rc = check_shape("cached_attention_scratch", Tq, q_heads, kv_heads, requests, max_q, max_kv, head_dim))
     return rc;
   if (!bytes) return set_error(QVGGT_ERR_INVALID, "cached_attention_scratch: null pointer");
-  *bytes = plan_scratch(make_plan(q_heads / kv_heads, kv_heads, requests, max_q, max_kv, head_dim), Tq, q_heads,
-                        head_dim);
+  *bytes = make_plan(Tq, q_heads / kv_heads, kv_heads, requests, max_q, max_kv, head_dim).scratch;
   return QVGGT_OK;
 }
 
@@ -381,21 +364,20 @@ extern "C" int qvggt_cached_attention(const void* q, int64_t q_tok, int64_t q_he
   a.max_q = max_q;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.ctl = make_ctl();
-  Plan p = make_plan(a.group, kv_heads, requests, max_q, max_kv, head_dim);
+  Plan p = make_plan(Tq, a.group, kv_heads, requests, max_q, max_kv, head_dim);
   if (p.tiles && !tiles_can_read(a)) {
     // strides no TMA map takes (a broadcast or reversed query): the row kernel, unsplit
     p.tiles = false;
     p.row_blocks = (int)(((long long)max_q * a.group + TOK_ROWS - 1) / TOK_ROWS);
     p.splits = 1;
+    p.scratch = 0;
   }
-  const int64_t need = plan_scratch(p, Tq, q_heads, head_dim);
+  const int64_t need = p.scratch;
   if (need && (!scratch || scratch_bytes < need || !aligned16(scratch)))
     return set_error(QVGGT_ERR_INVALID, "%s: needs %lld bytes of 16-byte aligned scratch, got %lld", name,
                      (long long)need, (long long)scratch_bytes);
   a.row_blocks = p.row_blocks;
   a.splits = p.splits;
-  a.part_o = static_cast<float*>(scratch);
-  a.part_lse = need ? a.part_o + (long long)p.splits * Tq * q_heads * head_dim : nullptr;
   const bool bf16 = dtype == QVGGT_DTYPE_BF16;
   using Kfn = void (*)(CacheAttnArgs);
   static const Kfn rows_fns[2][2] = {{attn_cache_rows_kernel<false, 64>, attn_cache_rows_kernel<false, 128>},
@@ -403,13 +385,14 @@ extern "C" int qvggt_cached_attention(const void* q, int64_t q_tok, int64_t q_he
   static const Kfn join_fns[2][2] = {{attn_cache_join_kernel<false, 64>, attn_cache_join_kernel<false, 128>},
                                      {attn_cache_join_kernel<true, 64>, attn_cache_join_kernel<true, 128>}};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int rc = p.tiles ? launch_tiles(a, head_dim, bf16, st)
-                         : check_cuda(launch_pdl(rows_fns[bf16][head_dim == 128],
-                                                 dim3((unsigned)p.row_blocks, (unsigned)(kv_heads * requests),
-                                                      (unsigned)p.splits),
-                                                 dim3(TOK_WARPS * 32), 0, st, 1u, a),
-                                      "cached_attention launch");
-  if (rc) return rc;
+  if (p.tiles) return launch_tiles(a, head_dim, bf16, max_kv, scratch, st);
+  a.part_o = static_cast<float*>(scratch);
+  a.part_lse = need ? a.part_o + (long long)p.splits * Tq * q_heads * head_dim : nullptr;
+  if (int rc = check_cuda(launch_pdl(rows_fns[bf16][head_dim == 128],
+                                     dim3((unsigned)p.row_blocks, (unsigned)(kv_heads * requests), (unsigned)p.splits),
+                                     dim3(TOK_WARPS * 32), 0, st, 1u, a),
+                          "cached_attention launch"))
+    return rc;
   count_launch(1);
   if (p.splits > 1) {
     if (int rc = check_cuda(launch_pdl(join_fns[bf16][head_dim == 128], dim3((unsigned)((Tq * q_heads + 7) / 8)),

@@ -21,11 +21,13 @@ struct CacheAttnArgs {
   const int8_t *kc, *vc;
   const float *ks, *vs;
   const int32_t *table, *cu_q, *kv_lens;
-  float *part_o, *part_lse;              // [splits][Tq * hq][D], [splits][Tq * hq] (splits > 1)
+  float *part_o, *part_lse;              // parts of rows, and their log2-sum-exp
   long long q_tok, q_head, o_tok, o_head, block_stride, Tq;
   int B, hq, hk, group, wide, num_blocks, bs_log2, chunk, max_q, splits;
-  int row_blocks;                        // Q blocks of the longest request (tile kernel)
+  int row_blocks;                        // Q blocks (16-row tiles) of the longest request
+  int can_split;                         // tile kernel: items may be cut, a join follows
   float scale_log2;
+  uint32_t wait_tries;                   // tile kernel: bound of every wait
   Ctl ctl;
 };
 
@@ -62,8 +64,10 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
   return BF16 ? codes_bf16<HI>(w) : codes_f16<HI>(w ^ 0x80808080u);
 }
 
-// attn_cache_sm100.cu: whether its TMA map can read these queries, and the launch (grid, shared memory, map).
+// attn_cache_sm100.cu (many rows): whether its TMA map can read these queries;
+// the scratch for `items` (request, Q block, kv head) triples; the launches.
 bool tiles_can_read(const CacheAttnArgs& a);
-int launch_tiles(const CacheAttnArgs& a, int D, bool bf16, cudaStream_t stream);
+int64_t tiles_scratch(long long items, long long max_kv, int D);
+int launch_tiles(CacheAttnArgs& a, int D, bool bf16, long long max_kv, void* scratch, cudaStream_t stream);
 
 }  // namespace qv

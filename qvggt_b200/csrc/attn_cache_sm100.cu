@@ -4,15 +4,25 @@
 // and both scales live in the softmax, per 32 keys (never across two blocks)
 //   x = ck S + lv,  ck = scale log2e ks_B, lv = log2 vs_B,  P = 2^(x - m),
 //   O += P c_v,  l += (1 / vs_B) sum P,  out = O / l.
-// One CTA per (request, kv head, two 128-row Q tiles, split of the keys); a
-// row is a (token, query head of the group) pair, so the heads that share K/V
-// share its tiles.  Per key tile of KT keys (128 for head_dim 64, 64 for 128):
+// An item is (request, block of two 128-row Q tiles, kv head); a row is a
+// (token, query head of the group) pair, so the heads that share K/V share its
+// tiles.  Lengths are ragged and known on the GPU only, and a causal mask gives
+// late blocks many times the keys of early ones, so the items' key tiles are
+// laid out as one line of cost and cut into equal pieces, one per SM: each CTA
+// scans the requests (a few KB), finds its piece and walks it.  Where a cut
+// falls inside an item, both sides park normalised rows and their log-sum-exp,
+// and the join kernel adds them; at most two parts per CTA, so the scratch does
+// not grow with the problem.  Per key tile of KT keys (128 for head_dim 64, 64
+// for 128):
 //   warp 0         block ids and scales, cp.async.bulk of the raw codes (RAW
 //                  stages of 16 KB), constants of the tile into a small ring
 //   warps 4..7     codes -> fp16 (bf16 for K with bf16 queries) into the
 //                  128-byte-swizzled operand tiles (two stages each of K, V)
 //   warp 1         S_i = Q_i K^T        warp 3   O_i += P_i V
 //   warps 8..15    softmax, one thread per row of Q tile i = 0, 1
+//   warp 2         the segments (an item, or the part of it that falls to this
+//                  CTA), a few ahead; every other role reads them from a ring
+// The next segment's loads and first S products run under the end of the one before.
 // The running maximum is raised lazily (2^8), as in attention_sm100.cu.  All
 // waits are bounded; on expiry every role leaves and the status word is set.
 //
@@ -28,6 +38,15 @@ constexpr int THREADS = 512;
 constexpr int RAW = 4;          // stages of raw codes
 constexpr int KV = 2;           // operand stages of K and of V
 constexpr int CRING = 8;        // constants: more than RAW + KV tiles back nothing reads them
+constexpr int SEGS = 4;         // segments handed out ahead
+constexpr int SEG_READERS = 15; // producer, two issuers, 4 + 8 warps
+constexpr int Q_ROWS = 256;     // rows of an item
+// Cost of an item on the line: a start-up (loads, first products, epilogue)
+// and its key tiles; with one Q tile a softmax warpgroup idles, but the other's
+// chain per tile is nearly as long.
+constexpr int COST_START = 20, COST_TILE2 = 10, COST_TILE1 = 9;
+// No piece is cut shorter than this (8 tiles): a join costs about as much.
+constexpr int COST_MIN = COST_START + 8 * COST_TILE2;
 constexpr int RAW_BYTES = 8192; // K or V codes of a tile
 constexpr int OP_BYTES = 16384; // the same as fp16
 constexpr uint32_t TMEM_COLS = 512;
@@ -44,11 +63,28 @@ struct Lay {
   static constexpr int RV = RK + RAW * RAW_BYTES;
   static constexpr int CONST = RV + RAW * RAW_BYTES;       // float4 [CRING][KT / 32]
   static constexpr int BAR = CONST + CRING * (KT / 32) * 16;
-  // q_full, raw_full[RAW], raw_empty[RAW], c_full[CRING], k_full[KV], k_empty[KV], v_full[KV], v_empty[KV],
-  // s_full[2], s_free[2], p_full[2], o_done[2], drain, drain2
-  static constexpr int NUM_BARS = 1 + 2 * RAW + CRING + 4 * KV + 8 + 2;
-  static constexpr int MISC = BAR + NUM_BARS * 8;          // TMEM base, abort flag, status pointer, timeout
-  static constexpr int TOTAL = MISC + 32 + 1024;
+  // q_full, q_empty, raw_full[RAW], raw_empty[RAW], k_full[KV], k_empty[KV], v_full[KV],
+  // v_empty[KV], seg_full[SEGS], seg_empty[SEGS], s_full[2], s_free[2], p_full[2], o_done[2], drain, drain2
+  static constexpr int NUM_BARS = 2 + 2 * RAW + 4 * KV + 2 * SEGS + 8 + 2;
+  static constexpr int MISC = BAR + NUM_BARS * 8;          // TMEM base
+  static constexpr int SEG = MISC + 32;                    // Segment [SEGS]
+  static constexpr int CUM = SEG + SEGS * 64;              // long long [THREADS + 1]
+  static constexpr int TOTAL = CUM + (THREADS + 1) * 8 + 64 + 1024;
+};
+
+// What a CTA does with one item: key tiles [t0, t0 + nt).
+struct __align__(16) Segment {
+  int b, kvh, tok0, q0;                  // tok0: first token (of the request) of the Q block
+  int ql, n, nqt, t0;
+  int nt;                                // -1: no more segments
+  int slot;                              // where the part is parked; -1: the item is whole
+  int pad[2];
+};
+
+// Where a cut lies, for the join: written by the CTA after it.
+struct __align__(16) Cut {
+  int first, last;                       // CTAs that hold parts of the item (first < 0: the cut is between items)
+  int kvh, tok0, q0, ql, pad[2];
 };
 
 // cp.async.bulk of contiguous bytes, completion on an mbarrier of this CTA.
@@ -58,48 +94,115 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
+// Bounded wait for the phase with parity `parity`: up to `tries` try_waits,
+// each of which the hardware suspends for about 1.4 us if nothing arrives.
+// Nothing but the loop, as it is inlined at every hand-off: the roles of an SM
+// run from one instruction cache, and its misses cost this kernel 12 % when
+// each wait carried its own time-out code.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, uint32_t tries) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+      "mov.u32 n, %3;\n\t"
+      "QV_TRY:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra QV_DONE;\n\t"
+      "sub.u32 n, n, 1;\n\t"
+      "setp.ne.u32 q, n, 0;\n\t"
+      "@q bra QV_TRY;\n\t"
+      "QV_DONE:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(tries)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait(const uint64_t* bar, uint32_t parity, uint32_t tries) {
+  return wait(smem_u32(bar), parity, tries);
+}
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
+}
+
+// Whether the phase is complete, without waiting.
+__device__ __forceinline__ bool test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// A wait of a whole warp that then stays converged.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint32_t tries) {
+  return __all_sync(0xffffffffu, wait(bar, parity, tries));
+}
+__device__ __forceinline__ bool warp_wait(const uint64_t* bar, uint32_t parity, uint32_t tries) {
+  return warp_wait(smem_u32(bar), parity, tries);
+}
+
 // K-major or MN-major operand with 128-byte swizzle; lead: bytes between the
 // 64-element panels of an MN-major operand (unused by K-major ones).
 __device__ __forceinline__ uint64_t sdesc_panels(uint32_t saddr, uint32_t lead) {
   return (sdesc_sw128(saddr) & ~(0x3fffull << 16)) | ((uint64_t)(lead >> 4) << 16);
 }
 
-// Max over the 32 scores of a chunk, of the first `valid` with PARTIAL.
-template <bool PARTIAL, int E0, int N>
-__device__ __forceinline__ float chunk_max(const uint32_t (&s)[N], int valid) {
-  float m0 = -INFINITY, m1 = -INFINITY;
+// Constants of a 32-key chunk.
+struct Chunk {
+  float ck, lv, inv_vs;
+};
+
+// A tile that the row sees in part (valid < KT keys, may be <= 0): hidden
+// scores become -inf, and a chunk without a visible key gets neutral constants
+// (whatever its block's scales are, the row takes nothing from them).
+template <int KT>
+__device__ __forceinline__ void hide_keys(uint32_t (&s)[KT], Chunk (&k)[KT / 32], int valid) {
 #pragma unroll
-  for (int e = E0; e < E0 + 32; e += 4) {
-    if (!PARTIAL) {
-      m0 = max3f(m0, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-      m1 = max3f(m1, __uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
-    } else {
-      if (e + 0 < valid) m0 = fmaxf(m0, __uint_as_float(s[e + 0]));
-      if (e + 1 < valid) m1 = fmaxf(m1, __uint_as_float(s[e + 1]));
-      if (e + 2 < valid) m0 = fmaxf(m0, __uint_as_float(s[e + 2]));
-      if (e + 3 < valid) m1 = fmaxf(m1, __uint_as_float(s[e + 3]));
+  for (int e = 0; e < KT; ++e)
+    if (e >= valid) s[e] = 0xff800000u;
+#pragma unroll
+  for (int c = 0; c < KT / 32; ++c)
+    if (32 * c >= valid) k[c] = {1.f, 0.f, 0.f};
+}
+
+// Max over the row of ck S + lv: each chunk's largest score first, four chains.
+template <int KT>
+__device__ __forceinline__ float tile_max(const uint32_t (&s)[KT], const Chunk (&k)[KT / 32], float mx) {
+#pragma unroll
+  for (int c = 0; c < KT / 32; ++c) {
+    float m[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const uint32_t* v = &s[32 * c + 8 * x];
+      m[x] = max3f(max3f(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2])), __uint_as_float(v[3]),
+                   __uint_as_float(v[4]));
+      m[x] = max3f(m[x], __uint_as_float(v[5]), fmaxf(__uint_as_float(v[6]), __uint_as_float(v[7])));
     }
+    mx = fmaxf(mx, fmaf(max3f(fmaxf(m[0], m[1]), m[2], m[3]), k[c].ck, k[c].lv));
   }
-  return fmaxf(m0, m1);
+  return mx;
 }
 
-__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-
-// P of chunk E0 / 16 (pairs E0..E0+15) as fp16 pairs into s[E0..), its sum
-// over 1 / vs into l.  POLY of 8 pairs take the FMA-pipe exponential.
-template <bool PARTIAL, int POLY, int E0, int N>
-__device__ __forceinline__ void exp_chunk(uint32_t (&s)[N], const float4& k, float neg_m, float& l, int valid) {
-  const uint64_t c2 = f2_pack(k.x, k.x), nm2 = f2_pack(k.y + neg_m, k.y + neg_m);
+// P of chunk C as fp16 pairs into s[16 C..16 C + 16) (no earlier chunk wrote
+// the scores it reads), its sum over 1 / vs into l.  POLY of 8 pairs take the
+// FMA-pipe exponential.
+template <int POLY, int C, int KT>
+__device__ __forceinline__ void exp_chunk(uint32_t (&s)[KT], const Chunk& k, float neg_m, float& l) {
+  const uint64_t c2 = f2_pack(k.ck, k.ck), nm2 = f2_pack(k.lv + neg_m, k.lv + neg_m);
   uint64_t la = f2_pack(0.f, 0.f), lb = f2_pack(0.f, 0.f);
 #pragma unroll
-  for (int e = E0; e < E0 + 16; ++e) {
+  for (int e = 16 * C; e < 16 * C + 16; ++e) {
     const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, nm2);
     float p0, p1;
     if ((e & 7) < POLY) {
@@ -110,19 +213,63 @@ __device__ __forceinline__ void exp_chunk(uint32_t (&s)[N], const float4& k, flo
       p0 = ex2(x0);
       p1 = ex2(x1);
     }
-    if (PARTIAL) {
-      if (2 * e >= valid) p0 = 0.f;
-      if (2 * e + 1 >= valid) p1 = 0.f;
-    }
     if (e & 1) lb = f2_add(lb, f2_pack(p0, p1));
     else la = f2_add(la, f2_pack(p0, p1));
     s[e] = pack_half2(p0, p1);
   }
   float l0, l1;
   f2_unpack(f2_add(la, lb), l0, l1);
-  const float sum = l0 + l1;
-  if (!PARTIAL || sum != 0.f) l += sum * k.z;   // a row that sees none of the keys takes nothing from their scale
+  l = fmaf(l0 + l1, k.inv_vs, l);
 }
+
+// P of the tile to TMEM, a chunk at a time (the stores overlap the
+// exponentials still to come).  P may be written once the PV product of the
+// tile before has read the previous one: that wait (unless `first`) comes
+// just before the first store.  False if it gave up.
+template <int POLY, int KT>
+__device__ __forceinline__ bool exp_store(uint32_t (&s)[KT], const Chunk (&k)[KT / 32], float neg_m, float& l,
+                                          uint32_t tP, bool first, uint32_t o_done, uint32_t o_parity, uint32_t tries) {
+  // asked before the first exponentials: a test's answer takes about 100 cycles
+  const bool ready = first || test(o_done, o_parity);
+  exp_chunk<POLY, 0>(s, k[0], neg_m, l);
+  if (!__all_sync(~0u, ready) && !warp_wait(o_done, o_parity, tries)) return false;
+  tc_fence_after();
+  tmem_st16(tP, *reinterpret_cast<const uint32_t(*)[16]>(&s[0]));
+  exp_chunk<POLY, 1>(s, k[1], neg_m, l);
+  tmem_st16(tP + 16, *reinterpret_cast<const uint32_t(*)[16]>(&s[16]));
+  if constexpr (KT == 128) {
+    exp_chunk<POLY, 2>(s, k[2], neg_m, l);
+    tmem_st16(tP + 32, *reinterpret_cast<const uint32_t(*)[16]>(&s[32]));
+    exp_chunk<POLY, 3>(s, k[3], neg_m, l);
+    tmem_st16(tP + 48, *reinterpret_cast<const uint32_t(*)[16]>(&s[48]));
+  }
+  tmem_st_wait();
+  return true;
+}
+
+// Q block `qb` of request b: its rows and keys.
+template <int KT>
+struct Block {
+  int q0, ql, n, tok0, nqt, tiles;
+  long long cost;                        // of one kv head; 0: no such block
+  __device__ __forceinline__ Block(const CacheAttnArgs& a, int b, int qb) {
+    q0 = a.cu_q[b];
+    ql = a.cu_q[b + 1] - q0;
+    n = a.kv_lens[b];
+    const int tpt = 128 / a.group;       // tokens of a Q tile
+    tok0 = qb * 2 * tpt;
+    nqt = tok0 + tpt < ql ? 2 : 1;
+    tiles = 0;
+    cost = 0;
+    if (tok0 >= ql) return;
+    if (q0 < 0 || ql > a.max_q || (long long)q0 + ql > a.Tq || n < 0 || n > (a.wide << a.bs_log2)) {
+      report_status(a.ctl, ST_BAD_LENGTH);
+      return;
+    }
+    tiles = (key_limit(min(ql, tok0 + 2 * tpt) - 1, ql, n, a.chunk) + KT - 1) / KT;
+    cost = COST_START + (long long)tiles * (nqt == 2 ? COST_TILE2 : COST_TILE1);
+  }
+};
 
 template <bool BF16, int D>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -134,48 +281,53 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::BAR);
-  uint64_t* raw_full = q_full + 1;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* raw_full = q_empty + 1;
   uint64_t* raw_empty = raw_full + RAW;
-  uint64_t* c_full = raw_empty + RAW;
-  uint64_t* k_full = c_full + CRING;
+  uint64_t* k_full = raw_empty + RAW;
   uint64_t* k_empty = k_full + KV;
   uint64_t* v_full = k_empty + KV;
   uint64_t* v_empty = v_full + KV;
+  uint64_t* seg_full = v_empty + KV;
+  uint64_t* seg_empty = seg_full + SEGS;
   // the softmax warps address the next four [2] arrays from s_full[i] at byte offsets 16, 32, 48
-  uint64_t* s_full = v_empty + KV;
+  uint64_t* s_full = seg_empty + SEGS;
   uint64_t* s_free = s_full + 2;
   uint64_t* p_full = s_free + 2;
   uint64_t* o_done = p_full + 2;
   uint64_t* drain = o_done + 2;
   uint64_t* drain2 = drain + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
-  const uint32_t misc = sbase + L::MISC;
+  volatile Segment* segs = reinterpret_cast<volatile Segment*>(smem + L::SEG);
+  long long* cum = reinterpret_cast<long long*>(smem + L::CUM);
+  const uint32_t tries = a.wait_tries;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int s = 0; s < RAW; ++s) {
       mbar_init(&raw_full[s], 1);
       mbar_init(&raw_empty[s], 4);
     }
-    for (int s = 0; s < CRING; ++s) mbar_init(&c_full[s], 1);
     for (int s = 0; s < KV; ++s) {
       mbar_init(&k_full[s], 4);
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_full[s], 4);
       mbar_init(&v_empty[s], 1);
     }
+    for (int s = 0; s < SEGS; ++s) {
+      mbar_init(&seg_full[s], 1);
+      mbar_init(&seg_empty[s], SEG_READERS);
+    }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
+      mbar_init(&s_full[i], 2);
       mbar_init(&s_free[i], 4);
       mbar_init(&p_full[i], 4);
       mbar_init(&o_done[i], 1);
     }
     mbar_init(drain, 1);
     mbar_init(drain2, 1);
-    *reinterpret_cast<int*>(smem + L::MISC + 4) = 0;
-    *reinterpret_cast<uint32_t**>(smem + L::MISC + 8) = a.ctl.status;
-    *reinterpret_cast<unsigned long long*>(smem + L::MISC + 16) = a.ctl.timeout_ns;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -183,236 +335,391 @@ __global__ void __launch_bounds__(THREADS, 1)
     tmem_relinquish();
   }
   if (warp == 0 && lane == 0) tma_prefetch_desc(&tmQ);
+  pdl_wait();
+  pdl_trigger();
+  // Running sums of the blocks' costs: thread x has blocks [x g, (x + 1) g).
+  const int blocks = a.B * a.row_blocks, g = (blocks + THREADS - 1) / THREADS;
+  {
+    long long sum = 0;
+    for (int p = threadIdx.x * g; p < min(blocks, ((int)threadIdx.x + 1) * g); ++p)
+      sum += Block<KT>(a, p / a.row_blocks, p % a.row_blocks).cost;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const long long o = __shfl_up_sync(~0u, sum, d);
+      if (lane >= d) sum += o;
+    }
+    cum[threadIdx.x + 1] = sum;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  pdl_wait();
-  pdl_trigger();
+  if (warp == 0) {
+    // sums of the warps before, added to every warp's
+    long long s = lane < THREADS / 32 ? cum[lane * 32 + 32] : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const long long o = __shfl_up_sync(~0u, s, d);
+      if (lane >= d) s += o;
+    }
+    cum[0] = 0;
+    __syncwarp();
+    for (int w = 1; w < THREADS / 32; ++w) {
+      const long long before = __shfl_sync(~0u, s, w - 1);
+      cum[w * 32 + lane + 1] += before;
+    }
+  }
+  __syncthreads();
   const uint32_t tmem = *tmem_slot;
-
-  // The item.  Blocks of later tokens first: under a causal mask they see the
-  // most keys, and the longest CTAs should not start last.
-  const int sp = blockIdx.x % a.splits;
-  const int bh = (blockIdx.x / a.splits) % (a.B * a.hk);
-  const int qb = a.row_blocks - 1 - blockIdx.x / (a.splits * a.B * a.hk);
-  const int b = bh / a.hk, kvh = bh % a.hk;
-  const int q0 = a.cu_q[b], ql = a.cu_q[b + 1] - q0, n = a.kv_lens[b];
   const int tpt = 128 / a.group;                           // tokens of a Q tile
-  const int tok0 = qb * 2 * tpt;
-  bool live = tok0 < ql;
-  if (q0 < 0 || ql < 0 || ql > a.max_q || (long long)q0 + ql > a.Tq || n < 0 || n > (a.wide << a.bs_log2)) {
-    if (threadIdx.x == 0) report_status(a.ctl, ST_BAD_LENGTH);
-    live = false;
-  }
-  const int nqt = tok0 + tpt < ql ? 2 : 1;                 // Q tiles that hold rows
-  int t0 = 0, nt = 0;                                      // key tiles of this CTA
-  if (live) {
-    const int lim = key_limit(min(ql, tok0 + 2 * tpt) - 1, ql, n, a.chunk);
-    const int tiles = (lim + KT - 1) / KT;
-    t0 = (int)((long long)sp * tiles / a.splits);
-    nt = (int)((long long)(sp + 1) * tiles / a.splits) - t0;
-  }
 
-  // Registers: launched at 128 each; 128 (48 + 80 + 2 * 192) = 128 * 512.
+  // Registers: launched at 128 each; 128 (64 + 64 + 2 * 192) = 128 * 512.
   // Every warp of a warpgroup runs the same setmaxnreg.
   if (warp < 4) {
-    regs_dec<48>();
-    if (warp == 0 && nt > 0) {
-      // ---------------------------------------------------------- producer
+    regs_dec<64>();
+    if (warp == 2) {
+      // ---------------------------------------------------------- segments
       if (lane == 0) {
-        const int rows = tpt * a.group;
-        mbar_arrive_expect_tx(q_full, nqt * L::PANELS * rows * 128);
-        for (int i = 0; i < nqt; ++i)
-          for (int p = 0; p < L::PANELS; ++p)
-            tma_load_3d(smem + L::Q + (i * L::PANELS + p) * L::Q_PANEL, &tmQ, q_full, p * 64, kvh * a.group,
-                        q0 + tok0 + i * tpt);
+        const long long total = cum[THREADS] * a.hk;
+        const int grid = gridDim.x, x = blockIdx.x;
+        long long W = (total + grid - 1) / grid;
+        if (a.can_split && W < COST_MIN) W = COST_MIN;
+        const long long begin = x * W, end = min(total, begin + W);
+        int seg = 0;
+        bool ok = true;
+        Cut cut{-1, -1, 0, 0, 0, 0, {0, 0}};
+        if (begin < end) {
+          // block and head that contain `begin`
+          int e = 0;
+          for (int len = THREADS; len > 1;) {
+            const int half = len / 2;
+            if (cum[e + half] * a.hk <= begin) e += half;
+            len -= half;
+          }
+          int p = e * g;
+          long long s = cum[e] * a.hk;                     // where block p starts
+          while (p < blocks) {
+            const Block<KT> blk(a, p / a.row_blocks, p % a.row_blocks);
+            const int c = blk.nqt == 2 ? COST_TILE2 : COST_TILE1;
+            if (blk.cost > 0 && s + blk.cost * a.hk > begin) {
+              if (s >= end) break;
+              int h = begin > s ? (int)((begin - s) / blk.cost) : 0;
+              for (; h < a.hk; ++h) {
+                const long long s0 = s + h * blk.cost, k0 = s0 + COST_START;   // the item, its first tile
+                if (s0 >= end) break;
+                Segment sg{};
+                sg.slot = -1;
+                int t_lo = 0, t_hi = blk.tiles;
+                if (a.can_split && blk.tiles > 0) {
+                  // tile t belongs to the CTA whose piece holds k0 + t c
+                  auto at = [&](long long pos) {
+                    return pos <= k0 ? 0 : (int)min((long long)blk.tiles, (pos - k0 + c - 1) / c);
+                  };
+                  t_lo = at(begin);
+                  t_hi = x == grid - 1 ? blk.tiles : at(begin + W);
+                  const int first = (int)min(k0 / W, (long long)grid - 1);
+                  const int last = (int)min((k0 + (long long)(blk.tiles - 1) * c) / W, (long long)grid - 1);
+                  if (t_lo >= t_hi) continue;
+                  if (first != last) {
+                    sg.slot = 2 * x + (t_lo == 0 ? 1 : 0);
+                    if (t_lo > 0)
+                      cut = Cut{first, last, h, blk.tok0, blk.q0, blk.ql, {0, 0}};
+                  }
+                } else if (s0 < begin) {
+                  continue;                                // whole items: the CTA that holds the start
+                }
+                const int st = seg % SEGS;
+                if (!wait(&seg_empty[st], ((seg / SEGS) & 1) ^ 1, tries)) { ok = false; break; }
+                segs[st].b = p / a.row_blocks;
+                segs[st].kvh = h;
+                segs[st].tok0 = blk.tok0;
+                segs[st].q0 = blk.q0;
+                segs[st].ql = blk.ql;
+                segs[st].n = blk.n;
+                segs[st].nqt = blk.nqt;
+                segs[st].t0 = t_lo;
+                segs[st].nt = t_hi - t_lo;
+                segs[st].slot = sg.slot;
+                mbar_arrive(&seg_full[st]);
+                ++seg;
+              }
+              if (!ok) break;
+            }
+            s += blk.cost * a.hk;
+            ++p;
+          }
+        }
+        if (a.can_split) reinterpret_cast<Cut*>(a.part_lse + 2LL * grid * Q_ROWS)[x] = cut;
+        const int st = seg % SEGS;
+        if (ok && wait(&seg_empty[st], ((seg / SEGS) & 1) ^ 1, tries)) {
+          segs[st].nt = -1;
+          mbar_arrive(&seg_full[st]);
+        }
       }
+    } else if (warp == 0) {
+      // ---------------------------------------------------------- producer
       const int bs = 1 << a.bs_log2;
       const int piece = min(bs, KT);                       // keys of one copy
       const int pieces = KT / piece;
-      const int32_t* row = a.table + (long long)b * a.wide;
-      // lane i holds the id and scales of block base + i; the next 32 are
-      // fetched while these are used
-      int base = (t0 * KT) >> a.bs_log2;
-      const int last = (min((t0 + nt) * KT, n) - 1) >> a.bs_log2;
-      auto fetch_id = [&](int j) { return j <= last ? row[j] : -1; };
-      auto fetch_scales = [&](int id, float& ks, float& vs) {
-        const bool good = id >= 0 && id < a.num_blocks;
-        ks = good ? a.ks[(long long)id * a.hk + kvh] : 0.f;
-        vs = good ? a.vs[(long long)id * a.hk + kvh] : 0.f;
-      };
-      int id = fetch_id(base + lane);
-      float ks, vs;
-      fetch_scales(id, ks, vs);
-      int id2 = fetch_id(base + 32 + lane);
       bool bad = false, ok = true;
-      int j = 0;
-      for (; j < nt; ++j) {
-        const int key0 = (t0 + j) * KT;
-        if (((key0 + KT - 1) >> a.bs_log2) >= base + 32) {
-          // blocks and tiles nest, so a tile starts on the batch's boundary
-          base += 32;
-          id = id2;
-          fetch_scales(id, ks, vs);
-          id2 = fetch_id(base + 32 + lane);
-        }
-        // constants of the tile's 32-key chunks
-        const int cj = min(((key0 + 32 * lane) >> a.bs_log2) - base, 31);
-        const int cid = __shfl_sync(~0u, id, cj);
-        const float cks = __shfl_sync(~0u, ks, cj), cvs = __shfl_sync(~0u, vs, cj);
-        // the copy of lane's piece
-        const int pkey = key0 + lane * piece;
-        const int pid = __shfl_sync(~0u, id, min((pkey >> a.bs_log2) - base, 31));
-        const bool mine = lane < pieces && pkey < n;
-        const bool good = mine && pid >= 0 && pid < a.num_blocks;
-        bad |= mine && !good;
-        const int st = j % RAW;
-        ok = __all_sync(~0u, wait(&raw_empty[st], ((j / RAW) & 1) ^ 1, misc, ST_TIMEOUT_TMA_EMPTY));
+      int jg = 0, it = 0;                                  // key tiles and Q blocks loaded so far
+      for (int seg = 0;; ++seg) {
+        const int ss = seg % SEGS;
+        ok = warp_wait(&seg_full[ss], (seg / SEGS) & 1, tries);
         if (!ok) break;
-        if (lane < CH) {
-          const bool have = cid >= 0 && cid < a.num_blocks && key0 + 32 * lane < n;
-          // a skipped block: every score -inf
-          const float4 k = have ? make_float4(cks * a.scale_log2, log2f(cvs), 1.f / cvs, 0.f)
-                                : make_float4(0.f, -INFINITY, 0.f, 0.f);
-          reinterpret_cast<float4*>(smem + L::CONST)[(j % CRING) * CH + lane] = k;
-        }
-        const uint32_t count = __popc(__ballot_sync(~0u, good));
-        if (lane == 0) {
-          mbar_arrive(&c_full[j % CRING]);
-          mbar_arrive_expect_tx(&raw_full[st], count * 2 * piece * D);
-        }
+        const int b = segs[ss].b, kvh = segs[ss].kvh, n = segs[ss].n, t0 = segs[ss].t0, nt = segs[ss].nt;
+        const int q_tok = segs[ss].q0 + segs[ss].tok0, nqt = segs[ss].nqt;
         __syncwarp();
-        if (good) {
-          const long long off = pid * a.block_stride + ((long long)kvh * bs + (pkey & (bs - 1))) * D;
-          const uint32_t at = st * RAW_BYTES + lane * piece * D, bar = smem_u32(&raw_full[st]);
-          bulk_load(sbase + L::RK + at, a.kc + off, piece * D, bar);
-          bulk_load(sbase + L::RV + at, a.vc + off, piece * D, bar);
+        if (lane == 0) mbar_arrive(&seg_empty[ss]);
+        if (nt < 0) break;
+        if (nt == 0) continue;
+        const int32_t* row = a.table + (long long)b * a.wide;
+        // lane i holds the id and scales of block base + i; the next 32 are
+        // fetched while these are used
+        int base = (t0 * KT) >> a.bs_log2;
+        const int last = (min((t0 + nt) * KT, n) - 1) >> a.bs_log2;
+        auto fetch_id = [&](int j) { return j <= last ? row[j] : -1; };
+        auto fetch_scales = [&](int id, float& ks, float& vs) {
+          const bool good = id >= 0 && id < a.num_blocks;
+          ks = good ? a.ks[(long long)id * a.hk + kvh] : 0.f;
+          vs = good ? a.vs[(long long)id * a.hk + kvh] : 0.f;
+        };
+        int id = fetch_id(base + lane);
+        float ks, vs;
+        fetch_scales(id, ks, vs);
+        int id2 = fetch_id(base + 32 + lane);
+        bool q_loaded = false;
+        for (int j = 0; j < nt; ++j, ++jg) {
+          const int key0 = (t0 + j) * KT;
+          if (((key0 + KT - 1) >> a.bs_log2) >= base + 32) {
+            // blocks and tiles nest, so a tile starts on the batch's boundary
+            base += 32;
+            id = id2;
+            fetch_scales(id, ks, vs);
+            id2 = fetch_id(base + 32 + lane);
+          }
+          // constants of the tile's 32-key chunks: seen by the softmax through
+          // raw_full, k_full and the S issuer's own arrival on s_full
+          const int cj = min(((key0 + 32 * lane) >> a.bs_log2) - base, 31);
+          const int cid = __shfl_sync(~0u, id, cj);
+          const float cks = __shfl_sync(~0u, ks, cj), cvs = __shfl_sync(~0u, vs, cj);
+          // the copy of lane's piece
+          const int pkey = key0 + lane * piece;
+          const int pid = __shfl_sync(~0u, id, min((pkey >> a.bs_log2) - base, 31));
+          const bool mine = lane < pieces && pkey < n;
+          const bool good = mine && pid >= 0 && pid < a.num_blocks;
+          bad |= mine && !good;
+          const int st = jg % RAW;
+          ok = warp_wait(&raw_empty[st], ((jg / RAW) & 1) ^ 1, tries);
+          if (!ok) break;
+          if (lane < CH) {
+            const bool have = cid >= 0 && cid < a.num_blocks && key0 + 32 * lane < n;
+            // a skipped block: every score -inf
+            const float4 k = have ? make_float4(cks * a.scale_log2, log2f(cvs), 1.f / cvs, 0.f)
+                                  : make_float4(1.f, -INFINITY, 0.f, 0.f);
+            reinterpret_cast<float4*>(smem + L::CONST)[(jg % CRING) * CH + lane] = k;
+          }
+          const uint32_t count = __popc(__ballot_sync(~0u, good));
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&raw_full[st], count * 2 * piece * D);
+          }
+          __syncwarp();
+          if (good) {
+            const long long off = pid * a.block_stride + ((long long)kvh * bs + (pkey & (bs - 1))) * D;
+            const uint32_t at = st * RAW_BYTES + lane * piece * D, bar = smem_u32(&raw_full[st]);
+            bulk_load(sbase + L::RK + at, a.kc + off, piece * D, bar);
+            bulk_load(sbase + L::RV + at, a.vc + off, piece * D, bar);
+          }
+          if (!q_loaded && (j == min(nt, 2) - 1)) {
+            // Q is free once the S products of the item before are done; by
+            // then this item's first codes are on their way
+            q_loaded = true;
+            ok = it == 0 || warp_wait(q_empty, (it - 1) & 1, tries);
+            if (!ok) { ++jg; break; }
+            if (lane == 0) {
+              mbar_arrive_expect_tx(q_full, nqt * L::PANELS * tpt * a.group * 128);
+              for (int i = 0; i < nqt; ++i)
+                for (int p = 0; p < L::PANELS; ++p)
+                  tma_load_3d(smem + L::Q + (i * L::PANELS + p) * L::Q_PANEL, &tmQ, q_full, p * 64, kvh * a.group,
+                              q_tok + i * tpt);
+            }
+            ++it;
+          }
         }
+        if (!ok) break;
       }
       if (bad) report_bad_block(a.ctl);
       if (!ok && lane == 0) {
-        // aborted: let the copies in flight land before the CTA exits
-        mbar_wait_drain(q_full, 0, 200000000ull);
-        for (int jj = max(0, j - RAW); jj < j; ++jj)
+        // gave up: let the copies in flight land before the CTA exits
+        report_status(a.ctl, ST_TIMEOUT_TMA_EMPTY);
+        if (it > 0) mbar_wait_drain(q_full, (it - 1) & 1, 200000000ull);
+        for (int jj = max(0, jg - RAW); jj < jg; ++jj)
           mbar_wait_drain(&raw_full[jj % RAW], (jj / RAW) & 1, 200000000ull);
       }
-    } else if (warp == 1 && nt > 0) {
+    } else if (warp == 1) {
       // ---------------------------------------------------------- S = Q K^T
-      if (lane == 0) {
-        constexpr uint32_t idesc = idesc_f16(128, KT, false, false, BF16);
-        bool ok = wait(q_full, 0, misc, ST_TIMEOUT_FULL);
-        for (int j = 0; ok && j < nt; ++j) {
-          const int st = j % KV;
-          if (!wait(&k_full[st], (j / KV) & 1, misc, ST_TIMEOUT_DEQ)) { ok = false; break; }
+      // The issuers walk their loops as whole warps and elect a lane for each
+      // group of MMAs: from inside a one-lane branch the same MMAs issue a
+      // third slower (their descriptors are then not warp-uniform).
+      constexpr uint32_t idesc = idesc_f16(128, KT, false, false, BF16);
+      uint32_t cs[2] = {0, 0};                             // S_i products issued so far
+      int jg = 0, it = 0;
+      bool ok = true;
+      for (int seg = 0; ok; ++seg) {
+        const int ss = seg % SEGS;
+        if (!warp_wait(&seg_full[ss], (seg / SEGS) & 1, tries)) { ok = false; break; }
+        const int nt = segs[ss].nt, nqt = segs[ss].nqt;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&seg_empty[ss]);
+        if (nt < 0) break;
+        if (nt == 0) continue;
+        if (!warp_wait(q_full, it & 1, tries)) { ok = false; break; }
+        ++it;
+        for (int j = 0; j < nt; ++j, ++jg) {
+          const int st = jg % KV;
+          if (!warp_wait(&k_full[st], (jg / KV) & 1, tries)) { ok = false; break; }
           for (int i = 0; i < nqt; ++i) {
-            if (j > 0 && !wait(&s_free[i], (j - 1) & 1, misc, ST_TIMEOUT_SOFTMAX)) { ok = false; break; }
+            if (cs[i] > 0 && !warp_wait(&s_free[i], (cs[i] - 1) & 1, tries)) { ok = false; break; }
+            ++cs[i];
             tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int p = 0; p < L::PANELS; ++p)
+              for (int p = 0; p < L::PANELS; ++p)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                mma_f16_ss(tmem + COL_S + i * KT,
-                           sdesc_sw128(sbase + L::Q + (i * L::PANELS + p) * L::Q_PANEL + k * 32),
-                           sdesc_sw128(sbase + L::K + st * OP_BYTES + p * KT * 128 + k * 32), idesc,
-                           (p | k) ? 1u : 0u);
-            tc_commit(&s_full[i]);
+                for (int k = 0; k < 4; ++k)
+                  mma_f16_ss(tmem + COL_S + i * KT,
+                             sdesc_sw128(sbase + L::Q + (i * L::PANELS + p) * L::Q_PANEL + k * 32),
+                             sdesc_sw128(sbase + L::K + st * OP_BYTES + p * KT * 128 + k * 32), idesc,
+                             (p | k) ? 1u : 0u);
+              tc_commit(&s_full[i]);
+              mbar_arrive(&s_full[i]);
+              if (i == nqt - 1) {
+                tc_commit(&k_empty[st]);
+                if (j == nt - 1) tc_commit(q_empty);
+              }
+            }
+            __syncwarp();
           }
           if (!ok) break;
-          tc_commit(&k_empty[st]);
-        }
-        if (!ok) {
-          tc_commit(drain);
-          mbar_wait_drain(drain, 0, 200000000ull);
         }
       }
-    } else if (warp == 3 && nt > 0) {
+      if (!ok && elect_one()) {
+        report_status(a.ctl, ST_TIMEOUT_FULL);
+        tc_commit(drain);
+        mbar_wait_drain(drain, 0, 200000000ull);
+      }
+      __syncwarp();
+    } else if (warp == 3) {
       // ---------------------------------------------------------- O += P V
-      if (lane == 0) {
-        constexpr uint32_t idesc = idesc_f16(128, D, false, true);
-        bool ok = true;
-        for (int j = 0; ok && j < nt; ++j) {
-          const int st = j % KV;
+      constexpr uint32_t idesc = idesc_f16(128, D, false, true);
+      uint32_t cp[2] = {0, 0};                             // PV_i products issued so far
+      int jg = 0;
+      bool ok = true;
+      for (int seg = 0; ok; ++seg) {
+        const int ss = seg % SEGS;
+        if (!warp_wait(&seg_full[ss], (seg / SEGS) & 1, tries)) { ok = false; break; }
+        const int nt = segs[ss].nt, nqt = segs[ss].nqt;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&seg_empty[ss]);
+        if (nt < 0) break;
+        for (int j = 0; j < nt; ++j, ++jg) {
+          const int st = jg % KV;
+          if (!warp_wait(&v_full[st], (jg / KV) & 1, tries)) { ok = false; break; }
           for (int i = 0; i < nqt; ++i) {
-            if (!wait(&p_full[i], j & 1, misc, ST_TIMEOUT_SOFTMAX)) { ok = false; break; }
-            if (i == 0 && !wait(&v_full[st], (j / KV) & 1, misc, ST_TIMEOUT_DEQ)) { ok = false; break; }
+            if (!warp_wait(&p_full[i], cp[i] & 1, tries)) { ok = false; break; }
+            ++cp[i];
             tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < KT / 16; ++k)
-              mma_f16_ts(tmem + COL_O + i * D, tmem + COL_P + i * (KT / 2) + k * 8,
-                         sdesc_panels(sbase + L::V + st * OP_BYTES + k * 2048, KT * 128), idesc,
-                         (j > 0 || k > 0) ? 1u : 0u);
-            tc_commit(&o_done[i]);
+              for (int k = 0; k < KT / 16; ++k)
+                mma_f16_ts(tmem + COL_O + i * D, tmem + COL_P + i * (KT / 2) + k * 8,
+                           sdesc_panels(sbase + L::V + st * OP_BYTES + k * 2048, KT * 128), idesc,
+                           (j > 0 || k > 0) ? 1u : 0u);
+              tc_commit(&o_done[i]);
+              if (i == nqt - 1) tc_commit(&v_empty[st]);
+            }
+            __syncwarp();
           }
           if (!ok) break;
-          tc_commit(&v_empty[st]);
-        }
-        if (!ok) {
-          tc_commit(drain2);
-          mbar_wait_drain(drain2, 0, 200000000ull);
         }
       }
+      if (!ok && elect_one()) {
+        report_status(a.ctl, ST_TIMEOUT_SOFTMAX);
+        tc_commit(drain2);
+        mbar_wait_drain(drain2, 0, 200000000ull);
+      }
+      __syncwarp();
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------ codes -> fp16 / bf16
-    regs_dec<80>();
+    regs_dec<64>();
     const int th = threadIdx.x - 128;                      // 0..127
     constexpr int PARTS = D / 16;                          // 16-code pieces of a row
     constexpr int IT = KT * PARTS / 128;                   // pieces per thread
     const int part = th % PARTS, row0 = th / PARTS, panel = part / 4;
-    bool ok = nt > 0;
-    for (int j = 0; ok && j < nt; ++j) {
-      const int rs = j % RAW, st = j % KV;
-      if (!__all_sync(~0u, wait(&raw_full[rs], (j / RAW) & 1, misc, ST_TIMEOUT_FULL))) { ok = false; break; }
+    bool ok = true;
+    int jg = 0;
+    for (int seg = 0; ok; ++seg) {
+      const int ss = seg % SEGS;
+      if (!warp_wait(&seg_full[ss], (seg / SEGS) & 1, tries)) { ok = false; break; }
+      const int nt = segs[ss].nt;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[ss]);
+      if (nt < 0) break;
+      for (int j = 0; ok && j < nt; ++j, ++jg) {
+        const int rs = jg % RAW, st = jg % KV;
+        if (!warp_wait(&raw_full[rs], (jg / RAW) & 1, tries)) { ok = false; break; }
+#pragma unroll(BF16 ? 2 : 1)
+        for (int side = 0; side < 2; ++side) {
+          const uint32_t src = sbase + (side ? L::RV : L::RK) + rs * RAW_BYTES;
+          const uint32_t dst = sbase + (side ? L::V : L::K) + st * OP_BYTES + panel * KT * 128;
+          uint4 w[IT];
 #pragma unroll
-      for (int side = 0; side < 2; ++side) {
-        const uint32_t src = sbase + (side ? L::RV : L::RK) + rs * RAW_BYTES;
-        const uint32_t dst = sbase + (side ? L::V : L::K) + st * OP_BYTES + panel * KT * 128;
-        uint4 w[IT];
+          for (int it = 0; it < IT; ++it)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[it].x), "=r"(w[it].y), "=r"(w[it].z), "=r"(w[it].w)
+                         : "r"(src + (row0 + it * (128 / PARTS)) * D + part * 16)
+                         : "memory");
+          uint64_t* empty = side ? &v_empty[st] : &k_empty[st];
+          if (!warp_wait(empty, ((jg / KV) & 1) ^ 1, tries)) { ok = false; break; }
 #pragma unroll
-        for (int it = 0; it < IT; ++it)
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w[it].x), "=r"(w[it].y), "=r"(w[it].z), "=r"(w[it].w)
-                       : "r"(src + (row0 + it * (128 / PARTS)) * D + part * 16)
-                       : "memory");
-        uint64_t* empty = side ? &v_empty[st] : &k_empty[st];
-        if (!__all_sync(~0u, wait(empty, ((j / KV) & 1) ^ 1, misc, ST_TIMEOUT_DEQ))) { ok = false; break; }
+          for (int it = 0; it < IT; ++it) {
+            const int r = row0 + it * (128 / PARTS);
+            const uint32_t x[4] = {w[it].x, w[it].y, w[it].z, w[it].w};
+            uint32_t y[8];
 #pragma unroll
-        for (int it = 0; it < IT; ++it) {
-          const int r = row0 + it * (128 / PARTS);
-          const uint32_t x[4] = {w[it].x, w[it].y, w[it].z, w[it].w};
-          uint32_t y[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (side || !BF16) {
-              y[2 * e] = codes2<false, false>(x[e]);
-              y[2 * e + 1] = codes2<false, true>(x[e]);
-            } else {
-              y[2 * e] = codes2<true, false>(x[e]);
-              y[2 * e + 1] = codes2<true, true>(x[e]);
+            for (int e = 0; e < 4; ++e) {
+              if (side || !BF16) {
+                y[2 * e] = codes2<false, false>(x[e]);
+                y[2 * e + 1] = codes2<false, true>(x[e]);
+              } else {
+                y[2 * e] = codes2<true, false>(x[e]);
+                y[2 * e + 1] = codes2<true, true>(x[e]);
+              }
             }
+            // 16-byte chunks 2 part and 2 part + 1 of the row, at chunk ^ (row & 7);
+            // lanes of the second panel write them in the other order, which
+            // keeps the banks of a quarter warp apart
+            const uint32_t line = dst + r * 128;
+            const uint32_t c0 = ((2 * (part & 3)) ^ (r & 7)) * 16, c1 = c0 ^ 16;
+            const bool swap = panel != 0;
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + (swap ? c1 : c0)),
+                         "r"(swap ? y[4] : y[0]), "r"(swap ? y[5] : y[1]), "r"(swap ? y[6] : y[2]),
+                         "r"(swap ? y[7] : y[3])
+                         : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + (swap ? c0 : c1)),
+                         "r"(swap ? y[0] : y[4]), "r"(swap ? y[1] : y[5]), "r"(swap ? y[2] : y[6]),
+                         "r"(swap ? y[3] : y[7])
+                         : "memory");
           }
-          // 16-byte chunks 2 part and 2 part + 1 of the row, at chunk ^ (row & 7);
-          // lanes of the second panel write them in the other order, which
-          // keeps the banks of a quarter warp apart
-          const uint32_t line = dst + r * 128;
-          const uint32_t c0 = ((2 * (part & 3)) ^ (r & 7)) * 16, c1 = c0 ^ 16;
-          const bool swap = panel != 0;
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + (swap ? c1 : c0)),
-                       "r"(swap ? y[4] : y[0]), "r"(swap ? y[5] : y[1]), "r"(swap ? y[6] : y[2]),
-                       "r"(swap ? y[7] : y[3])
-                       : "memory");
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + (swap ? c0 : c1)),
-                       "r"(swap ? y[0] : y[4]), "r"(swap ? y[1] : y[5]), "r"(swap ? y[2] : y[6]),
-                       "r"(swap ? y[3] : y[7])
-                       : "memory");
-        }
-        // orders these stores before the MMA's reads, and the loads of the raw
-        // stage before the copy that refills it
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(side ? &v_full[st] : &k_full[st]);
-          if (side) mbar_arrive(&raw_empty[rs]);
+          // orders these stores before the MMA's reads, and the loads of the raw
+          // stage before the copy that refills it
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(side ? &v_full[st] : &k_full[st]);
+            if (side) mbar_arrive(&raw_empty[rs]);
+          }
         }
       }
     }
@@ -428,127 +735,130 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t tO = tmem + lane_base + COL_O + i * D;
     const uint32_t bar_s_full = smem_u32(&s_full[i]);
     const uint32_t bar_s_free = bar_s_full + 16, bar_p_full = bar_s_full + 32, bar_o_done = bar_s_full + 48;
-    const uint32_t consts = sbase + L::CONST;
-    const int tok = tok0 + i * tpt + r / a.group;          // within the request
-    const bool row_ok = live && r < tpt * a.group && tok < ql;
-    // rows past the end compute on whatever their tile holds and are not stored
-    const int lim = row_ok ? key_limit(tok, ql, n, a.chunk) : n;
-    float m_used = -INFINITY, l = 0.f;
-    bool ok = live;
-    const int ntr = (live && i < nqt) ? nt : 0;
-    for (int j = 0; j < ntr; ++j) {
-      if (!softmax_wait(bar_s_full, j & 1, misc)) { ok = false; break; }
-      if (!softmax_wait(smem_u32(&c_full[j % CRING]), (j / CRING) & 1, misc)) { ok = false; break; }
-      tc_fence_after();
-      uint32_t s[KT];
-#pragma unroll
-      for (int c = 0; c < CH; ++c) tmem_ld32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
-      tmem_ld_wait();
-      reg_fence<0, KT>(s);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive(bar_s_free);
-      const uint32_t cb = consts + (j % CRING) * (CH * 16);
-      const int valid = lim - (t0 + j) * KT;               // keys of the tile that the row sees (may be <= 0)
-      const bool full = __all_sync(~0u, valid >= KT);
-      float mx = m_used;
-#define QV_MAX(C)                                                                                            \
-  if (C < CH) {                                                                                              \
-    const float4 k = lds_f4(cb + 16 * C);                                                                    \
-    const float v = full ? chunk_max<false, 32 * (C % CH)>(s, valid) : chunk_max<true, 32 * (C % CH)>(s, valid); \
-    mx = fmaxf(mx, fmaf(v, k.x, k.y));                                                                       \
-  }
-      QV_MAX(0) QV_MAX(1) QV_MAX(2) QV_MAX(3)
-#undef QV_MAX
-      const bool need = mx > m_used + 8.0f;
-      float alpha = 1.f;
-      bool rescale = false;
-      if (__any_sync(~0u, need)) {
-        const float m_target = need ? mx : m_used;
-        alpha = m_target == m_used ? 1.f : ex2(m_used - m_target);
-        rescale = j > 0;
-        m_used = m_target;
+    const float4* consts = reinterpret_cast<const float4*>(smem + L::CONST);
+    bool ok = true;
+    uint32_t cnt = 0;                                      // tiles of this warpgroup so far
+    int jg = 0;                                            // tiles of the CTA so far
+    for (int seg = 0; ok; ++seg) {
+      const int ss = seg % SEGS;
+      if (!warp_wait(&seg_full[ss], (seg / SEGS) & 1, tries)) break;
+      const int nt = segs[ss].nt;
+      if (nt < 0) break;
+      const int ntr = i < segs[ss].nqt ? nt : 0;
+      // keys the row sees, from the segment's first tile on; rows past the end
+      // compute on whatever their tile holds and are not stored
+      int left;
+      {
+        const int ql = segs[ss].ql, tok = segs[ss].tok0 + i * tpt + r / a.group;
+        left = (r < tpt * a.group && tok < ql ? key_limit(tok, ql, segs[ss].n, a.chunk) : segs[ss].n) -
+               segs[ss].t0 * KT;
       }
-      const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
-      float lj = 0.f;
-      bool stored = true;
-      // P_i may be written once PV_i(j-1) has read the one before
-#define QV_EXP(C)                                                                                \
-  if (C < CH) {                                                                                  \
-    const float4 k = lds_f4(cb + 16 * C);                                                        \
-    if (full) exp_chunk<false, 1, 16 * (C % CH)>(s, k, neg_m, lj, valid);                        \
-    else exp_chunk<true, 1, 16 * (C % CH)>(s, k, neg_m, lj, valid);                              \
-    if (C == 0 && j > 0) {                                                                       \
-      stored = softmax_wait(bar_o_done, (j - 1) & 1, misc);                                      \
-      tc_fence_after();                                                                          \
-    }                                                                                            \
-    if (stored) tmem_st16(tP + 16 * C, *reinterpret_cast<const uint32_t(*)[16]>(&s[16 * (C % CH)])); \
-  }
-      QV_EXP(0) QV_EXP(1) QV_EXP(2) QV_EXP(3)
-#undef QV_EXP
-      if (!stored) { ok = false; break; }
-      tmem_st_wait();
-      l = l * alpha + lj;
-      if (rescale) {
+      float m_used = -INFINITY, l = 0.f;
+      bool ready = false;
+      for (int j = 0; j < ntr; ++j, ++cnt) {
+        if (!__all_sync(~0u, ready) && !warp_wait(bar_s_full, cnt & 1, tries)) { ok = false; break; }
+        const int cj = (jg + j) % CRING;
+        tc_fence_after();
+        uint32_t s[KT];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) tmem_ld32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+        tmem_ld_wait();
+        reg_fence<0, KT>(s);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(bar_s_free);
+        Chunk k[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const float4* at = &consts[cj * CH + c];
+          k[c] = {at->x, at->y, at->z};
+        }
+        const int valid = left - j * KT;                   // keys of the tile that the row sees (may be <= 0)
+        if (__any_sync(~0u, valid < KT)) hide_keys(s, k, valid);
+        const float mx = tile_max(s, k, m_used);
+        const bool need = mx > m_used + 8.0f;
+        float alpha = 1.f;
+        bool rescale = false;
+        if (__any_sync(~0u, need)) {
+          const float m_target = need ? mx : m_used;
+          alpha = m_target == m_used ? 1.f : ex2(m_used - m_target);
+          rescale = j > 0;
+          m_used = m_target;
+        }
+        const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+        float lj = 0.f;
+        // (the previous item's epilogue has waited for its last PV product)
+        if (!exp_store<1>(s, k, neg_m, lj, tP, j == 0, bar_o_done, (cnt - 1) & 1, tries)) { ok = false; break; }
+        ready = j + 1 < ntr && test(bar_s_full, (cnt + 1) & 1);
+        l = l * alpha + lj;
+        if (rescale) {
+#pragma unroll 1
+          for (int cc = 0; cc < D / 16; ++cc) {
+            uint32_t v[16];
+            tmem_ld16(tO + cc * 16, v);
+            tmem_ld_wait();
+            reg_fence<0, 16>(v);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+            tmem_st16(tO + cc * 16, v);
+          }
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(bar_p_full);
+      }
+      jg += nt;
+      // ---------------------------------------------------------- epilogue
+      if (ok && ntr > 0) {
+        ok = warp_wait(bar_o_done, (cnt - 1) & 1, tries);
+        tc_fence_after();
+      }
+      if (ok) {                                            // warp-uniform
+        const int tok = segs[ss].tok0 + i * tpt + r / a.group, slot = segs[ss].slot;
+        const bool row_ok = r < tpt * a.group && tok < segs[ss].ql;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float lse2 = l == 0.f ? -INFINITY : m_used + log2f(l);
+        const long long gtok = segs[ss].q0 + tok;
+        const int h = segs[ss].kvh * a.group + r % a.group;
+        const long long part = (long long)slot * Q_ROWS + i * 128 + r;
 #pragma unroll 1
         for (int cc = 0; cc < D / 16; ++cc) {
           uint32_t v[16];
-          tmem_ld16(tO + cc * 16, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
-          tmem_st16(tO + cc * 16, v);
-        }
-        tmem_st_wait();
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive(bar_p_full);
-    }
-    // ------------------------------------------------------------ epilogue
-    if (ok && ntr > 0) {
-      ok = softmax_wait(bar_o_done, (ntr - 1) & 1, misc);
-      tc_fence_after();
-    }
-    if (ok) {                                              // warp-uniform
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const float lse2 = l == 0.f ? -INFINITY : m_used + log2f(l);
-      const long long gtok = q0 + tok;
-      const int h = kvh * a.group + r % a.group;
-      const long long part = (long long)sp * a.Tq * a.hq + gtok * a.hq + h;
-#pragma unroll 1
-      for (int cc = 0; cc < D / 16; ++cc) {
-        uint32_t v[16];
-        if (ntr > 0) {
-          tmem_ld16(tO + cc * 16, v);
-          tmem_ld_wait();
-          reg_fence<0, 16>(v);
-        }
-        if (!row_ok) continue;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(v[e]) * inv);
-        if (a.splits > 1) {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + part * D + cc * 16);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            dst[e] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
-                                 __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
-        } else {
-          uint32_t o[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x = __uint_as_float(v[2 * e]), y = __uint_as_float(v[2 * e + 1]);
-            o[e] = BF16 ? pack_bf162(x, y) : pack_half2(x, y);
+          if (ntr > 0) {
+            tmem_ld16(tO + cc * 16, v);
+            tmem_ld_wait();
+            reg_fence<0, 16>(v);
           }
-          uint4* dst = reinterpret_cast<uint4*>(a.out + gtok * a.o_tok + h * a.o_head + cc * 16);
-          dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-          dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+          if (!row_ok) continue;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(v[e]) * inv);
+          if (slot >= 0) {
+            float4* dst = reinterpret_cast<float4*>(a.part_o + part * D + cc * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              dst[e] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
+                                   __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
+          } else {
+            uint32_t o[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float x = __uint_as_float(v[2 * e]), y = __uint_as_float(v[2 * e + 1]);
+              o[e] = BF16 ? pack_bf162(x, y) : pack_half2(x, y);
+            }
+            uint4* dst = reinterpret_cast<uint4*>(a.out + gtok * a.o_tok + h * a.o_head + cc * 16);
+            dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        }
+        if (row_ok) {
+          if (slot >= 0) a.part_lse[part] = lse2;
+          else if (a.lse) a.lse[h * a.Tq + gtok] = lse2 * 0.6931471805599453f;
         }
       }
-      if (row_ok) {
-        if (a.splits > 1) a.part_lse[part] = lse2;
-        else if (a.lse) a.lse[h * a.Tq + gtok] = lse2 * 0.6931471805599453f;
-      }
+      tc_fence_before();                                   // O_i read before the next item's products
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[ss]);
     }
   }
 
@@ -560,17 +870,80 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
+// Adds the parts of the items that a cut went through.  CTA (x, y) looks at
+// the cut before piece x + 1; the item's first cut does the work, 16 rows a
+// CTA, half a warp's registers a row.
+template <bool BF16, int D>
+__global__ void __launch_bounds__(256) attn_cache_tiles_join_kernel(CacheAttnArgs a, int grid) {
+  pdl_wait();
+  pdl_trigger();
+  const int x = blockIdx.x + 1;
+  const Cut cut = reinterpret_cast<const Cut*>(a.part_lse + 2LL * grid * Q_ROWS)[x];
+  if (cut.first != x - 1) return;
+  const int lane = threadIdx.x % 32;
+  constexpr int E = D / 32;
+#pragma unroll 1
+  for (int rr = 0; rr < 2; ++rr) {
+    const int row = blockIdx.y * 16 + (threadIdx.x / 32) * 2 + rr, r = row & 127;
+    const int tpt = 128 / a.group, tok = cut.tok0 + (row >> 7) * tpt + r / a.group;
+    if (r >= tpt * a.group || tok >= cut.ql) continue;
+    auto at = [&](int k) { return (long long)(2 * k + (k == cut.first)) * Q_ROWS + row; };
+    float mx = -INFINITY;
+    for (int k = cut.first + lane; k <= cut.last; k += 32) mx = fmaxf(mx, a.part_lse[at(k)]);
+    mx = warp_max(mx);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float l = 0.f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int k = cut.first; k <= cut.last; ++k) {
+      const float w = ex2(a.part_lse[at(k)] - base);
+      if (w == 0.f) continue;
+      l += w;
+      const float* p = a.part_o + at(k) * D + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += w * p[e];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const long long gtok = cut.q0 + tok;
+    const int h = cut.kvh * a.group + r % a.group;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + gtok * a.o_tok + h * a.o_head + lane * E);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e)
+      dst[e] = BF16 ? pack_bf162(acc[2 * e] * inv, acc[2 * e + 1] * inv)
+                    : pack_half2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    if (lane == 0 && a.lse) a.lse[h * a.Tq + gtok] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
+  }
+}
+
 }  // namespace
 
 bool tiles_can_read(const CacheAttnArgs& a) {
   return a.group <= 128 && (a.hq == 1 || a.q_head > 0) && (a.Tq == 1 || a.q_tok > 0);
 }
 
-int launch_tiles(const CacheAttnArgs& a, int D, bool bf16, cudaStream_t stream) {
+// Whether items may be cut (a rule on the hint alone: the join is launched by it).
+static bool tiles_split(long long max_kv, int D) { return max_kv > 8 * (D == 64 ? 128 : 64); }
+
+// One CTA per SM at most, and no more than there can be pieces.
+static int tiles_grid(long long items, long long max_kv, int D) {
+  const int kt = D == 64 ? 128 : 64;
+  const long long cost = items * (COST_START + (max_kv + kt - 1) / kt * COST_TILE2);
+  const long long pieces = tiles_split(max_kv, D) ? (cost + COST_MIN - 1) / COST_MIN : items;
+  return (int)std::max<long long>(1, std::min<long long>(pieces, device_info().num_sms));
+}
+
+int64_t tiles_scratch(long long items, long long max_kv, int D) {
+  if (!tiles_split(max_kv, D)) return 0;
+  const int64_t grid = tiles_grid(items, max_kv, D);
+  return grid > 1 ? grid * (2 * Q_ROWS * (D + 1) * (int64_t)sizeof(float) + (int64_t)sizeof(Cut)) : 0;
+}
+
+int launch_tiles(CacheAttnArgs& a, int D, bool bf16, long long max_kv, void* scratch, cudaStream_t stream) {
   const int smem = D == 64 ? Lay<64>::TOTAL : Lay<128>::TOTAL;
   if (smem > device_info().max_smem_optin)
     return set_error(QVGGT_ERR_UNSUPPORTED, "cached_attention: shared memory %d > %d", smem,
                      device_info().max_smem_optin);
+  if ((long long)a.B * a.row_blocks > 1 << 30) return set_error(QVGGT_ERR_UNSUPPORTED, "cached_attention: too many rows");
   CUtensorMap tmQ;
   const uint64_t dims[3] = {(uint64_t)D, (uint64_t)a.hq, (uint64_t)a.Tq};
   const uint64_t strides[2] = {(uint64_t)(a.hq == 1 ? D : a.q_head) * 2,
@@ -579,16 +952,34 @@ int launch_tiles(const CacheAttnArgs& a, int D, bool bf16, cudaStream_t stream) 
   if (int rc = encode_tmap(&tmQ, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, a.q,
                            dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
+  const long long items = (long long)a.B * a.row_blocks * a.hk;
+  const int grid = tiles_grid(items, max_kv, D);
+  // a try_wait that fails takes about 1.4 us
+  a.wait_tries = (uint32_t)std::min<unsigned long long>(1u << 26, a.ctl.timeout_ns / 1024 + 1);
+  a.can_split = grid > 1 && tiles_split(max_kv, D);
+  a.part_o = static_cast<float*>(scratch);
+  a.part_lse = a.can_split ? a.part_o + 2LL * grid * Q_ROWS * D : nullptr;
   using Kfn = void (*)(CUtensorMap, CacheAttnArgs);
   static const Kfn fns[2][2] = {{attn_cache_tiles_kernel<false, 64>, attn_cache_tiles_kernel<false, 128>},
                                 {attn_cache_tiles_kernel<true, 64>, attn_cache_tiles_kernel<true, 128>}};
+  using Jfn = void (*)(CacheAttnArgs, int);
+  static const Jfn joins[2][2] = {{attn_cache_tiles_join_kernel<false, 64>, attn_cache_tiles_join_kernel<false, 128>},
+                                  {attn_cache_tiles_join_kernel<true, 64>, attn_cache_tiles_join_kernel<true, 128>}};
   static DeviceFlags attr[2][2];
   const Kfn fn = fns[bf16][D == 128];
   if (int rc = ensure_smem(attr[bf16][D == 128], fn, smem, "cudaFuncSetAttribute(cached_attention)")) return rc;
-  const long long grid = (long long)a.row_blocks * a.B * a.hk * a.splits;
-  if (grid > 2147483647LL) return set_error(QVGGT_ERR_UNSUPPORTED, "cached_attention: grid too large");
-  return check_cuda(launch_pdl(fn, dim3((unsigned)grid), dim3(THREADS), smem, stream, 1u, tmQ, a),
-                    "cached_attention launch");
+  if (int rc = check_cuda(launch_pdl(fn, dim3((unsigned)grid), dim3(THREADS), smem, stream, 1u, tmQ, a),
+                          "cached_attention launch"))
+    return rc;
+  count_launch(1);
+  if (a.can_split) {
+    if (int rc = check_cuda(launch_pdl(joins[bf16][D == 128], dim3((unsigned)(grid - 1), Q_ROWS / 16), dim3(256), 0,
+                                       stream, 1u, a, grid),
+                            "cached_attention join launch"))
+      return rc;
+    count_launch(1);
+  }
+  return QVGGT_OK;
 }
 
 }  // namespace qv
