@@ -23,11 +23,11 @@ struct CacheAttnArgs {
   const int32_t *table, *cu_q, *kv_lens;
   float *part_o, *part_lse;              // parts of rows, and their log2-sum-exp
   long long q_tok, q_head, o_tok, o_head, block_stride, Tq;
-  int B, hq, hk, group, wide, num_blocks, bs_log2, chunk, max_q, splits;
+  int B, hq, hk, group, wide, num_blocks, bs_log2, chunk, max_q;
   int row_blocks;                        // Q blocks (16-row tiles) of the longest request
-  int can_split;                         // tile kernel: items may be cut, a join follows
+  int can_split;                         // items may be cut, a join follows
   float scale_log2;
-  uint32_t wait_tries;                   // tile kernel: bound of every wait
+  uint32_t wait_tries;                   // bound of every wait
   Ctl ctl;
 };
 
@@ -62,6 +62,231 @@ __device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
 template <bool BF16, bool HI>
 __device__ __forceinline__ uint32_t codes2(uint32_t w) {
   return BF16 ? codes_bf16<HI>(w) : codes_f16<HI>(w ^ 0x80808080u);
+}
+
+__device__ __forceinline__ bool lengths_ok(const CacheAttnArgs& a, int q0, int ql, int n) {
+  if (q0 >= 0 && ql >= 0 && ql <= a.max_q && (long long)q0 + ql <= a.Tq && n >= 0 && n <= (a.wide << a.bs_log2)) return true;
+  report_status(a.ctl, ST_BAD_LENGTH);
+  return false;
+}
+
+// cp.async.bulk of contiguous bytes, completion on an mbarrier of this CTA.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// Bounded wait for the phase with parity `parity`: up to `tries` try_waits,
+// each of which the hardware suspends for about 1.4 us if nothing arrives.
+// Nothing but the loop, as it is inlined at every hand-off: the roles of an SM
+// run from one instruction cache, and its misses cost this kernel 12 % when
+// each wait carried its own time-out code.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, uint32_t tries) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+      "mov.u32 n, %3;\n\t"
+      "QV_TRY:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra QV_DONE;\n\t"
+      "sub.u32 n, n, 1;\n\t"
+      "setp.ne.u32 q, n, 0;\n\t"
+      "@q bra QV_TRY;\n\t"
+      "QV_DONE:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(tries)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait(const uint64_t* bar, uint32_t parity, uint32_t tries) {
+  return wait(smem_u32(bar), parity, tries);
+}
+// Whether the phase is complete, without waiting.
+__device__ __forceinline__ bool test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// A wait of a whole warp that then stays converged.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint32_t tries) {
+  return __all_sync(0xffffffffu, wait(bar, parity, tries));
+}
+__device__ __forceinline__ bool warp_wait(const uint64_t* bar, uint32_t parity, uint32_t tries) {
+  return warp_wait(smem_u32(bar), parity, tries);
+}
+
+// ------------------------------------------------------------------ pieces
+// What a CTA does with one item (request, block of rows, kv head): key tiles
+// [t0, t0 + nt).
+struct __align__(16) Segment {
+  int b, kvh, tok0, q0;                  // tok0: first token (tile kernel) or row (row kernel) of the block
+  int ql, n, nqt, t0;
+  int nt;                                // -1: no more segments
+  int slot;                              // where the part is parked; -1: the item is whole
+  int pad[2];
+};
+
+// Where a cut lies, for the join: written by the CTA after it.
+struct __align__(16) Cut {
+  int first, last;                       // CTAs that hold parts of the item (first < 0: the cut is between items)
+  int kvh, tok0, q0, ql, pad[2];
+};
+
+// Running sums of the blocks' costs in shared memory, cum[0 .. THREADS]: entry
+// x starts at block x * g.  All THREADS threads call it; ends with a barrier.
+template <int THREADS, class Blk>
+__device__ __forceinline__ void scan_blocks(const CacheAttnArgs& a, long long* cum, int blocks, int g) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  long long sum = 0;
+  for (int p = threadIdx.x * g; p < min(blocks, ((int)threadIdx.x + 1) * g); ++p)
+    sum += Blk(a, p / a.row_blocks, p % a.row_blocks).cost;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long o = __shfl_up_sync(~0u, sum, d);
+    if (lane >= d) sum += o;
+  }
+  cum[threadIdx.x + 1] = sum;
+  __syncthreads();
+  if (warp == 0) {
+    // sums of the warps before, added to every warp's
+    long long s = lane < THREADS / 32 ? cum[lane * 32 + 32] : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const long long o = __shfl_up_sync(~0u, s, d);
+      if (lane >= d) s += o;
+    }
+    cum[0] = 0;
+    __syncwarp();
+    for (int w = 1; w < THREADS / 32; ++w) {
+      const long long before = __shfl_sync(~0u, s, w - 1);
+      cum[w * 32 + lane + 1] += before;
+    }
+  }
+  __syncthreads();
+}
+
+// The items laid out as one line of cost (block after block, in a block one kv
+// head after another), cut into equal pieces of at least Blk::MIN; CTA x walks
+// piece x.  Tile t of an item belongs to the piece that holds its place on the
+// line, so every CTA finds the others' parts by arithmetic alone.  An item's
+// part that starts at tile 0 is parked in slot 2x + 1, any other in 2x: a CTA
+// has at most one of each.
+template <int THREADS, class Blk>
+struct PieceWalk {
+  long long W, begin, end, s;            // length of a piece, this one's ends, where block p starts
+  int p, h, g;
+  Blk blk;
+  Cut cut;
+
+  __device__ __forceinline__ PieceWalk(const CacheAttnArgs& a, const long long* cum, int blocks, int g_) : g(g_) {
+    const long long total = cum[THREADS] * a.hk;
+    const int grid = gridDim.x;
+    W = (total + grid - 1) / grid;
+    if (a.can_split && W < Blk::MIN) W = Blk::MIN;
+    begin = blockIdx.x * W;
+    end = min(total, begin + W);
+    cut.first = -1;
+    int e = 0;                           // entry that holds `begin`
+    for (int len = THREADS; len > 1;) {
+      const int half = len / 2;
+      if (cum[e + half] * a.hk <= begin) e += half;
+      len -= half;
+    }
+    p = e * g;
+    s = cum[e] * a.hk;
+    h = 0;
+    if (begin < end) load(a, blocks);
+    else p = blocks;
+  }
+
+  __device__ __forceinline__ void load(const CacheAttnArgs& a, int blocks) {
+    for (; p < blocks; ++p) {
+      blk = Blk(a, p / a.row_blocks, p % a.row_blocks);
+      if (blk.cost > 0 && s + blk.cost * a.hk > begin) {
+        h = begin > s ? (int)((begin - s) / blk.cost) : 0;
+        return;
+      }
+      s += blk.cost * a.hk;
+    }
+  }
+
+  // The next segment; false at the end of the piece.
+  __device__ __forceinline__ bool next(const CacheAttnArgs& a, int blocks, Segment& sg) {
+    const int grid = gridDim.x, x = blockIdx.x;
+    while (p < blocks) {
+      if (h == a.hk) {
+        s += blk.cost * a.hk;
+        ++p;
+        load(a, blocks);
+        continue;
+      }
+      const long long s0 = s + h * blk.cost, k0 = s0 + Blk::START;        // the item, its first tile
+      if (s0 >= end) return false;
+      const int head = h++;
+      const int c = blk.tile_cost();
+      int t_lo = 0, t_hi = blk.tiles, slot = -1;
+      if (a.can_split && blk.tiles > 0) {
+        auto at = [&](long long pos) { return pos <= k0 ? 0 : (int)min((long long)blk.tiles, (pos - k0 + c - 1) / c); };
+        t_lo = at(begin);
+        t_hi = x == grid - 1 ? blk.tiles : at(begin + W);
+        if (t_lo >= t_hi) continue;
+        const int first = (int)min(k0 / W, (long long)grid - 1);
+        const int last = (int)min((k0 + (long long)(blk.tiles - 1) * c) / W, (long long)grid - 1);
+        if (first != last) {
+          slot = 2 * x + (t_lo == 0 ? 1 : 0);
+          if (t_lo > 0) cut = Cut{first, last, head, blk.tok0, blk.q0, blk.ql, {0, 0}};
+        }
+      } else if (s0 < begin) {
+        continue;                        // whole items: the CTA that holds the start
+      }
+      sg = Segment{p / a.row_blocks, head, blk.tok0, blk.q0, blk.ql, blk.n, blk.nqt, t_lo, t_hi - t_lo, slot, {0, 0}};
+      return true;
+    }
+    return false;
+  }
+};
+
+// Row `row` of a cut item, joined from its parts (rows_per_slot rows a slot) by
+// one warp: the parts' normalised rows weighted by their sums, in the pieces' order.
+template <bool BF16, int D>
+__device__ __forceinline__ void join_parts(const CacheAttnArgs& a, const Cut& cut, int rows_per_slot, int row, int lane,
+                                           long long tok, int h) {
+  constexpr int E = D / 32;
+  auto at = [&](int k) { return (long long)(2 * k + (k == cut.first)) * rows_per_slot + row; };
+  float mx = -INFINITY;
+  for (int k = cut.first + lane; k <= cut.last; k += 32) mx = fmaxf(mx, a.part_lse[at(k)]);
+  mx = warp_max(mx);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float l = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 2
+  for (int k = cut.first; k <= cut.last; ++k) {
+    const float w = exp2f(a.part_lse[at(k)] - base);
+    const float* p = a.part_o + at(k) * D + lane * E;
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = p[e];
+    l += w;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += w * v[e];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + tok * a.o_tok + h * a.o_head + lane * E);
+#pragma unroll
+  for (int e = 0; e < E / 2; ++e)
+    dst[e] = BF16 ? pack_bf162(acc[2 * e] * inv, acc[2 * e + 1] * inv)
+                  : pack_half2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  if (lane == 0 && a.lse) a.lse[h * a.Tq + tok] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
 }
 
 // attn_cache_sm100.cu (many rows): whether its TMA map can read these queries;

@@ -72,54 +72,6 @@ struct Lay {
   static constexpr int TOTAL = CUM + (THREADS + 1) * 8 + 64 + 1024;
 };
 
-// What a CTA does with one item: key tiles [t0, t0 + nt).
-struct __align__(16) Segment {
-  int b, kvh, tok0, q0;                  // tok0: first token (of the request) of the Q block
-  int ql, n, nqt, t0;
-  int nt;                                // -1: no more segments
-  int slot;                              // where the part is parked; -1: the item is whole
-  int pad[2];
-};
-
-// Where a cut lies, for the join: written by the CTA after it.
-struct __align__(16) Cut {
-  int first, last;                       // CTAs that hold parts of the item (first < 0: the cut is between items)
-  int kvh, tok0, q0, ql, pad[2];
-};
-
-// cp.async.bulk of contiguous bytes, completion on an mbarrier of this CTA.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-
-// Bounded wait for the phase with parity `parity`: up to `tries` try_waits,
-// each of which the hardware suspends for about 1.4 us if nothing arrives.
-// Nothing but the loop, as it is inlined at every hand-off: the roles of an SM
-// run from one instruction cache, and its misses cost this kernel 12 % when
-// each wait carried its own time-out code.
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, uint32_t tries) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
-      "mov.u32 n, %3;\n\t"
-      "QV_TRY:\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "@p bra QV_DONE;\n\t"
-      "sub.u32 n, n, 1;\n\t"
-      "setp.ne.u32 q, n, 0;\n\t"
-      "@q bra QV_TRY;\n\t"
-      "QV_DONE:\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity), "r"(tries)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool wait(const uint64_t* bar, uint32_t parity, uint32_t tries) {
-  return wait(smem_u32(bar), parity, tries);
-}
 // One lane of a converged warp, the same one every time.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -129,27 +81,6 @@ __device__ __forceinline__ bool elect_one() {
       "selp.u32 %0, 1, 0, p;\n\t}\n"
       : "=r"(p));
   return p != 0;
-}
-
-// Whether the phase is complete, without waiting.
-__device__ __forceinline__ bool test(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// A wait of a whole warp that then stays converged.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, uint32_t tries) {
-  return __all_sync(0xffffffffu, wait(bar, parity, tries));
-}
-__device__ __forceinline__ bool warp_wait(const uint64_t* bar, uint32_t parity, uint32_t tries) {
-  return warp_wait(smem_u32(bar), parity, tries);
 }
 
 // K-major or MN-major operand with 128-byte swizzle; lead: bytes between the
@@ -250,8 +181,11 @@ __device__ __forceinline__ bool exp_store(uint32_t (&s)[KT], const Chunk (&k)[KT
 // Q block `qb` of request b: its rows and keys.
 template <int KT>
 struct Block {
+  static constexpr int START = COST_START, MIN = COST_MIN;
   int q0, ql, n, tok0, nqt, tiles;
   long long cost;                        // of one kv head; 0: no such block
+  __device__ __forceinline__ int tile_cost() const { return nqt == 2 ? COST_TILE2 : COST_TILE1; }
+  __device__ __forceinline__ Block() {}
   __device__ __forceinline__ Block(const CacheAttnArgs& a, int b, int qb) {
     q0 = a.cu_q[b];
     ql = a.cu_q[b + 1] - q0;
@@ -262,12 +196,9 @@ struct Block {
     tiles = 0;
     cost = 0;
     if (tok0 >= ql) return;
-    if (q0 < 0 || ql > a.max_q || (long long)q0 + ql > a.Tq || n < 0 || n > (a.wide << a.bs_log2)) {
-      report_status(a.ctl, ST_BAD_LENGTH);
-      return;
-    }
+    if (!lengths_ok(a, q0, ql, n)) return;
     tiles = (key_limit(min(ql, tok0 + 2 * tpt) - 1, ql, n, a.chunk) + KT - 1) / KT;
-    cost = COST_START + (long long)tiles * (nqt == 2 ? COST_TILE2 : COST_TILE1);
+    cost = COST_START + (long long)tiles * tile_cost();
   }
 };
 
@@ -337,38 +268,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == 0 && lane == 0) tma_prefetch_desc(&tmQ);
   pdl_wait();
   pdl_trigger();
-  // Running sums of the blocks' costs: thread x has blocks [x g, (x + 1) g).
   const int blocks = a.B * a.row_blocks, g = (blocks + THREADS - 1) / THREADS;
-  {
-    long long sum = 0;
-    for (int p = threadIdx.x * g; p < min(blocks, ((int)threadIdx.x + 1) * g); ++p)
-      sum += Block<KT>(a, p / a.row_blocks, p % a.row_blocks).cost;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const long long o = __shfl_up_sync(~0u, sum, d);
-      if (lane >= d) sum += o;
-    }
-    cum[threadIdx.x + 1] = sum;
-  }
   tc_fence_before();
-  __syncthreads();
+  scan_blocks<THREADS, Block<KT>>(a, cum, blocks, g);
   tc_fence_after();
-  if (warp == 0) {
-    // sums of the warps before, added to every warp's
-    long long s = lane < THREADS / 32 ? cum[lane * 32 + 32] : 0;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const long long o = __shfl_up_sync(~0u, s, d);
-      if (lane >= d) s += o;
-    }
-    cum[0] = 0;
-    __syncwarp();
-    for (int w = 1; w < THREADS / 32; ++w) {
-      const long long before = __shfl_sync(~0u, s, w - 1);
-      cum[w * 32 + lane + 1] += before;
-    }
-  }
-  __syncthreads();
   const uint32_t tmem = *tmem_slot;
   const int tpt = 128 / a.group;                           // tokens of a Q tile
 
@@ -379,81 +282,26 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == 2) {
       // ---------------------------------------------------------- segments
       if (lane == 0) {
-        const long long total = cum[THREADS] * a.hk;
-        const int grid = gridDim.x, x = blockIdx.x;
-        long long W = (total + grid - 1) / grid;
-        if (a.can_split && W < COST_MIN) W = COST_MIN;
-        const long long begin = x * W, end = min(total, begin + W);
-        int seg = 0;
-        bool ok = true;
-        Cut cut{-1, -1, 0, 0, 0, 0, {0, 0}};
-        if (begin < end) {
-          // block and head that contain `begin`
-          int e = 0;
-          for (int len = THREADS; len > 1;) {
-            const int half = len / 2;
-            if (cum[e + half] * a.hk <= begin) e += half;
-            len -= half;
-          }
-          int p = e * g;
-          long long s = cum[e] * a.hk;                     // where block p starts
-          while (p < blocks) {
-            const Block<KT> blk(a, p / a.row_blocks, p % a.row_blocks);
-            const int c = blk.nqt == 2 ? COST_TILE2 : COST_TILE1;
-            if (blk.cost > 0 && s + blk.cost * a.hk > begin) {
-              if (s >= end) break;
-              int h = begin > s ? (int)((begin - s) / blk.cost) : 0;
-              for (; h < a.hk; ++h) {
-                const long long s0 = s + h * blk.cost, k0 = s0 + COST_START;   // the item, its first tile
-                if (s0 >= end) break;
-                Segment sg{};
-                sg.slot = -1;
-                int t_lo = 0, t_hi = blk.tiles;
-                if (a.can_split && blk.tiles > 0) {
-                  // tile t belongs to the CTA whose piece holds k0 + t c
-                  auto at = [&](long long pos) {
-                    return pos <= k0 ? 0 : (int)min((long long)blk.tiles, (pos - k0 + c - 1) / c);
-                  };
-                  t_lo = at(begin);
-                  t_hi = x == grid - 1 ? blk.tiles : at(begin + W);
-                  const int first = (int)min(k0 / W, (long long)grid - 1);
-                  const int last = (int)min((k0 + (long long)(blk.tiles - 1) * c) / W, (long long)grid - 1);
-                  if (t_lo >= t_hi) continue;
-                  if (first != last) {
-                    sg.slot = 2 * x + (t_lo == 0 ? 1 : 0);
-                    if (t_lo > 0)
-                      cut = Cut{first, last, h, blk.tok0, blk.q0, blk.ql, {0, 0}};
-                  }
-                } else if (s0 < begin) {
-                  continue;                                // whole items: the CTA that holds the start
-                }
-                const int st = seg % SEGS;
-                if (!wait(&seg_empty[st], ((seg / SEGS) & 1) ^ 1, tries)) { ok = false; break; }
-                segs[st].b = p / a.row_blocks;
-                segs[st].kvh = h;
-                segs[st].tok0 = blk.tok0;
-                segs[st].q0 = blk.q0;
-                segs[st].ql = blk.ql;
-                segs[st].n = blk.n;
-                segs[st].nqt = blk.nqt;
-                segs[st].t0 = t_lo;
-                segs[st].nt = t_hi - t_lo;
-                segs[st].slot = sg.slot;
-                mbar_arrive(&seg_full[st]);
-                ++seg;
-              }
-              if (!ok) break;
-            }
-            s += blk.cost * a.hk;
-            ++p;
-          }
-        }
-        if (a.can_split) reinterpret_cast<Cut*>(a.part_lse + 2LL * grid * Q_ROWS)[x] = cut;
-        const int st = seg % SEGS;
-        if (ok && wait(&seg_empty[st], ((seg / SEGS) & 1) ^ 1, tries)) {
-          segs[st].nt = -1;
+        PieceWalk<THREADS, Block<KT>> walk(a, cum, blocks, g);
+        Segment sg;
+        for (int seg = 0;; ++seg) {
+          const bool more = walk.next(a, blocks, sg);
+          const int st = seg % SEGS;
+          if (!wait(&seg_empty[st], ((seg / SEGS) & 1) ^ 1, tries)) break;
+          segs[st].b = sg.b;
+          segs[st].kvh = sg.kvh;
+          segs[st].tok0 = sg.tok0;
+          segs[st].q0 = sg.q0;
+          segs[st].ql = sg.ql;
+          segs[st].n = sg.n;
+          segs[st].nqt = sg.nqt;
+          segs[st].t0 = sg.t0;
+          segs[st].nt = more ? sg.nt : -1;
+          segs[st].slot = sg.slot;
           mbar_arrive(&seg_full[st]);
+          if (!more) break;
         }
+        if (a.can_split) reinterpret_cast<Cut*>(a.part_lse + 2LL * gridDim.x * Q_ROWS)[blockIdx.x] = walk.cut;
       }
     } else if (warp == 0) {
       // ---------------------------------------------------------- producer
@@ -881,37 +729,12 @@ __global__ void __launch_bounds__(256) attn_cache_tiles_join_kernel(CacheAttnArg
   const Cut cut = reinterpret_cast<const Cut*>(a.part_lse + 2LL * grid * Q_ROWS)[x];
   if (cut.first != x - 1) return;
   const int lane = threadIdx.x % 32;
-  constexpr int E = D / 32;
 #pragma unroll 1
   for (int rr = 0; rr < 2; ++rr) {
     const int row = blockIdx.y * 16 + (threadIdx.x / 32) * 2 + rr, r = row & 127;
     const int tpt = 128 / a.group, tok = cut.tok0 + (row >> 7) * tpt + r / a.group;
     if (r >= tpt * a.group || tok >= cut.ql) continue;
-    auto at = [&](int k) { return (long long)(2 * k + (k == cut.first)) * Q_ROWS + row; };
-    float mx = -INFINITY;
-    for (int k = cut.first + lane; k <= cut.last; k += 32) mx = fmaxf(mx, a.part_lse[at(k)]);
-    mx = warp_max(mx);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float l = 0.f, acc[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int k = cut.first; k <= cut.last; ++k) {
-      const float w = ex2(a.part_lse[at(k)] - base);
-      if (w == 0.f) continue;
-      l += w;
-      const float* p = a.part_o + at(k) * D + lane * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += w * p[e];
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const long long gtok = cut.q0 + tok;
-    const int h = cut.kvh * a.group + r % a.group;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + gtok * a.o_tok + h * a.o_head + lane * E);
-#pragma unroll
-    for (int e = 0; e < E / 2; ++e)
-      dst[e] = BF16 ? pack_bf162(acc[2 * e] * inv, acc[2 * e + 1] * inv)
-                    : pack_half2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-    if (lane == 0 && a.lse) a.lse[h * a.Tq + gtok] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
+    join_parts<BF16, D>(a, cut, Q_ROWS, row, lane, cut.q0 + tok, cut.kvh * a.group + r % a.group);
   }
 }
 
@@ -954,8 +777,6 @@ int launch_tiles(CacheAttnArgs& a, int D, bool bf16, long long max_kv, void* scr
     return rc;
   const long long items = (long long)a.B * a.row_blocks * a.hk;
   const int grid = tiles_grid(items, max_kv, D);
-  // a try_wait that fails takes about 1.4 us
-  a.wait_tries = (uint32_t)std::min<unsigned long long>(1u << 26, a.ctl.timeout_ns / 1024 + 1);
   a.can_split = grid > 1 && tiles_split(max_kv, D);
   a.part_o = static_cast<float*>(scratch);
   a.part_lse = a.can_split ? a.part_o + 2LL * grid * Q_ROWS * D : nullptr;
