@@ -9,14 +9,15 @@
 namespace qv {
 namespace {
 
-constexpr int TOK_ROWS = 16;             // (query, head) rows of an item: the M of mma.m16n8k16
 constexpr int UNIT = 32;                 // keys a warp takes at a time: never across two blocks
 
-template <int D>
+// NT: 8-row tiles of an item, a row being a (token, query head of the group) pair.
+template <int D, int NT>
 struct RowLay {
-  static constexpr int WARPS = D == 64 ? 16 : 8;
+  static constexpr int ROWS = 8 * NT;
+  static constexpr int WARPS = D == 64 && NT < 4 ? 16 : 8;
   static constexpr int THREADS = WARPS * 32;
-  static constexpr int STAGES = 3;                         // units in flight per warp
+  static constexpr int STAGES = 192 * 1024 / (WARPS * 2 * UNIT * D);   // units in flight per warp: 3 or 6
   static constexpr int SIDE = UNIT * D;                    // K or V codes of a unit
   static constexpr int RING = 0;                           // [warp][stage][K, V]
   static constexpr int RING_BYTES = WARPS * STAGES * 2 * SIDE;
@@ -24,18 +25,18 @@ struct RowLay {
   static constexpr int CUM = BAR + WARPS * STAGES * 8;     // long long [THREADS + 1]
   static constexpr int SEG = CUM + (THREADS + 2) * 8;      // Segment [2]
   static constexpr int ML = SEG + 2 * (int)sizeof(Segment);   // float [warp][row] maxima, then sums
-  static constexpr int WALK = ML + 2 * WARPS * TOK_ROWS * 4;   // PieceWalk, one thread's
+  static constexpr int WALK = ML + 2 * WARPS * ROWS * 4;   // PieceWalk, one thread's
   static constexpr int TOTAL = WALK + 256;
   // the warps' O, merged at the end of a segment, lie in the drained ring
-  static_assert(WARPS * TOK_ROWS * D * 4 <= RING_BYTES, "O does not fit the ring");
+  static_assert(WARPS * ROWS * D * 4 <= RING_BYTES, "O does not fit the ring");
 };
 
-// 16 rows of a request, their keys in units.
-template <int D>
+// The rows of an item, their keys in units.
+template <int D, int NT>
 struct RowBlock {
   // A segment's start and merge cost about as much as two units on each warp;
   // a piece is not cut below four units for each (a join costs about that).
-  static constexpr int START = 2 * RowLay<D>::WARPS, MIN = START + 4 * RowLay<D>::WARPS;
+  static constexpr int START = 2 * RowLay<D, NT>::WARPS, MIN = START + 4 * RowLay<D, NT>::WARPS;
   int q0, ql, n, tok0, nqt, tiles;       // tok0: first row (token * group + head)
   long long cost;
   __device__ __forceinline__ int tile_cost() const { return 1; }
@@ -44,12 +45,12 @@ struct RowBlock {
     q0 = a.cu_q[b];
     ql = a.cu_q[b + 1] - q0;
     n = a.kv_lens[b];
-    tok0 = qb * TOK_ROWS;
+    tok0 = qb * RowLay<D, NT>::ROWS;
     nqt = 1;
     tiles = 0;
     cost = 0;
     if (tok0 >= (long long)ql * a.group || !lengths_ok(a, q0, ql, n)) return;
-    const int last = (min(ql * a.group, tok0 + TOK_ROWS) - 1) / a.group;
+    const int last = (min(ql * a.group, tok0 + RowLay<D, NT>::ROWS) - 1) / a.group;
     tiles = (key_limit(last, ql, n, a.chunk) + UNIT - 1) / UNIT;
     cost = START + (long long)tiles;
   }
@@ -78,14 +79,27 @@ __device__ __forceinline__ uint2 lds64(uint32_t at) {
   return v;
 }
 
+// 8 x 8 transpose of 16-bit elements across the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 // One CTA per SM walks its piece of the items' line (attn_cache.cuh); the
 // units of a segment go round its warps.  Each warp streams its own units
 // through a ring of bulk copies that only it fills and reads, so nothing but
 // its own mbarriers holds it up: up to 192 KB in flight per SM, well over what
 // the memory's latency needs.  The warps' softmax states merge at the segment's end.
-template <bool BF16, int D>
-__global__ void __launch_bounds__(RowLay<D>::THREADS, 1) attn_cache_rows_kernel(CacheAttnArgs a) {
-  using L = RowLay<D>;
+//
+// The codes are the M operand of mma.m16n8k16 and the rows its N: S^T = K q^T,
+// O^T += V^T P^T.  The instructions that unpack a code are then paid once for
+// all rows (they bound the kernel: with the rows as M, 668 instructions a unit
+// against 340 now, 150 us against XXX at 8 x 16 heads x 43,968 keys), and each
+// of up to 8 rows costs what one does.
+template <bool BF16, int D, int NT>
+__global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 1) attn_cache_rows_kernel(CacheAttnArgs a) {
+  using L = RowLay<D, NT>;
   constexpr int KC = D / 64;              // 64-dim chunks
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
@@ -93,7 +107,7 @@ __global__ void __launch_bounds__(RowLay<D>::THREADS, 1) attn_cache_rows_kernel(
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR) + warp * L::STAGES;
   Segment* segs = reinterpret_cast<Segment*>(smem + L::SEG);
   float* sm_m = reinterpret_cast<float*>(smem + L::ML);
-  float* sm_l = sm_m + L::WARPS * TOK_ROWS;
+  float* sm_l = sm_m + L::WARPS * L::ROWS;
   float* sm_o = reinterpret_cast<float*>(smem + L::RING);
   const uint32_t ring = sbase + L::RING + warp * L::STAGES * 2 * L::SIDE;
   if (lane == 0) {
@@ -105,10 +119,10 @@ __global__ void __launch_bounds__(RowLay<D>::THREADS, 1) attn_cache_rows_kernel(
   pdl_trigger();
   const int blocks = a.B * a.row_blocks, bg = (blocks + L::THREADS - 1) / L::THREADS;
   long long* cum = reinterpret_cast<long long*>(smem + L::CUM);
-  scan_blocks<L::THREADS, RowBlock<D>>(a, cum, blocks, bg);
+  scan_blocks<L::THREADS, RowBlock<D, NT>>(a, cum, blocks, bg);
   // one thread walks (its state in shared memory, not in every thread's
   // registers); it finds the next segment before it starts on this one's units
-  using Walk = PieceWalk<L::THREADS, RowBlock<D>>;
+  using Walk = PieceWalk<L::THREADS, RowBlock<D, NT>>;
   static_assert(sizeof(Walk) <= 256, "no room for the walk");
   Walk* walk = reinterpret_cast<Walk*>(smem + L::WALK);
   auto advance = [&](int slot) {
@@ -139,11 +153,17 @@ __global__ void __launch_bounds__(RowLay<D>::THREADS, 1) attn_cache_rows_kernel(
     auto fetch_id = [&](int i) {
       return i < count ? table[((first + i * L::WARPS) * UNIT) >> a.bs_log2] : -1;
     };
-    auto fetch_scale = [&](const float* sc, int id) {
-      return id >= 0 && id < a.num_blocks ? sc[(long long)id * a.hk + kvh] : 0.f;
+    // the constants of the lane's unit: the score's factor, log2 and inverse of the V scale
+    float ck, lv, inv_vs;
+    auto constants = [&](int id) {
+      const bool good = id >= 0 && id < a.num_blocks;
+      const float vs = good ? a.vs[(long long)id * a.hk + kvh] : 1.f;
+      ck = good ? a.ks[(long long)id * a.hk + kvh] * a.scale_log2 : 1.f;
+      lv = log2f(vs);
+      inv_vs = 1.f / vs;
     };
     int id = fetch_id(lane), id2 = fetch_id(32 + lane);
-    float ks = fetch_scale(a.ks, id), vs = fetch_scale(a.vs, id);
+    constants(id);
     bool bad = false;
     // starts the copies of unit i (a block outside the cache: none)
     auto issue = [&](int i, int block) {
@@ -163,119 +183,148 @@ __global__ void __launch_bounds__(RowLay<D>::THREADS, 1) attn_cache_rows_kernel(
     };
     for (int i = 0; i < L::STAGES && i < count; ++i) issue(i, __shfl_sync(~0u, id, i));
 
-    // rows g and g + 8 of the tile
-    int lim[2];
-    const uint16_t* qp[2];
+    // rows 2t and 2t + 1 of each 8-row tile
+    int lim[NT][2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = min(row0 + g + 8 * r, rows - 1);
-      const int i = row / a.group, h = kvh * a.group + row % a.group;
-      lim[r] = row0 + g + 8 * r < rows ? key_limit(i, ql, n, a.chunk) : 0;
-      qp[r] = a.q + (long long)(sg.q0 + i) * a.q_tok + (long long)h * a.q_head;
-    }
-    // A fragments: step s of chunk c takes dims 64c + 16t + 4s + {0, 1} as k
-    // columns 2t, 2t+1 and {2, 3} as 2t+8, 2t+9 (any order of the dims will do,
-    // as K's fragments use the same)
-    uint32_t qa[KC][4][4];
+    for (int x = 0; x < NT; ++x)
 #pragma unroll
-    for (int c = 0; c < KC; ++c)
+      for (int e = 0; e < 2; ++e) {
+        const int row = row0 + 8 * x + 2 * t + e;
+        lim[x][e] = row < rows ? key_limit(row / a.group, ql, n, a.chunk) : 0;
+      }
+    const int all = key_limit(row0 / a.group, ql, n, a.chunk);   // keys that every row sees
+    // B fragments of q (row g of each tile): step s of chunk c takes dims
+    // 64c + 16t + 4s + {0, 1} as k rows 2t, 2t+1 and {2, 3} as 2t+8, 2t+9 (any
+    // order of the dims will do, as K's fragments use the same)
+    uint32_t qb[NT][KC][4][2];
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+    for (int x = 0; x < NT; ++x) {
+      const int row = min(row0 + 8 * x + g, rows - 1);
+      const uint16_t* qp = a.q + (long long)(sg.q0 + row / a.group) * a.q_tok +
+                           (long long)(kvh * a.group + row % a.group) * a.q_head;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint2 w = *reinterpret_cast<const uint2*>(qp[r] + 64 * c + 16 * t + 4 * s);
-          qa[c][s][r] = w.x;
-          qa[c][s][2 + r] = w.y;
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const uint2 w = *reinterpret_cast<const uint2*>(qp + 64 * c + 16 * t + 4 * s);
+          qb[x][c][s][0] = w.x;
+          qb[x][c][s][1] = w.y;
         }
-    float o[D / 8][4];
+    }
+    float o[NT][D / 16][4];               // O^T: tile 4c + 2w + j, slots (dim, dim + 1) x rows (2t, 2t + 1)
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
+    for (int x = 0; x < NT; ++x)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[x][d][e] = 0.f;
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[x][e] = -INFINITY;
+        l[x][e] = 0.f;
+      }
+    // Slot g of 8 keys is key (g >> 1) + 4 (g & 1): the four t lanes, which
+    // need slots 2t, 2t + 1 of V, then read rows in both halves of the
+    // shared-memory banks.
+    const int kappa = (g >> 1) + 4 * (g & 1);
 
     int i = 0;
     for (; i < count; ++i) {
       if (i && (i & 31) == 0) {
         id = id2;
         id2 = fetch_id(i + 32 + lane);
-        ks = fetch_scale(a.ks, id);
-        vs = fetch_scale(a.vs, id);
+        constants(id);
       }
       const int blk = __shfl_sync(~0u, id, i & 31);
-      const float uks = __shfl_sync(~0u, ks, i & 31), uvs = __shfl_sync(~0u, vs, i & 31);
+      const float uck = __shfl_sync(~0u, ck, i & 31), ulv = __shfl_sync(~0u, lv, i & 31);
+      const float uinv = __shfl_sync(~0u, inv_vs, i & 31);
       const uint32_t u = used + i, st = u % L::STAGES;
       if (!warp_wait(&bars[st], (u / L::STAGES) & 1, a.wait_tries)) { ok = false; break; }
       const int key0 = (first + i * L::WARPS) * UNIT;
       const uint32_t kb = ring + st * 2 * L::SIDE, vb = kb + L::SIDE;
       if (blk >= 0 && blk < a.num_blocks) {
-        const float ck = uks * a.scale_log2, lv = log2f(uvs), inv_vs = 1.f / uvs;
-        // column c of 8-key tile nt is key 8 nt + (c >> 1) + 4 (c & 1): with
-        // this order the four t lanes' V rows below fall into both halves of
-        // the shared-memory banks
-        float s[4][4];
+        float s[NT][2][4];                // S^T: 16 keys x 8 rows; keys kappa, kappa + 8 x rows 2t, 2t + 1
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
+        for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+          for (int x = 0; x < NT; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[x][mt][e] = 0.f;
 #pragma unroll
           for (int c = 0; c < KC; ++c) {
-            const uint4 w = lds128(kb + (nt * 8 + (g >> 1) + 4 * (g & 1)) * D + 64 * c + 16 * t);
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+            const uint4 w0 = lds128(kb + (16 * mt + kappa) * D + 64 * c + 16 * t);
+            const uint4 w1 = lds128(kb + (16 * mt + 8 + kappa) * D + 64 * c + 16 * t);
+            const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-            for (int sp = 0; sp < 4; ++sp)
-              mma16816<BF16>(s[nt], qa[c][sp], codes2<BF16, false>(ww[sp]), codes2<BF16, true>(ww[sp]));
-          }
-        }
-        float mx[2] = {-INFINITY, -INFINITY};
+            for (int sp = 0; sp < 4; ++sp) {
+              const uint32_t ka[4] = {codes2<BF16, false>(x0[sp]), codes2<BF16, false>(x1[sp]),
+                                      codes2<BF16, true>(x0[sp]), codes2<BF16, true>(x1[sp])};
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = key0 + nt * 8 + t + 4 * (e & 1);
-            s[nt][e] = key < lim[e >> 1] ? s[nt][e] * ck + lv : -INFINITY;
-            mx[e >> 1] = fmaxf(mx[e >> 1], s[nt][e]);
-          }
-        float base[2], alpha[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          mx[r] = fmaxf(mx[r], __shfl_xor_sync(~0u, mx[r], 1));
-          mx[r] = fmaxf(mx[r], __shfl_xor_sync(~0u, mx[r], 2));
-          const float mn = fmaxf(m[r], mx[r]);
-          base[r] = mn == -INFINITY ? 0.f : mn;
-          alpha[r] = ex2(m[r] - base[r]);                  // 0 while the row has seen no key
-          m[r] = mn;
-        }
-        if (__any_sync(~0u, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            l[r] *= alpha[r];
-#pragma unroll
-            for (int d = 0; d < D / 8; ++d) {
-              o[d][2 * r] *= alpha[r];
-              o[d][2 * r + 1] *= alpha[r];
+              for (int x = 0; x < NT; ++x) mma16816<BF16>(s[x][mt], ka, qb[x][c][sp][0], qb[x][c][sp][1]);
             }
           }
         }
-        float ps[2] = {0.f, 0.f};
+        uint32_t pb[NT][2][2];
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
+        for (int x = 0; x < NT; ++x) {
+          float cx[2] = {uck, uck}, ix[2] = {uinv, uinv}, lx[2] = {ulv, ulv};
+          if (key0 + UNIT > all) {        // warp-uniform
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[nt][e] = ex2(s[nt][e] - base[e >> 1]);
-            ps[e >> 1] += s[nt][e];
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (key0 + 16 * mt + kappa + 8 * (e >> 1) >= lim[x][e & 1]) s[x][mt][e] = -INFINITY;
+            // a row that sees none of these keys takes nothing from their scale either
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (key0 >= lim[x][e]) {
+                cx[e] = 1.f;
+                lx[e] = 0.f;
+                ix[e] = 0.f;
+              }
           }
-        // (a row that sees none of these keys takes nothing from their scale either)
-        if (ps[0] != 0.f) l[0] += ps[0] * inv_vs;
-        if (ps[1] != 0.f) l[1] += ps[1] * inv_vs;
-        // O += P V: 16 keys a step, lane t's four are t + {0, 4, 8, 12}; column n
-        // of dim tile d is dim 8n + d of a 64-dim chunk, so lane g's operands are
-        // 8 consecutive bytes of a row
+          float alpha[2], nm[2];
 #pragma unroll
-        for (int sp = 0; sp < 2; ++sp) {
-          const uint32_t pa[4] = {pack_half2(s[2 * sp][0], s[2 * sp][1]), pack_half2(s[2 * sp][2], s[2 * sp][3]),
-                                  pack_half2(s[2 * sp + 1][0], s[2 * sp + 1][1]),
-                                  pack_half2(s[2 * sp + 1][2], s[2 * sp + 1][3])};
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(fmaxf(s[x][0][e], s[x][0][e + 2]), fmaxf(s[x][1][e], s[x][1][e + 2]));
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, d));
+            const float mn = fmaxf(m[x][e], fmaf(mx, cx[e], lx[e]));
+            const float base = mn == -INFINITY ? 0.f : mn;
+            alpha[e] = ex2(m[x][e] - base);                // 0 while the row has seen no key
+            m[x][e] = mn;
+            nm[e] = lx[e] - base;
+          }
+          if (__any_sync(~0u, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              l[x][e] *= alpha[e];
+#pragma unroll
+              for (int d = 0; d < D / 16; ++d) {
+                o[x][d][e] *= alpha[e];
+                o[x][d][e + 2] *= alpha[e];
+              }
+            }
+          }
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[x][mt][e] = ex2(fmaf(s[x][mt][e], cx[e & 1], nm[e & 1]));
+            // P^T as the B operand: keys 2t, 2t + 1 (slots) x row g
+            pb[x][mt][0] = transpose8(pack_half2(s[x][mt][0], s[x][mt][1]));
+            pb[x][mt][1] = transpose8(pack_half2(s[x][mt][2], s[x][mt][3]));
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            l[x][e] = fmaf((s[x][0][e] + s[x][0][e + 2]) + (s[x][1][e] + s[x][1][e + 2]), ix[e], l[x][e]);
+        }
+        // O^T += V^T P^T, 16 keys a step: lane t's rows of V are slots 2t, 2t + 1,
+        // 2t + 8, 2t + 9 = keys t + {0, 4, 8, 12}, of which it takes 8 bytes
+#pragma unroll
+        for (int sp = 0; sp < 2; ++sp)
 #pragma unroll
           for (int c = 0; c < KC; ++c) {
             uint2 w[4];
@@ -283,18 +332,19 @@ __global__ void __launch_bounds__(RowLay<D>::THREADS, 1) attn_cache_rows_kernel(
             for (int k = 0; k < 4; ++k) w[k] = lds64(vb + (16 * sp + t + 4 * k) * D + 64 * c + 8 * g);
 #pragma unroll
             for (int hw = 0; hw < 2; ++hw) {
-              const uint32_t x0 = (hw ? w[0].y : w[0].x) ^ 0x80808080u, x1 = (hw ? w[1].y : w[1].x) ^ 0x80808080u;
-              const uint32_t y0 = (hw ? w[2].y : w[2].x) ^ 0x80808080u, y1 = (hw ? w[3].y : w[3].x) ^ 0x80808080u;
-              const uint32_t xl = __byte_perm(x0, x1, 0x5140), xh = __byte_perm(x0, x1, 0x7362);
-              const uint32_t yl = __byte_perm(y0, y1, 0x5140), yh = __byte_perm(y0, y1, 0x7362);
-              float(*oc)[4] = &o[8 * c + 4 * hw];
-              mma16816<false>(oc[0], pa, codes_f16<false>(xl), codes_f16<false>(yl));
-              mma16816<false>(oc[1], pa, codes_f16<true>(xl), codes_f16<true>(yl));
-              mma16816<false>(oc[2], pa, codes_f16<false>(xh), codes_f16<false>(yh));
-              mma16816<false>(oc[3], pa, codes_f16<true>(xh), codes_f16<true>(yh));
+              const uint32_t x0 = hw ? w[0].y : w[0].x, x1 = hw ? w[1].y : w[1].x;
+              const uint32_t y0 = hw ? w[2].y : w[2].x, y1 = hw ? w[3].y : w[3].x;
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const uint32_t xx = __byte_perm(x0, x1, j ? 0x7362 : 0x5140) ^ 0x80808080u;
+                const uint32_t yy = __byte_perm(y0, y1, j ? 0x7362 : 0x5140) ^ 0x80808080u;
+                const uint32_t va[4] = {codes_f16<false>(xx), codes_f16<true>(xx), codes_f16<false>(yy),
+                                        codes_f16<true>(yy)};
+#pragma unroll
+                for (int x = 0; x < NT; ++x) mma16816<false>(o[x][4 * c + 2 * hw + j], va, pb[x][sp][0], pb[x][sp][1]);
+              }
             }
           }
-        }
       }
       // refill the stage once every lane has read it (ordinary loads before the
       // copy's writes)
@@ -319,41 +369,43 @@ __global__ void __launch_bounds__(RowLay<D>::THREADS, 1) attn_cache_rows_kernel(
     // every warp is done with its ring before any writes O over it
     if (__syncthreads_or(!ok)) break;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(~0u, l[r], 1);
-      l[r] += __shfl_xor_sync(~0u, l[r], 2);
-      if (t == 0) {
-        sm_m[warp * TOK_ROWS + g + 8 * r] = m[r];
-        sm_l[warp * TOK_ROWS + g + 8 * r] = l[r];
+    for (int x = 0; x < NT; ++x)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) l[x][e] += __shfl_xor_sync(~0u, l[x][e], d);
+        const int r = 8 * x + 2 * t + e;
+        if (g == 0) {
+          sm_m[warp * L::ROWS + r] = m[x][e];
+          sm_l[warp * L::ROWS + r] = l[x][e];
+        }
+        if (row0 + r < rows) {
+          // dims 64c + 8g + 4w + 2j + (0, 1) of the row
+          float* dst = sm_o + (warp * L::ROWS + r) * D + 8 * g;
+#pragma unroll
+          for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int hw = 0; hw < 2; ++hw) {
+              const int d = 4 * c + 2 * hw;
+              *reinterpret_cast<float4*>(dst + 64 * c + 4 * hw) =
+                  make_float4(o[x][d][e], o[x][d][e + 2], o[x][d + 1][e], o[x][d + 1][e + 2]);
+            }
+        }
       }
-      if (row0 + g + 8 * r < rows) {
-        // dims 64c + 16t + 8e + (0..7) of the row
-        float* dst = sm_o + (warp * TOK_ROWS + g + 8 * r) * D;
-#pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int d = 0; d < 8; d += 4)
-              *reinterpret_cast<float4*>(dst + 64 * c + 16 * t + 8 * e + d) =
-                  make_float4(o[8 * c + d][2 * r + e], o[8 * c + d + 1][2 * r + e], o[8 * c + d + 2][2 * r + e],
-                              o[8 * c + d + 3][2 * r + e]);
-      }
-    }
     __syncthreads();
-    const int live = min(TOK_ROWS, rows - row0);
+    const int live = min(L::ROWS, rows - row0);
     for (int x = threadIdx.x; x < live * (D / 2); x += L::THREADS) {
       const int r = x / (D / 2), d = 2 * (x % (D / 2)), row = row0 + r;
       float mt = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < L::WARPS; ++w) mt = fmaxf(mt, sm_m[w * TOK_ROWS + r]);
+      for (int w = 0; w < L::WARPS; ++w) mt = fmaxf(mt, sm_m[w * L::ROWS + r]);
       const float base = mt == -INFINITY ? 0.f : mt;
       float lt = 0.f, p = 0.f, q = 0.f;
 #pragma unroll
       for (int w = 0; w < L::WARPS; ++w) {
-        const float f = ex2(sm_m[w * TOK_ROWS + r] - base);
-        const float2 v = *reinterpret_cast<const float2*>(sm_o + (w * TOK_ROWS + r) * D + d);
-        lt += f * sm_l[w * TOK_ROWS + r];
+        const float f = ex2(sm_m[w * L::ROWS + r] - base);
+        const float2 v = *reinterpret_cast<const float2*>(sm_o + (w * L::ROWS + r) * D + d);
+        lt += f * sm_l[w * L::ROWS + r];
         p += f * v.x;
         q += f * v.y;
       }
@@ -362,7 +414,7 @@ __global__ void __launch_bounds__(RowLay<D>::THREADS, 1) attn_cache_rows_kernel(
       const long long tok = sg.q0 + row / a.group;
       const int h = kvh * a.group + row % a.group;
       if (sg.slot >= 0) {
-        const long long part = (long long)sg.slot * TOK_ROWS + r;
+        const long long part = (long long)sg.slot * L::ROWS + r;
         *reinterpret_cast<float2*>(a.part_o + part * D + d) = make_float2(p * inv, q * inv);
         if (d == 0) a.part_lse[part] = lse2;
       } else {
@@ -376,97 +428,98 @@ __global__ void __launch_bounds__(RowLay<D>::THREADS, 1) attn_cache_rows_kernel(
     __syncthreads();
   }
   if (threadIdx.x == L::THREADS - 32 && a.can_split)
-    reinterpret_cast<Cut*>(a.part_lse + 2LL * gridDim.x * TOK_ROWS)[blockIdx.x] = walk->cut;
+    reinterpret_cast<Cut*>(a.part_lse + 2LL * gridDim.x * L::ROWS)[blockIdx.x] = walk->cut;
 }
 
 // Adds the parts of the items that a cut went through: CTA x looks at the cut
 // before piece x + 1, and the item's first cut does the work, a warp per row.
-template <bool BF16, int D>
-__global__ void __launch_bounds__(TOK_ROWS * 32) attn_cache_rows_join_kernel(CacheAttnArgs a, int grid) {
+template <bool BF16, int D, int NT>
+__global__ void __launch_bounds__(NT * 256) attn_cache_rows_join_kernel(CacheAttnArgs a, int grid) {
   pdl_wait();
   pdl_trigger();
   const int x = blockIdx.x + 1, lane = threadIdx.x % 32, r = threadIdx.x / 32;
-  const Cut cut = reinterpret_cast<const Cut*>(a.part_lse + 2LL * grid * TOK_ROWS)[x];
+  const Cut cut = reinterpret_cast<const Cut*>(a.part_lse + 2LL * grid * 8 * NT)[x];
   if (cut.first != x - 1) return;
   const int row = cut.tok0 + r;
   if (row >= cut.ql * a.group) return;
-  join_parts<BF16, D>(a, cut, TOK_ROWS, r, lane, cut.q0 + row / a.group, cut.kvh * a.group + row % a.group);
+  join_parts<BF16, D>(a, cut, 8 * NT, r, lane, cut.q0 + row / a.group, cut.kvh * a.group + row % a.group);
 }
+
+// Sizes and launch of the row kernel with NT 8-row tiles.
+template <int D, int NT>
+struct Rows {
+  using L = RowLay<D, NT>;
+  using B = RowBlock<D, NT>;
+  // Whether items may be cut (a rule on the hint alone: the join is launched
+  // by it): above four units for each warp.
+  static bool split(long long max_kv) { return max_kv > 4 * UNIT * L::WARPS; }
+  static int grid(long long items, long long max_kv) {
+    const long long cost = items * (B::START + (max_kv + UNIT - 1) / UNIT);
+    const long long pieces = split(max_kv) ? (cost + B::MIN - 1) / B::MIN : items;
+    return (int)std::max<long long>(1, std::min<long long>(pieces, device_info().num_sms));
+  }
+  static int64_t scratch(long long items, long long max_kv) {
+    const int64_t n = grid(items, max_kv);
+    return split(max_kv) && n > 1 ? n * (2 * L::ROWS * (D + 1) * (int64_t)sizeof(float) + (int64_t)sizeof(Cut)) : 0;
+  }
+  static int launch(CacheAttnArgs& a, bool bf16, long long max_kv, bool may_split, void* scratch, cudaStream_t stream) {
+    if (L::TOTAL > device_info().max_smem_optin)
+      return set_error(QVGGT_ERR_UNSUPPORTED, "cached_attention: shared memory %d > %d", L::TOTAL,
+                       device_info().max_smem_optin);
+    const int n = grid((long long)a.B * a.row_blocks * a.hk, max_kv);
+    a.can_split = may_split && n > 1 && split(max_kv);
+    a.part_o = static_cast<float*>(scratch);
+    a.part_lse = a.can_split ? a.part_o + 2LL * n * L::ROWS * D : nullptr;
+    static DeviceFlags attr[2];
+    const auto fn = bf16 ? attn_cache_rows_kernel<true, D, NT> : attn_cache_rows_kernel<false, D, NT>;
+    if (int rc = ensure_smem(attr[bf16], fn, L::TOTAL, "cudaFuncSetAttribute(cached_attention)")) return rc;
+    if (int rc = check_cuda(launch_pdl(fn, dim3((unsigned)n), dim3(L::THREADS), L::TOTAL, stream, 1u, a),
+                            "cached_attention launch"))
+      return rc;
+    count_launch(1);
+    if (a.can_split) {
+      const auto join = bf16 ? attn_cache_rows_join_kernel<true, D, NT> : attn_cache_rows_join_kernel<false, D, NT>;
+      if (int rc = check_cuda(launch_pdl(join, dim3((unsigned)(n - 1)), dim3(NT * 256), 0, stream, 1u, a, n),
+                              "cached_attention join launch"))
+        return rc;
+      count_launch(1);
+    }
+    return QVGGT_OK;
+  }
+};
+
+// Rows (of a kv head) up to which the row kernel serves a call.  It reads the
+// cache once for each 8, 16 or 32 rows at up to memory speed; the tile kernel
+// reads it once for up to 256, at a rate that its softmax sets.
+constexpr int ROWS_MAX_64 = 32, ROWS_MAX_128 = 16;
 
 // How a call is laid out, by its sizes alone.
 struct Plan {
   bool tiles;                            // attn_cache_sm100.cu's kernel
-  int row_blocks;                        // 16-row tiles or Q blocks of a request
+  int nt;                                // 8-row tiles of the row kernel's items
+  int row_blocks;                        // blocks of rows of a request
   int64_t scratch;
 };
 
-// Rows served by the row kernel: it reads the cache at memory speed for each 16
-// rows, the tile kernel at about a third of that for any number up to 256.
-constexpr int ROWS_MAX = 16;
-
-// Whether the row kernel's items may be cut (a rule on the hint alone: the join
-// is launched by it): above four units for each warp.
-bool rows_split(long long max_kv, int D) { return max_kv > 4 * UNIT * (D == 64 ? RowLay<64>::WARPS : RowLay<128>::WARPS); }
-
-int rows_grid(long long items, long long max_kv, int D) {
-  const long long start = D == 64 ? RowBlock<64>::START : RowBlock<128>::START;
-  const long long least = D == 64 ? RowBlock<64>::MIN : RowBlock<128>::MIN;
-  const long long cost = items * (start + (max_kv + UNIT - 1) / UNIT);
-  const long long pieces = rows_split(max_kv, D) ? (cost + least - 1) / least : items;
-  return (int)std::max<long long>(1, std::min<long long>(pieces, device_info().num_sms));
+// Calls f with the row kernel's sizes for head_dim and 8-row tiles.
+template <class F>
+auto with_rows(int head_dim, int nt, F f) {
+  if (head_dim == 64) return nt == 1 ? f(Rows<64, 1>()) : nt == 2 ? f(Rows<64, 2>()) : f(Rows<64, 4>());
+  return nt == 1 ? f(Rows<128, 1>()) : f(Rows<128, 2>());
 }
 
-int64_t rows_scratch(long long items, long long max_kv, int D) {
-  if (!rows_split(max_kv, D)) return 0;
-  const int64_t grid = rows_grid(items, max_kv, D);
-  return grid > 1 ? grid * (2 * TOK_ROWS * (D + 1) * (int64_t)sizeof(float) + (int64_t)sizeof(Cut)) : 0;
-}
-
-int launch_rows(CacheAttnArgs& a, int D, bool bf16, long long max_kv, bool split, void* scratch, cudaStream_t stream) {
-  const int smem = D == 64 ? RowLay<64>::TOTAL : RowLay<128>::TOTAL;
-  const int threads = D == 64 ? RowLay<64>::THREADS : RowLay<128>::THREADS;
-  if (smem > device_info().max_smem_optin)
-    return set_error(QVGGT_ERR_UNSUPPORTED, "cached_attention: shared memory %d > %d", smem,
-                     device_info().max_smem_optin);
-  const long long items = (long long)a.B * a.row_blocks * a.hk;
-  const int grid = rows_grid(items, max_kv, D);
-  a.can_split = split && grid > 1 && rows_split(max_kv, D);
-  a.part_o = static_cast<float*>(scratch);
-  a.part_lse = a.can_split ? a.part_o + 2LL * grid * TOK_ROWS * D : nullptr;
-  using Kfn = void (*)(CacheAttnArgs);
-  static const Kfn fns[2][2] = {{attn_cache_rows_kernel<false, 64>, attn_cache_rows_kernel<false, 128>},
-                                {attn_cache_rows_kernel<true, 64>, attn_cache_rows_kernel<true, 128>}};
-  using Jfn = void (*)(CacheAttnArgs, int);
-  static const Jfn joins[2][2] = {{attn_cache_rows_join_kernel<false, 64>, attn_cache_rows_join_kernel<false, 128>},
-                                  {attn_cache_rows_join_kernel<true, 64>, attn_cache_rows_join_kernel<true, 128>}};
-  static DeviceFlags attr[2][2];
-  if (int rc = ensure_smem(attr[bf16][D == 128], fns[bf16][D == 128], smem, "cudaFuncSetAttribute(cached_attention)"))
-    return rc;
-  if (int rc = check_cuda(launch_pdl(fns[bf16][D == 128], dim3((unsigned)grid), dim3(threads), smem, stream, 1u, a),
-                          "cached_attention launch"))
-    return rc;
-  count_launch(1);
-  if (a.can_split) {
-    if (int rc = check_cuda(launch_pdl(joins[bf16][D == 128], dim3((unsigned)(grid - 1)), dim3(TOK_ROWS * 32), 0,
-                                       stream, 1u, a, grid),
-                            "cached_attention join launch"))
-      return rc;
-    count_launch(1);
-  }
-  return QVGGT_OK;
-}
-
-Plan make_plan(int group, int kv_heads, int requests, int max_q, long long max_kv, int head_dim) {
+Plan make_plan(int group, int kv_heads, int requests, int max_q, long long max_kv, int head_dim, bool force_rows) {
   Plan p{};
-  const long long rows = (long long)max_q * group;
-  p.tiles = rows > ROWS_MAX && group <= 128;
+  const long long rows = (long long)max_q * group, pairs = (long long)kv_heads * requests;
+  p.nt = rows <= 8 ? 1 : rows <= 16 || head_dim == 128 ? 2 : 4;
+  p.tiles = rows > (head_dim == 64 ? ROWS_MAX_64 : ROWS_MAX_128) && group <= 128 && !force_rows;
   if (p.tiles) {
     const int tokens = 2 * (128 / group);
     p.row_blocks = (int)(((long long)max_q + tokens - 1) / tokens);
-    p.scratch = tiles_scratch((long long)p.row_blocks * kv_heads * requests, max_kv, head_dim);
+    p.scratch = tiles_scratch(p.row_blocks * pairs, max_kv, head_dim);
   } else {
-    p.row_blocks = (int)((rows + TOK_ROWS - 1) / TOK_ROWS);
-    p.scratch = rows_scratch((long long)p.row_blocks * kv_heads * requests, max_kv, head_dim);
+    p.row_blocks = (int)((rows + 8 * p.nt - 1) / (8 * p.nt));
+    p.scratch = with_rows(head_dim, p.nt, [&](auto k) { return k.scratch(p.row_blocks * pairs, max_kv); });
   }
   return p;
 }
@@ -494,7 +547,7 @@ extern "C" int qvggt_cached_attention_scratch(int64_t Tq, int32_t q_heads, int32
   if (int rc = check_shape("cached_attention_scratch", Tq, q_heads, kv_heads, requests, max_q, max_kv, head_dim))
     return rc;
   if (!bytes) return set_error(QVGGT_ERR_INVALID, "cached_attention_scratch: null pointer");
-  *bytes = make_plan(q_heads / kv_heads, kv_heads, requests, max_q, max_kv, head_dim).scratch;
+  *bytes = make_plan(q_heads / kv_heads, kv_heads, requests, max_q, max_kv, head_dim, false).scratch;
   return QVGGT_OK;
 }
 
@@ -551,12 +604,13 @@ extern "C" int qvggt_cached_attention(const void* q, int64_t q_tok, int64_t q_he
   a.max_q = max_q;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.ctl = make_ctl();
-  Plan p = make_plan(a.group, kv_heads, requests, max_q, max_kv, head_dim);
-  const bool strided = p.tiles && !tiles_can_read(a);
-  if (strided) {
-    // strides no TMA map takes (a broadcast or reversed query): the row kernel, items whole
-    p.tiles = false;
-    p.row_blocks = (int)(((long long)max_q * a.group + TOK_ROWS - 1) / TOK_ROWS);
+  // strides no TMA map takes (a broadcast or reversed query): the row kernel,
+  // items whole where the scratch is laid out for the tile kernel
+  const bool strided = !tiles_can_read(a);
+  Plan p = make_plan(a.group, kv_heads, requests, max_q, max_kv, head_dim, false);
+  const bool fits = !(strided && p.tiles);
+  if (!fits) {
+    p = make_plan(a.group, kv_heads, requests, max_q, max_kv, head_dim, true);
     p.scratch = 0;
   }
   const int64_t need = p.scratch;
@@ -568,6 +622,6 @@ extern "C" int qvggt_cached_attention(const void* q, int64_t q_tok, int64_t q_he
   a.wait_tries = (uint32_t)std::min<unsigned long long>(1u << 26, a.ctl.timeout_ns / 1024 + 1);
   const bool bf16 = dtype == QVGGT_DTYPE_BF16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return p.tiles ? launch_tiles(a, head_dim, bf16, max_kv, scratch, st)
-                 : launch_rows(a, head_dim, bf16, max_kv, !strided, scratch, st);
+  if (p.tiles) return launch_tiles(a, head_dim, bf16, max_kv, scratch, st);
+  return with_rows(head_dim, p.nt, [&](auto k) { return k.launch(a, bf16, max_kv, fits, scratch, st); });
 }
