@@ -15,9 +15,9 @@ constexpr int UNIT = 32;                 // keys a warp takes at a time: never a
 template <int D, int NT>
 struct RowLay {
   static constexpr int ROWS = 8 * NT;
-  static constexpr int WARPS = D == 64 && NT < 4 ? 16 : 8;
+  static constexpr int WARPS = D == 128 ? 6 : NT < 4 ? 8 : 4;
   static constexpr int THREADS = WARPS * 32;
-  static constexpr int STAGES = 192 * 1024 / (WARPS * 2 * UNIT * D);   // units in flight per warp: 3 or 6
+  static constexpr int STAGES = 96 * 1024 / (WARPS * 2 * UNIT * D);   // units in flight per warp: 3, 6 or 2
   static constexpr int SIDE = UNIT * D;                    // K or V codes of a unit
   static constexpr int RING = 0;                           // [warp][stage][K, V]
   static constexpr int RING_BYTES = WARPS * STAGES * 2 * SIDE;
@@ -26,7 +26,9 @@ struct RowLay {
   static constexpr int SEG = CUM + (THREADS + 2) * 8;      // Segment [2]
   static constexpr int ML = SEG + 2 * (int)sizeof(Segment);   // float [warp][row] maxima, then sums
   static constexpr int WALK = ML + 2 * WARPS * ROWS * 4;   // PieceWalk, one thread's
-  static constexpr int TOTAL = WALK + 256;
+  static constexpr int Q = WALK + 256;                     // q's fragments, where they do not fit registers
+  static constexpr bool Q_SHARED = D == 128 && NT == 2;
+  static constexpr int TOTAL = Q + (Q_SHARED ? NT * (D / 16) * 32 * 8 : 0);
   // the warps' O, merged at the end of a segment, lie in the drained ring
   static_assert(WARPS * ROWS * D * 4 <= RING_BYTES, "O does not fit the ring");
 };
@@ -56,16 +58,10 @@ struct RowBlock {
   }
 };
 
-template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t at) {
@@ -98,7 +94,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // against 340 now, 150 us against XXX at 8 x 16 heads x 43,968 keys), and each
 // of up to 8 rows costs what one does.
 template <bool BF16, int D, int NT>
-__global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 1) attn_cache_rows_kernel(CacheAttnArgs a) {
+__global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 2) attn_cache_rows_kernel(CacheAttnArgs a) {
   using L = RowLay<D, NT>;
   constexpr int KC = D / 64;              // 64-dim chunks
   extern __shared__ __align__(128) uint8_t smem[];
@@ -163,7 +159,6 @@ __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 1) attn_cache_rows_ker
       inv_vs = 1.f / vs;
     };
     int id = fetch_id(lane), id2 = fetch_id(32 + lane);
-    constants(id);
     bool bad = false;
     // starts the copies of unit i (a block outside the cache: none)
     auto issue = [&](int i, int block) {
@@ -182,6 +177,7 @@ __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 1) attn_cache_rows_ker
       }
     };
     for (int i = 0; i < L::STAGES && i < count; ++i) issue(i, __shfl_sync(~0u, id, i));
+    constants(id);
 
     // rows 2t and 2t + 1 of each 8-row tile
     int lim[NT][2];
@@ -195,22 +191,64 @@ __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 1) attn_cache_rows_ker
     const int all = key_limit(row0 / a.group, ql, n, a.chunk);   // keys that every row sees
     // B fragments of q (row g of each tile): step s of chunk c takes dims
     // 64c + 16t + 4s + {0, 1} as k rows 2t, 2t+1 and {2, 3} as 2t+8, 2t+9 (any
-    // order of the dims will do, as K's fragments use the same)
-    uint32_t qb[NT][KC][4][2];
+    // order of the dims will do, as K's fragments use the same).  bf16 queries
+    // become fp16 times a power of two per row (its largest element near 2^13;
+    // what fp16 then cannot hold exactly is below 2^-37 of that), because codes
+    // unpack to fp16 in five instructions a word and to bf16 in eight: 61 us
+    // against XXX at 16 ragged requests x 8 heads x 128.
+    uint32_t qb[L::Q_SHARED ? 1 : NT][KC][4][2];
+    float row_ck[NT][2];                  // what undoes it, of rows 2t and 2t + 1
+    if (L::Q_SHARED) __syncthreads();     // the segment before is done with the shared fragments
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
       const int row = min(row0 + 8 * x + g, rows - 1);
       const uint16_t* qp = a.q + (long long)(sg.q0 + row / a.group) * a.q_tok +
                            (long long)(kvh * a.group + row % a.group) * a.q_head;
+      uint2 w[KC][4];
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) w[c][s] = *reinterpret_cast<const uint2*>(qp + 64 * c + 16 * t + 4 * s);
+      float back = 1.f;
+      if (BF16) {
+        float mx = 0.f;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const float2 p = unpack_bf162(w[c][s].x), q = unpack_bf162(w[c][s].y);
+            mx = fmaxf(mx, fmaxf(fmaxf(fabsf(p.x), fabsf(p.y)), fmaxf(fabsf(q.x), fabsf(q.y))));
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+        // exponents of 2^up and 2^-up; rows of zeros, infinities or NaN (and
+        // magnitudes whose factor would leave the normal range) stay within it
+        const int up = max(-115, min(110, 13 - ((int)(__float_as_uint(mx) >> 23) - 127)));
+        const float f = __int_as_float((127 + up) << 23);
+        back = __int_as_float((127 - up) << 23);
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const float2 p = unpack_bf162(w[c][s].x), q = unpack_bf162(w[c][s].y);
+            w[c][s] = make_uint2(pack_half2(p.x * f, p.y * f), pack_half2(q.x * f, q.y * f));
+          }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) row_ck[x][e] = __shfl_sync(~0u, back, (2 * t + e) * 4);
 #pragma unroll
       for (int c = 0; c < KC; ++c)
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const uint2 w = *reinterpret_cast<const uint2*>(qp + 64 * c + 16 * t + 4 * s);
-          qb[x][c][s][0] = w.x;
-          qb[x][c][s][1] = w.y;
+          if constexpr (L::Q_SHARED) {
+            if (warp == 0) reinterpret_cast<uint2*>(smem + L::Q)[((x * KC + c) * 4 + s) * 32 + lane] = w[c][s];
+          } else {
+            qb[x][c][s][0] = w[c][s].x;
+            qb[x][c][s][1] = w[c][s].y;
+          }
         }
     }
+    if (L::Q_SHARED) __syncthreads();
     float o[NT][D / 16][4];               // O^T: tile 4c + 2w + j, slots (dim, dim + 1) x rows (2t, 2t + 1)
 #pragma unroll
     for (int x = 0; x < NT; ++x)
@@ -260,17 +298,24 @@ __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 1) attn_cache_rows_ker
             const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
             for (int sp = 0; sp < 4; ++sp) {
-              const uint32_t ka[4] = {codes2<BF16, false>(x0[sp]), codes2<BF16, false>(x1[sp]),
-                                      codes2<BF16, true>(x0[sp]), codes2<BF16, true>(x1[sp])};
+              const uint32_t ka[4] = {codes2<false, false>(x0[sp]), codes2<false, false>(x1[sp]),
+                                      codes2<false, true>(x0[sp]), codes2<false, true>(x1[sp])};
 #pragma unroll
-              for (int x = 0; x < NT; ++x) mma16816<BF16>(s[x][mt], ka, qb[x][c][sp][0], qb[x][c][sp][1]);
+              for (int x = 0; x < NT; ++x) {
+                if constexpr (L::Q_SHARED) {
+                  const uint2 q2 = lds64(sbase + L::Q + (((x * KC + c) * 4 + sp) * 32 + lane) * 8);
+                  mma16816(s[x][mt], ka, q2.x, q2.y);
+                } else {
+                  mma16816(s[x][mt], ka, qb[x][c][sp][0], qb[x][c][sp][1]);
+                }
+              }
             }
           }
         }
         uint32_t pb[NT][2][2];
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-          float cx[2] = {uck, uck}, ix[2] = {uinv, uinv}, lx[2] = {ulv, ulv};
+          float cx[2] = {BF16 ? uck * row_ck[x][0] : uck, BF16 ? uck * row_ck[x][1] : uck}, ix[2] = {uinv, uinv}, lx[2] = {ulv, ulv};
           if (key0 + UNIT > all) {        // warp-uniform
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
@@ -341,7 +386,7 @@ __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 1) attn_cache_rows_ker
                 const uint32_t va[4] = {codes_f16<false>(xx), codes_f16<true>(xx), codes_f16<false>(yy),
                                         codes_f16<true>(yy)};
 #pragma unroll
-                for (int x = 0; x < NT; ++x) mma16816<false>(o[x][4 * c + 2 * hw + j], va, pb[x][sp][0], pb[x][sp][1]);
+                for (int x = 0; x < NT; ++x) mma16816(o[x][4 * c + 2 * hw + j], va, pb[x][sp][0], pb[x][sp][1]);
               }
             }
           }
@@ -456,7 +501,7 @@ struct Rows {
   static int grid(long long items, long long max_kv) {
     const long long cost = items * (B::START + (max_kv + UNIT - 1) / UNIT);
     const long long pieces = split(max_kv) ? (cost + B::MIN - 1) / B::MIN : items;
-    return (int)std::max<long long>(1, std::min<long long>(pieces, device_info().num_sms));
+    return (int)std::max<long long>(1, std::min<long long>(pieces, 2LL * device_info().num_sms));
   }
   static int64_t scratch(long long items, long long max_kv) {
     const int64_t n = grid(items, max_kv);
