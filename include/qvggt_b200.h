@@ -295,24 +295,38 @@ int qvggt_attention_small(const void* q, int64_t q_stride, const void* kv, int64
                           int64_t v_col0, void* out, int64_t o_stride, int64_t batches, int64_t L, int32_t heads,
                           void* stream);
 
-/* --------------------------------------------------- streaming K/V cache */
+/* --------------------------------------------------- streaming K/V cache
+ * These calls take their arguments in a structure of 64-bit fields (sizes,
+ * strides in elements, device pointers).  Sizes that have to fit 32 bits are
+ * checked. */
 
 /* Rotary positions with 1..4 axes (time, height, width, ...), q and k in one
  * launch.  x [T, heads, head_dim] with element strides (tok, head) and unit
  * stride inside a head; fp16 or bf16 (dtype); out may be the input itself.
- * Axis a owns sections[a] consecutive pairs (sections is a host array) of the
- * R/2 = sum(sections) pairs, and pair j turns by positions[axis_j][t] *
- * inv_freq[j]:  y[lo] = x[lo] cos - x[hi] sin,  y[hi] = x[hi] cos + x[lo] sin.
+ * Axis a owns sections[a] consecutive pairs of the R/2 = sum(sections) pairs,
+ * and pair j turns by positions[axis_j][t] * inv_freq[j]:
+ *   y[lo] = x[lo] cos - x[hi] sin,  y[hi] = x[hi] cos + x[lo] sin.
  * layout 0 (axial): each axis' pairs are the two halves of its own 2 *
  *   sections[a] dims; 1 (split): pair j is dims (j, j + R/2); 2 (interleaved):
  *   dims (2j, 2j + 1).  Dims >= R are copied.  inverse != 0 turns back (the
  * gradient).  positions int32 [n_axes, T] with row stride pos_stride, inv_freq
  * fp32 [R/2].  head_dim <= 256.  k_heads may be 0.  New entry point. */
-int qvggt_rope_axes(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok, int64_t qo_head,
-                    int32_t q_heads, const void* k, int64_t k_tok, int64_t k_head, void* k_out, int64_t ko_tok,
-                    int64_t ko_head, int32_t k_heads, int64_t T, int32_t head_dim, const int32_t* positions,
-                    int64_t pos_stride, const float* inv_freq, const int32_t* sections, int32_t n_axes,
-                    int32_t layout, int32_t inverse, int32_t dtype, void* stream);
+typedef struct {
+  const void* q;
+  int64_t q_tok, q_head;
+  void* q_out;
+  int64_t qo_tok, qo_head, q_heads;
+  const void* k;
+  int64_t k_tok, k_head;
+  void* k_out;
+  int64_t ko_tok, ko_head, k_heads;
+  int64_t T, head_dim;
+  const int32_t* positions;
+  int64_t pos_stride;
+  const float* inv_freq;
+  int64_t sections[4], n_axes, layout, inverse, dtype;
+} qvggt_rope_axes_args;
+int qvggt_rope_axes(const qvggt_rope_axes_args* args, void* stream);
 
 /* Block tables and slot maps of a paged cache, from request lengths.  Request
  * b goes from cached_lens[b] to target_lens[b] tokens (more: blocks are taken
@@ -325,45 +339,73 @@ int qvggt_rope_axes(const void* q, int64_t q_tok, int64_t q_head, void* q_out, i
  * cu_blocks [requests + 1], the running sums of new tokens and of blocks that
  * get new tokens; slots [max_new], block * block_size + offset of each new
  * token in request order, then -1; status[0].
- * status: 0 done; otherwise nothing is changed, no token gets a slot and lens_out =
- * cached_lens: 1 too few free blocks, 2 a table row too short, 3 a negative length,
- * 4 more than max_new tokens.  One launch, no host synchronisation; the same
- * inputs give the same result again.  At most 8192 requests; block_size a
- * power of two.  New entry point. */
-int qvggt_block_plan(const int32_t* cached_lens, const int32_t* target_lens, int32_t requests, int32_t* block_tables,
-                     int32_t max_blocks, int32_t* free_ring, int32_t num_blocks, const int64_t* free_range,
-                     int32_t block_size, int32_t max_new, int32_t* slots, int32_t* cu_new, int32_t* cu_blocks,
-                     int32_t* lens_out, int64_t* free_range_out, int32_t* status, void* stream);
+ * status: 0 done; otherwise nothing is changed, no token gets a slot and
+ * lens_out = cached_lens: 1 too few free blocks, 2 a table row too short, 3 a
+ * negative length, 4 more than max_new tokens.  One launch, no host
+ * synchronisation; the same inputs give the same result again.  At most 8192
+ * requests; block_size a power of two.  New entry point. */
+typedef struct {
+  const int32_t *cached_lens, *target_lens;
+  int64_t requests;
+  int32_t* block_tables;
+  int64_t max_blocks;
+  int32_t* free_ring;
+  int64_t num_blocks;
+  const int64_t* free_range;
+  int64_t block_size, max_new;
+  int32_t *slots, *cu_new, *cu_blocks, *lens_out;
+  int64_t* free_range_out;
+  int32_t* status;
+} qvggt_block_plan_args;
+int qvggt_block_plan(const qvggt_block_plan_args* args, void* stream);
+
+/* The 8-bit cache: k_cache / v_cache int8 [num_blocks][kv_heads][block_size]
+ * [head_dim] (block_stride codes between blocks, 16-byte aligned), k_scale /
+ * v_scale fp32 [num_blocks][kv_heads], all positive; an element is code *
+ * scale.  block_size 32, 64 or 128, head_dim 64 or 128. */
+typedef struct {
+  int8_t *k_cache, *v_cache;
+  int64_t block_stride;
+  float *k_scale, *v_scale;
+  int64_t num_blocks, kv_heads, block_size, head_dim;
+} qvggt_kv_cache;
 
 /* Writes new K and V rows into the 8-bit cache.
- * Cache: k_cache / v_cache int8 [num_blocks][kv_heads][block_size][head_dim]
- * (block_stride codes between blocks, 16-byte aligned), k_scale / v_scale fp32
- * [num_blocks][kv_heads]; an element is code * scale.  block_size 32, 64 or
- * 128, head_dim 64 or 128.
  * k, v [tokens, kv_heads, head_dim] (element strides of token and head, unit
  * stride inside, rows 16-byte aligned), fp16 or bf16, requests packed one
  * after another as cu_new says; cu_new and cu_blocks as qvggt_block_plan
  * writes them, cached_lens the lengths before.  max_units: an upper bound of
  * cu_blocks[requests] (tokens / block_size + 2 * requests always is one).
  * Per (block, head): s = max(s_old if the block holds earlier tokens, amax /
- * 127, 2^-60), code = rint(x / s) within +-127 (computed as x * (1 / s)); earlier codes c of the
- * block become rint(c * s_old / s).  Only finite values count in amax;
- * infinities are stored as the largest code, NaN as 0.  A block id or length
- * outside its range sets the device status word (0x201 / 0x202) and skips the
- * block.  New entry point. */
-int qvggt_kv_append(const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok, int64_t v_head,
-                    int64_t tokens, int32_t dtype, int8_t* k_cache, int8_t* v_cache, int64_t block_stride,
-                    float* k_scale, float* v_scale, int32_t num_blocks, int32_t kv_heads, int32_t block_size,
-                    int32_t head_dim, const int32_t* block_tables, int32_t max_blocks, const int32_t* cached_lens,
-                    const int32_t* cu_new, const int32_t* cu_blocks, int32_t requests, int32_t max_units,
-                    void* stream);
+ * 127, 2^-60), code = rint(x / s) within +-127 (computed as x * (1 / s));
+ * earlier codes c of the block become rint(c * s_old / s).  Only finite values
+ * count in amax; infinities are stored as the largest code, NaN as 0.  A block
+ * id or length outside its range sets the device status word (0x201 / 0x202)
+ * and skips the block.  New entry point. */
+typedef struct {
+  qvggt_kv_cache cache;
+  const void* k;
+  int64_t k_tok, k_head;
+  const void* v;
+  int64_t v_tok, v_head, tokens, dtype;
+  const int32_t* block_tables;
+  int64_t max_blocks;
+  const int32_t *cached_lens, *cu_new, *cu_blocks;
+  int64_t requests, max_units;
+} qvggt_kv_append_args;
+int qvggt_kv_append(const qvggt_kv_append_args* args, void* stream);
 
 /* Reads cache rows back: out [n][out_stride] fp16 or bf16, row i = [K of all
  * heads | V of all heads] of slots[i] (the layout qvggt_attention reads as
  * kv); a negative slot gives zeros.  New entry point. */
-int qvggt_kv_gather(const int8_t* k_cache, const int8_t* v_cache, int64_t block_stride, const float* k_scale,
-                    const float* v_scale, int32_t num_blocks, int32_t kv_heads, int32_t block_size, int32_t head_dim,
-                    const int32_t* slots, int64_t n, void* out, int64_t out_stride, int32_t dtype, void* stream);
+typedef struct {
+  qvggt_kv_cache cache;
+  const int32_t* slots;
+  int64_t n;
+  void* out;
+  int64_t out_stride, dtype;
+} qvggt_kv_gather_args;
+int qvggt_kv_gather(const qvggt_kv_gather_args* args, void* stream);
 
 /* Attention over the 8-bit cache: softmax(scale q k^T + mask) v for ragged
  * requests whose query rows are packed one after another.
@@ -371,27 +413,37 @@ int qvggt_kv_gather(const int8_t* k_cache, const int8_t* v_cache, int64_t block_
  * head, rows 16-byte aligned; query head h reads key head h / (q_heads /
  * kv_heads).  Request b's queries are rows [cu_q[b], cu_q[b + 1]) (at most
  * max_q of them) and its keys the first kv_lens[b] tokens of table row b;
- * max_kv is the largest length the launch is laid out for (any length up to the
- * table's is served).
+ * max_kv is about the largest length (it sets how the work is laid out; any
+ * length up to the table's is served).
  * Mask: query i of ql sits at position p = kv_len - ql + i.  causal_chunk 0:
  * it sees every key; c > 0: keys j < (p / c + 1) * c (1: causal; the tokens of
- * a frame: its own and all earlier frames), none when p < 0.  A row that sees no key
- * gives 0.  lse (fp32 [q_heads][Tq], may be NULL): ln sum_j exp(scale q.k_j),
- * -inf for such a row.
+ * a frame: its own and all earlier frames), none when p < 0.  A row that sees
+ * no key gives 0.  lse (fp32 [q_heads][Tq], may be NULL): ln sum_j exp(scale
+ * q.k_j), -inf for such a row.
  * Sums, maxima and products are held in fp32; the weights are rounded to fp16
  * for the product with V.
  * scratch: qvggt_cached_attention_scratch() bytes (0 for some shapes), 16-byte
- * aligned; its contents need no preparation and are free after the call, and calls that may
- * overlap on the GPU may not share it.  A block id or length outside its range
- * sets the device status word (0x201: the block's keys are skipped, 0x202: the
- * request is skipped).  New entry points. */
-int qvggt_cached_attention(const void* q, int64_t q_tok, int64_t q_head, void* out, int64_t o_tok, int64_t o_head,
-                           float* lse, int64_t Tq, int32_t q_heads, int32_t dtype, const int8_t* k_cache,
-                           const int8_t* v_cache, int64_t block_stride, const float* k_scale, const float* v_scale,
-                           int32_t num_blocks, int32_t kv_heads, int32_t block_size, int32_t head_dim,
-                           const int32_t* block_tables, int32_t max_blocks, const int32_t* cu_q,
-                           const int32_t* kv_lens, int32_t requests, int32_t max_q, int64_t max_kv,
-                           int32_t causal_chunk, float scale, void* scratch, int64_t scratch_bytes, void* stream);
+ * aligned; its contents need no preparation and are free after the call, and
+ * calls that may overlap on the GPU may not share it.  A block id or length
+ * outside its range sets the device status word (0x201: the block's keys are
+ * skipped, 0x202: the request is skipped).  New entry points. */
+typedef struct {
+  qvggt_kv_cache cache;
+  const void* q;
+  int64_t q_tok, q_head;
+  void* out;
+  int64_t o_tok, o_head;
+  float* lse;
+  int64_t Tq, q_heads, dtype;
+  const int32_t* block_tables;
+  int64_t max_blocks;
+  const int32_t *cu_q, *kv_lens;
+  int64_t requests, max_q, max_kv, causal_chunk;
+  double scale;
+  void* scratch;
+  int64_t scratch_bytes;
+} qvggt_cached_attention_args;
+int qvggt_cached_attention(const qvggt_cached_attention_args* args, void* stream);
 int qvggt_cached_attention_scratch(int64_t Tq, int32_t q_heads, int32_t kv_heads, int32_t requests, int32_t max_q,
                                    int64_t max_kv, int32_t head_dim, int64_t* bytes);
 

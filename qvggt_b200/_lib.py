@@ -54,14 +54,12 @@ SIGNATURES = {
     "qvggt_selftest_wait_timeout": [u64, u32p],
     "qvggt_patchify": [vp, vp, i64, i32, i32, i32, i32, C.POINTER(f32), C.POINTER(f32), vp],
     "qvggt_assemble_tokens": [vp, i64, i64, vp, i32, i32, vp, vp, i64, i32, i32, i64, vp],
-    "qvggt_rope_axes": [vp, i64, i64, vp, i64, i64, i32, vp, i64, i64, vp, i64, i64, i32, i64, i32, vp, i64, vp,
-                        C.POINTER(i32), i32, i32, i32, i32, vp],
-    "qvggt_block_plan": [vp, vp, i32, vp, i32, vp, i32, vp, i32, i32, vp, vp, vp, vp, vp, vp, vp],
-    "qvggt_kv_append": [vp, i64, i64, vp, i64, i64, i64, i32, vp, vp, i64, vp, vp, i32, i32, i32, i32, vp, i32, vp, vp,
-                        vp, i32, i32, vp],
-    "qvggt_kv_gather": [vp, vp, i64, vp, vp, i32, i32, i32, i32, vp, i64, vp, i64, i32, vp],
-    "qvggt_cached_attention": [vp, i64, i64, vp, i64, i64, vp, i64, i32, i32, vp, vp, i64, vp, vp, i32, i32, i32, i32,
-                               vp, i32, vp, vp, i32, i32, i64, i32, f32, vp, i64, vp],
+    # the argument structures come packed, as bytes (qvggt_b200/kv_cache.py)
+    "qvggt_rope_axes": [C.c_char_p, vp],
+    "qvggt_block_plan": [C.c_char_p, vp],
+    "qvggt_kv_append": [C.c_char_p, vp],
+    "qvggt_kv_gather": [C.c_char_p, vp],
+    "qvggt_cached_attention": [C.c_char_p, vp],
     "qvggt_cached_attention_scratch": [i64, i32, i32, i32, i32, i64, i32, i64p],
     "qvggt_pose_encoding_to_extri_intri": [vp, i64, i32, i32, vp, vp, vp],
     "qvggt_unproject_depth": [vp, i64, i32, i32, vp, vp, vp, vp],

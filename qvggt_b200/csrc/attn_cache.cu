@@ -569,15 +569,17 @@ Plan make_plan(int group, int kv_heads, int requests, int max_q, long long max_k
   return p;
 }
 
-int check_shape(const char* name, int64_t Tq, int32_t q_heads, int32_t kv_heads, int32_t requests, int32_t max_q,
-                int64_t max_kv, int32_t head_dim) {
+int check_shape(const char* name, int64_t Tq, int64_t q_heads, int64_t kv_heads, int64_t requests, int64_t max_q,
+                int64_t max_kv, int64_t head_dim) {
   if (Tq < 0 || requests < 0 || max_q < 0 || max_kv < 0 || q_heads <= 0 || kv_heads <= 0)
     return set_error(QVGGT_ERR_INVALID, "%s: bad shape", name);
   if (q_heads % kv_heads)
-    return set_error(QVGGT_ERR_INVALID, "%s: %d query heads do not share %d key heads evenly", name, q_heads, kv_heads);
+    return set_error(QVGGT_ERR_INVALID, "%s: %lld query heads do not share %lld key heads evenly", name,
+                     (long long)q_heads, (long long)kv_heads);
   if (head_dim != 64 && head_dim != 128)
     return set_error(QVGGT_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128", name);
-  if (Tq > 2147483647LL / q_heads || (int64_t)requests * kv_heads > 65535 || max_kv > 2147483647LL)
+  if (q_heads > 65535 || Tq > 2147483647LL / q_heads || max_q > 2147483647LL / q_heads || max_kv > 2147483647LL ||
+      requests > 1 << 24)
     return set_error(QVGGT_ERR_UNSUPPORTED, "%s: too many rows, requests or keys", name);
   return QVGGT_OK;
 }
@@ -596,77 +598,72 @@ extern "C" int qvggt_cached_attention_scratch(int64_t Tq, int32_t q_heads, int32
   return QVGGT_OK;
 }
 
-extern "C" int qvggt_cached_attention(const void* q, int64_t q_tok, int64_t q_head, void* out, int64_t o_tok,
-                                      int64_t o_head, float* lse, int64_t Tq, int32_t q_heads, int32_t dtype,
-                                      const int8_t* k_cache, const int8_t* v_cache, int64_t block_stride,
-                                      const float* k_scale, const float* v_scale, int32_t num_blocks,
-                                      int32_t kv_heads, int32_t block_size, int32_t head_dim,
-                                      const int32_t* block_tables, int32_t max_blocks, const int32_t* cu_q,
-                                      const int32_t* kv_lens, int32_t requests, int32_t max_q, int64_t max_kv,
-                                      int32_t causal_chunk, float scale, void* scratch, int64_t scratch_bytes,
-                                      void* stream) {
+extern "C" int qvggt_cached_attention(const qvggt_cached_attention_args* p, void* stream) {
   const char* name = "cached_attention";
-  if (int rc = check_shape(name, Tq, q_heads, kv_heads, requests, max_q, max_kv, head_dim)) return rc;
-  if (int rc = check_cache(name, k_cache, v_cache, k_scale, v_scale, block_stride, num_blocks, kv_heads, block_size,
-                           head_dim))
-    return rc;
-  if (dtype != QVGGT_DTYPE_F16 && dtype != QVGGT_DTYPE_BF16)
+  if (!p) return set_error(QVGGT_ERR_INVALID, "%s: null arguments", name);
+  const qvggt_kv_cache& c = p->cache;
+  if (int rc = check_shape(name, p->Tq, p->q_heads, c.kv_heads, p->requests, p->max_q, p->max_kv, c.head_dim)) return rc;
+  if (int rc = check_cache(name, c)) return rc;
+  if (p->dtype != QVGGT_DTYPE_F16 && p->dtype != QVGGT_DTYPE_BF16)
     return set_error(QVGGT_ERR_UNSUPPORTED, "%s: dtype must be fp16 or bf16", name);
-  if (causal_chunk < 0 || max_blocks < 0) return set_error(QVGGT_ERR_INVALID, "%s: bad causal_chunk or table", name);
-  if (!(scale > 0.f) || scale > 3.0e38f) return set_error(QVGGT_ERR_INVALID, "%s: scale must be positive", name);
-  if ((int64_t)max_blocks * block_size > 2147483647LL)
+  if (p->causal_chunk < 0 || p->max_blocks < 0)
+    return set_error(QVGGT_ERR_INVALID, "%s: bad causal_chunk or table", name);
+  if (!(p->scale > 1e-30) || p->scale > 1e30) return set_error(QVGGT_ERR_INVALID, "%s: scale must be positive", name);
+  if (p->max_blocks > 2147483647LL / c.block_size)
     return set_error(QVGGT_ERR_UNSUPPORTED, "%s: block tables hold more than 2^31 keys", name);
-  if (Tq == 0 || requests == 0 || max_q == 0) return QVGGT_OK;
-  if (!q || !out || !cu_q || !kv_lens || (!block_tables && max_blocks))
+  if (p->Tq == 0 || p->requests == 0 || p->max_q == 0) return QVGGT_OK;
+  if (!p->q || !p->out || !p->cu_q || !p->kv_lens || (!p->block_tables && p->max_blocks))
     return set_error(QVGGT_ERR_INVALID, "%s: null tensor", name);
-  if (!aligned16(q) || !aligned16(out) || q_tok % 8 || q_head % 8 || o_tok % 8 || o_head % 8)
+  if (!aligned16(p->q) || !aligned16(p->out) || p->q_tok % 8 || p->q_head % 8 || p->o_tok % 8 || p->o_head % 8)
     return set_error(QVGGT_ERR_ALIGN, "%s: q and out rows must be 16-byte aligned", name);
   CacheAttnArgs a{};
-  a.q = static_cast<const uint16_t*>(q);
-  a.out = static_cast<uint16_t*>(out);
-  a.lse = lse;
-  a.kc = k_cache;
-  a.vc = v_cache;
-  a.ks = k_scale;
-  a.vs = v_scale;
-  a.table = block_tables;
-  a.cu_q = cu_q;
-  a.kv_lens = kv_lens;
-  a.q_tok = q_tok;
-  a.q_head = q_head;
-  a.o_tok = o_tok;
-  a.o_head = o_head;
-  a.block_stride = block_stride;
-  a.Tq = Tq;
-  a.B = requests;
-  a.hq = q_heads;
-  a.hk = kv_heads;
-  a.group = q_heads / kv_heads;
-  a.wide = max_blocks;
-  a.num_blocks = num_blocks;
-  a.bs_log2 = block_size == 32 ? 5 : block_size == 64 ? 6 : 7;
-  a.chunk = causal_chunk;
-  a.max_q = max_q;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.out = static_cast<uint16_t*>(p->out);
+  a.lse = p->lse;
+  a.kc = c.k_cache;
+  a.vc = c.v_cache;
+  a.ks = c.k_scale;
+  a.vs = c.v_scale;
+  a.table = p->block_tables;
+  a.cu_q = p->cu_q;
+  a.kv_lens = p->kv_lens;
+  a.q_tok = p->q_tok;
+  a.q_head = p->q_head;
+  a.o_tok = p->o_tok;
+  a.o_head = p->o_head;
+  a.block_stride = c.block_stride;
+  a.Tq = p->Tq;
+  a.B = (int)p->requests;
+  a.hq = (int)p->q_heads;
+  a.hk = (int)c.kv_heads;
+  a.group = a.hq / a.hk;
+  a.wide = (int)p->max_blocks;
+  a.num_blocks = (int)c.num_blocks;
+  a.bs_log2 = c.block_size == 32 ? 5 : c.block_size == 64 ? 6 : 7;
+  a.chunk = (int)std::min<int64_t>(p->causal_chunk, 1 << 30);
+  a.max_q = (int)p->max_q;
+  a.scale_log2 = (float)(p->scale * 1.4426950408889634);
   a.ctl = make_ctl();
+  const int head_dim = (int)c.head_dim;
   // strides no TMA map takes (a broadcast or reversed query): the row kernel,
   // items whole where the scratch is laid out for the tile kernel
   const bool strided = !tiles_can_read(a);
-  Plan p = make_plan(a.group, kv_heads, requests, max_q, max_kv, head_dim, false);
-  const bool fits = !(strided && p.tiles);
+  Plan plan = make_plan(a.group, a.hk, a.B, a.max_q, p->max_kv, head_dim, false);
+  const bool fits = !(strided && plan.tiles);
   if (!fits) {
-    p = make_plan(a.group, kv_heads, requests, max_q, max_kv, head_dim, true);
-    p.scratch = 0;
+    plan = make_plan(a.group, a.hk, a.B, a.max_q, p->max_kv, head_dim, true);
+    plan.scratch = 0;
   }
-  const int64_t need = p.scratch;
-  if (need && (!scratch || scratch_bytes < need || !aligned16(scratch)))
+  if (plan.scratch && (!p->scratch || p->scratch_bytes < plan.scratch || !aligned16(p->scratch)))
     return set_error(QVGGT_ERR_INVALID, "%s: needs %lld bytes of 16-byte aligned scratch, got %lld", name,
-                     (long long)need, (long long)scratch_bytes);
-  a.row_blocks = p.row_blocks;
+                     (long long)plan.scratch, (long long)p->scratch_bytes);
+  if ((long long)a.B * plan.row_blocks > 1 << 30)
+    return set_error(QVGGT_ERR_UNSUPPORTED, "%s: too many rows", name);
+  a.row_blocks = plan.row_blocks;
   // a try_wait that fails takes about 1.4 us
   a.wait_tries = (uint32_t)std::min<unsigned long long>(1u << 26, a.ctl.timeout_ns / 1024 + 1);
-  const bool bf16 = dtype == QVGGT_DTYPE_BF16;
+  const bool bf16 = p->dtype == QVGGT_DTYPE_BF16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (p.tiles) return launch_tiles(a, head_dim, bf16, max_kv, scratch, st);
-  return with_rows(head_dim, p.nt, [&](auto k) { return k.launch(a, bf16, max_kv, fits, scratch, st); });
+  if (plan.tiles) return launch_tiles(a, head_dim, bf16, p->max_kv, p->scratch, st);
+  return with_rows(head_dim, plan.nt, [&](auto k) { return k.launch(a, bf16, p->max_kv, fits, p->scratch, st); });
 }

@@ -766,7 +766,6 @@ int launch_tiles(CacheAttnArgs& a, int D, bool bf16, long long max_kv, void* scr
   if (smem > device_info().max_smem_optin)
     return set_error(QVGGT_ERR_UNSUPPORTED, "cached_attention: shared memory %d > %d", smem,
                      device_info().max_smem_optin);
-  if ((long long)a.B * a.row_blocks > 1 << 30) return set_error(QVGGT_ERR_UNSUPPORTED, "cached_attention: too many rows");
   CUtensorMap tmQ;
   const uint64_t dims[3] = {(uint64_t)D, (uint64_t)a.hq, (uint64_t)a.Tq};
   const uint64_t strides[2] = {(uint64_t)(a.hq == 1 ? D : a.q_head) * 2,

@@ -290,19 +290,20 @@ __global__ void __launch_bounds__(GATHER_THREADS) kv_gather_kernel(GatherArgs a)
 
 }  // namespace
 
-int check_cache(const char* name, const void* kc, const void* vc, const void* ks, const void* vs, int64_t block_stride,
-                int32_t num_blocks, int32_t heads, int32_t block_size, int32_t head_dim) {
-  if (num_blocks <= 0 || heads <= 0) return set_error(QVGGT_ERR_INVALID, "%s: empty cache", name);
-  if (block_size != 32 && block_size != 64 && block_size != 128)
+int check_cache(const char* name, const qvggt_kv_cache& c) {
+  if (c.num_blocks <= 0 || c.kv_heads <= 0 || c.kv_heads > 65535)
+    return set_error(QVGGT_ERR_INVALID, "%s: bad cache shape", name);
+  if (c.block_size != 32 && c.block_size != 64 && c.block_size != 128)
     return set_error(QVGGT_ERR_UNSUPPORTED, "%s: block_size must be 32, 64 or 128", name);
-  if (head_dim != 64 && head_dim != 128)
+  if (c.head_dim != 64 && c.head_dim != 128)
     return set_error(QVGGT_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128", name);
-  if (!kc || !vc || !ks || !vs) return set_error(QVGGT_ERR_INVALID, "%s: null cache tensor", name);
-  if (!aligned16(kc) || !aligned16(vc) || block_stride % 16)
+  if (!c.k_cache || !c.v_cache || !c.k_scale || !c.v_scale)
+    return set_error(QVGGT_ERR_INVALID, "%s: null cache tensor", name);
+  if (!aligned16(c.k_cache) || !aligned16(c.v_cache) || c.block_stride % 16)
     return set_error(QVGGT_ERR_ALIGN, "%s: cache codes and their block stride must be 16-byte aligned", name);
-  if (block_stride < (int64_t)heads * block_size * head_dim)
+  if (c.block_stride < c.kv_heads * c.block_size * c.head_dim)
     return set_error(QVGGT_ERR_INVALID, "%s: block stride smaller than a block", name);
-  if ((int64_t)num_blocks * block_size > 2147483647LL)
+  if (c.num_blocks > 2147483647LL / c.block_size)
     return set_error(QVGGT_ERR_UNSUPPORTED, "%s: more than 2^31 slots", name);
   return QVGGT_OK;
 }
@@ -311,34 +312,34 @@ int check_cache(const char* name, const void* kc, const void* vc, const void* ks
 
 using namespace qv;
 
-extern "C" int qvggt_block_plan(const int32_t* cached_lens, const int32_t* target_lens, int32_t requests,
-                                int32_t* block_tables, int32_t max_blocks, int32_t* free_ring, int32_t num_blocks,
-                                const int64_t* free_range, int32_t block_size, int32_t max_new, int32_t* slots,
-                                int32_t* cu_new, int32_t* cu_blocks, int32_t* lens_out, int64_t* free_range_out,
-                                int32_t* status, void* stream) {
-  if (requests < 0 || max_blocks < 0 || num_blocks <= 0 || max_new < 0)
+extern "C" int qvggt_block_plan(const qvggt_block_plan_args* p, void* stream) {
+  if (!p || p->requests < 0 || p->max_blocks < 0 || p->num_blocks <= 0 || p->max_new < 0)
     return set_error(QVGGT_ERR_INVALID, "block_plan: bad shape");
-  if (requests > PLAN_MAX_REQUESTS)
+  if (p->requests > PLAN_MAX_REQUESTS)
     return set_error(QVGGT_ERR_UNSUPPORTED, "block_plan: at most %d requests", PLAN_MAX_REQUESTS);
-  if (block_size <= 0 || (block_size & (block_size - 1)))
+  if (p->block_size <= 0 || (p->block_size & (p->block_size - 1)))
     return set_error(QVGGT_ERR_INVALID, "block_plan: block_size must be a power of two");
-  if ((int64_t)num_blocks * block_size > 2147483647LL)
+  if (p->num_blocks > 2147483647LL / p->block_size || p->max_blocks > 2147483647LL / p->block_size ||
+      p->max_new > 2147483647LL)
     return set_error(QVGGT_ERR_UNSUPPORTED, "block_plan: more than 2^31 slots");
-  if (!free_ring || !free_range || !cu_new || !cu_blocks || !free_range_out || !status || (max_new && !slots) ||
-      (requests && (!cached_lens || !target_lens || !lens_out)) || (requests && max_blocks && !block_tables))
+  if (!p->free_ring || !p->free_range || !p->cu_new || !p->cu_blocks || !p->free_range_out || !p->status ||
+      (p->max_new && !p->slots) || (p->requests && (!p->cached_lens || !p->target_lens || !p->lens_out)) ||
+      (p->requests && p->max_blocks && !p->block_tables))
     return set_error(QVGGT_ERR_INVALID, "block_plan: null tensor");
-  if (lens_out == cached_lens || lens_out == target_lens || free_range_out == free_range)
+  if ((p->requests && (p->lens_out == p->cached_lens || p->lens_out == p->target_lens)) ||
+      p->free_range_out == p->free_range)
     return set_error(QVGGT_ERR_INVALID, "block_plan: the outputs must not be the inputs");
-  PlanArgs a{cached_lens, target_lens, block_tables, free_ring, reinterpret_cast<const long long*>(free_range),
-             slots, cu_new, cu_blocks, lens_out, status, reinterpret_cast<long long*>(free_range_out),
-             requests, max_blocks, block_size, num_blocks, max_new};
-  const int smem = 4 * (requests + 1) * (int)sizeof(int);
+  PlanArgs a{p->cached_lens, p->target_lens, p->block_tables, p->free_ring,
+             reinterpret_cast<const long long*>(p->free_range), p->slots, p->cu_new, p->cu_blocks, p->lens_out,
+             p->status, reinterpret_cast<long long*>(p->free_range_out), (int)p->requests, (int)p->max_blocks,
+             (int)p->block_size, (int)p->num_blocks, (int)p->max_new};
+  const int smem = 4 * (a.B + 1) * (int)sizeof(int);
   static DeviceFlags attr;
   if (int rc = ensure_smem(attr, block_plan_kernel, 4 * (PLAN_MAX_REQUESTS + 1) * (int)sizeof(int),
                            "cudaFuncSetAttribute(block_plan)"))
     return rc;
   const int sms = device_info().num_sms;
-  const int grid = (int)std::min<int64_t>(sms, std::max<int64_t>(1, ((int64_t)max_new + PLAN_THREADS - 1) / PLAN_THREADS));
+  const int grid = (int)std::min<int64_t>(sms, std::max<int64_t>(1, (p->max_new + PLAN_THREADS - 1) / PLAN_THREADS));
   int rc = check_cuda(launch_pdl(block_plan_kernel, dim3(grid), dim3(PLAN_THREADS), (size_t)smem,
                                  static_cast<cudaStream_t>(stream), 1u, a),
                       "block_plan launch");
@@ -346,75 +347,68 @@ extern "C" int qvggt_block_plan(const int32_t* cached_lens, const int32_t* targe
   return rc;
 }
 
-extern "C" int qvggt_kv_append(const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok,
-                               int64_t v_head, int64_t tokens, int32_t dtype, int8_t* k_cache, int8_t* v_cache, int64_t block_stride,
-                               float* k_scale, float* v_scale, int32_t num_blocks, int32_t kv_heads,
-                               int32_t block_size, int32_t head_dim, const int32_t* block_tables, int32_t max_blocks,
-                               const int32_t* cached_lens, const int32_t* cu_new, const int32_t* cu_blocks,
-                               int32_t requests, int32_t max_units, void* stream) {
-  if (int rc = check_cache("kv_append", k_cache, v_cache, k_scale, v_scale, block_stride, num_blocks, kv_heads,
-                           block_size, head_dim))
-    return rc;
-  if (dtype != QVGGT_DTYPE_F16 && dtype != QVGGT_DTYPE_BF16)
+extern "C" int qvggt_kv_append(const qvggt_kv_append_args* p, void* stream) {
+  if (!p) return set_error(QVGGT_ERR_INVALID, "kv_append: null arguments");
+  if (int rc = check_cache("kv_append", p->cache)) return rc;
+  if (p->dtype != QVGGT_DTYPE_F16 && p->dtype != QVGGT_DTYPE_BF16)
     return set_error(QVGGT_ERR_UNSUPPORTED, "kv_append: dtype must be fp16 or bf16");
-  if (tokens < 0 || requests < 0 || max_blocks < 0 || max_units < 0) return set_error(QVGGT_ERR_INVALID, "kv_append: bad shape");
-  if (tokens == 0 || requests == 0 || max_units == 0) return QVGGT_OK;
-  if (!k || !v || !block_tables || !cached_lens || !cu_new || !cu_blocks)
+  if (p->tokens < 0 || p->requests < 0 || p->max_blocks < 0 || p->max_units < 0 || p->requests > 2147483646LL ||
+      p->max_blocks > 2147483647LL || p->max_units > 2147483647LL)
+    return set_error(QVGGT_ERR_INVALID, "kv_append: bad shape");
+  if (p->tokens == 0 || p->requests == 0 || p->max_units == 0) return QVGGT_OK;
+  if (!p->k || !p->v || !p->block_tables || !p->cached_lens || !p->cu_new || !p->cu_blocks)
     return set_error(QVGGT_ERR_INVALID, "kv_append: null tensor");
-  if (!aligned16(k) || !aligned16(v) || k_tok % 8 || k_head % 8 || v_tok % 8 || v_head % 8)
+  if (!aligned16(p->k) || !aligned16(p->v) || p->k_tok % 8 || p->k_head % 8 || p->v_tok % 8 || p->v_head % 8)
     return set_error(QVGGT_ERR_ALIGN, "kv_append: k and v rows must be 16-byte aligned");
-  if (kv_heads > 65535) return set_error(QVGGT_ERR_UNSUPPORTED, "kv_append: too many heads");
   AppendArgs a{};
-  a.x[0] = static_cast<const uint16_t*>(k);
-  a.x[1] = static_cast<const uint16_t*>(v);
-  a.tok_stride[0] = k_tok;
-  a.tok_stride[1] = v_tok;
-  a.head_stride[0] = k_head;
-  a.head_stride[1] = v_head;
-  a.codes[0] = k_cache;
-  a.codes[1] = v_cache;
-  a.scales[0] = k_scale;
-  a.scales[1] = v_scale;
-  a.table = block_tables;
-  a.cached = cached_lens;
-  a.cu_new = cu_new;
-  a.cu_blocks = cu_blocks;
-  a.block_stride = block_stride;
-  a.tokens = tokens;
-  a.B = requests;
-  a.wide = max_blocks;
-  a.bs = block_size;
-  a.num_blocks = num_blocks;
-  a.heads = kv_heads;
-  a.D = head_dim;
+  a.x[0] = static_cast<const uint16_t*>(p->k);
+  a.x[1] = static_cast<const uint16_t*>(p->v);
+  a.tok_stride[0] = p->k_tok;
+  a.tok_stride[1] = p->v_tok;
+  a.head_stride[0] = p->k_head;
+  a.head_stride[1] = p->v_head;
+  a.codes[0] = p->cache.k_cache;
+  a.codes[1] = p->cache.v_cache;
+  a.scales[0] = p->cache.k_scale;
+  a.scales[1] = p->cache.v_scale;
+  a.table = p->block_tables;
+  a.cached = p->cached_lens;
+  a.cu_new = p->cu_new;
+  a.cu_blocks = p->cu_blocks;
+  a.block_stride = p->cache.block_stride;
+  a.tokens = p->tokens;
+  a.B = (int)p->requests;
+  a.wide = (int)p->max_blocks;
+  a.bs = (int)p->cache.block_size;
+  a.num_blocks = (int)p->cache.num_blocks;
+  a.heads = (int)p->cache.kv_heads;
+  a.D = (int)p->cache.head_dim;
   a.ctl = make_ctl();
-  const auto fn = dtype == QVGGT_DTYPE_BF16 ? kv_append_kernel<true> : kv_append_kernel<false>;
-  int rc = check_cuda(launch_pdl(fn, dim3(max_units, kv_heads, 2), dim3(APPEND_THREADS), 0,
+  const auto fn = p->dtype == QVGGT_DTYPE_BF16 ? kv_append_kernel<true> : kv_append_kernel<false>;
+  int rc = check_cuda(launch_pdl(fn, dim3((unsigned)p->max_units, a.heads, 2), dim3(APPEND_THREADS), 0,
                                  static_cast<cudaStream_t>(stream), 1u, a),
                       "kv_append launch");
   if (!rc) count_launch(1);
   return rc;
 }
 
-extern "C" int qvggt_kv_gather(const int8_t* k_cache, const int8_t* v_cache, int64_t block_stride,
-                               const float* k_scale, const float* v_scale, int32_t num_blocks, int32_t kv_heads,
-                               int32_t block_size, int32_t head_dim, const int32_t* slots, int64_t n, void* out,
-                               int64_t out_stride, int32_t dtype, void* stream) {
-  if (int rc = check_cache("kv_gather", k_cache, v_cache, k_scale, v_scale, block_stride, num_blocks, kv_heads,
-                           block_size, head_dim))
-    return rc;
-  if (dtype != QVGGT_DTYPE_F16 && dtype != QVGGT_DTYPE_BF16)
+extern "C" int qvggt_kv_gather(const qvggt_kv_gather_args* p, void* stream) {
+  if (!p) return set_error(QVGGT_ERR_INVALID, "kv_gather: null arguments");
+  if (int rc = check_cache("kv_gather", p->cache)) return rc;
+  if (p->dtype != QVGGT_DTYPE_F16 && p->dtype != QVGGT_DTYPE_BF16)
     return set_error(QVGGT_ERR_UNSUPPORTED, "kv_gather: dtype must be fp16 or bf16");
-  if (n < 0) return set_error(QVGGT_ERR_INVALID, "kv_gather: bad shape");
-  if (n == 0) return QVGGT_OK;
-  if (!slots || !out) return set_error(QVGGT_ERR_INVALID, "kv_gather: null tensor");
-  if (!aligned16(out) || out_stride % 8 || out_stride < 2LL * kv_heads * head_dim)
+  if (p->n < 0) return set_error(QVGGT_ERR_INVALID, "kv_gather: bad shape");
+  if (p->n == 0) return QVGGT_OK;
+  if (!p->slots || !p->out) return set_error(QVGGT_ERR_INVALID, "kv_gather: null tensor");
+  const qvggt_kv_cache& c = p->cache;
+  if (!aligned16(p->out) || p->out_stride % 8 || p->out_stride < 2 * c.kv_heads * c.head_dim)
     return set_error(QVGGT_ERR_ALIGN, "kv_gather: out rows must be 16-byte aligned and hold K and V");
-  GatherArgs a{{k_cache, v_cache}, {k_scale, v_scale}, slots, static_cast<uint16_t*>(out), out_stride, block_stride,
-               n, block_size, num_blocks, kv_heads, head_dim, make_ctl()};
-  const long long work = (n * 2 * kv_heads * (head_dim / 16) + GATHER_THREADS - 1) / GATHER_THREADS;
+  GatherArgs a{{c.k_cache, c.v_cache}, {c.k_scale, c.v_scale}, p->slots, static_cast<uint16_t*>(p->out),
+               p->out_stride, c.block_stride, p->n, (int)c.block_size, (int)c.num_blocks, (int)c.kv_heads,
+               (int)c.head_dim, make_ctl()};
+  const long long work = (p->n * 2 * a.heads * (a.D / 16) + GATHER_THREADS - 1) / GATHER_THREADS;
   const long long grid = std::min<long long>(work, 16LL * device_info().num_sms);
-  const auto fn = dtype == QVGGT_DTYPE_BF16 ? kv_gather_kernel<true> : kv_gather_kernel<false>;
+  const auto fn = p->dtype == QVGGT_DTYPE_BF16 ? kv_gather_kernel<true> : kv_gather_kernel<false>;
   int rc = check_cuda(launch_pdl(fn, dim3((unsigned)grid), dim3(GATHER_THREADS), 0,
                                  static_cast<cudaStream_t>(stream), 1u, a),
                       "kv_gather launch");

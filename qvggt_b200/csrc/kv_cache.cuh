@@ -3,6 +3,7 @@
 
 #include <algorithm>
 
+#include "../../include/qvggt_b200.h"
 #include "common.cuh"
 
 namespace qv {
@@ -32,7 +33,6 @@ __device__ __forceinline__ int8_t kv_code(float x) {
 }
 
 // Checks of the cache's tensors that every entry point makes; sets the error.
-int check_cache(const char* name, const void* kc, const void* vc, const void* ks, const void* vs, int64_t block_stride,
-                int32_t num_blocks, int32_t heads, int32_t block_size, int32_t head_dim);
+int check_cache(const char* name, const qvggt_kv_cache& c);
 
 }  // namespace qv

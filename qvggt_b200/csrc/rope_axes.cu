@@ -161,44 +161,45 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(RopeArgs a) {
 
 using namespace qv;
 
-extern "C" int qvggt_rope_axes(const void* q, int64_t q_tok, int64_t q_head, void* q_out, int64_t qo_tok,
-                               int64_t qo_head, int32_t q_heads, const void* k, int64_t k_tok, int64_t k_head,
-                               void* k_out, int64_t ko_tok, int64_t ko_head, int32_t k_heads, int64_t T,
-                               int32_t head_dim, const int32_t* positions, int64_t pos_stride, const float* inv_freq,
-                               const int32_t* sections, int32_t n_axes, int32_t layout, int32_t inverse,
-                               int32_t dtype, void* stream) {
-  if (T < 0 || q_heads < 0 || k_heads < 0 || q_heads + k_heads == 0)
+extern "C" int qvggt_rope_axes(const qvggt_rope_axes_args* p, void* stream) {
+  if (!p) return set_error(QVGGT_ERR_INVALID, "rope_axes: null arguments");
+  if (p->T < 0 || p->q_heads < 0 || p->k_heads < 0 || p->q_heads + p->k_heads == 0 || p->q_heads > 65535 ||
+      p->k_heads > 65535)
     return set_error(QVGGT_ERR_INVALID, "rope_axes: bad shape");
-  if (dtype != QVGGT_DTYPE_F16 && dtype != QVGGT_DTYPE_BF16)
+  if (p->dtype != QVGGT_DTYPE_F16 && p->dtype != QVGGT_DTYPE_BF16)
     return set_error(QVGGT_ERR_UNSUPPORTED, "rope_axes: dtype must be fp16 or bf16");
-  if (layout < 0 || layout > 2) return set_error(QVGGT_ERR_INVALID, "rope_axes: layout must be 0, 1 or 2");
-  if (n_axes < 1 || n_axes > ROPE_AXES || sections == nullptr)
+  if (p->layout < 0 || p->layout > 2) return set_error(QVGGT_ERR_INVALID, "rope_axes: layout must be 0, 1 or 2");
+  if (p->n_axes < 1 || p->n_axes > ROPE_AXES)
     return set_error(QVGGT_ERR_INVALID, "rope_axes: 1 to %d axes", ROPE_AXES);
-  if (T == 0) return QVGGT_OK;
-  if (!positions || !inv_freq || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out)))
-    return set_error(QVGGT_ERR_INVALID, "rope_axes: null tensor");
+  const int n_axes = (int)p->n_axes, layout = (int)p->layout;
+  const int64_t T = p->T, head_dim = p->head_dim, *sections = p->sections;
   RopeArgs a{};
   int pairs = 0;
   for (int x = 0; x < n_axes; ++x) {
     if (sections[x] <= 0) return set_error(QVGGT_ERR_INVALID, "rope_axes: section sizes must be positive");
-    pairs += sections[x] > ROPE_MAX_PAIRS ? ROPE_MAX_PAIRS + 1 : sections[x];
+    pairs += sections[x] > ROPE_MAX_PAIRS ? ROPE_MAX_PAIRS + 1 : (int)sections[x];
     a.sect_end[x] = pairs;
   }
   for (int x = n_axes; x < ROPE_AXES; ++x) a.sect_end[x] = pairs;
   if (pairs > ROPE_MAX_PAIRS || head_dim > 2 * ROPE_MAX_PAIRS)
     return set_error(QVGGT_ERR_UNSUPPORTED, "rope_axes: head_dim up to %d", 2 * ROPE_MAX_PAIRS);
   if (2 * pairs > head_dim)
-    return set_error(QVGGT_ERR_INVALID, "rope_axes: %d rotated pairs do not fit head_dim %d", pairs, head_dim);
-  a.s[0] = {static_cast<const uint16_t*>(q), static_cast<uint16_t*>(q_out), q_tok, q_head, qo_tok, qo_head, q_heads};
-  a.s[1] = {static_cast<const uint16_t*>(k), static_cast<uint16_t*>(k_out), k_tok, k_head, ko_tok, ko_head, k_heads};
-  a.pos = positions;
-  a.inv_freq = inv_freq;
-  a.pos_stride = pos_stride;
+    return set_error(QVGGT_ERR_INVALID, "rope_axes: %d rotated pairs do not fit head_dim %d", pairs, (int)head_dim);
+  if (T == 0) return QVGGT_OK;
+  if (!p->positions || !p->inv_freq || (p->q_heads && (!p->q || !p->q_out)) || (p->k_heads && (!p->k || !p->k_out)))
+    return set_error(QVGGT_ERR_INVALID, "rope_axes: null tensor");
+  a.s[0] = {static_cast<const uint16_t*>(p->q), static_cast<uint16_t*>(p->q_out), p->q_tok, p->q_head, p->qo_tok,
+            p->qo_head, (int)p->q_heads};
+  a.s[1] = {static_cast<const uint16_t*>(p->k), static_cast<uint16_t*>(p->k_out), p->k_tok, p->k_head, p->ko_tok,
+            p->ko_head, (int)p->k_heads};
+  a.pos = p->positions;
+  a.inv_freq = p->inv_freq;
+  a.pos_stride = p->pos_stride;
   a.T = T;
-  a.D = head_dim;
+  a.D = (int)head_dim;
   a.pairs = pairs;
   a.layout = layout;
-  a.sign = inverse ? -1.f : 1.f;
+  a.sign = p->inverse ? -1.f : 1.f;
   // Widest vector that divides every run of pairs, the pass-through tail, the
   // strides and the addresses.
   long long align = 8;
@@ -230,7 +231,7 @@ extern "C" int qvggt_rope_axes(const void* q, int64_t q_tok, int64_t q_head, voi
       {rope_axes_kernel<false, 1>, rope_axes_kernel<false, 2>, rope_axes_kernel<false, 4>, rope_axes_kernel<false, 8>},
       {rope_axes_kernel<true, 1>, rope_axes_kernel<true, 2>, rope_axes_kernel<true, 4>, rope_axes_kernel<true, 8>}};
   const int vi = align == 8 ? 3 : align == 4 ? 2 : align == 2 ? 1 : 0;
-  int rc = check_cuda(launch_pdl(fns[dtype == QVGGT_DTYPE_BF16][vi], dim3((unsigned)grid), dim3(ROPE_THREADS),
+  int rc = check_cuda(launch_pdl(fns[p->dtype == QVGGT_DTYPE_BF16][vi], dim3((unsigned)grid), dim3(ROPE_THREADS),
                                  (size_t)a.tok * pairs * sizeof(float2), static_cast<cudaStream_t>(stream), 1u, a),
                       "rope_axes launch");
   if (!rc) count_launch(1);

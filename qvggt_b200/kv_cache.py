@@ -25,6 +25,8 @@ outside its range is skipped and sets the library's status word
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import struct
 from typing import NamedTuple
 
 import torch
@@ -37,9 +39,30 @@ __all__ = ["rope_axes", "block_plan", "BlockPlan", "kv_append", "kv_gather", "ca
 
 _HALF = {torch.float16: 0, torch.bfloat16: 1}      # QVGGT_DTYPE_F16 / _BF16
 _LAYOUTS = {"axial": 0, "split": 1, "interleaved": 2}
+_I32, _F32 = torch.int32, torch.float32
 
 PLAN_STATUS = {0: "done", 1: "too few free blocks", 2: "a request needs more blocks than its table row holds",
                3: "a negative length", 4: "more new tokens than max_new"}
+
+# The argument structures of include/qvggt_b200.h: 64-bit fields only.  Packed
+# in one go: converting some thirty ctypes arguments took longer than the rest
+# of a call.
+_ROPE = struct.Struct("=27q").pack
+_PLAN = struct.Struct("=16q").pack
+_APPEND = struct.Struct("=24q").pack
+_GATHER = struct.Struct("=14q").pack
+_ATTEND = struct.Struct("=27qd2q").pack
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _run(name, dev, t, args):
+    """The C call `name` on the current stream of the tensor t's device (index dev)."""
+    if _current_device() == dev:
+        _lib.call(name, args, _stream(t))
+    else:
+        with _Dev(t.device):
+            _lib.call(name, args, _stream(t))
 
 
 def _half(name, t, what):
@@ -50,17 +73,27 @@ def _half(name, t, what):
 
 
 def _rows3(name, t, what):
-    """[tokens, heads, head_dim] with unit stride inside a head."""
-    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
-        raise ValueError(f"{name}: {what} {tuple(t.shape)} (strides {t.stride()}) must be [tokens, heads, head_dim] "
+    """[tokens, heads, head_dim] with unit stride inside a head; returns its strides."""
+    st = t.stride()
+    if len(st) != 3 or (st[2] != 1 and t.shape[2] > 1):
+        raise ValueError(f"{name}: {what} {tuple(t.shape)} (strides {st}) must be [tokens, heads, head_dim] "
                          "with unit stride in head_dim")
+    return st
 
 
 def _ints(name, t, what, shape=None):
-    if t.dtype != torch.int32 or not t.is_contiguous():
+    if t.dtype is not _I32 or not t.is_contiguous():
         raise TypeError(f"{name}: {what} must be contiguous int32, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != shape:
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name}: {what} {tuple(t.shape)} must be {shape}")
+
+
+def _table(name, t, B):
+    _ints(name, t, "block_tables")
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != B:
+        raise ValueError(f"{name}: block_tables {tuple(shape)} must be [{B}, max_blocks]")
+    return shape[1]
 
 
 # ---------------------------------------------------------------------- RoPE
@@ -77,43 +110,60 @@ def rope_axes(q, k, positions, inv_freq, sections, layout: str = "axial", invers
     of the forward turn.  Any token and head strides; fp16 or bf16; ``q_out`` /
     ``k_out`` may be q / k.  Returns (q, k) turned."""
     name = "rope_axes"
-    dev = _check_cuda(name, q, k, positions, inv_freq, q_out, k_out)
+    dev = q.get_device()
+    if dev < 0 or not dev == positions.get_device() == inv_freq.get_device():
+        _check_cuda(name, q, k, positions, inv_freq)
     dt = _half(name, q, "q")
-    _rows3(name, q, "q")
+    sq = _rows3(name, q, "q")
     T, hq, D = q.shape
-    hk = 0
-    if k is not None:
-        _rows3(name, k, "k")
-        _check_dtype(name, k, q.dtype)
-        hk = k.shape[1]
-        _check_shape(name, k.shape[0] == T and k.shape[2] == D, f"k {tuple(k.shape)} must be [{T}, heads, {D}]")
+    axes = len(sections)
     if layout not in _LAYOUTS:
         raise ValueError(f"{name}: layout must be one of {sorted(_LAYOUTS)}, got {layout!r}")
-    axes = len(sections)
-    _check_shape(name, 1 <= axes <= 4, f"1 to 4 axes, got {axes}")
-    _check_shape(name, inv_freq.dtype == torch.float32 and inv_freq.is_contiguous()
-                 and inv_freq.numel() == sum(sections), f"inv_freq must be float32 with {sum(sections)} entries")
-    _check_shape(name, positions.dtype == torch.int32 and tuple(positions.shape) == (axes, T)
-                 and (positions.stride(1) == 1 or T <= 1),
-                 f"positions {tuple(positions.shape)} must be int32 [{axes}, {T}] with unit stride in tokens")
-    outs = []
-    for x, o, what in ((q, q_out, "q_out"), (k, k_out, "k_out")):
-        if x is not None and o is None:
-            o = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        elif o is not None:
-            _rows3(name, o, what)
-            _check_dtype(name, o, x.dtype)
-            _check_shape(name, o.shape == x.shape, f"{what} {tuple(o.shape)} must be {tuple(x.shape)}")
-        outs.append(o)
-    qo, ko = outs
-    sect = (C.c_int32 * axes)(*sections)
-    with _Dev(dev):
-        _lib.call("qvggt_rope_axes", q.data_ptr(), q.stride(0), q.stride(1), qo.data_ptr(), qo.stride(0),
-                  qo.stride(1), hq, k.data_ptr() if hk else None, k.stride(0) if hk else 0,
-                  k.stride(1) if hk else 0, ko.data_ptr() if hk else None, ko.stride(0) if hk else 0,
-                  ko.stride(1) if hk else 0, hk, T, D, positions.data_ptr(), positions.stride(0),
-                  inv_freq.data_ptr(), sect, axes, _LAYOUTS[layout], 1 if inverse else 0, dt, _stream(q))
-    return qo, ko
+    if not 1 <= axes <= 4:
+        raise ValueError(f"{name}: 1 to 4 axes, got {axes}")
+    if inv_freq.dtype is not _F32 or not inv_freq.is_contiguous() or inv_freq.numel() != sum(sections):
+        raise ValueError(f"{name}: inv_freq must be float32 with {sum(sections)} entries")
+    sp = positions.stride()
+    if positions.dtype is not _I32 or positions.shape != (axes, T) or (sp[1] != 1 and T > 1):
+        raise ValueError(f"{name}: positions {tuple(positions.shape)} must be int32 [{axes}, {T}] with unit stride in "
+                         "tokens")
+    if q_out is None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        so = (hq * D, D)
+    else:
+        so = _out3(name, q_out, q, dev, "q_out")
+    if k is None:
+        tail = (0,) * 7
+        k_out = None
+    else:
+        if k.get_device() != dev:
+            _check_cuda(name, q, k)
+        sk = _rows3(name, k, "k")
+        _check_dtype(name, k, q.dtype)
+        Tk, hk, Dk = k.shape
+        if Tk != T or Dk != D:
+            raise ValueError(f"{name}: k {tuple(k.shape)} must be [{T}, heads, {D}]")
+        if k_out is None:
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+            sko = (hk * D, D)
+        else:
+            sko = _out3(name, k_out, k, dev, "k_out")
+        tail = (k.data_ptr(), sk[0], sk[1], k_out.data_ptr(), sko[0], sko[1], hk)
+    _run("qvggt_rope_axes", dev, q,
+         _ROPE(q.data_ptr(), sq[0], sq[1], q_out.data_ptr(), so[0], so[1], hq, *tail, T, D, positions.data_ptr(), sp[0],
+               inv_freq.data_ptr(), *sections, *(0,) * (4 - axes), axes, _LAYOUTS[layout], 1 if inverse else 0, dt))
+    return q_out, k_out
+
+
+def _out3(name, out, like, dev, what):
+    """Strides of a given output that has to match `like`."""
+    if out.get_device() != dev:
+        _check_cuda(name, like, out)
+    st = _rows3(name, out, what)
+    _check_dtype(name, out, like.dtype)
+    if out.shape != like.shape:
+        raise ValueError(f"{name}: {what} {tuple(out.shape)} must be {tuple(like.shape)}")
+    return st
 
 
 # -------------------------------------------------------------- block tables
@@ -139,41 +189,40 @@ def block_plan(cached_lens, target_lens, block_tables, free_ring, free_range, bl
     returned; if a request cannot be served nothing is changed and ``status``
     says why.  ``max_new`` bounds the new tokens."""
     name = "block_plan"
-    dev = _check_cuda(name, cached_lens, target_lens, block_tables, free_ring, free_range)
+    dev = cached_lens.get_device()
+    if dev < 0 or not (dev == target_lens.get_device() == block_tables.get_device() == free_ring.get_device()
+                       == free_range.get_device()):
+        _check_cuda(name, cached_lens, target_lens, block_tables, free_ring, free_range)
     _ints(name, cached_lens, "cached_lens")
     B = cached_lens.numel()
     _ints(name, target_lens, "target_lens", (B,))
-    _ints(name, block_tables, "block_tables")
+    wide = _table(name, block_tables, B)
     _ints(name, free_ring, "free_ring")
-    _check_shape(name, block_tables.dim() == 2 and block_tables.shape[0] == B,
-                 f"block_tables {tuple(block_tables.shape)} must be [{B}, max_blocks]")
-    _check_shape(name, free_range.dtype == torch.int64 and free_range.is_contiguous() and free_range.numel() == 2,
-                 "free_range must be int64 [2]")
+    if free_range.dtype is not torch.int64 or not free_range.is_contiguous() or free_range.numel() != 2:
+        raise ValueError(f"{name}: free_range must be int64 [2]")
     # one allocation: the 64-bit pair first, then the 32-bit arrays
-    buf = torch.empty(4 + 3 * B + 3 + max_new, dtype=torch.int32, device=dev)
-    free_out = buf[:4].view(torch.int64)
-    cu_new, cu_blocks, lens, status, slots = buf[4:].split_with_sizes([B + 1, B + 1, B, 1, max_new])
+    buf = cached_lens.new_empty(3 * B + 7 + max_new)
+    free_out, cu_new, cu_blocks, lens, status, slots = buf.split_with_sizes([4, B + 1, B + 1, B, 1, max_new])
     at = buf.data_ptr()
-    with _Dev(dev):
-        _lib.call("qvggt_block_plan", cached_lens.data_ptr(), target_lens.data_ptr(), B, block_tables.data_ptr(),
-                  block_tables.shape[1], free_ring.data_ptr(), free_ring.numel(), free_range.data_ptr(), block_size,
-                  max_new, at + 4 * (3 * B + 7), at + 16, at + 4 * (B + 5), at + 4 * (2 * B + 6), at,
-                  at + 4 * (3 * B + 6), _stream(cached_lens))
-    return BlockPlan(slots, cu_new, cu_blocks, lens, free_out, status)
+    _run("qvggt_block_plan", dev, buf,
+         _PLAN(cached_lens.data_ptr(), target_lens.data_ptr(), B, block_tables.data_ptr(), wide, free_ring.data_ptr(),
+               free_ring.numel(), free_range.data_ptr(), block_size, max_new, at + 12 * B + 28, at + 16,
+               at + 4 * B + 20, at + 8 * B + 24, at, at + 12 * B + 24))
+    return BlockPlan(slots, cu_new, cu_blocks, lens, free_out.view(torch.int64), status)
 
 
 # --------------------------------------------------------------------- cache
 def _check_cache(name, k_cache, v_cache, k_scale, v_scale):
     """Cache tensors -> (num_blocks, kv_heads, block_size, head_dim)."""
-    if k_cache.dim() != 4 or k_cache.dtype != torch.int8 or v_cache.dtype != torch.int8:
+    shape, st = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or k_cache.dtype is not torch.int8 or v_cache.dtype is not torch.int8:
         raise TypeError(f"{name}: the caches must be int8 [num_blocks, kv_heads, block_size, head_dim]")
-    nb, h, bs, d = k_cache.shape
-    inner = (bs * d, d, 1)
-    if v_cache.shape != k_cache.shape or k_cache.stride()[1:] != inner or v_cache.stride() != k_cache.stride():
+    nb, h, bs, d = shape
+    if v_cache.shape != shape or st[1:] != (bs * d, d, 1) or v_cache.stride() != st:
         raise ValueError(f"{name}: K and V caches must have the same shape and strides, dense inside a block")
-    for s, what in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        if s.dtype != torch.float32 or tuple(s.shape) != (nb, h) or not s.is_contiguous():
-            raise ValueError(f"{name}: {what} must be contiguous float32 [{nb}, {h}]")
+    if (k_scale.dtype is not _F32 or v_scale.dtype is not _F32 or k_scale.shape != (nb, h) or v_scale.shape != (nb, h)
+            or not k_scale.is_contiguous() or not v_scale.is_contiguous()):
+        raise ValueError(f"{name}: k_scale and v_scale must be contiguous float32 [{nb}, {h}]")
     return nb, h, bs, d
 
 
@@ -188,59 +237,69 @@ def kv_append(k, v, k_cache, v_cache, k_scale, v_scale, block_tables, cached_len
     bound of ``cu_blocks[-1]`` if one tighter than ``tokens // block_size + 2
     * B`` is known."""
     name = "kv_append"
-    dev = _check_cuda(name, k, v, k_cache, v_cache, k_scale, v_scale, block_tables, cached_lens, cu_new, cu_blocks)
+    dev = k.get_device()
+    if dev < 0 or not (dev == v.get_device() == k_cache.get_device() == v_cache.get_device() == k_scale.get_device()
+                       == v_scale.get_device() == block_tables.get_device() == cached_lens.get_device()
+                       == cu_new.get_device() == cu_blocks.get_device()):
+        _check_cuda(name, k, v, k_cache, v_cache, k_scale, v_scale, block_tables, cached_lens, cu_new, cu_blocks)
     nb, h, bs, d = _check_cache(name, k_cache, v_cache, k_scale, v_scale)
     dt = _half(name, k, "k")
     _check_dtype(name, v, k.dtype)
-    _rows3(name, k, "k")
-    _rows3(name, v, "v")
-    T = k.shape[0]
-    _check_shape(name, tuple(k.shape) == (T, h, d) and v.shape == k.shape,
-                 f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [tokens, {h}, {d}]")
+    sk, sv = _rows3(name, k, "k"), _rows3(name, v, "v")
+    shape = k.shape
+    T = shape[0]
+    if shape != (T, h, d) or v.shape != shape:
+        raise ValueError(f"{name}: k {tuple(shape)} and v {tuple(v.shape)} must be [tokens, {h}, {d}]")
     B = cached_lens.numel()
-    _ints(name, block_tables, "block_tables")
+    wide = _table(name, block_tables, B)
     _ints(name, cached_lens, "cached_lens")
     _ints(name, cu_new, "cu_new", (B + 1,))
     _ints(name, cu_blocks, "cu_blocks", (B + 1,))
-    _check_shape(name, block_tables.dim() == 2 and block_tables.shape[0] == B,
-                 f"block_tables {tuple(block_tables.shape)} must be [{B}, max_blocks]")
     if max_units is None:
         max_units = T // bs + 2 * B
-    with _Dev(dev):
-        _lib.call("qvggt_kv_append", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                  T, dt, k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_scale.data_ptr(),
-                  v_scale.data_ptr(), nb, h, bs, d, block_tables.data_ptr(), block_tables.shape[1],
-                  cached_lens.data_ptr(), cu_new.data_ptr(), cu_blocks.data_ptr(), B, max_units, _stream(k))
+    _run("qvggt_kv_append", dev, k,
+         _APPEND(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_scale.data_ptr(), v_scale.data_ptr(), nb,
+                 h, bs, d, k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], T, dt, block_tables.data_ptr(), wide,
+                 cached_lens.data_ptr(), cu_new.data_ptr(), cu_blocks.data_ptr(), B, max_units))
 
 
 def kv_gather(k_cache, v_cache, k_scale, v_scale, slots, dtype=torch.float16, out=None):
     """The cache rows of ``slots`` (int32 ``[n]``) as ``[n, 2 * kv_heads * head_dim]`` rows ``[k | v]``, the layout
     :func:`~qvggt_b200.awq_inference_engine.attention` reads; a negative slot gives zeros."""
     name = "kv_gather"
-    dev = _check_cuda(name, k_cache, v_cache, k_scale, v_scale, slots, out)
+    dev = slots.get_device()
+    if dev < 0 or not (dev == k_cache.get_device() == v_cache.get_device() == k_scale.get_device()
+                       == v_scale.get_device()):
+        _check_cuda(name, k_cache, v_cache, k_scale, v_scale, slots)
     nb, h, bs, d = _check_cache(name, k_cache, v_cache, k_scale, v_scale)
     _ints(name, slots, "slots")
     n = slots.numel()
     if out is None:
-        out = torch.empty(n, 2 * h * d, dtype=dtype, device=dev)
-    _check_shape(name, out.dim() == 2 and tuple(out.shape) == (n, 2 * h * d) and out.stride(1) == 1,
-                 f"out {tuple(out.shape)} must be [{n}, {2 * h * d}]")
+        out = slots.new_empty((n, 2 * h * d), dtype=dtype)
+    elif out.get_device() != dev:
+        _check_cuda(name, slots, out)
+    if out.shape != (n, 2 * h * d) or out.stride()[1] != 1:
+        raise ValueError(f"{name}: out {tuple(out.shape)} must be [{n}, {2 * h * d}]")
     dt = _half(name, out, "out")
-    with _Dev(dev):
-        _lib.call("qvggt_kv_gather", k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_scale.data_ptr(),
-                  v_scale.data_ptr(), nb, h, bs, d, slots.data_ptr(), n, out.data_ptr(), out.stride(0), dt,
-                  _stream(slots))
+    _run("qvggt_kv_gather", dev, slots,
+         _GATHER(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_scale.data_ptr(), v_scale.data_ptr(), nb,
+                 h, bs, d, slots.data_ptr(), n, out.data_ptr(), out.stride(0), dt))
     return out
 
 
 # ----------------------------------------------------------------- attention
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(dev, *sizes):
+    nb = C.c_int64(0)
+    with torch.cuda.device(dev):
+        _lib.call("qvggt_cached_attention_scratch", *sizes, C.byref(nb))
+    return int(nb.value)
+
+
 def attention_scratch_bytes(tokens: int, q_heads: int, kv_heads: int, requests: int, max_q: int, max_kv: int,
                             head_dim: int) -> int:
     """Scratch :func:`cached_attention` needs for these sizes on the current device."""
-    nb = C.c_int64(0)
-    _lib.call("qvggt_cached_attention_scratch", tokens, q_heads, kv_heads, requests, max_q, max_kv, head_dim,
-              C.byref(nb))
-    return int(nb.value)
+    return _scratch_bytes(_current_device(), tokens, q_heads, kv_heads, requests, max_q, max_kv, head_dim)
 
 
 def cached_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, cu_q, kv_lens, max_q: int, max_kv: int,
@@ -258,42 +317,51 @@ def cached_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, cu_q, 
     to be filled.  ``scratch``: uint8, at least :func:`attention_scratch_bytes`
     (allocated here if None).  Returns ``out`` ``[tokens, Hq, head_dim]``."""
     name = "cached_attention"
-    dev = _check_cuda(name, q, k_cache, v_cache, k_scale, v_scale, block_tables, cu_q, kv_lens, out, lse, scratch)
+    dev = q.get_device()
+    if dev < 0 or not (dev == k_cache.get_device() == v_cache.get_device() == k_scale.get_device()
+                       == v_scale.get_device() == block_tables.get_device() == cu_q.get_device()
+                       == kv_lens.get_device()):
+        _check_cuda(name, q, k_cache, v_cache, k_scale, v_scale, block_tables, cu_q, kv_lens)
     nb, hk, bs, d = _check_cache(name, k_cache, v_cache, k_scale, v_scale)
     dt = _half(name, q, "q")
-    _rows3(name, q, "q")
+    sq = _rows3(name, q, "q")
     T, hq, dq = q.shape
-    _check_shape(name, dq == d, f"q has head_dim {dq}, the cache {d}")
+    if dq != d:
+        raise ValueError(f"{name}: q has head_dim {dq}, the cache {d}")
     B = kv_lens.numel()
-    _ints(name, block_tables, "block_tables")
+    wide = _table(name, block_tables, B)
     _ints(name, cu_q, "cu_q", (B + 1,))
     _ints(name, kv_lens, "kv_lens")
-    _check_shape(name, block_tables.dim() == 2 and block_tables.shape[0] == B,
-                 f"block_tables {tuple(block_tables.shape)} must be [{B}, max_blocks]")
     if out is None:
-        out = torch.empty((T, hq, d), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        so = (hq * d, d)
     else:
-        _rows3(name, out, "out")
-        _check_dtype(name, out, q.dtype)
-        _check_shape(name, out.shape == q.shape, f"out {tuple(out.shape)} must be {tuple(q.shape)}")
-    if lse is not None:
-        _check_shape(name, lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (hq, T),
+        so = _out3(name, out, q, dev, "out")
+    if lse is None:
+        lse_at = 0
+    else:
+        if lse.get_device() != dev:
+            _check_cuda(name, q, lse)
+        _check_shape(name, lse.dtype is _F32 and lse.is_contiguous() and lse.shape == (hq, T),
                      f"lse must be contiguous float32 [{hq}, {T}]")
-    with _Dev(dev):
-        nbytes = attention_scratch_bytes(T, hq, hk, B, max_q, max_kv, d)
-        if scratch is None:
-            if nbytes:
-                scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        else:
-            _check_shape(name, scratch.dtype == torch.uint8 and scratch.is_contiguous() and scratch.numel() >= nbytes,
-                         f"scratch must be a contiguous uint8 tensor of >= {nbytes} bytes")
-        _lib.call("qvggt_cached_attention", q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
-                  out.stride(1), None if lse is None else lse.data_ptr(), T, hq, dt, k_cache.data_ptr(),
-                  v_cache.data_ptr(), k_cache.stride(0), k_scale.data_ptr(), v_scale.data_ptr(), nb, hk, bs, d,
-                  block_tables.data_ptr(), block_tables.shape[1], cu_q.data_ptr(), kv_lens.data_ptr(), B, max_q,
-                  max_kv, causal_chunk, d ** -0.5 if scale is None else float(scale),
-                  None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel(),
-                  _stream(q))
+        lse_at = lse.data_ptr()
+    nbytes = _scratch_bytes(dev, T, hq, hk, B, max_q, max_kv, d)
+    scratch_at = scratch_len = 0
+    if scratch is not None:
+        if scratch.get_device() != dev:
+            _check_cuda(name, q, scratch)
+        scratch_len = scratch.numel()
+        _check_shape(name, scratch.dtype is torch.uint8 and scratch.is_contiguous() and scratch_len >= nbytes,
+                     f"scratch must be a contiguous uint8 tensor of >= {nbytes} bytes")
+        scratch_at = scratch.data_ptr()
+    elif nbytes:
+        scratch = q.new_empty(nbytes, dtype=torch.uint8)
+        scratch_at, scratch_len = scratch.data_ptr(), nbytes
+    _run("qvggt_cached_attention", dev, q,
+         _ATTEND(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_scale.data_ptr(), v_scale.data_ptr(), nb,
+                 hk, bs, d, q.data_ptr(), sq[0], sq[1], out.data_ptr(), so[0], so[1], lse_at, T, hq, dt,
+                 block_tables.data_ptr(), wide, cu_q.data_ptr(), kv_lens.data_ptr(), B, max_q, max_kv, causal_chunk,
+                 d ** -0.5 if scale is None else scale, scratch_at, scratch_len))
     return out
 
 

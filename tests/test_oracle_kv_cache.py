@@ -175,14 +175,46 @@ def test_library_refuses_bad_arguments_without_a_gpu():
                        ((-1, 4, 4, 1, 8, 64, 64), b"shape")]:
         assert lib.qvggt_cached_attention_scratch(*args, n) in (1, 2)
         assert word in lib.qvggt_last_error()
-    assert lib.qvggt_block_plan(None, None, 9000, None, 1, None, 8, None, 32, 0, None, None, None, None, None, None,
-                                None) == 2
-    assert lib.qvggt_block_plan(None, None, 1, None, 1, None, 8, None, 33, 0, None, None, None, None, None, None,
-                                None) == 1
-    sect = (_lib.i32 * 1)(40)
-    assert lib.qvggt_rope_axes(1, 64, 64, 1, 64, 64, 1, None, 0, 0, None, 0, 0, 0, 4, 64, 1, 4, 1, sect, 1, 0, 0, 0,
-                               None) == 1
-    assert b"fit" in lib.qvggt_last_error()
-    assert lib.qvggt_kv_append(16, 64, 64, 16, 64, 64, 1, 0, 16, 16, 4096, 16, 16, 4, 1, 48, 64, 16, 1, 16, 16, 16, 1,
-                               1, None) == 2
-    assert lib.qvggt_kv_gather(16, 16, 100, 16, 16, 4, 1, 32, 64, 16, 1, 16, 128, 0, None) == 5
+    plan = lambda requests, bs: kc._PLAN(0, 0, requests, 0, 1, 0, 8, 0, bs, 0, 0, 0, 0, 0, 0, 0)
+    assert lib.qvggt_block_plan(plan(9000, 32), None) == 2
+    assert lib.qvggt_block_plan(plan(1, 33), None) == 1
+    assert lib.qvggt_block_plan(plan(1, 32), None) == 1 and b"null" in lib.qvggt_last_error()
+    rope = lambda pairs, dtype: kc._ROPE(16, 64, 64, 16, 64, 64, 1, *(0,) * 7, 4, 64, 16, 4, 16, pairs, 0, 0, 0, 1, 0,
+                                         0, dtype)
+    assert lib.qvggt_rope_axes(rope(40, 0), None) == 1 and b"fit" in lib.qvggt_last_error()
+    assert lib.qvggt_rope_axes(rope(32, 2), None) == 2
+    cache = lambda bs, stride: (16, 16, stride, 16, 16, 4, 1, bs, 64)
+    assert lib.qvggt_kv_append(kc._APPEND(*cache(48, 4096), 16, 64, 64, 16, 64, 64, 1, 0, 16, 1, 16, 16, 16, 1, 1),
+                               None) == 2
+    assert lib.qvggt_kv_gather(kc._GATHER(*cache(32, 2056), 16, 1, 16, 128, 0), None) == 5
+    attend = lambda scale, chunk: kc._ATTEND(*cache(32, 2048), 16, 64, 64, 16, 64, 64, 0, 1, 1, 0, 16, 1, 16, 16, 1, 1,
+                                             32, chunk, scale, 0, 0)
+    for args, word in [((0.0, 0), b"scale"), ((float("nan"), 0), b"scale"), ((0.1, -1), b"chunk")]:
+        assert lib.qvggt_cached_attention(attend(*args), None) == 1 and word in lib.qvggt_last_error()
+
+
+def test_packed_structures_match_the_header():
+    """Every field of the header's argument structures is 64 bits wide, so their number is the packed size."""
+    import os
+    import re
+    hdr = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include",
+                            "qvggt_b200.h")).read()
+    hdr = re.sub(r"/\*.*?\*/", "", hdr, flags=re.S)
+    fields = {}
+    for body, name in re.findall(r"typedef struct \{(.*?)\} (qvggt_\w+);", hdr, flags=re.S):
+        n = 0
+        for decl in body.split(";"):
+            decl = " ".join(decl.split())
+            if not decl:
+                continue
+            if decl.startswith("qvggt_kv_cache"):
+                n += fields["qvggt_kv_cache"]
+                continue
+            assert "*" in decl or decl.startswith(("int64_t", "double")), decl
+            for item in decl.split(","):
+                m = re.search(r"\[(\d+)\]", item)
+                n += int(m.group(1)) if m else 1
+        fields[name] = n
+    for name, pack in [("rope_axes", kc._ROPE), ("block_plan", kc._PLAN), ("kv_append", kc._APPEND),
+                       ("kv_gather", kc._GATHER), ("cached_attention", kc._ATTEND)]:
+        assert fields[f"qvggt_{name}_args"] * 8 == pack.__self__.size, name
