@@ -174,7 +174,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(PlanArgs a) {
 }
 
 // ------------------------------------------------------------------ append
-constexpr int APPEND_THREADS = 128;
+constexpr int APPEND_SIDE = 128;          // threads for K, and as many for V
+constexpr int APPEND_THREADS = 2 * APPEND_SIDE;
 
 struct AppendArgs {
   const uint16_t* x[2];                  // K, V: [tokens][heads][D], unit stride in D
@@ -188,49 +189,138 @@ struct AppendArgs {
   Ctl ctl;
 };
 
-// One CTA per (written block, head, K or V): the new rows' largest magnitude,
-// the block's scale, the codes.
+// Largest i in [0, n) with a[i] <= x, a whole warp looking at 32 places at a time.
+__device__ __forceinline__ int warp_last_le(const int32_t* a, int n, int x) {
+  const int lane = threadIdx.x % 32;
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int at = lane * step;
+    const unsigned le = __ballot_sync(~0u, at < n && a[lo + at] <= x);
+    const int k = 31 - __clz(le);        // a[lo] <= x always
+    lo += k * step;
+    n = min(step, n - k * step);
+  }
+  return lo;
+}
+
+// Four codes of x * inv.  Adding 1.5 * 2^23 rounds to the nearest integer,
+// ties to even, and leaves it in the low byte: two instructions an element
+// where a conversion would go through the 16-a-clock pipe.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inv) {
+  const float M = 12582912.f;
+  const uint32_t x = __byte_perm(__float_as_uint(__fadd_rn(__fmul_rn(a, inv), M)),
+                                 __float_as_uint(__fadd_rn(__fmul_rn(b, inv), M)), 0x0040);
+  const uint32_t y = __byte_perm(__float_as_uint(__fadd_rn(__fmul_rn(c, inv), M)),
+                                 __float_as_uint(__fadd_rn(__fmul_rn(d, inv), M)), 0x0040);
+  return __byte_perm(x, y, 0x5410);
+}
+__device__ __forceinline__ uint32_t codes4_any(float a, float b, float c, float d, float inv) {
+  return (uint32_t)(uint8_t)kv_code(a * inv) | (uint32_t)(uint8_t)kv_code(b * inv) << 8 |
+         (uint32_t)(uint8_t)kv_code(c * inv) << 16 | (uint32_t)(uint8_t)kv_code(d * inv) << 24;
+}
+
 template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t u) {
+  return BF16 ? unpack_bf162(u) : unpack_half2(u);
+}
+
+// One CTA per (written block, head): half the threads for K, half for V.  The
+// new rows are read once, all loads of a thread at once, and stay in registers
+// (NV 16-byte pieces a thread) while the largest magnitude is found; then the
+// scale, the codes.  Bound by memory: 2 bytes in and 1 out per element.
+template <bool BF16, int NV>
 __global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(AppendArgs a) {
-  __shared__ float red[APPEND_THREADS / 32];
+  __shared__ uint32_t red[APPEND_THREADS / 32];
+  constexpr uint32_t INF = BF16 ? 0x7f80u : 0x7c00u;
   pdl_wait();
   pdl_trigger();
-  const int unit = blockIdx.x, h = blockIdx.y, side = blockIdx.z;
+  const int unit = blockIdx.x, h = blockIdx.y, side = threadIdx.x / APPEND_SIDE, th = threadIdx.x % APPEND_SIDE;
   if (unit >= a.cu_blocks[a.B]) return;
-  const int b = last_le(a.cu_blocks, a.B, unit);
+  const int b = warp_last_le(a.cu_blocks, a.B, unit);
   const int c = a.cached[b], n0 = a.cu_new[b], end = c + a.cu_new[b + 1] - n0;
   const int j = c / a.bs + unit - a.cu_blocks[b];
   const int lo = max(c, j * a.bs), hi = min(end, (j + 1) * a.bs);      // new tokens of the block
   const int blk = j < a.wide ? a.table[(long long)b * a.wide + j] : -1;
-  if (c < 0 || n0 < 0 || hi <= lo || (long long)n0 + end - c > a.tokens || blk < 0 || blk >= a.num_blocks) {
-    if (threadIdx.x == 0) report_status(a.ctl, c < 0 || hi <= lo ? ST_BAD_LENGTH : ST_BAD_BLOCK);
+  const bool lengths = c >= 0 && n0 >= 0 && hi > lo && (long long)n0 + end - c <= a.tokens;
+  const int per_row = a.D / 8, pieces = lengths ? (hi - lo) * per_row : 0;
+  const uint16_t* x = a.x[side] + (long long)(n0 + lo - c) * a.tok_stride[side] + h * a.head_stride[side];
+  uint4 v[NV];
+  uint32_t m = 0;                        // magnitudes of two elements, as integers
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int p = th + i * APPEND_SIDE;
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (p < pieces) {
+      const int r = p / per_row;
+      v[i] = __ldg(reinterpret_cast<const uint4*>(x + r * a.tok_stride[side] + (p - r * per_row) * 8));
+    }
+  }
+  if (!lengths || blk < 0 || blk >= a.num_blocks) {
+    if (threadIdx.x == 0) report_status(a.ctl, lengths ? ST_BAD_BLOCK : ST_BAD_LENGTH);
     return;
   }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = __vmaxu2(m, w[e] & 0x7fff7fffu);
+  }
   const int older = lo - j * a.bs;                                     // earlier tokens of the block
-  const uint16_t* x = a.x[side] + (n0 + lo - c) * a.tok_stride[side] + h * a.head_stride[side];
   int8_t* codes = a.codes[side] + blk * a.block_stride + (long long)h * a.bs * a.D;
   float* scale = a.scales[side] + (long long)blk * a.heads + h;
-  const int total = (hi - lo) * a.D;
-  float m = 0.f;
-  for (int i = threadIdx.x; i < total; i += APPEND_THREADS) {
-    const float v = fabsf(half_bits_to_f32<BF16>(x[(i / a.D) * a.tok_stride[side] + i % a.D]));
-    if (v <= 3.4028235e38f) m = fmaxf(m, v);                           // finite values only
-  }
-  m = warp_max(m);
-  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float before = older > 0 ? *scale : 0.f;
-  const float s = fmaxf(fmaxf(before, __fdiv_rn(m, 127.f)), KV_SCALE_MIN);
-  const float inv = __frcp_rn(s);
-  __syncthreads();                                                     // everyone has read the old scale
-  if (threadIdx.x == 0) *scale = s;
-  if (older > 0 && s != before) {
-    const float r = before * inv;
-    for (int i = threadIdx.x; i < older * a.D; i += APPEND_THREADS) codes[i] = kv_code((float)codes[i] * r);
+  m = __reduce_max_sync(~0u, max(m & 0xffffu, m >> 16));
+  if (th % 32 == 0) red[threadIdx.x / 32] = m;
+  __syncthreads();
+  const uint32_t* r4 = red + side * (APPEND_SIDE / 32);
+  m = max(max(r4[0], r4[1]), max(r4[2], r4[3]));
+  const bool odd = m >= INF;             // an infinity or NaN among them
+  if (odd) {
+    // the largest finite magnitude instead (both halves of the CTA pass this barrier or neither)
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t l = w[e] & 0x7fffu, u = (w[e] >> 16) & 0x7fffu;
+        m = max(m, max(l < INF ? l : 0u, u < INF ? u : 0u));
+      }
+    }
+    m = __reduce_max_sync(~0u, m);
   }
-  for (int i = threadIdx.x; i < total; i += APPEND_THREADS)
-    codes[older * a.D + i] = kv_code(half_bits_to_f32<BF16>(x[(i / a.D) * a.tok_stride[side] + i % a.D]) * inv);
+  if (__syncthreads_or(odd)) {
+    if (odd && th % 32 == 0) red[threadIdx.x / 32] = m;
+    __syncthreads();
+    if (odd) m = max(max(r4[0], r4[1]), max(r4[2], r4[3]));
+  }
+  const float s = fmaxf(fmaxf(before, __fdiv_rn(half_bits_to_f32<BF16>((uint16_t)m), 127.f)), KV_SCALE_MIN);
+  const float inv = __frcp_rn(s);
+  if (th == 0) *scale = s;               // (everyone read the old one before the barriers)
+  if (older > 0 && s != before) {
+    const float f = before * inv;
+    uint4* old = reinterpret_cast<uint4*>(codes);
+    for (int i = th; i < older * a.D / 16; i += APPEND_SIDE) {
+      uint4 q = old[i];
+      uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = codes4_any((float)(int8_t)w[e], (float)(int8_t)(w[e] >> 8), (float)(int8_t)(w[e] >> 16),
+                          (float)(int8_t)(w[e] >> 24), f);
+      old[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  uint2* out = reinterpret_cast<uint2*>(codes + older * a.D);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int p = th + i * APPEND_SIDE;
+    if (p >= pieces) continue;
+    const float2 p0 = unpack2<BF16>(v[i].x), p1 = unpack2<BF16>(v[i].y), p2 = unpack2<BF16>(v[i].z),
+                 p3 = unpack2<BF16>(v[i].w);
+    out[p] = odd ? make_uint2(codes4_any(p0.x, p0.y, p1.x, p1.y, inv), codes4_any(p2.x, p2.y, p3.x, p3.y, inv))
+                 : make_uint2(codes4(p0.x, p0.y, p1.x, p1.y, inv), codes4(p2.x, p2.y, p3.x, p3.y, inv));
+  }
 }
 
 // ------------------------------------------------------------------ gather
@@ -242,7 +332,7 @@ struct GatherArgs {
   const int32_t* slots;
   uint16_t* out;                         // [n][2][heads][D], rows of out_stride
   long long out_stride, block_stride, n;
-  int bs, num_blocks, heads, D;
+  int bs, bs_log2, num_blocks, heads, D;
   Ctl ctl;
 };
 
@@ -261,19 +351,21 @@ __global__ void __launch_bounds__(GATHER_THREADS) kv_gather_kernel(GatherArgs a)
     const int slot = a.slots[row];
     uint4 o[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
     if (slot >= 0) {
-      const int blk = slot / a.bs;
+      const int blk = slot >> a.bs_log2;
       if (blk < a.num_blocks) {
-        const int8_t* src = a.codes[side] + blk * a.block_stride +
-                            ((long long)h * a.bs + (slot - blk * a.bs)) * a.D + part * 16;
+        const int8_t* src = (side ? a.codes[1] : a.codes[0]) + blk * a.block_stride +
+                            ((long long)h * a.bs + (slot & (a.bs - 1))) * a.D + part * 16;
         const uint4 c = *reinterpret_cast<const uint4*>(src);
-        const float s = a.scales[side][(long long)blk * a.heads + h];
+        const float s = (side ? a.scales[1] : a.scales[0])[(long long)blk * a.heads + h];
         const uint32_t w[4] = {c.x, c.y, c.z, c.w};
         uint32_t r[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const uint32_t u = w[k / 2] >> (16 * (k & 1));
-          const float x0 = (float)(int8_t)u * s, x1 = (float)(int8_t)(u >> 8) * s;
-          r[k] = BF16 ? pack_bf162(x0, x1) : pack_half2(x0, x1);
+          // the code as a float: its byte, sign bit flipped, under the exponent of 2^23
+          const uint32_t f = w[k / 2] ^ 0x80808080u;
+          const float x0 = __uint_as_float(__byte_perm(f, 0x4b000000u, k & 1 ? 0x7442 : 0x7440)) - 8388736.f;
+          const float x1 = __uint_as_float(__byte_perm(f, 0x4b000000u, k & 1 ? 0x7443 : 0x7441)) - 8388736.f;
+          r[k] = BF16 ? pack_bf162(x0 * s, x1 * s) : pack_half2(x0 * s, x1 * s);
         }
         o[0] = make_uint4(r[0], r[1], r[2], r[3]);
         o[1] = make_uint4(r[4], r[5], r[6], r[7]);
@@ -281,8 +373,7 @@ __global__ void __launch_bounds__(GATHER_THREADS) kv_gather_kernel(GatherArgs a)
         report_bad_block(a.ctl);
       }
     }
-    uint4* dst = reinterpret_cast<uint4*>(a.out + row * a.out_stride + (long long)side * a.heads * a.D + h * a.D +
-                                          part * 16);
+    uint4* dst = reinterpret_cast<uint4*>(a.out + row * a.out_stride + (long long)rem * 16);
     dst[0] = o[0];
     dst[1] = o[1];
   }
@@ -384,8 +475,13 @@ extern "C" int qvggt_kv_append(const qvggt_kv_append_args* p, void* stream) {
   a.heads = (int)p->cache.kv_heads;
   a.D = (int)p->cache.head_dim;
   a.ctl = make_ctl();
-  const auto fn = p->dtype == QVGGT_DTYPE_BF16 ? kv_append_kernel<true> : kv_append_kernel<false>;
-  int rc = check_cuda(launch_pdl(fn, dim3((unsigned)p->max_units, a.heads, 2), dim3(APPEND_THREADS), 0,
+  using Kfn = void (*)(AppendArgs);
+  static const Kfn fns[2][4] = {
+      {kv_append_kernel<false, 2>, kv_append_kernel<false, 4>, kv_append_kernel<false, 8>, kv_append_kernel<false, 16>},
+      {kv_append_kernel<true, 2>, kv_append_kernel<true, 4>, kv_append_kernel<true, 8>, kv_append_kernel<true, 16>}};
+  const int nv = a.bs * a.D / 8 / APPEND_SIDE;             // 2, 4, 8 or 16 pieces a thread
+  int rc = check_cuda(launch_pdl(fns[p->dtype == QVGGT_DTYPE_BF16][nv == 2 ? 0 : nv == 4 ? 1 : nv == 8 ? 2 : 3],
+                                 dim3((unsigned)p->max_units, a.heads), dim3(APPEND_THREADS), 0,
                                  static_cast<cudaStream_t>(stream), 1u, a),
                       "kv_append launch");
   if (!rc) count_launch(1);
@@ -404,7 +500,8 @@ extern "C" int qvggt_kv_gather(const qvggt_kv_gather_args* p, void* stream) {
   if (!aligned16(p->out) || p->out_stride % 8 || p->out_stride < 2 * c.kv_heads * c.head_dim)
     return set_error(QVGGT_ERR_ALIGN, "kv_gather: out rows must be 16-byte aligned and hold K and V");
   GatherArgs a{{c.k_cache, c.v_cache}, {c.k_scale, c.v_scale}, p->slots, static_cast<uint16_t*>(p->out),
-               p->out_stride, c.block_stride, p->n, (int)c.block_size, (int)c.num_blocks, (int)c.kv_heads,
+               p->out_stride, c.block_stride, p->n, (int)c.block_size,
+               c.block_size == 32 ? 5 : c.block_size == 64 ? 6 : 7, (int)c.num_blocks, (int)c.kv_heads,
                (int)c.head_dim, make_ctl()};
   const long long work = (p->n * 2 * a.heads * (a.D / 16) + GATHER_THREADS - 1) / GATHER_THREADS;
   const long long grid = std::min<long long>(work, 16LL * device_info().num_sms);
