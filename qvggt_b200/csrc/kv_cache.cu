@@ -235,7 +235,9 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(AppendArgs a)
   constexpr uint32_t INF = BF16 ? 0x7f80u : 0x7c00u;
   pdl_wait();
   pdl_trigger();
-  const int unit = blockIdx.x, h = blockIdx.y, side = threadIdx.x / APPEND_SIDE, th = threadIdx.x % APPEND_SIDE;
+  // heads fastest: neighbouring CTAs then read neighbouring pieces of the same rows
+  const int unit = blockIdx.x / a.heads, h = blockIdx.x - unit * a.heads;
+  const int side = threadIdx.x / APPEND_SIDE, th = threadIdx.x % APPEND_SIDE;
   if (unit >= a.cu_blocks[a.B]) return;
   const int b = warp_last_le(a.cu_blocks, a.B, unit);
   const int c = a.cached[b], n0 = a.cu_new[b], end = c + a.cu_new[b + 1] - n0;
@@ -243,18 +245,19 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(AppendArgs a)
   const int lo = max(c, j * a.bs), hi = min(end, (j + 1) * a.bs);      // new tokens of the block
   const int blk = j < a.wide ? a.table[(long long)b * a.wide + j] : -1;
   const bool lengths = c >= 0 && n0 >= 0 && hi > lo && (long long)n0 + end - c <= a.tokens;
-  const int per_row = a.D / 8, pieces = lengths ? (hi - lo) * per_row : 0;
-  const uint16_t* x = a.x[side] + (long long)(n0 + lo - c) * a.tok_stride[side] + h * a.head_stride[side];
+  // 8 or 16 16-byte pieces to a row; a thread's pieces are 16 or 8 rows apart
+  const int row_log2 = a.D == 64 ? 3 : 4, pieces = lengths ? (hi - lo) << row_log2 : 0;
+  const long long stride = side ? a.tok_stride[1] : a.tok_stride[0];
+  const uint16_t* x = (side ? a.x[1] + h * a.head_stride[1] : a.x[0] + h * a.head_stride[0]) +
+                      ((long long)(n0 + lo - c) + (th >> row_log2)) * stride + (th & ((1 << row_log2) - 1)) * 8;
+  const long long step = stride * (APPEND_SIDE >> row_log2);
   uint4 v[NV];
   uint32_t m = 0;                        // magnitudes of two elements, as integers
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int p = th + i * APPEND_SIDE;
     v[i] = make_uint4(0, 0, 0, 0);
-    if (p < pieces) {
-      const int r = p / per_row;
-      v[i] = __ldg(reinterpret_cast<const uint4*>(x + r * a.tok_stride[side] + (p - r * per_row) * 8));
-    }
+    if (p < pieces) v[i] = __ldg(reinterpret_cast<const uint4*>(x + i * step));
   }
   if (!lengths || blk < 0 || blk >= a.num_blocks) {
     if (threadIdx.x == 0) report_status(a.ctl, lengths ? ST_BAD_BLOCK : ST_BAD_LENGTH);
@@ -267,8 +270,8 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(AppendArgs a)
     for (int e = 0; e < 4; ++e) m = __vmaxu2(m, w[e] & 0x7fff7fffu);
   }
   const int older = lo - j * a.bs;                                     // earlier tokens of the block
-  int8_t* codes = a.codes[side] + blk * a.block_stride + (long long)h * a.bs * a.D;
-  float* scale = a.scales[side] + (long long)blk * a.heads + h;
+  int8_t* codes = (side ? a.codes[1] : a.codes[0]) + blk * a.block_stride + (long long)h * a.bs * a.D;
+  float* scale = (side ? a.scales[1] : a.scales[0]) + (long long)blk * a.heads + h;
   const float before = older > 0 ? *scale : 0.f;
   m = __reduce_max_sync(~0u, max(m & 0xffffu, m >> 16));
   if (th % 32 == 0) red[threadIdx.x / 32] = m;
@@ -336,46 +339,50 @@ struct GatherArgs {
   Ctl ctl;
 };
 
-// 16 codes per thread; a slot of -1 gives a row of zeros.
+// 16 codes per thread and step; the grid sweeps the rows' pieces in order.  A
+// slot of -1 gives a row of zeros.  Bound by memory latency at full occupancy:
+// 5.3 TB/s read and written at 43,968 rows of 2 x 16 x 64 (8 codes a thread:
+// 61 us against 51; several rows a thread in flight, which costs occupancy: 62).
 template <bool BF16>
-__global__ void __launch_bounds__(GATHER_THREADS) kv_gather_kernel(GatherArgs a) {
+__global__ void __launch_bounds__(GATHER_THREADS, 8) kv_gather_kernel(GatherArgs a) {
   pdl_wait();
   pdl_trigger();
-  const int per_head = a.D / 16, per_side = a.heads * per_head, per_row = 2 * per_side;
-  const long long total = a.n * per_row;
-  for (long long i = (long long)blockIdx.x * GATHER_THREADS + threadIdx.x; i < total;
-       i += (long long)gridDim.x * GATHER_THREADS) {
-    const long long row = i / per_row;
-    const int rem = (int)(i - row * per_row);
-    const int side = rem >= per_side, hp = rem - side * per_side, h = hp / per_head, part = hp - h * per_head;
-    const int slot = a.slots[row];
-    uint4 o[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-    if (slot >= 0) {
-      const int blk = slot >> a.bs_log2;
-      if (blk < a.num_blocks) {
-        const int8_t* src = (side ? a.codes[1] : a.codes[0]) + blk * a.block_stride +
-                            ((long long)h * a.bs + (slot & (a.bs - 1))) * a.D + part * 16;
-        const uint4 c = *reinterpret_cast<const uint4*>(src);
-        const float s = (side ? a.scales[1] : a.scales[0])[(long long)blk * a.heads + h];
-        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-        uint32_t r[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          // the code as a float: its byte, sign bit flipped, under the exponent of 2^23
-          const uint32_t f = w[k / 2] ^ 0x80808080u;
-          const float x0 = __uint_as_float(__byte_perm(f, 0x4b000000u, k & 1 ? 0x7442 : 0x7440)) - 8388736.f;
-          const float x1 = __uint_as_float(__byte_perm(f, 0x4b000000u, k & 1 ? 0x7443 : 0x7441)) - 8388736.f;
-          r[k] = BF16 ? pack_bf162(x0 * s, x1 * s) : pack_half2(x0 * s, x1 * s);
-        }
-        o[0] = make_uint4(r[0], r[1], r[2], r[3]);
-        o[1] = make_uint4(r[4], r[5], r[6], r[7]);
-      } else if (rem == 0) {
-        report_bad_block(a.ctl);
-      }
+  const int head_log2 = a.D == 64 ? 2 : 3, per_side = a.heads << head_log2, per_row = 2 * per_side;
+  const int t = blockIdx.x * GATHER_THREADS + threadIdx.x, threads = gridDim.x * GATHER_THREADS;
+  const int d_row = threads / per_row, d_rem = threads - d_row * per_row;   // a step of the sweep
+  int rem = t % per_row;
+  for (long long row = t / per_row; row < a.n;) {
+    const int side = rem >= per_side, hp = rem - side * per_side, h = hp >> head_log2;
+    const int slot = a.slots[row], blk = slot >> a.bs_log2;
+    uint4 c = make_uint4(0, 0, 0, 0);
+    float s = 0.f;
+    if (slot >= 0 && blk < a.num_blocks) {
+      c = __ldg(reinterpret_cast<const uint4*>((side ? a.codes[1] : a.codes[0]) + blk * a.block_stride +
+                                               ((long long)h * a.bs + (slot & (a.bs - 1))) * a.D +
+                                               (hp - (h << head_log2)) * 16));
+      s = (side ? a.scales[1] : a.scales[0])[(long long)blk * a.heads + h];
+    } else if (slot >= 0 && rem == 0) {
+      report_bad_block(a.ctl);
     }
-    uint4* dst = reinterpret_cast<uint4*>(a.out + row * a.out_stride + (long long)rem * 16);
-    dst[0] = o[0];
-    dst[1] = o[1];
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    uint32_t o[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      // the code as a float: its byte, sign bit flipped, under the exponent of 2^23
+      const uint32_t f = w[k / 2] ^ 0x80808080u;
+      const float x0 = __uint_as_float(__byte_perm(f, 0x4b000000u, k & 1 ? 0x7442 : 0x7440)) - 8388736.f;
+      const float x1 = __uint_as_float(__byte_perm(f, 0x4b000000u, k & 1 ? 0x7443 : 0x7441)) - 8388736.f;
+      o[k] = BF16 ? pack_bf162(x0 * s, x1 * s) : pack_half2(x0 * s, x1 * s);
+    }
+    uint4* dst = reinterpret_cast<uint4*>(a.out + row * a.out_stride + rem * 16);
+    dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    row += d_row;
+    rem += d_rem;
+    if (rem >= per_row) {
+      rem -= per_row;
+      ++row;
+    }
   }
 }
 
@@ -444,7 +451,7 @@ extern "C" int qvggt_kv_append(const qvggt_kv_append_args* p, void* stream) {
   if (p->dtype != QVGGT_DTYPE_F16 && p->dtype != QVGGT_DTYPE_BF16)
     return set_error(QVGGT_ERR_UNSUPPORTED, "kv_append: dtype must be fp16 or bf16");
   if (p->tokens < 0 || p->requests < 0 || p->max_blocks < 0 || p->max_units < 0 || p->requests > 2147483646LL ||
-      p->max_blocks > 2147483647LL || p->max_units > 2147483647LL)
+      p->max_blocks > 2147483647LL || p->max_units > 2147483647LL / p->cache.kv_heads)
     return set_error(QVGGT_ERR_INVALID, "kv_append: bad shape");
   if (p->tokens == 0 || p->requests == 0 || p->max_units == 0) return QVGGT_OK;
   if (!p->k || !p->v || !p->block_tables || !p->cached_lens || !p->cu_new || !p->cu_blocks)
@@ -481,7 +488,7 @@ extern "C" int qvggt_kv_append(const qvggt_kv_append_args* p, void* stream) {
       {kv_append_kernel<true, 2>, kv_append_kernel<true, 4>, kv_append_kernel<true, 8>, kv_append_kernel<true, 16>}};
   const int nv = a.bs * a.D / 8 / APPEND_SIDE;             // 2, 4, 8 or 16 pieces a thread
   int rc = check_cuda(launch_pdl(fns[p->dtype == QVGGT_DTYPE_BF16][nv == 2 ? 0 : nv == 4 ? 1 : nv == 8 ? 2 : 3],
-                                 dim3((unsigned)p->max_units, a.heads), dim3(APPEND_THREADS), 0,
+                                 dim3((unsigned)(p->max_units * a.heads)), dim3(APPEND_THREADS), 0,
                                  static_cast<cudaStream_t>(stream), 1u, a),
                       "kv_append launch");
   if (!rc) count_launch(1);
@@ -503,8 +510,9 @@ extern "C" int qvggt_kv_gather(const qvggt_kv_gather_args* p, void* stream) {
                p->out_stride, c.block_stride, p->n, (int)c.block_size,
                c.block_size == 32 ? 5 : c.block_size == 64 ? 6 : 7, (int)c.num_blocks, (int)c.kv_heads,
                (int)c.head_dim, make_ctl()};
-  const long long work = (p->n * 2 * a.heads * (a.D / 16) + GATHER_THREADS - 1) / GATHER_THREADS;
-  const long long grid = std::min<long long>(work, 16LL * device_info().num_sms);
+  // up to 16 CTAs per SM (8 at a time)
+  const long long want = (p->n * 2 * a.heads * (a.D / 16) + GATHER_THREADS - 1) / GATHER_THREADS;
+  const long long grid = std::min<long long>(want, 16LL * device_info().num_sms);
   const auto fn = p->dtype == QVGGT_DTYPE_BF16 ? kv_gather_kernel<true> : kv_gather_kernel<false>;
   int rc = check_cuda(launch_pdl(fn, dim3((unsigned)grid), dim3(GATHER_THREADS), 0,
                                  static_cast<cudaStream_t>(stream), 1u, a),
