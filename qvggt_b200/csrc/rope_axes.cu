@@ -15,7 +15,7 @@ namespace {
 
 constexpr int ROPE_THREADS = 256;
 constexpr int ROPE_MAX_PAIRS = 128;     // head_dim <= 256
-constexpr int ROPE_MAX_TOK = 16;        // tokens of one CTA
+constexpr int ROPE_MAX_TOK = 8;         // tokens of one CTA
 constexpr int ROPE_AXES = 4;
 
 enum RopeLayout : int32_t { ROPE_AXIAL = 0, ROPE_SPLIT = 1, ROPE_INTERLEAVED = 2 };
@@ -55,15 +55,28 @@ __device__ __forceinline__ uint16_t from_f32(float x) {
   return __half_as_ushort(__float2half_rn(x));
 }
 
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t u) {
+  return BF16 ? unpack_bf162(u) : unpack_half2(u);
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  return BF16 ? pack_bf162(x, y) : pack_half2(x, y);
+}
+
 // V pairs per item: two V-element vectors in, two out.
 template <bool BF16, int V>
-__global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(RopeArgs a) {
+__global__ void __launch_bounds__(ROPE_THREADS, 8) rope_axes_kernel(RopeArgs a) {
   using Vec = typename VecBits<V>::T;
   union Pack {
     Vec v;
     uint16_t e[V];
+    uint32_t w[(V + 1) / 2];
   };
-  extern __shared__ float2 cs[];         // [tok][pairs] (cos, sin)
+  // [tok][pairs] cosines, then sines: apart, so that the 16-byte reads of a
+  // warp's items lie 32 bytes apart, not 64 (half the bank conflicts)
+  extern __shared__ __align__(16) float cosines[];
+  float* sines = cosines + a.tok * a.pairs;
   pdl_wait();
   pdl_trigger();
   const long long t0 = (long long)blockIdx.x * a.tok;
@@ -79,7 +92,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(RopeArgs a) {
     const double r = t - rint(t * 0.15915494309189533577) * 6.28318530717958647693;
     float sn, cn;
     sincosf((float)r, &sn, &cn);
-    cs[i] = make_float2(cn, sn * a.sign);
+    cosines[i] = cn;
+    sines[i] = sn * a.sign;
   }
   __syncthreads();
   const int rot = a.pairs / V;                            // rotation items of a head
@@ -87,15 +101,32 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(RopeArgs a) {
   const int per_head = rot + copy;
   const int heads = a.s[0].heads + a.s[1].heads;
   const int per_tok = heads * per_head;
-  for (int i = threadIdx.x; i < nt * per_tok; i += ROPE_THREADS) {
-    const int tt = i / per_tok, rem = i - tt * per_tok;
-    int h = rem / per_head;
-    const int item = rem - h * per_head;
-    const int side = h >= a.s[0].heads;
-    if (side) h -= a.s[0].heads;
-    const RopeSide& s = a.s[side];
-    const uint16_t* in = s.in + (t0 + tt) * s.in_ts + h * s.in_hs;
-    uint16_t* out = s.out + (t0 + tt) * s.out_ts + h * s.out_hs;
+  // a thread's items are ROPE_THREADS apart: token, head and item advance by
+  // fixed amounts with carries, so nothing is divided in the loop
+  const int d_tok = ROPE_THREADS / per_tok, d_rem = ROPE_THREADS - d_tok * per_tok;
+  const int d_head = d_rem / per_head, d_item = d_rem - d_head * per_head;
+  int tt = threadIdx.x / per_tok, hh = (threadIdx.x - tt * per_tok) / per_head;
+  int item = threadIdx.x - tt * per_tok - hh * per_head;
+  auto advance = [&] {
+    item += d_item;
+    hh += d_head;
+    tt += d_tok;
+    if (item >= per_head) {
+      item -= per_head;
+      ++hh;
+    }
+    if (hh >= heads) {
+      hh -= heads;
+      ++tt;
+    }
+  };
+  for (; tt < nt; advance()) {
+    const bool side = hh >= a.s[0].heads;
+    const int h = side ? hh - a.s[0].heads : hh;
+    const uint16_t* in = side ? a.s[1].in + (t0 + tt) * a.s[1].in_ts + h * a.s[1].in_hs
+                              : a.s[0].in + (t0 + tt) * a.s[0].in_ts + h * a.s[0].in_hs;
+    uint16_t* out = side ? a.s[1].out + (t0 + tt) * a.s[1].out_ts + h * a.s[1].out_hs
+                         : a.s[0].out + (t0 + tt) * a.s[0].out_ts + h * a.s[0].out_hs;
     if (item >= rot) {
       const int d = 2 * a.pairs + (item - rot) * V;
       *reinterpret_cast<Vec*>(out + d) = *reinterpret_cast<const Vec*>(in + d);
@@ -123,32 +154,29 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(RopeArgs a) {
     Pack x, y;
     x.v = *reinterpret_cast<const Vec*>(in + lo);
     y.v = *reinterpret_cast<const Vec*>(in + hi);
-    const float2* c = cs + tt * a.pairs + j;
-    if (a.layout == ROPE_INTERLEAVED) {
-      // the 2V consecutive elements are (x | y): pair e is elements 2e, 2e + 1
-      uint16_t z[2 * V];
+    const float* c = cosines + tt * a.pairs + j;
+    const float* s = sines + tt * a.pairs + j;
+    if constexpr (V == 1) {
+      const float p = to_f32<BF16>(x.e[0]), q = to_f32<BF16>(y.e[0]);
+      x.e[0] = from_f32<BF16>(p * c[0] - q * s[0]);
+      y.e[0] = from_f32<BF16>(q * c[0] + p * s[0]);
+    } else if (a.layout == ROPE_INTERLEAVED) {
+      // each word of the 2V consecutive elements (x | y) is a pair
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        z[e] = x.e[e];
-        z[V + e] = y.e[e];
-      }
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float p = to_f32<BF16>(z[2 * e]), q = to_f32<BF16>(z[2 * e + 1]);
-        z[2 * e] = from_f32<BF16>(p * c[e].x - q * c[e].y);
-        z[2 * e + 1] = from_f32<BF16>(q * c[e].x + p * c[e].y);
-      }
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        x.e[e] = z[e];
-        y.e[e] = z[V + e];
+      for (int e = 0; e < V / 2; ++e) {
+        const float2 u = unpack2<BF16>(x.w[e]), w = unpack2<BF16>(y.w[e]);
+        const float c0 = c[e], s0 = s[e], c1 = c[V / 2 + e], s1 = s[V / 2 + e];
+        x.w[e] = pack2<BF16>(u.x * c0 - u.y * s0, u.y * c0 + u.x * s0);
+        y.w[e] = pack2<BF16>(w.x * c1 - w.y * s1, w.y * c1 + w.x * s1);
       }
     } else {
+      // two pairs to a word of x and y
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float p = to_f32<BF16>(x.e[e]), q = to_f32<BF16>(y.e[e]);
-        x.e[e] = from_f32<BF16>(p * c[e].x - q * c[e].y);
-        y.e[e] = from_f32<BF16>(q * c[e].x + p * c[e].y);
+      for (int e = 0; e < V / 2; ++e) {
+        const float2 p = unpack2<BF16>(x.w[e]), q = unpack2<BF16>(y.w[e]);
+        const float2 cc = *reinterpret_cast<const float2*>(c + 2 * e), ss = *reinterpret_cast<const float2*>(s + 2 * e);
+        x.w[e] = pack2<BF16>(p.x * cc.x - q.x * ss.x, p.y * cc.y - q.y * ss.y);
+        y.w[e] = pack2<BF16>(q.x * cc.x + p.x * ss.x, q.y * cc.y + p.y * ss.y);
       }
     }
     *reinterpret_cast<Vec*>(out + lo) = x.v;
@@ -219,9 +247,10 @@ extern "C" int qvggt_rope_axes(const qvggt_rope_axes_args* p, void* stream) {
     limit((long long)(reinterpret_cast<uintptr_t>(s.in) / 2 % 8));
     limit((long long)(reinterpret_cast<uintptr_t>(s.out) / 2 % 8));
   }
-  // Tokens per CTA: few enough that every SM has several CTAs, up to 16 so
-  // that the per-CTA start-up is paid for many rows.
-  const long long want = 8LL * device_info().num_sms;
+  // Tokens per CTA: few enough that every SM has several CTAs, up to 8 so that
+  // the per-CTA start-up is paid for several rows (16: 94 us against 80 at
+  // 20,000 tokens x 32 heads x 128, as the angles' phase then stands alone).
+  const long long want = 4LL * device_info().num_sms;
   a.tok = 1;
   while (a.tok < ROPE_MAX_TOK && T / (2 * a.tok) >= want) a.tok *= 2;
   const long long grid = (T + a.tok - 1) / a.tok;
@@ -232,7 +261,7 @@ extern "C" int qvggt_rope_axes(const qvggt_rope_axes_args* p, void* stream) {
       {rope_axes_kernel<true, 1>, rope_axes_kernel<true, 2>, rope_axes_kernel<true, 4>, rope_axes_kernel<true, 8>}};
   const int vi = align == 8 ? 3 : align == 4 ? 2 : align == 2 ? 1 : 0;
   int rc = check_cuda(launch_pdl(fns[p->dtype == QVGGT_DTYPE_BF16][vi], dim3((unsigned)grid), dim3(ROPE_THREADS),
-                                 (size_t)a.tok * pairs * sizeof(float2), static_cast<cudaStream_t>(stream), 1u, a),
+                                 (size_t)a.tok * pairs * 2 * sizeof(float), static_cast<cudaStream_t>(stream), 1u, a),
                       "rope_axes launch");
   if (!rc) count_launch(1);
   return rc;
