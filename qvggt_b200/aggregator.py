@@ -379,7 +379,7 @@ class VGGTAggregator:
         self.cfg = cfg
         self.pe = pe
         self.agg_specials = agg_specials            # [2, 5, C]: camera + 4 registers, frame 0 / others
-        self.runner = AggregatorRunner(cfg, frame_blocks, global_blocks, frames_local, device, group, world, rank)
+        self.runner = self._make_runner(cfg, frame_blocks, global_blocks, frames_local, device, group, world, rank)
         self.S_local = frames_local
         self.rank = rank
         self.img_hw = img_hw
@@ -390,15 +390,20 @@ class VGGTAggregator:
         self.x_pe = torch.empty(frames_local, cfg.tokens_per_frame, C, dtype=F16, device=dev)
         self.tokens = torch.empty(frames_local, cfg.tokens_per_frame, C, dtype=F16, device=dev)
 
+    def _make_runner(self, *args):
+        return AggregatorRunner(*args)
+
     def forward(self, images: torch.Tensor, keep: tuple[int, ...] = ()) -> dict:
         """The DINOv2 front, then the frame / global pairs (which update
         ``self.tokens`` in place); returns the runner's outputs."""
         return self.runner.forward(self.embed(images), keep)
 
-    def embed(self, images: torch.Tensor) -> torch.Tensor:
+    def embed(self, images: torch.Tensor, frame_offset: int | None = None) -> torch.Tensor:
         """images [S_local, 3, H, W] -> the aggregator's input tokens
         ``self.tokens`` [S_local, P, C]: DINOv2 front, final LayerNorm, then
-        camera / register tokens in place of DINOv2's special rows."""
+        camera / register tokens in place of DINOv2's special rows.
+        ``frame_offset``: place of the first image in the sequence (default:
+        this rank's first frame)."""
         cfg, pe = self.cfg, self.pe
         P, C = cfg.tokens_per_frame, cfg.dim
         eng.patchify(images, pe.patch, pe.k_pad, out=self.patches)
@@ -411,7 +416,7 @@ class VGGTAggregator:
         h = self.runner.ws.h
         eng.layernorm(x, pe.norm_w, pe.norm_b, cfg.eps, out=h)
         eng.assemble_tokens(h, P, cfg.patch_start, self.agg_specials, cfg.patch_start, True, None, self.tokens,
-                            self.S_local, P, frame_offset=self.rank * self.S_local)
+                            self.S_local, P, frame_offset=self.rank * self.S_local if frame_offset is None else frame_offset)
         return self.tokens
 
     def infer(self, images_host: torch.Tensor, out_host: torch.Tensor | None = None):
