@@ -477,17 +477,18 @@ __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 2) attn_cache_rows_ker
 }
 
 // Adds the parts of the items that a cut went through: CTA x looks at the cut
-// before piece x + 1, and the item's first cut does the work, a warp per row.
+// before piece x + 1, and the item's first cut does the work.
 template <bool BF16, int D, int NT>
-__global__ void __launch_bounds__(NT * 256) attn_cache_rows_join_kernel(CacheAttnArgs a, int grid) {
+__global__ void __launch_bounds__(NT * 2 * D) attn_cache_rows_join_kernel(CacheAttnArgs a, int grid) {
   pdl_wait();
   pdl_trigger();
-  const int x = blockIdx.x + 1, lane = threadIdx.x % 32, r = threadIdx.x / 32;
+  const int x = blockIdx.x + 1, r = threadIdx.x / (D / 4);
   const Cut cut = reinterpret_cast<const Cut*>(a.part_lse + 2LL * grid * 8 * NT)[x];
   if (cut.first != x - 1) return;
   const int row = cut.tok0 + r;
   if (row >= cut.ql * a.group) return;
-  join_parts<BF16, D>(a, cut, 8 * NT, r, lane, cut.q0 + row / a.group, cut.kvh * a.group + row % a.group);
+  join_parts<BF16, D>(a, cut, 8 * NT, r, threadIdx.x % (D / 4), cut.q0 + row / a.group,
+                      cut.kvh * a.group + row % a.group);
 }
 
 // Sizes and launch of the row kernel with NT 8-row tiles.
@@ -524,7 +525,7 @@ struct Rows {
     count_launch(1);
     if (a.can_split) {
       const auto join = bf16 ? attn_cache_rows_join_kernel<true, D, NT> : attn_cache_rows_join_kernel<false, D, NT>;
-      if (int rc = check_cuda(launch_pdl(join, dim3((unsigned)(n - 1)), dim3(NT * 256), 0, stream, 1u, a, n),
+      if (int rc = check_cuda(launch_pdl(join, dim3((unsigned)(n - 1)), dim3(NT * 2 * D), 0, stream, 1u, a, n),
                               "cached_attention join launch"))
         return rc;
       count_launch(1);

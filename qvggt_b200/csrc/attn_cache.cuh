@@ -256,37 +256,34 @@ struct PieceWalk {
 };
 
 // Row `row` of a cut item, joined from its parts (rows_per_slot rows a slot) by
-// one warp: the parts' normalised rows weighted by their sums, in the pieces' order.
+// D / 4 threads, four columns each: the parts' normalised rows weighted by
+// their sums, in the pieces' order.
 template <bool BF16, int D>
-__device__ __forceinline__ void join_parts(const CacheAttnArgs& a, const Cut& cut, int rows_per_slot, int row, int lane,
+__device__ __forceinline__ void join_parts(const CacheAttnArgs& a, const Cut& cut, int rows_per_slot, int row, int col4,
                                            long long tok, int h) {
-  constexpr int E = D / 32;
   auto at = [&](int k) { return (long long)(2 * k + (k == cut.first)) * rows_per_slot + row; };
   float mx = -INFINITY;
-  for (int k = cut.first + lane; k <= cut.last; k += 32) mx = fmaxf(mx, a.part_lse[at(k)]);
-  mx = warp_max(mx);
+#pragma unroll 4
+  for (int k = cut.first; k <= cut.last; ++k) mx = fmaxf(mx, a.part_lse[at(k)]);
   const float base = mx == -INFINITY ? 0.f : mx;
-  float l = 0.f, acc[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 2
+  float l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
   for (int k = cut.first; k <= cut.last; ++k) {
     const float w = exp2f(a.part_lse[at(k)] - base);
-    const float* p = a.part_o + at(k) * D + lane * E;
-    float v[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = p[e];
+    const float4 v = *reinterpret_cast<const float4*>(a.part_o + at(k) * D + col4 * 4);
     l += w;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += w * v[e];
+    acc.x += w * v.x;
+    acc.y += w * v.y;
+    acc.z += w * v.z;
+    acc.w += w * v.w;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + tok * a.o_tok + h * a.o_head + lane * E);
-#pragma unroll
-  for (int e = 0; e < E / 2; ++e)
-    dst[e] = BF16 ? pack_bf162(acc[2 * e] * inv, acc[2 * e + 1] * inv)
-                  : pack_half2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-  if (lane == 0 && a.lse) a.lse[h * a.Tq + tok] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
+  acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(a.out + tok * a.o_tok + h * a.o_head + col4 * 4) =
+      BF16 ? make_uint2(pack_bf162(acc.x, acc.y), pack_bf162(acc.z, acc.w))
+           : make_uint2(pack_half2(acc.x, acc.y), pack_half2(acc.z, acc.w));
+  if (col4 == 0 && a.lse) a.lse[h * a.Tq + tok] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
 }
 
 // attn_cache_sm100.cu (many rows): whether its TMA map can read these queries;

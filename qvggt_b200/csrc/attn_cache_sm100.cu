@@ -44,7 +44,7 @@ constexpr int Q_ROWS = 256;     // rows of an item
 // Cost of an item on the line: a start-up (loads, first products, epilogue)
 // and its key tiles; with one Q tile a softmax warpgroup idles, but the other's
 // chain per tile is nearly as long.
-constexpr int COST_START = 20, COST_TILE2 = 10, COST_TILE1 = 9;
+constexpr int COST_START = 30, COST_TILE2 = 10, COST_TILE1 = 8;
 // No piece is cut shorter than this (8 tiles): a join costs about as much.
 constexpr int COST_MIN = COST_START + 8 * COST_TILE2;
 constexpr int RAW_BYTES = 8192; // K or V codes of a tile
@@ -69,7 +69,8 @@ struct Lay {
   static constexpr int MISC = BAR + NUM_BARS * 8;          // TMEM base
   static constexpr int SEG = MISC + 32;                    // Segment [SEGS]
   static constexpr int CUM = SEG + SEGS * 64;              // long long [THREADS + 1]
-  static constexpr int TOTAL = CUM + (THREADS + 1) * 8 + 64 + 1024;
+  static constexpr int ROWS = CUM + (THREADS + 2) * 8;     // int2 [256]: token and head of each row
+  static constexpr int TOTAL = ROWS + 256 * 8 + 1024;
 };
 
 // One lane of a converged warp, the same one every time.
@@ -584,6 +585,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t bar_s_full = smem_u32(&s_full[i]);
     const uint32_t bar_s_free = bar_s_full + 16, bar_p_full = bar_s_full + 32, bar_o_done = bar_s_full + 48;
     const float4* consts = reinterpret_cast<const float4*>(smem + L::CONST);
+    // the row's token in the block (past any block's for a row that holds none)
+    // and head in the group: kept in shared memory, as registers held through
+    // the tile loop push scores to local memory
+    volatile int2* row_at = reinterpret_cast<volatile int2*>(smem + L::ROWS) + (threadIdx.x - 256);
+    row_at->x = r < tpt * a.group ? i * tpt + r / a.group : 1 << 30;
+    row_at->y = r % a.group;
     bool ok = true;
     uint32_t cnt = 0;                                      // tiles of this warpgroup so far
     int jg = 0;                                            // tiles of the CTA so far
@@ -597,9 +604,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       // compute on whatever their tile holds and are not stored
       int left;
       {
-        const int ql = segs[ss].ql, tok = segs[ss].tok0 + i * tpt + r / a.group;
-        left = (r < tpt * a.group && tok < ql ? key_limit(tok, ql, segs[ss].n, a.chunk) : segs[ss].n) -
-               segs[ss].t0 * KT;
+        const int ql = segs[ss].ql, in_block = ql - segs[ss].tok0, x = row_at->x;
+        left = (x < in_block ? key_limit(segs[ss].tok0 + x, ql, segs[ss].n, a.chunk) : segs[ss].n) - segs[ss].t0 * KT;
       }
       float m_used = -INFINITY, l = 0.f;
       bool ready = false;
@@ -663,40 +669,46 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_fence_after();
       }
       if (ok) {                                            // warp-uniform
-        const int tok = segs[ss].tok0 + i * tpt + r / a.group, slot = segs[ss].slot;
-        const bool row_ok = r < tpt * a.group && tok < segs[ss].ql;
+        const int x = row_at->x, tok = segs[ss].tok0 + x, slot = segs[ss].slot;
+        const bool row_ok = x < segs[ss].ql - segs[ss].tok0;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const float lse2 = l == 0.f ? -INFINITY : m_used + log2f(l);
         const long long gtok = segs[ss].q0 + tok;
-        const int h = segs[ss].kvh * a.group + r % a.group;
+        const int h = segs[ss].kvh * a.group + row_at->y;
         const long long part = (long long)slot * Q_ROWS + i * 128 + r;
+        float4* part_dst = reinterpret_cast<float4*>(a.part_o + part * D);
+        uint4* dst = reinterpret_cast<uint4*>(a.out + gtok * a.o_tok + h * a.o_head);
+        // 16 columns at a time where the score row is 128 wide: more would cost
+        // the tile loop registers
+        constexpr int W = D == 64 ? 16 : 32;
 #pragma unroll 1
-        for (int cc = 0; cc < D / 16; ++cc) {
-          uint32_t v[16];
+        for (int cc = 0; cc < D; cc += W) {
+          uint32_t v[W];
           if (ntr > 0) {
-            tmem_ld16(tO + cc * 16, v);
+            if constexpr (W == 16) tmem_ld16(tO + cc, v);
+            else tmem_ld32(tO + cc, v);
             tmem_ld_wait();
-            reg_fence<0, 16>(v);
+            reg_fence<0, W>(v);
           }
           if (!row_ok) continue;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(v[e]) * inv);
+          for (int e = 0; e < W; ++e) v[e] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(v[e]) * inv);
           if (slot >= 0) {
-            float4* dst = reinterpret_cast<float4*>(a.part_o + part * D + cc * 16);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              dst[e] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
-                                   __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
+            for (int e = 0; e < W / 4; ++e)
+              part_dst[cc / 4 + e] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
+                                                 __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
           } else {
-            uint32_t o[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float x = __uint_as_float(v[2 * e]), y = __uint_as_float(v[2 * e + 1]);
-              o[e] = BF16 ? pack_bf162(x, y) : pack_half2(x, y);
+            for (int e = 0; e < W / 8; ++e) {
+              uint32_t o[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float p = __uint_as_float(v[8 * e + 2 * x]), q = __uint_as_float(v[8 * e + 2 * x + 1]);
+                o[x] = BF16 ? pack_bf162(p, q) : pack_half2(p, q);
+              }
+              dst[cc / 8 + e] = make_uint4(o[0], o[1], o[2], o[3]);
             }
-            uint4* dst = reinterpret_cast<uint4*>(a.out + gtok * a.o_tok + h * a.o_head + cc * 16);
-            dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
           }
         }
         if (row_ok) {
@@ -719,8 +731,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 }
 
 // Adds the parts of the items that a cut went through.  CTA (x, y) looks at
-// the cut before piece x + 1; the item's first cut does the work, 16 rows a
-// CTA, half a warp's registers a row.
+// the cut before piece x + 1; the item's first cut does the work, 256 / (D / 4)
+// rows a CTA.
 template <bool BF16, int D>
 __global__ void __launch_bounds__(256) attn_cache_tiles_join_kernel(CacheAttnArgs a, int grid) {
   pdl_wait();
@@ -728,14 +740,10 @@ __global__ void __launch_bounds__(256) attn_cache_tiles_join_kernel(CacheAttnArg
   const int x = blockIdx.x + 1;
   const Cut cut = reinterpret_cast<const Cut*>(a.part_lse + 2LL * grid * Q_ROWS)[x];
   if (cut.first != x - 1) return;
-  const int lane = threadIdx.x % 32;
-#pragma unroll 1
-  for (int rr = 0; rr < 2; ++rr) {
-    const int row = blockIdx.y * 16 + (threadIdx.x / 32) * 2 + rr, r = row & 127;
-    const int tpt = 128 / a.group, tok = cut.tok0 + (row >> 7) * tpt + r / a.group;
-    if (r >= tpt * a.group || tok >= cut.ql) continue;
-    join_parts<BF16, D>(a, cut, Q_ROWS, row, lane, cut.q0 + tok, cut.kvh * a.group + r % a.group);
-  }
+  const int row = blockIdx.y * (1024 / D) + threadIdx.x / (D / 4), r = row & 127;
+  const int tpt = 128 / a.group, tok = cut.tok0 + (row >> 7) * tpt + r / a.group;
+  if (r >= tpt * a.group || tok >= cut.ql) return;
+  join_parts<BF16, D>(a, cut, Q_ROWS, row, threadIdx.x % (D / 4), cut.q0 + tok, cut.kvh * a.group + r % a.group);
 }
 
 }  // namespace
@@ -793,7 +801,7 @@ int launch_tiles(CacheAttnArgs& a, int D, bool bf16, long long max_kv, void* scr
     return rc;
   count_launch(1);
   if (a.can_split) {
-    if (int rc = check_cuda(launch_pdl(joins[bf16][D == 128], dim3((unsigned)(grid - 1), Q_ROWS / 16), dim3(256), 0,
+    if (int rc = check_cuda(launch_pdl(joins[bf16][D == 128], dim3((unsigned)(grid - 1), Q_ROWS * D / 1024), dim3(256), 0,
                                        stream, 1u, a, grid),
                             "cached_attention join launch"))
       return rc;

@@ -54,15 +54,21 @@ _GATHER = struct.Struct("=14q").pack
 _ATTEND = struct.Struct("=27qd2q").pack
 
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_functions: dict = {}
 
 
 def _run(name, dev, t, args):
     """The C call `name` on the current stream of the tensor t's device (index dev)."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(_lib.load(), name)
     if _current_device() == dev:
-        _lib.call(name, args, _stream(t))
+        rc = fn(args, _stream(t))
     else:
         with _Dev(t.device):
-            _lib.call(name, args, _stream(t))
+            rc = fn(args, _stream(t))
+    if rc:
+        raise _lib.QvggtError(name, rc, _lib.load().qvggt_last_error().decode(errors="replace"))
 
 
 def _half(name, t, what):
