@@ -82,16 +82,17 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// One CTA per SM walks its piece of the items' line (attn_cache.cuh); the
+// A CTA walks its piece of the items' line (attn_cache.cuh); the
 // units of a segment go round its warps.  Each warp streams its own units
 // through a ring of bulk copies that only it fills and reads, so nothing but
 // its own mbarriers holds it up: up to 192 KB in flight per SM, well over what
-// the memory's latency needs.  The warps' softmax states merge at the segment's end.
+// the memory's latency needs.  Two CTAs share an SM, so one streams while the
+// other starts or merges.  The warps' softmax states merge at the segment's end.
 //
 // The codes are the M operand of mma.m16n8k16 and the rows its N: S^T = K q^T,
 // O^T += V^T P^T.  The instructions that unpack a code are then paid once for
 // all rows (they bound the kernel: with the rows as M, 668 instructions a unit
-// against 340 now, 150 us against XXX at 8 x 16 heads x 43,968 keys), and each
+// against 458 now, 150 us against 113 at 8 x 16 heads x 37,000 keys, 632 MB), and each
 // of up to 8 rows costs what one does.
 template <bool BF16, int D, int NT>
 __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 2) attn_cache_rows_kernel(CacheAttnArgs a) {
@@ -194,8 +195,8 @@ __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 2) attn_cache_rows_ker
     // order of the dims will do, as K's fragments use the same).  bf16 queries
     // become fp16 times a power of two per row (its largest element near 2^13;
     // what fp16 then cannot hold exactly is below 2^-37 of that), because codes
-    // unpack to fp16 in five instructions a word and to bf16 in eight: 61 us
-    // against XXX at 16 ragged requests x 8 heads x 128.
+    // unpack to fp16 in five instructions a word and to bf16 in eight: 63 us
+    // against 56 at 16 ragged requests x 8 heads x 128, 177 MB.
     uint32_t qb[L::Q_SHARED ? 1 : NT][KC][4][2];
     float row_ck[NT][2];                  // what undoes it, of rows 2t and 2t + 1
     if (L::Q_SHARED) __syncthreads();     // the segment before is done with the shared fragments
@@ -536,7 +537,11 @@ struct Rows {
 
 // Rows (of a kv head) up to which the row kernel serves a call.  It reads the
 // cache once for each 8, 16 or 32 rows at up to memory speed; the tile kernel
-// reads it once for up to 256, at a rate that its softmax sets.
+// reads it once for up to 256, at a rate that its softmax sets.  Measured on 8
+// requests of 37,000 keys, 16 heads x 64: 1 row 113 us, 16 rows 157, 17 to 32
+// rows 267 here and 341 there (33 rows or 64).  With head_dim 128 a second pass
+// over the keys for rows 17 to 32 takes what the tile kernel does (92 us at 20
+// rows of 16 ragged requests, 58 at 16), and its registers do not hold 32 rows.
 constexpr int ROWS_MAX_64 = 32, ROWS_MAX_128 = 16;
 
 // How a call is laid out, by its sizes alone.

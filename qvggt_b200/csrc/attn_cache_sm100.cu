@@ -276,10 +276,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tmem = *tmem_slot;
   const int tpt = 128 / a.group;                           // tokens of a Q tile
 
-  // Registers: launched at 128 each; 128 (64 + 64 + 2 * 192) = 128 * 512.
+  // Registers: launched at 128 each; 128 (56 + 56 + 2 * 200) = 128 * 512.
   // Every warp of a warpgroup runs the same setmaxnreg.
   if (warp < 4) {
-    regs_dec<64>();
+    regs_dec<56>();
     if (warp == 2) {
       // ---------------------------------------------------------- segments
       if (lane == 0) {
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------ codes -> fp16 / bf16
-    regs_dec<64>();
+    regs_dec<56>();
     const int th = threadIdx.x - 128;                      // 0..127
     constexpr int PARTS = D / 16;                          // 16-code pieces of a row
     constexpr int IT = KT * PARTS / 128;                   // pieces per thread
@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------ softmax of Q tile i
-    regs_inc<192>();
+    regs_inc<200>();
     const int i = (warp - 8) / 4;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
