@@ -133,7 +133,8 @@ __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 2) attn_cache_rows_ker
   }
   __syncthreads();
   const int bs = 1 << a.bs_log2;
-  uint32_t used = 0;                      // units this warp has taken from its ring
+  int st = 0;                             // the ring's next stage and its phase
+  uint32_t phase = 0;
   bool ok = true;
   for (int seg = 0;; ++seg) {
     const Segment sg = segs[seg & 1];
@@ -161,23 +162,22 @@ __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 2) attn_cache_rows_ker
     };
     int id = fetch_id(lane), id2 = fetch_id(32 + lane);
     bool bad = false;
-    // starts the copies of unit i (a block outside the cache: none)
-    auto issue = [&](int i, int block) {
-      const uint32_t u = used + i, st = u % L::STAGES;
+    // starts the copies of unit i into stage x (a block outside the cache: none)
+    auto issue = [&](int i, int block, int x) {
       const int key0 = (first + i * L::WARPS) * UNIT;
       if (lane == 0) {
         const bool good = block >= 0 && block < a.num_blocks;
         bad |= !good;
-        mbar_arrive_expect_tx(&bars[st], good ? 2 * L::SIDE : 0);
+        mbar_arrive_expect_tx(&bars[x], good ? 2 * L::SIDE : 0);
         if (good) {
           const long long off = block * a.block_stride + ((long long)kvh * bs + (key0 & (bs - 1))) * D;
-          const uint32_t dst = ring + st * 2 * L::SIDE;
-          bulk_load(dst, a.kc + off, L::SIDE, smem_u32(&bars[st]));
-          bulk_load(dst + L::SIDE, a.vc + off, L::SIDE, smem_u32(&bars[st]));
+          const uint32_t dst = ring + x * 2 * L::SIDE;
+          bulk_load(dst, a.kc + off, L::SIDE, smem_u32(&bars[x]));
+          bulk_load(dst + L::SIDE, a.vc + off, L::SIDE, smem_u32(&bars[x]));
         }
       }
     };
-    for (int i = 0; i < L::STAGES && i < count; ++i) issue(i, __shfl_sync(~0u, id, i));
+    for (int i = 0; i < L::STAGES && i < count; ++i) issue(i, __shfl_sync(~0u, id, i), (st + i) % L::STAGES);
     constants(id);
 
     // rows 2t and 2t + 1 of each 8-row tile
@@ -280,8 +280,7 @@ __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 2) attn_cache_rows_ker
       const int blk = __shfl_sync(~0u, id, i & 31);
       const float uck = __shfl_sync(~0u, ck, i & 31), ulv = __shfl_sync(~0u, lv, i & 31);
       const float uinv = __shfl_sync(~0u, inv_vs, i & 31);
-      const uint32_t u = used + i, st = u % L::STAGES;
-      if (!warp_wait(&bars[st], (u / L::STAGES) & 1, a.wait_tries)) { ok = false; break; }
+      if (!warp_wait(&bars[st], phase, a.wait_tries)) { ok = false; break; }
       const int key0 = (first + i * L::WARPS) * UNIT;
       const uint32_t kb = ring + st * 2 * L::SIDE, vb = kb + L::SIDE;
       if (blk >= 0 && blk < a.num_blocks) {
@@ -399,16 +398,24 @@ __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 2) attn_cache_rows_ker
       if (nx < count) {
         fence_proxy_async_smem();
         __syncwarp();
-        issue(nx, nblk);
+        issue(nx, nblk, st);             // (STAGES units on: the same stage)
+      }
+      if (++st == L::STAGES) {
+        st = 0;
+        phase ^= 1;
       }
     }
-    used += count;
     if (bad) report_bad_block(a.ctl);
     if (!ok) {
       if (lane == 0) {
         report_status(a.ctl, ST_TIMEOUT_FULL);
-        for (int x = i; x < min(count, i + L::STAGES); ++x)
-          mbar_wait_drain(&bars[(used - count + x) % L::STAGES], ((used - count + x) / L::STAGES) & 1, 200000000ull);
+        for (int x = i; x < min(count, i + L::STAGES); ++x) {
+          mbar_wait_drain(&bars[st], phase, 200000000ull);
+          if (++st == L::STAGES) {
+            st = 0;
+            phase ^= 1;
+          }
+        }
       }
       __syncwarp();
     }
