@@ -92,7 +92,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // The codes are the M operand of mma.m16n8k16 and the rows its N: S^T = K q^T,
 // O^T += V^T P^T.  The instructions that unpack a code are then paid once for
 // all rows (they bound the kernel: with the rows as M, 668 instructions a unit
-// against 458 now, 150 us against 113 at 8 x 16 heads x 37,000 keys, 632 MB), and each
+// against 450 now, 150 us against 113 at 8 x 16 heads x 37,000 keys, 632 MB), and each
 // of up to 8 rows costs what one does.
 template <bool BF16, int D, int NT>
 __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 2) attn_cache_rows_kernel(CacheAttnArgs a) {
@@ -545,7 +545,7 @@ struct Rows {
 // Rows (of a kv head) up to which the row kernel serves a call.  It reads the
 // cache once for each 8, 16 or 32 rows at up to memory speed; the tile kernel
 // reads it once for up to 256, at a rate that its softmax sets.  Measured on 8
-// requests of 37,000 keys, 16 heads x 64: 1 row 113 us, 16 rows 157, 17 to 32
+// requests of 37,000 keys, 16 heads x 64: 1 row 113 us, 16 rows 152, 17 to 32
 // rows 267 here and 341 there (33 rows or 64).  With head_dim 128 a second pass
 // over the keys for rows 17 to 32 takes what the tile kernel does (92 us at 20
 // rows of 16 ragged requests, 58 at 16), and its registers do not hold 32 rows.
