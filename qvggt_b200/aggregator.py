@@ -176,7 +176,8 @@ class AggregatorRunner:
         self.T = frames_local * P
         self.w8a8 = any(b.qkv.kind == "w8" for b in list(frame_blocks) + list(global_blocks))
         self.ws = Workspace(self.T, self.T * world, cfg, self.device, self.w8a8)
-        self.cos, self.sin = rope_tables(cfg, self.device)
+        # what q and k turn by: in the global blocks, and in the frame blocks
+        self.cos, self.sin = self.frame_rope = rope_tables(cfg, self.device)
         # With more than one rank the global attention runs as a local-keys
         # pass overlapping the K/V all-gather and a remote-keys pass
         # (overlap_kv), or after the whole gather (overlap_kv=False).
@@ -226,7 +227,8 @@ class AggregatorRunner:
         else:
             kv_dst = ws.kv_local
         # qkv projection with the q/k/v split and 2-D RoPE in the GEMM epilogue
-        eng.qkv_rope_linear(ws.h, blk.qkv, cfg.heads, self.cos, self.sin, P, cfg.patch_start, cfg.grid_w, 0,
+        cos, sin = (self.cos, self.sin) if glob else self.frame_rope
+        eng.qkv_rope_linear(ws.h, blk.qkv, cfg.heads, cos, sin, P, cfg.patch_start, cfg.grid_w, 0,
                             q_out=ws.q, kv_out=kv_dst, qk_norm=blk.qk_norm, eps=cfg.eps)
         if glob:
             self._global_attention()
@@ -300,7 +302,8 @@ class AggregatorRunner:
         eng.w8a8_gemm_fuse_bias_forward_cuda(ws.xq, q.w8, q.wscale, ws.xs, ws.qkv, q.bias)
         glob = kind == "global"
         kv_dst = kv_slice(ws.kv_global, self.T, self.rank) if (glob and self.world > 1) else ws.kv_local
-        eng.qkv_rope2d(ws.qkv, cfg.heads, self.cos, self.sin, P, cfg.patch_start, cfg.grid_w, 0, q_out=ws.q,
+        cos, sin = (self.cos, self.sin) if glob else self.frame_rope
+        eng.qkv_rope2d(ws.qkv, cfg.heads, cos, sin, P, cfg.patch_start, cfg.grid_w, 0, q_out=ws.q,
                        kv_out=kv_dst, qk_norm=blk.qk_norm, eps=cfg.eps)
         self._attend(kind, kv_dst)
         eng.invoke_quant(ws.xq, ws.attn, ws.xs)

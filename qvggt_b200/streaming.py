@@ -12,9 +12,10 @@ its causal form, as for frames from a live camera.)
 
     plan -> [per layer] qkv (+ q/k norm, RoPE) -> append -> attend -> proj ...
 
-With ``time_axis`` q and k turn by (time, height, width) positions
-(:func:`~qvggt_b200.kv_cache.rope_axes`) in place of the model's (height,
-width).  A 518 x 518 frame's K/V of all 24 layers take 68 MB of the cache.
+With ``time_axis`` q and k of the global blocks turn by (time, height, width)
+positions (:func:`~qvggt_b200.kv_cache.rope_axes`) in place of the model's
+(height, width); the frame blocks, whose tokens all have one time, keep the
+model's.  A 518 x 518 frame's K/V of all 24 layers take 68 MB of the cache.
 
     python -m qvggt_b200.streaming [--frames N] [--depth D] [--time-axis]
 
@@ -46,7 +47,7 @@ class StreamingRunner(AggregatorRunner):
                                   block_size, self.device)
         self.time_axis = time_axis
         if time_axis:
-            # the projection's own RoPE turns by nothing; rope_axes follows it
+            # the global blocks' projection turns by nothing; rope_axes follows it
             self.cos, self.sin = torch.ones_like(self.cos), torch.zeros_like(self.sin)
             self.sections = (8, 12, 12)
             self.inv_freq = torch.cat([cfg.rope_base ** (-torch.arange(n, dtype=torch.float32) / n)
