@@ -16,7 +16,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def reference_path() -> str | None:
-    """The reference checkout directory, or None when it is not present."""
+    """The reference checkout directory, or None when it is not present (or empty, as an unfilled mount is)."""
     p = os.environ.get("QVGGT_REFERENCE")
     if not p:
         try:
@@ -24,4 +24,4 @@ def reference_path() -> str | None:
                 p = json.load(f).get("reference_path")
         except (OSError, ValueError):
             p = None
-    return p if p and os.path.isdir(p) else None
+    return p if p and os.path.isdir(p) and os.listdir(p) else None
