@@ -315,7 +315,11 @@ __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 2) attn_cache_rows_ker
         uint32_t pb[NT][2][2];
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-          float cx[2] = {BF16 ? uck * row_ck[x][0] : uck, BF16 ? uck * row_ck[x][1] : uck}, ix[2] = {uinv, uinv}, lx[2] = {ulv, ulv};
+          float cx[2] = {uck, uck}, ix[2] = {uinv, uinv}, lx[2] = {ulv, ulv};
+          if (BF16) {                     // (small rows over small keys: 2^-110 times 2^-60 and less)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) cx[e] = nonzero_factor(uck * row_ck[x][e]);
+          }
           if (key0 + UNIT > all) {        // warp-uniform
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)

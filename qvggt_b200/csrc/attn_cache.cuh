@@ -64,6 +64,11 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
   return BF16 ? codes_bf16<HI>(w) : codes_f16<HI>(w ^ 0x80808080u);
 }
 
+// A score's factor (scales times a power of two) kept from rounding to 0: a
+// hidden key's -inf times 0 would be NaN.  What it is raised to is 0 for a
+// score all the same, |q . c| being under 2^28 where this is called.  NaN stays.
+__device__ __forceinline__ float nonzero_factor(float x) { return x < 1.17549435e-38f ? 1.17549435e-38f : x; }
+
 __device__ __forceinline__ bool lengths_ok(const CacheAttnArgs& a, int q0, int ql, int n) {
   if (q0 >= 0 && ql >= 0 && ql <= a.max_q && (long long)q0 + ql <= a.Tq && n >= 0 && n <= (a.wide << a.bs_log2)) return true;
   report_status(a.ctl, ST_BAD_LENGTH);

@@ -1,0 +1,69 @@
+"""GPU: the streaming K/V cache operators where their numbers or their inputs leave the ordinary range."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_cache as ok
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TINY = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126}     # half the smallest step
+DTYPES = [torch.float16, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def kc():
+    from qvggt_b200 import _lib, kv_cache
+    _lib.device_status(clear=True)
+    yield kv_cache
+    assert _lib.device_status(clear=True) == 0
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def _one_request(seed, ql, n, hq, hk, D, bs, dtype):
+    """q and a cache of one request whose blocks are shuffled."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    nb = -(-n // bs)
+    kcodes, vcodes = (torch.randint(-127, 128, (nb + 3, hk, bs, D), generator=g, device="cuda", dtype=torch.int8)
+                      for _ in range(2))
+    ks, vs = (torch.exp(0.7 * torch.randn(nb + 3, hk, generator=g, device="cuda")) / 80 for _ in range(2))
+    q = torch.randn(ql, hq, D, generator=g, device="cuda").to(dtype)
+    table = torch.randperm(nb + 3, generator=g, device="cuda")[None, :nb].to(torch.int32).contiguous()
+    return q, kcodes, vcodes, ks, vs, table, ints([0, ql]), ints([n])
+
+
+def _check(got, lse, ref, dtype, vmax, n):
+    """As in test_gpu_kv_cache: output rounding; the weights' fp16 rounding 2^-11 and the scores' and exponentials'
+    2^-13, of sum w |v|; weights under fp16's normal range, 2^-25 of the largest |v| for each key."""
+    out, want_lse, mag = ref
+    bound = U[dtype] * out.abs() * 1.01 + (2.0 ** -11 + 2.0 ** -13) * mag + n * 2.0 ** -25 * vmax + TINY[dtype]
+    assert torch.isfinite(got).all() and torch.isfinite(lse).all()
+    assert ((got.double() - out).abs() <= bound).all(), float(((got.double() - out).abs() / bound).max())
+    assert ((lse.double() - want_lse).abs() <= 2e-4).all()
+
+
+# --------------------------------------------------------------- tiny scores
+@pytest.mark.parametrize("chunk", [0, 1])
+@pytest.mark.parametrize("ql,n", [(1, 1), (1, 31), (1, 33), (3, 100), (16, 47), (140, 200)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [0.0, 2.0 ** -100])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_queries_and_keys_of_nothing(kc, dtype, size, D, ql, n, chunk):
+    """Zero (or, in bf16, tiny) queries over keys stored with the smallest scale, a unit of 32 keys seen in part: every
+    visible key weighs the same.  (fp16 holds no 2^-100: zeros again.)"""
+    q, kcodes, vcodes, ks, vs, table, cu, lens = _one_request(D + n, ql, n, 2, 1, D, 32, dtype)
+    q = (q.float() * size).to(dtype)
+    if size == 0:
+        kcodes.zero_()
+    ks.fill_(2.0 ** -60)
+    args = (q, kcodes, vcodes, ks, vs, table, cu, lens)
+    lse = torch.empty(2, ql, device="cuda")
+    got = kc.cached_attention(*args, ql, n, chunk, lse=lse)
+    ref = ok.cached_attention(*args, chunk)
+    none = torch.isinf(ref[1]).t()                # (a causal query before the first key)
+    assert not none.any()
+    _check(got, lse, ref, dtype, float(vs.max() * 127), n)
