@@ -157,6 +157,7 @@ __global__ void __launch_bounds__(RowLay<D, NT>::THREADS, 2) attn_cache_rows_ker
       const bool good = id >= 0 && id < a.num_blocks;
       const float vs = good ? a.vs[(long long)id * a.hk + kvh] : 1.f;
       ck = good ? a.ks[(long long)id * a.hk + kvh] * a.scale_log2 : 1.f;
+      if (!BF16) ck = nonzero_factor(ck);   // (bf16: with the row's own factor, below)
       lv = log2f(vs);
       inv_vs = 1.f / vs;
     };

@@ -65,8 +65,8 @@ __device__ __forceinline__ uint32_t codes2(uint32_t w) {
 }
 
 // A score's factor (scales times a power of two) kept from rounding to 0: a
-// hidden key's -inf times 0 would be NaN.  What it is raised to is 0 for a
-// score all the same, |q . c| being under 2^28 where this is called.  NaN stays.
+// hidden key's -inf times 0 would be NaN.  What it is raised to leaves a score
+// 0 all the same (|q . c| is under 2^30 for fp16 queries).  NaN stays.
 __device__ __forceinline__ float nonzero_factor(float x) { return x < 1.17549435e-38f ? 1.17549435e-38f : x; }
 
 __device__ __forceinline__ bool lengths_ok(const CacheAttnArgs& a, int q0, int ql, int n) {

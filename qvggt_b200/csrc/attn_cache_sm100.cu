@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (lane < CH) {
             const bool have = cid >= 0 && cid < a.num_blocks && key0 + 32 * lane < n;
             // a skipped block: every score -inf
-            const float4 k = have ? make_float4(cks * a.scale_log2, log2f(cvs), 1.f / cvs, 0.f)
+            const float4 k = have ? make_float4(nonzero_factor(cks * a.scale_log2), log2f(cvs), 1.f / cvs, 0.f)
                                   : make_float4(1.f, -INFINITY, 0.f, 0.f);
             reinterpret_cast<float4*>(smem + L::CONST)[(jg % CRING) * CH + lane] = k;
           }

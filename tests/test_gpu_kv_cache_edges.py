@@ -67,3 +67,16 @@ def test_queries_and_keys_of_nothing(kc, dtype, size, D, ql, n, chunk):
     none = torch.isinf(ref[1]).t()                # (a causal query before the first key)
     assert not none.any()
     _check(got, lse, ref, dtype, float(vs.max() * 127), n)
+
+
+@pytest.mark.parametrize("ql,n", [(1, 17), (3, 100), (140, 200)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_scale_as_small_as_it_may_be(kc, dtype, D, ql, n):
+    """A scale near the smallest that is accepted: times a block's smallest scale it is no float any more, and every
+    visible key weighs the same."""
+    args = _one_request(D + ql, ql, n, 2, 1, D, 32, dtype)
+    args[3].fill_(2.0 ** -60)
+    lse = torch.empty(2, ql, device="cuda")
+    got = kc.cached_attention(*args, ql, n, 1, scale=2e-30, lse=lse)
+    _check(got, lse, ok.cached_attention(*args, 1, scale=2e-30), dtype, float(args[4].max() * 127), n)
