@@ -341,7 +341,9 @@ int qvggt_rope_axes(const qvggt_rope_axes_args* args, void* stream);
  * token in request order, then -1; status[0].
  * status: 0 done; otherwise nothing is changed, no token gets a slot and
  * lens_out = cached_lens: 1 too few free blocks, 2 a table row too short, 3 a
- * negative length, 4 more than max_new tokens.  One launch, no host
+ * negative length, 4 more than max_new tokens, 5 free_range is not 0 <= first <=
+ * second <= first + num_blocks or more blocks come back than it leaves room for
+ * (lengths that do not fit the pool).  One launch, no host
  * synchronisation; the same inputs give the same result again.  At most 8192
  * requests; block_size a power of two.  New entry point. */
 typedef struct {

@@ -55,6 +55,8 @@ def block_plan(cached, target, table, ring, free_range, bs, max_new):
         status = 2
     elif sum(max(0, t - c) for c, t in zip(cached, target)) > max_new:
         status = 4
+    elif not 0 <= head <= tail <= head + n or sum(max(0, blocks(c) - blocks(t)) for c, t in zip(cached, target)) > n - (tail - head):
+        status = 5
     elif sum(max(0, blocks(t) - blocks(c)) for c, t in zip(cached, target)) > tail - head:
         status = 1
     slots, cu_new, cu_blocks = [], [0], [0]

@@ -15,7 +15,9 @@ namespace {
 constexpr int PLAN_THREADS = 512;
 constexpr int PLAN_MAX_REQUESTS = 8192;   // 4 prefix arrays of it fit shared memory
 
-enum : int32_t { PLAN_OK = 0, PLAN_NO_BLOCKS = 1, PLAN_TABLE_FULL = 2, PLAN_BAD_LENGTH = 3, PLAN_MORE_TOKENS = 4 };
+enum : int32_t {
+  PLAN_OK = 0, PLAN_NO_BLOCKS = 1, PLAN_TABLE_FULL = 2, PLAN_BAD_LENGTH = 3, PLAN_MORE_TOKENS = 4, PLAN_BAD_POOL = 5
+};
 
 struct PlanArgs {
   const int32_t *cached, *target;
@@ -107,10 +109,15 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(PlanArgs a) {
   int flags = bad;
   if (total.new_tok > a.most || total.new_tok < 0) flags |= 1 << PLAN_MORE_TOKENS;
   if (total.grow > tail - head || total.grow < 0) flags |= 1 << PLAN_NO_BLOCKS;
+  // The free blocks and those given back have to fit the ring: then no place of
+  // it is written that holds a free block, nor one outside it.
+  if (head < 0 || tail < head || tail - head > a.num_blocks || total.drop > a.num_blocks - (tail - head))
+    flags |= 1 << PLAN_BAD_POOL;
   // the first reason in this order is reported
   const int status = flags & (1 << PLAN_BAD_LENGTH)    ? PLAN_BAD_LENGTH
                      : flags & (1 << PLAN_TABLE_FULL)  ? PLAN_TABLE_FULL
                      : flags & (1 << PLAN_MORE_TOKENS) ? PLAN_MORE_TOKENS
+                     : flags & (1 << PLAN_BAD_POOL)    ? PLAN_BAD_POOL
                      : flags & (1 << PLAN_NO_BLOCKS)   ? PLAN_NO_BLOCKS
                                                        : PLAN_OK;
   const bool ok = status == PLAN_OK;

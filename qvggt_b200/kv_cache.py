@@ -42,7 +42,8 @@ _LAYOUTS = {"axial": 0, "split": 1, "interleaved": 2}
 _I32, _F32 = torch.int32, torch.float32
 
 PLAN_STATUS = {0: "done", 1: "too few free blocks", 2: "a request needs more blocks than its table row holds",
-               3: "a negative length", 4: "more new tokens than max_new"}
+               3: "a negative length", 4: "more new tokens than max_new",
+               5: "the free range is no range of the ring, or more blocks come back than are out"}
 
 # The argument structures of include/qvggt_b200.h: 64-bit fields only.  Packed
 # in one go: converting some thirty ctypes arguments took longer than the rest

@@ -80,3 +80,47 @@ def test_scale_as_small_as_it_may_be(kc, dtype, D, ql, n):
     lse = torch.empty(2, ql, device="cuda")
     got = kc.cached_attention(*args, ql, n, 1, scale=2e-30, lse=lse)
     _check(got, lse, ok.cached_attention(*args, 1, scale=2e-30), dtype, float(args[4].max() * 127), n)
+
+
+# ------------------------------------------------------------------- plan
+def _plan(kc, cached, target, table, ring, free, bs, max_new, guard=16):
+    """block_plan with guard words on both sides of the ring and the table; checks them and that the call repeats."""
+    def guarded(a):
+        buf = torch.full((a.size + 2 * guard,), -77, dtype=torch.int32, device="cuda")
+        buf[guard:guard + a.size] = torch.tensor(a.reshape(-1), device="cuda")
+        return buf, buf[guard:guard + a.size].view(a.shape)
+    (tb, t), (rb, r) = guarded(table), guarded(ring)
+    c, g, f = ints(cached), ints(target), torch.tensor(free, dtype=torch.int64, device="cuda")
+    outs = []
+    for _ in range(2):
+        p = kc.block_plan(c, g, t, r, f, bs, max_new)
+        outs.append(dict(table=t.tolist(), ring=r.tolist(), slots=p.slots.tolist(), cu_new=p.cu_new.tolist(),
+                         cu_blocks=p.cu_blocks.tolist(), lens=p.lens.tolist(), free_range=p.free_range.tolist(),
+                         status=p.status.item()))
+        for buf in (tb, rb):
+            assert (buf[:guard] == -77).all() and (buf[-guard:] == -77).all()
+    assert outs[0] == outs[1]
+    return outs[0]
+
+
+def _same(got, want):
+    want = dict(want, table=want["table"].tolist(), ring=want["ring"].tolist())
+    for key in want:
+        assert got[key] == want[key], key
+
+
+@pytest.mark.parametrize("cached,target,free,status", [
+    ([64, 96, 96], [0, 0, 0], [2, 4], 5),        # eight blocks come back into a ring of four that has two free
+    ([96, 96, 96], [0, 0, 0], [3, 5], 5),        # nine: the last would land behind the ring
+    ([64, 64, 0], [32, 0, 0], [1, 3], 5),        # three into room for two: would overwrite a free one
+    ([64, 0, 0], [0, 64, 0], [1, 3], 0),         # two back into room for two, two taken
+    ([32, 0, 0], [64, 0, 0], [-3, 1], 5), ([32, 0, 0], [64, 0, 0], [3, 2], 5), ([32, 0, 0], [32, 0, 0], [3, 2], 5),
+    ([32, 0, 0], [64, 64, 64], [0, 5], 5), ([32, 0, 0], [64, 64, 64], [2 ** 62, 2 ** 62 + 4], 1),
+    ([32, 0, 0], [64, 64, 32], [2 ** 62 + 1, 2 ** 62 + 5], 0), ([64, 64, -1], [0, 0, 0], [0, 4], 3)])
+def test_plan_refuses_lengths_and_ranges_that_do_not_fit_the_pool(kc, cached, target, free, status):
+    """Stale lengths or a range out of order: all or nothing, and nothing outside the ring is touched."""
+    table = np.array([[3, 2, 0], [1, 0, 3], [2, 1, 1]], np.int32)
+    ring = np.arange(4, dtype=np.int32)
+    want = ok.block_plan(cached, target, table, ring, free, 32, 200)
+    assert want["status"] == status
+    _same(_plan(kc, cached, target, table, ring, free, 32, 200), want)
