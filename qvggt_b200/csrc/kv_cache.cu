@@ -29,10 +29,14 @@ struct PlanArgs {
   int B, wide, bs, num_blocks, most;
 };
 
+// New tokens and blocks given back add up to at most 2^32 - 1 and stay there:
+// 8192 requests' can be more than 32 bits hold, and no sum that large is served.
+// (The other two counts are not above the new tokens.)
+__device__ __forceinline__ unsigned add_sat(unsigned a, unsigned b) { return a + b < a ? ~0u : a + b; }
 struct Quad {
-  int new_tok, grow, drop, touched;
+  unsigned new_tok, grow, drop, touched;
   __device__ Quad operator+(const Quad& o) const {
-    return {new_tok + o.new_tok, grow + o.grow, drop + o.drop, touched + o.touched};
+    return {add_sat(new_tok, o.new_tok), grow + o.grow, add_sat(drop, o.drop), touched + o.touched};
   }
 };
 __device__ __forceinline__ Quad shfl_up(const Quad& v, int d) {
@@ -43,7 +47,8 @@ __device__ __forceinline__ Quad shfl_up(const Quad& v, int d) {
 // What request i contributes when it goes from `c` to `t` tokens.
 __device__ __forceinline__ Quad plan_counts(int c, int t, int bs) {
   const int have = (int)(((long long)c + bs - 1) / bs), need = (int)(((long long)t + bs - 1) / bs);
-  return {max(t - c, 0), max(need - have, 0), max(have - need, 0), t > c ? (t - 1) / bs - c / bs + 1 : 0};
+  return {(unsigned)max(t - c, 0), (unsigned)max(need - have, 0), (unsigned)max(have - need, 0),
+          t > c ? (unsigned)((t - 1) / bs - c / bs + 1) : 0u};
 }
 
 // Largest i in [0, n) with a[i] <= x (a[0] = 0 <= x, a non-decreasing).
@@ -78,7 +83,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(PlanArgs a) {
   __syncthreads();
   Quad sum{0, 0, 0, 0};
   int my_bad = 0;
-  unsigned long long tokens = 0;
   for (int i = i0; i < i1; ++i) {
     const int c = a.cached[i], t = a.target[i];
     if (c < 0 || t < 0) {
@@ -87,8 +91,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(PlanArgs a) {
     }
     if (((long long)t + a.bs - 1) / a.bs > a.wide || ((long long)c + a.bs - 1) / a.bs > a.wide)
       my_bad |= 1 << PLAN_TABLE_FULL;
-    tokens += t > c ? t - c : 0;
-    if (tokens > (unsigned long long)a.most) my_bad |= 1 << PLAN_MORE_TOKENS;
     sum = sum + plan_counts(c, t, a.bs);
   }
   if (my_bad) atomicOr(&bad, my_bad);
@@ -107,11 +109,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(PlanArgs a) {
   }
   const long long head = a.free_range[0], tail = a.free_range[1];
   int flags = bad;
-  if (total.new_tok > a.most || total.new_tok < 0) flags |= 1 << PLAN_MORE_TOKENS;
-  if (total.grow > tail - head || total.grow < 0) flags |= 1 << PLAN_NO_BLOCKS;
+  if (total.new_tok > (unsigned)a.most) flags |= 1 << PLAN_MORE_TOKENS;
+  if ((long long)total.grow > tail - head) flags |= 1 << PLAN_NO_BLOCKS;
   // The free blocks and those given back have to fit the ring: then no place of
   // it is written that holds a free block, nor one outside it.
-  if (head < 0 || tail < head || tail - head > a.num_blocks || total.drop > a.num_blocks - (tail - head))
+  if (head < 0 || tail < head || tail - head > a.num_blocks ||
+      (long long)total.drop > a.num_blocks - (tail - head))
     flags |= 1 << PLAN_BAD_POOL;
   // the first reason in this order is reported
   const int status = flags & (1 << PLAN_BAD_LENGTH)    ? PLAN_BAD_LENGTH
@@ -122,6 +125,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(PlanArgs a) {
                                                        : PLAN_OK;
   const bool ok = status == PLAN_OK;
   if (!ok) total = Quad{0, 0, 0, 0};
+  const int new_tok = (int)total.new_tok, grow = (int)total.grow, drop = (int)total.drop;
   Quad run = base + Quad{inc.new_tok - sum.new_tok, inc.grow - sum.grow, inc.drop - sum.drop,
                          inc.touched - sum.touched};
   for (int i = i0; i < i1; ++i) {
@@ -134,9 +138,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(PlanArgs a) {
     if (ok) run = run + plan_counts(c, t, a.bs);
   }
   if (tid == 0) {
-    cu_new[a.B] = total.new_tok;
-    first[a.B] = total.grow;
-    freed[a.B] = total.drop;
+    cu_new[a.B] = new_tok;
+    first[a.B] = grow;
+    freed[a.B] = drop;
     cu_blk[a.B] = total.touched;
   }
   __syncthreads();
@@ -146,8 +150,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(PlanArgs a) {
       a.cu_blocks[i] = cu_blk[i];
     }
     if (tid == 0) {
-      a.free_out[0] = head + total.grow;
-      a.free_out[1] = tail + total.drop;
+      a.free_out[0] = head + grow;
+      a.free_out[1] = tail + drop;
       a.status[0] = status;
     }
   }
@@ -159,21 +163,21 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(PlanArgs a) {
   };
   for (int n = gtid; n < a.most; n += gsize) {
     int slot = -1;
-    if (n < total.new_tok) {
+    if (n < new_tok) {
       const int b = last_le(cu_new, a.B, n);
-      const int c = a.cached[b], pos = c + n - cu_new[b];
+      const int c = a.cached[b], pos = c + (n - cu_new[b]);
       const int have = (c + a.bs - 1) / a.bs, j = pos / a.bs;
       const int blk = j < have ? a.table[(long long)b * a.wide + j] : a.ring[ring_at(head_m, first[b] + j - have)];
       slot = blk * a.bs + pos - j * a.bs;
     }
     a.slots[n] = slot;
   }
-  for (int n = gtid; n < total.grow; n += gsize) {
+  for (int n = gtid; n < grow; n += gsize) {
     const int b = last_le(first, a.B, n);
     const int have = (a.cached[b] + a.bs - 1) / a.bs;
     a.table[(long long)b * a.wide + have + n - first[b]] = a.ring[ring_at(head_m, n)];
   }
-  for (int n = gtid; n < total.drop; n += gsize) {
+  for (int n = gtid; n < drop; n += gsize) {
     const int b = last_le(freed, a.B, n);
     const int need = (a.target[b] + a.bs - 1) / a.bs;
     a.ring[ring_at(tail_m, n)] = a.table[(long long)b * a.wide + need + n - freed[b]];

@@ -124,3 +124,20 @@ def test_plan_refuses_lengths_and_ranges_that_do_not_fit_the_pool(kc, cached, ta
     want = ok.block_plan(cached, target, table, ring, free, 32, 200)
     assert want["status"] == status
     _same(_plan(kc, cached, target, table, ring, free, 32, 200), want)
+
+
+@pytest.mark.parametrize("bs,wide,num,first", [(2 ** 20, 8, 2047, 0), (2 ** 24, 1, 127, 1)])
+def test_plan_counts_more_tokens_than_32_bits_hold(kc, bs, wide, num, first):
+    """512 requests of 2^23 new tokens each: 2^32 in all, far over max_new, which holds one of them."""
+    B, most = 512, 2 ** 23
+    table = torch.zeros(B, wide, dtype=torch.int32, device="cuda")
+    ring = torch.arange(num, dtype=torch.int32, device="cuda")
+    cached = torch.full((B,), first, dtype=torch.int32, device="cuda")
+    free = torch.tensor([0, num], dtype=torch.int64, device="cuda")
+    p = kc.block_plan(cached, cached + most, table, ring, free, bs, most)
+    assert p.status.item() == 4
+    assert (p.cu_new == 0).all() and (p.slots == -1).all() and torch.equal(p.lens, cached)
+    p = kc.block_plan(cached[:1], cached[:1] + most, table[:1], ring, free, bs, most)      # one of them is served
+    assert p.status.item() == 0 and p.cu_new.tolist() == [0, most] and torch.equal(p.lens, cached[:1] + most)
+    want = first + torch.arange(most, device="cuda")       # blocks 0, 1, ... of the ring, or block 0 of the table
+    assert torch.equal(p.slots.long(), want)
