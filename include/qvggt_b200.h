@@ -343,7 +343,9 @@ int qvggt_rope_axes(const qvggt_rope_axes_args* args, void* stream);
  * lens_out = cached_lens: 1 too few free blocks, 2 a table row too short, 3 a
  * negative length, 4 more than max_new tokens, 5 free_range is not 0 <= first <=
  * second <= first + num_blocks or more blocks come back than it leaves room for
- * (lengths that do not fit the pool).  One launch, no host
+ * (lengths that do not fit the pool).  Block ids are handed on as they stand;
+ * one outside the cache sets the device status word (0x201) and gives its
+ * tokens the slot -1.  One launch, no host
  * synchronisation; the same inputs give the same result again.  At most 8192
  * requests; block_size a power of two.  New entry point. */
 typedef struct {

@@ -27,6 +27,7 @@ struct PlanArgs {
   int32_t *slots, *cu_new, *cu_blocks, *lens, *status;
   long long* free_out;
   int B, wide, bs, num_blocks, most;
+  Ctl ctl;
 };
 
 // New tokens and blocks given back add up to at most 2^32 - 1 and stay there:
@@ -161,6 +162,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(PlanArgs a) {
     const int x = from + off;
     return x >= a.num_blocks ? x - a.num_blocks : x;
   };
+  // Block ids are handed on as they stand; one outside the cache is reported,
+  // and its tokens get no slot (a product of it could look like one).
+  auto in_cache = [&](int blk) {
+    if (blk >= 0 && blk < a.num_blocks) return true;
+    report_bad_block(a.ctl);
+    return false;
+  };
   for (int n = gtid; n < a.most; n += gsize) {
     int slot = -1;
     if (n < new_tok) {
@@ -168,19 +176,23 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_plan_kernel(PlanArgs a) {
       const int c = a.cached[b], pos = c + (n - cu_new[b]);
       const int have = (c + a.bs - 1) / a.bs, j = pos / a.bs;
       const int blk = j < have ? a.table[(long long)b * a.wide + j] : a.ring[ring_at(head_m, first[b] + j - have)];
-      slot = blk * a.bs + pos - j * a.bs;
+      if (in_cache(blk)) slot = blk * a.bs + pos - j * a.bs;
     }
     a.slots[n] = slot;
   }
   for (int n = gtid; n < grow; n += gsize) {
     const int b = last_le(first, a.B, n);
     const int have = (a.cached[b] + a.bs - 1) / a.bs;
-    a.table[(long long)b * a.wide + have + n - first[b]] = a.ring[ring_at(head_m, n)];
+    const int blk = a.ring[ring_at(head_m, n)];
+    in_cache(blk);
+    a.table[(long long)b * a.wide + have + n - first[b]] = blk;
   }
   for (int n = gtid; n < drop; n += gsize) {
     const int b = last_le(freed, a.B, n);
     const int need = (a.target[b] + a.bs - 1) / a.bs;
-    a.ring[ring_at(tail_m, n)] = a.table[(long long)b * a.wide + need + n - freed[b]];
+    const int blk = a.table[(long long)b * a.wide + need + n - freed[b]];
+    in_cache(blk);
+    a.ring[ring_at(tail_m, n)] = blk;
   }
 }
 
@@ -441,7 +453,7 @@ extern "C" int qvggt_block_plan(const qvggt_block_plan_args* p, void* stream) {
   PlanArgs a{p->cached_lens, p->target_lens, p->block_tables, p->free_ring,
              reinterpret_cast<const long long*>(p->free_range), p->slots, p->cu_new, p->cu_blocks, p->lens_out,
              p->status, reinterpret_cast<long long*>(p->free_range_out), (int)p->requests, (int)p->max_blocks,
-             (int)p->block_size, (int)p->num_blocks, (int)p->max_new};
+             (int)p->block_size, (int)p->num_blocks, (int)p->max_new, make_ctl()};
   const int smem = 4 * (a.B + 1) * (int)sizeof(int);
   static DeviceFlags attr;
   if (int rc = ensure_smem(attr, block_plan_kernel, 4 * (PLAN_MAX_REQUESTS + 1) * (int)sizeof(int),

@@ -193,8 +193,10 @@ def block_plan(cached_lens, target_lens, block_tables, free_ring, free_range, bl
     ``free_range[1]``, int64 ``[2]``, modulo its size); one that shrinks (0:
     ends) gives its surplus blocks back.  ``block_tables`` (int32 ``[B,
     max_blocks]``) and ``free_ring`` are updated in place, the rest is
-    returned; if a request cannot be served nothing is changed and ``status``
-    says why.  ``max_new`` bounds the new tokens."""
+    returned; if a request cannot be served, or the lengths and the free range
+    do not fit the pool, nothing is changed and ``status`` says why.  Block ids
+    are handed on as they stand; one outside the pool sets the status word
+    (0x201) and its tokens get the slot -1.  ``max_new`` bounds the new tokens."""
     name = "block_plan"
     dev = cached_lens.get_device()
     if dev < 0 or not (dev == target_lens.get_device() == block_tables.get_device() == free_ring.get_device()

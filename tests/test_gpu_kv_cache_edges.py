@@ -141,3 +141,22 @@ def test_plan_counts_more_tokens_than_32_bits_hold(kc, bs, wide, num, first):
     assert p.status.item() == 0 and p.cu_new.tolist() == [0, most] and torch.equal(p.lens, cached[:1] + most)
     want = first + torch.arange(most, device="cuda")       # blocks 0, 1, ... of the ring, or block 0 of the table
     assert torch.equal(p.slots.long(), want)
+
+
+@pytest.mark.parametrize("cached,target,where,bad,lost", [
+    ([10, 64], [40, 64], "ring", 4, range(22, 30)),          # taken: the second block's tokens have no slot
+    ([10, 64], [40, 64], "table", -1, range(0, 22)),         # held: those that go into the first block
+    ([10, 64], [20, 0], "table", 2 ** 27 + 1, range(0, 10)), # times 32 it wraps to the slot 32
+    ([32, 64], [32, 0], "returned", 4, [])])                 # given back
+def test_plan_reports_block_ids_outside_the_pool(kc, cached, target, where, bad, lost):
+    from qvggt_b200 import _lib
+    table, ring, free = np.array([[3, -1], [1, 0]], np.int32), np.array([2, 9, 9, 9], np.int32), [0, 1]
+    if where == "ring":
+        ring[0] = bad
+    else:
+        table[(0, 0) if where == "table" else (1, 1)] = bad
+    want = ok.block_plan(cached, target, table, ring, free, 32, 40)
+    want["slots"] = [-1 if i in lost else x for i, x in enumerate(want["slots"])]
+    assert want["status"] == 0
+    _same(_plan(kc, cached, target, table, ring, free, 32, 40), want)
+    assert _lib.device_status(clear=True) == 0x201
