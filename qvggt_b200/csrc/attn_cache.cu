@@ -51,7 +51,8 @@ struct RowBlock {
     nqt = 1;
     tiles = 0;
     cost = 0;
-    if (tok0 >= (long long)ql * a.group || !lengths_ok(a, q0, ql, n)) return;
+    // (a negative number of queries is for lengths_ok to report)
+    if ((ql >= 0 && tok0 >= (long long)ql * a.group) || !lengths_ok(a, q0, ql, n)) return;
     const int last = (min(ql * a.group, tok0 + RowLay<D, NT>::ROWS) - 1) / a.group;
     tiles = (key_limit(last, ql, n, a.chunk) + UNIT - 1) / UNIT;
     cost = START + (long long)tiles;

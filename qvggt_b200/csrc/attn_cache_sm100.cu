@@ -196,8 +196,8 @@ struct Block {
     nqt = tok0 + tpt < ql ? 2 : 1;
     tiles = 0;
     cost = 0;
-    if (tok0 >= ql) return;
-    if (!lengths_ok(a, q0, ql, n)) return;
+    // (a negative number of queries is for lengths_ok to report)
+    if ((ql >= 0 && tok0 >= ql) || !lengths_ok(a, q0, ql, n)) return;
     tiles = (key_limit(min(ql, tok0 + 2 * tpt) - 1, ql, n, a.chunk) + KT - 1) / KT;
     cost = COST_START + (long long)tiles * tile_cost();
   }

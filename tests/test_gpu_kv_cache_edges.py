@@ -160,3 +160,20 @@ def test_plan_reports_block_ids_outside_the_pool(kc, cached, target, where, bad,
     assert want["status"] == 0
     _same(_plan(kc, cached, target, table, ring, free, 32, 40), want)
     assert _lib.device_status(clear=True) == 0x201
+
+
+# ------------------------------------------------------- lengths out of order
+@pytest.mark.parametrize("ql", [3, 80])
+def test_attention_reports_decreasing_query_starts(kc, ql):
+    """A request with a negative number of queries is skipped and reported; its neighbours are served."""
+    from qvggt_b200 import _lib
+    q, kcodes, vcodes, ks, vs, table, _, _ = _one_request(3, 3 * ql, 90, 2, 2, 64, 32, torch.float16)
+    three, lens = table.expand(3, -1).contiguous(), ints([90, 70, 50])
+    args = (q, kcodes, vcodes, ks, vs, three)
+    got = kc.cached_attention(*args, ints([0, ql, ql - 2, 2 * ql]), lens, ql + 2, 90)
+    assert _lib.device_status(clear=True) == 0x202
+    want = kc.cached_attention(*args, ints([0, ql, ql, 2 * ql]), lens, ql + 2, 90)
+    assert _lib.device_status(clear=True) == 0
+    assert torch.equal(got[:ql - 2], want[:ql - 2])       # rows [ql - 2, ql) belong to two requests here
+    part = kc.cached_attention(*args, ints([0, 0, ql - 2, 2 * ql]), lens, ql + 2, 90)
+    assert torch.equal(got[ql:2 * ql], part[ql:2 * ql])
