@@ -212,7 +212,8 @@ struct AppendArgs {
   Ctl ctl;
 };
 
-// Largest i in [0, n) with a[i] <= x, a whole warp looking at 32 places at a time.
+// Largest i in [0, n) with a[i] <= x, a whole warp looking at 32 places at a
+// time; a place in [0, n) whatever a holds.
 __device__ __forceinline__ int warp_last_le(const int32_t* a, int n, int x) {
   const int lane = threadIdx.x % 32;
   int lo = 0;
@@ -220,7 +221,7 @@ __device__ __forceinline__ int warp_last_le(const int32_t* a, int n, int x) {
     const int step = (n + 31) / 32;
     const int at = lane * step;
     const unsigned le = __ballot_sync(~0u, at < n && a[lo + at] <= x);
-    const int k = 31 - __clz(le);        // a[lo] <= x always
+    const int k = 31 - __clz(le | 1);    // a[lo] <= x, if a is what it should be
     lo += k * step;
     n = min(step, n - k * step);
   }
@@ -263,11 +264,15 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(AppendArgs a)
   const int side = threadIdx.x / APPEND_SIDE, th = threadIdx.x % APPEND_SIDE;
   if (unit >= a.cu_blocks[a.B]) return;
   const int b = warp_last_le(a.cu_blocks, a.B, unit);
-  const int c = a.cached[b], n0 = a.cu_new[b], end = c + a.cu_new[b + 1] - n0;
-  const int j = c / a.bs + unit - a.cu_blocks[b];
-  const int lo = max(c, j * a.bs), hi = min(end, (j + 1) * a.bs);      // new tokens of the block
-  const int blk = j < a.wide ? a.table[(long long)b * a.wide + j] : -1;
-  const bool lengths = c >= 0 && n0 >= 0 && hi > lo && (long long)n0 + end - c <= a.tokens;
+  const int c = a.cached[b], n0 = a.cu_new[b], n1 = a.cu_new[b + 1];
+  // the block's place in the request's row of the table; outside it where a
+  // length is negative or too large or the running sums are out of order
+  const int j = (int)((unsigned)(c / a.bs) + (unsigned)unit - (unsigned)a.cu_blocks[b]);
+  const bool in_row = (unsigned)j < (unsigned)a.wide;
+  const int blk = in_row ? a.table[(long long)b * a.wide + j] : -1;
+  const int start = in_row ? j * a.bs : 0;
+  const int lo = max(c, start), hi = (int)min((long long)c + n1 - n0, (long long)start + a.bs);  // new tokens of the block
+  const bool lengths = in_row && c >= 0 && n0 >= 0 && n1 <= a.tokens && hi > lo;
   // 8 or 16 16-byte pieces to a row; a thread's pieces are 16 or 8 rows apart
   const int row_log2 = a.D == 64 ? 3 : 4, pieces = lengths ? (hi - lo) << row_log2 : 0;
   const long long stride = side ? a.tok_stride[1] : a.tok_stride[0];
@@ -292,7 +297,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(AppendArgs a)
 #pragma unroll
     for (int e = 0; e < 4; ++e) m = __vmaxu2(m, w[e] & 0x7fff7fffu);
   }
-  const int older = lo - j * a.bs;                                     // earlier tokens of the block
+  const int older = lo - start;                                        // earlier tokens of the block
   int8_t* codes = (side ? a.codes[1] : a.codes[0]) + blk * a.block_stride + (long long)h * a.bs * a.D;
   float* scale = (side ? a.scales[1] : a.scales[0]) + (long long)blk * a.heads + h;
   const float before = older > 0 ? *scale : 0.f;
@@ -474,7 +479,7 @@ extern "C" int qvggt_kv_append(const qvggt_kv_append_args* p, void* stream) {
   if (p->dtype != QVGGT_DTYPE_F16 && p->dtype != QVGGT_DTYPE_BF16)
     return set_error(QVGGT_ERR_UNSUPPORTED, "kv_append: dtype must be fp16 or bf16");
   if (p->tokens < 0 || p->requests < 0 || p->max_blocks < 0 || p->max_units < 0 || p->requests > 2147483646LL ||
-      p->max_blocks > 2147483647LL || p->max_units > 2147483647LL / p->cache.kv_heads)
+      p->max_blocks > 2147483647LL / p->cache.block_size || p->max_units > 2147483647LL / p->cache.kv_heads)
     return set_error(QVGGT_ERR_INVALID, "kv_append: bad shape");
   if (p->tokens == 0 || p->requests == 0 || p->max_units == 0) return QVGGT_OK;
   if (!p->k || !p->v || !p->block_tables || !p->cached_lens || !p->cu_new || !p->cu_blocks)

@@ -177,3 +177,29 @@ def test_attention_reports_decreasing_query_starts(kc, ql):
     assert torch.equal(got[:ql - 2], want[:ql - 2])       # rows [ql - 2, ql) belong to two requests here
     part = kc.cached_attention(*args, ints([0, 0, ql - 2, 2 * ql]), lens, ql + 2, 90)
     assert torch.equal(got[ql:2 * ql], part[ql:2 * ql])
+
+
+@pytest.mark.parametrize("cached,cu_new,cu_blocks,served", [
+    ([-1000, 0], [0, 2, 5], [0, 1, 2], 1), ([-2 ** 31, 0], [0, 2, 5], [0, 1, 2], 1),         # negative lengths
+    ([2 ** 31 - 1, 0], [0, 2, 5], [0, 1, 2], 1), ([64, 0], [0, 2, 5], [0, 1, 2], 1),         # past the row's end
+    ([0, 0], [0, 2, 5], [900, 901, 902], None), ([0, 0], [0, 2, 5], [40, 1, 2], 1),          # no such blocks
+    ([0, 0], [0, 2, 5], [-2 ** 31, 1, 2], 1), ([0, 0], [5, 2, 0], [0, 1, 2], None),
+    ([0, 0], [-9, -7, 5], [0, 1, 2], None), ([0, 0], [0, 2, 6], [0, 1, 2], 0)])              # no such rows
+def test_append_reports_lengths_out_of_order(kc, cached, cu_new, cu_blocks, served):
+    """Lengths and running sums that no plan gives: what they name is skipped and reported, the other request is served,
+    and no other block is touched."""
+    from qvggt_b200 import _lib
+    g = torch.Generator(device="cuda").manual_seed(1)
+    codes = [np.full((6, 2, 32, 64), 7, np.int8) for _ in range(2)]
+    scales = [np.ones((6, 2), np.float32) for _ in range(2)]
+    dev = [torch.tensor(a, device="cuda") for a in codes + scales]
+    kv = torch.randn(5, 2, 2, 64, generator=g, device="cuda").half()
+    # the table stands between rows that name block 2
+    table = ints([[2, 2], [1, 4], [3, 5], [2, 2]])[1:3]
+    kc.kv_append(kv[:, 0], kv[:, 1], *dev, table, ints(cached), ints(cu_new), ints(cu_blocks), 4)
+    assert _lib.device_status(clear=True) == 0x202
+    for s in range(2):
+        if served is not None:
+            rows = kv[cu_new[served]:cu_new[served + 1], s].cpu()
+            ok.append_f32(rows, codes[s], scales[s], [[1 + 2 * served]], [0], [0, len(rows)])
+        assert (dev[s].cpu().numpy() == codes[s]).all() and (dev[2 + s].cpu().numpy() == scales[s]).all()
