@@ -385,7 +385,8 @@ typedef struct {
  * earlier codes c of the block become rint(c * s_old / s).  Only finite values
  * count in amax; infinities are stored as the largest code, NaN as 0.  A block
  * id or length outside its range sets the device status word (0x201 / 0x202)
- * and skips the block.  New entry point. */
+ * and skips the block; so does a max_units that is too small (0x202, the blocks
+ * past it are not written).  New entry point. */
 typedef struct {
   qvggt_kv_cache cache;
   const void* k;

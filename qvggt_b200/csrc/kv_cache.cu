@@ -208,7 +208,7 @@ struct AppendArgs {
   const int32_t *table, *cached, *cu_new, *cu_blocks;
   long long block_stride;                // codes between blocks
   long long tokens;
-  int B, wide, bs, num_blocks, heads, D;
+  int B, wide, bs, num_blocks, heads, D, max_units;
   Ctl ctl;
 };
 
@@ -262,7 +262,9 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(AppendArgs a)
   // heads fastest: neighbouring CTAs then read neighbouring pieces of the same rows
   const int unit = blockIdx.x / a.heads, h = blockIdx.x - unit * a.heads;
   const int side = threadIdx.x / APPEND_SIDE, th = threadIdx.x % APPEND_SIDE;
-  if (unit >= a.cu_blocks[a.B]) return;
+  const int units = a.cu_blocks[a.B];
+  if (units > a.max_units && blockIdx.x == 0 && threadIdx.x == 0) report_status(a.ctl, ST_BAD_LENGTH);   // some have no CTA
+  if (unit >= units) return;
   const int b = warp_last_le(a.cu_blocks, a.B, unit);
   const int c = a.cached[b], n0 = a.cu_new[b], n1 = a.cu_new[b + 1];
   // the block's place in the request's row of the table; outside it where a
@@ -509,6 +511,7 @@ extern "C" int qvggt_kv_append(const qvggt_kv_append_args* p, void* stream) {
   a.num_blocks = (int)p->cache.num_blocks;
   a.heads = (int)p->cache.kv_heads;
   a.D = (int)p->cache.head_dim;
+  a.max_units = (int)p->max_units;
   a.ctl = make_ctl();
   using Kfn = void (*)(AppendArgs);
   static const Kfn fns[2][4] = {

@@ -244,7 +244,7 @@ def kv_append(k, v, k_cache, v_cache, k_scale, v_scale, block_tables, cached_len
     are the lengths before.  A block's scale grows when its new rows need it,
     and its earlier codes are rounded to the new scale.  ``max_units``: a
     bound of ``cu_blocks[-1]`` if one tighter than ``tokens // block_size + 2
-    * B`` is known."""
+    * B`` is known; blocks past it are not written, and the status word says so."""
     name = "kv_append"
     dev = k.get_device()
     if dev < 0 or not (dev == v.get_device() == k_cache.get_device() == v_cache.get_device() == k_scale.get_device()

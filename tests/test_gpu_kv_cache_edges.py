@@ -203,3 +203,18 @@ def test_append_reports_lengths_out_of_order(kc, cached, cu_new, cu_blocks, serv
             rows = kv[cu_new[served]:cu_new[served + 1], s].cpu()
             ok.append_f32(rows, codes[s], scales[s], [[1 + 2 * served]], [0], [0, len(rows)])
         assert (dev[s].cpu().numpy() == codes[s]).all() and (dev[2 + s].cpu().numpy() == scales[s]).all()
+
+
+def test_append_reports_a_bound_that_is_too_small(kc):
+    """max_units 1 where the new rows touch two blocks: the first is written, the loss of the second reported."""
+    from qvggt_b200 import _lib
+    codes = [torch.zeros(2, 1, 32, 64, dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.ones(2, 1, device="cuda") for _ in range(2)]
+    x = torch.ones(40, 1, 64, device="cuda").half()
+    args = (x, x, *codes, *scales, ints([[1, 0]]), ints([0]), ints([0, 40]), ints([0, 2]))
+    kc.kv_append(*args, 1)
+    assert _lib.device_status(clear=True) == 0x202
+    assert all((c[1] == 127).all() and (c[0] == 0).all() for c in codes)
+    kc.kv_append(*args, 2)
+    assert _lib.device_status(clear=True) == 0
+    assert all((c[1] == 127).all() and (c[0, :, :8] == 127).all() and (c[0, :, 8:] == 0).all() for c in codes)
