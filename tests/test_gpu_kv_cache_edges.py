@@ -218,3 +218,31 @@ def test_append_reports_a_bound_that_is_too_small(kc):
     kc.kv_append(*args, 2)
     assert _lib.device_status(clear=True) == 0
     assert all((c[1] == 127).all() and (c[0, :, :8] == 127).all() and (c[0, :, 8:] == 0).all() for c in codes)
+
+
+# -------------------------------------------------------------------- strides
+@pytest.mark.parametrize("ql", [3, 150])
+@pytest.mark.parametrize("hq,hk,D", [(4, 4, 64), (6, 2, 64), (4, 2, 128)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_takes_queries_in_any_order(kc, dtype, hq, hk, D, ql):
+    """Heads outermost, a token stride that is no multiple of the head stride, one head or one token broadcast: what the
+    same queries give densely (the broadcast ones within the bounds, as another kernel may serve them)."""
+    n, T = 400, ql + 7
+    q, *cache = _one_request(D + hq, T, n, hq, hk, D, 64, dtype)
+    cu, lens = ints([7, T]), ints([n])            # the first rows are no request's
+    args = (*cache[:5], cu, lens, ql, n, 1)
+    want = kc.cached_attention(q, *args)[7:]
+    outermost = q.transpose(0, 1).contiguous().transpose(0, 1)
+    padded = torch.zeros(T, 3 * hq * D + 8, device="cuda", dtype=dtype)[:, 8 + hq * D:8 + 2 * hq * D].view(T, hq, D)
+    spread = torch.zeros(T, hq, 3, D + 8, device="cuda", dtype=dtype)[:, :, 1, :D]
+    out = torch.zeros(hq, T, D + 8, device="cuda", dtype=dtype).transpose(0, 1)[..., :D]
+    for x in (outermost, padded.copy_(q), spread.copy_(q)):
+        assert torch.equal(kc.cached_attention(x, *args)[7:], want)
+        kc.cached_attention(x, *args, out=out)
+        assert torch.equal(out[7:], want) and (out[:7] == 0).all()
+    lse = torch.zeros(hq, T, device="cuda")
+    for x in (q[:, 1:2].expand(-1, hq, -1), q[9:10].expand(T, -1, -1)):
+        got = kc.cached_attention(x, *args, lse=lse)
+        ref = ok.cached_attention(x, *cache[:5], cu, lens, 1)
+        assert (lse[:, :7] == 0).all()
+        _check(got[7:], lse[:, 7:], (ref[0][7:], ref[1][:, 7:], ref[2][7:]), dtype, float(cache[3].max() * 127), n)
