@@ -82,6 +82,19 @@ def test_scale_as_small_as_it_may_be(kc, dtype, D, ql, n):
     _check(got, lse, ok.cached_attention(*args, 1, scale=2e-30), dtype, float(args[4].max() * 127), n)
 
 
+@pytest.mark.parametrize("ql", [3, 150])
+@pytest.mark.parametrize("D", [64, 128])
+def test_value_scales_far_apart(kc, D, ql):
+    """V scales 2^-60 and 2^20: the keys of the small ones weigh what their scores say."""
+    args = _one_request(D, ql, 640, 2, 1, D, 32, torch.bfloat16)
+    q, kcodes, vcodes, ks, vs, table, cu, lens = args
+    vs.fill_(2.0 ** -60)
+    vs[table[0, 3].long()] = 2.0 ** 20
+    lse = torch.empty(2, ql, device="cuda")
+    got = kc.cached_attention(*args, ql, 640, lse=lse)
+    _check(got, lse, ok.cached_attention(*args), torch.bfloat16, 2.0 ** 27, 640)
+
+
 # ------------------------------------------------------------------- plan
 def _plan(kc, cached, target, table, ring, free, bs, max_new, guard=16):
     """block_plan with guard words on both sides of the ring and the table; checks them and that the call repeats."""
