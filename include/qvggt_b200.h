@@ -423,15 +423,19 @@ int qvggt_kv_gather(const qvggt_kv_gather_args* args, void* stream);
  * Mask: query i of ql sits at position p = kv_len - ql + i.  causal_chunk 0:
  * it sees every key; c > 0: keys j < (p / c + 1) * c (1: causal; the tokens of
  * a frame: its own and all earlier frames), none when p < 0.  A row that sees
- * no key gives 0.  lse (fp32 [q_heads][Tq], may be NULL): ln sum_j exp(scale
- * q.k_j), -inf for such a row.
- * Sums, maxima and products are held in fp32; the weights are rounded to fp16
- * for the product with V.
+ * no key gives 0; rows outside cu_q are left as they are.  lse (fp32
+ * [q_heads][Tq], may be NULL): ln sum_j exp(scale q.k_j), -inf for a row
+ * without a key.
+ * scale: above 1e-30, at most 1e30.  Sums, maxima and products are held in fp32;
+ * the weights are rounded to fp16 for the product with V, and with many rows one
+ * in eight of them comes from a polynomial (relative error up to 7.5e-5, a sixth of
+ * that rounding's).  The V scales of one request's blocks may lie 2^80 apart.
  * scratch: qvggt_cached_attention_scratch() bytes (0 for some shapes), 16-byte
  * aligned; its contents need no preparation and are free after the call, and
  * calls that may overlap on the GPU may not share it.  A block id or length
  * outside its range sets the device status word (0x201: the block's keys are
- * skipped, 0x202: the request is skipped).  New entry points. */
+ * skipped, 0x202: the request is skipped, its rows of out and lse are left as
+ * they are).  New entry points. */
 typedef struct {
   qvggt_kv_cache cache;
   const void* q;

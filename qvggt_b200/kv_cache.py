@@ -18,9 +18,10 @@ apart), scales fp32 ``[num_blocks, kv_heads]``; token j of request b is row
 
 Every call launches on the current stream of its tensors' device and returns
 without waiting; CPU tensors, wrong types and shapes raise.  Lengths and tables
-live on the GPU, so their contents are checked there: a block id or length
-outside its range is skipped and sets the library's status word
-(``_lib.device_status()``, 0x201 / 0x202).
+live on the GPU, so their contents are checked there: what a block id or length
+outside its range names is skipped, and the library's status word is set
+(``_lib.device_status()``, 0x201 / 0x202); :func:`block_plan` refuses lengths
+in its own status.
 """
 from __future__ import annotations
 
@@ -321,8 +322,11 @@ def cached_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, cu_q, 
     sets how the work is split).  ``Hq`` is a multiple of the cache's heads.
     Query i of ql sits at position ``kv_len - ql + i``.  ``causal_chunk`` 0:
     every query sees every key; 1: causal; the tokens of a frame: its own and
-    all earlier frames.  A query that sees no key gives 0 (and ``lse`` -inf).
-    ``scale`` defaults to ``head_dim ** -0.5``.  ``lse``: fp32 ``[Hq, tokens]``
+    all earlier frames.  A query that sees no key gives 0 (and ``lse`` -inf);
+    rows outside ``cu_q``, and those of a request that is skipped for its
+    lengths (status word 0x202), are left as they are.  ``scale``: positive
+    (more than 1e-30, at most 1e30), ``head_dim ** -0.5`` by default.  The V
+    scales of one request's blocks may lie 2^80 apart.  ``lse``: fp32 ``[Hq, tokens]``
     to be filled.  ``scratch``: uint8, at least :func:`attention_scratch_bytes`
     (allocated here if None).  Returns ``out`` ``[tokens, Hq, head_dim]``."""
     name = "cached_attention"
@@ -387,7 +391,10 @@ class PagedKVCache:
         cache.commit(plan)                             # the plan's lengths become the cache's
 
     Nothing waits for the GPU; :meth:`check` does, and raises if the plan
-    could not be served.  One stream at a time."""
+    could not be served (its tokens then have no place: :meth:`append` writes
+    nothing and :meth:`attend` leaves its output as allocated).  One stream at
+    a time.  :meth:`commit` takes the plan's tensors for the cache's, so a step
+    captured in a CUDA graph would start from the same lengths at each replay."""
 
     def __init__(self, layers: int, num_blocks: int, kv_heads: int, head_dim: int, requests: int, max_len: int,
                  block_size: int = 64, device="cuda"):
