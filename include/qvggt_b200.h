@@ -456,6 +456,130 @@ int qvggt_cached_attention(const qvggt_cached_attention_args* args, void* stream
 int qvggt_cached_attention_scratch(int64_t Tq, int32_t q_heads, int32_t kv_heads, int32_t requests, int32_t max_q,
                                    int64_t max_kv, int32_t head_dim, int64_t* bytes);
 
+/* What a cached key has gathered: for the keys of each request, out = old +
+ * sum of exp(scale q_i . k_j - lse_i) over the queries i that see key j and the
+ * query heads that read its head, where old is decay * weights for tokens before
+ * fresh_from[b] (of all tokens, if it is NULL) and 0 for the others, whose places
+ * may hold anything.
+ * weights, out fp32 [num_blocks][kv_heads][block_size], the cache's order, and
+ * may be the same; places that hold no key of a request are left as they are.
+ * lse fp32 [q_heads][Tq] as the attention over the same keys gives it; a row
+ * whose lse is not finite (no key, or NaN) counts for nothing.  q, cu_q, kv_lens,
+ * block_tables, max_q, max_kv, causal_chunk, scale as in qvggt_cached_attention;
+ * requests have their own blocks.  decay: 0 to 1.  Sums are held in fp32 and
+ * taken in one order, so they repeat bit for bit.  A block id or length outside
+ * its range sets the device status word (0x201: the block is skipped, 0x202: the
+ * request is).  New entry point. */
+typedef struct {
+  const int8_t* k_cache;
+  int64_t block_stride;
+  const float* k_scale;
+  int64_t num_blocks, kv_heads, block_size, head_dim;
+  const void* q;
+  int64_t q_tok, q_head, Tq, q_heads, dtype;
+  const float* lse;
+  const int32_t* block_tables;
+  int64_t max_blocks;
+  const int32_t *cu_q, *kv_lens, *fresh_from;
+  int64_t requests, max_q, max_kv, causal_chunk;
+  const float* weights;
+  float* out;
+  double scale, decay;
+} qvggt_key_weights_args;
+int qvggt_key_weights(const qvggt_key_weights_args* args, void* stream);
+
+/* Which tokens stay when request b goes from lens[b] to keep[b] tokens, for
+ * every layer and kv head apart: the first `sink` and the last `recent` (as
+ * far as keep[b] goes, the first ones before the last), then those of largest
+ * weight; of equal ones the lower position.  NaN counts as the lowest weight,
+ * infinities as the largest finite ones.  A token that stays although it stands
+ * at keep[b] or later moves into the place of one that goes: dst
+ * [layers][requests][kv_heads][max_moves] holds the places below keep[b] that
+ * fall free and src the tokens that move, both ascending, then -1; counts
+ * [layers][requests][kv_heads] how many.  keep[b] >= lens[b]: none.
+ * weights fp32 [layers][num_blocks][kv_heads][block_size], 16-byte aligned.
+ * max_moves: at least the largest min(keep[b], lens[b] - keep[b]); moves past it
+ * are dropped and the status word says so (0x202).  max_len: about the longest
+ * length (0: what the tables hold); it sets how the work is laid out.  A length
+ * outside its range gives no moves, a block outside the cache lowest weights;
+ * the status word says so (0x202, 0x201).  At most 2^30 tokens a request.
+ * New entry point. */
+typedef struct {
+  const float* weights;
+  int64_t layers, num_blocks, kv_heads, block_size;
+  const int32_t* block_tables;
+  int64_t max_blocks;
+  const int32_t *lens, *keep;
+  int64_t requests, sink, recent, max_moves, max_len;
+  int32_t *src, *dst, *counts;
+} qvggt_evict_plan_args;
+int qvggt_evict_plan(const qvggt_evict_plan_args* args, void* stream);
+
+/* Carries out the moves of qvggt_evict_plan in the cache: codes, scales and, if
+ * not NULL, weights [layers][num_blocks][kv_heads][block_size] of token src[i]
+ * enter the place of token dst[i].
+ * cache: the tensors of the first layer; layer_stride codes between layers
+ * (16-byte aligned), the scales [layers][num_blocks][kv_heads].  Per (layer,
+ * head) and block that receives rows of magnitude amax: s = max(s_old, amax /
+ * 127, 2^-60), incoming values x become rint(x * (1 / s)), and if s grew all
+ * other codes c of the block rint(c * (s_old * (1 / s))).  Blocks that receive
+ * nothing are left as they are, and so is what stands at keep[b] or later, but
+ * for the rest of the block that keep[b] falls into.  Places outside [0,
+ * keep[b]) in dst, or before keep[b] in src, and block ids outside the cache are
+ * skipped and reported (0x202, 0x201).  New entry point. */
+typedef struct {
+  qvggt_kv_cache cache;
+  int64_t layers, layer_stride;
+  float* weights;
+  const int32_t* block_tables;
+  int64_t max_blocks;
+  const int32_t* keep;
+  int64_t requests;
+  const int32_t *src, *dst, *counts;
+  int64_t max_moves;
+} qvggt_kv_evict_args;
+int qvggt_kv_evict(const qvggt_kv_evict_args* args, void* stream);
+
+/* Attention over whole sequences packed one after another: softmax(scale q k^T +
+ * mask) v within each.
+ * q, out [T, q_heads, head_dim], k, v [T, kv_heads, head_dim], fp16 or bf16,
+ * element strides of token and head (positive multiples of 8 where there is more
+ * than one; out's may not overlap), unit stride inside, 16-byte aligned;
+ * head_dim 64 or 128; query head h reads key head h / (q_heads / kv_heads), at
+ * most 128 query heads to a key head.  Sequence b is rows [cu[b], cu[b + 1]), at
+ * most max_len of them.
+ * Mask: causal_chunk 0: every token sees its whole sequence; c > 0: token i sees
+ * tokens j < (i / c + 1) * c (1: causal; the tokens of a frame: its own and all
+ * earlier frames).  What a token does not see adds nothing to it, NaN and
+ * infinities among it.  Rows outside cu are left as they are.  lse (fp32
+ * [q_heads][T], may be NULL): ln sum_j exp(scale q.k_j).
+ * scale: above 1e-30, at most 1e30.  Sums, maxima and products are held in fp32;
+ * the weights are rounded to the inputs' type for the product with V.
+ * scratch: qvggt_prompt_attention_scratch() bytes (0 for some shapes), 16-byte
+ * aligned; calls that may overlap on the GPU may not share it.  A sequence
+ * outside [0, T) or longer than max_len is skipped and sets the device status
+ * word (0x202).  New entry points. */
+typedef struct {
+  const void* q;
+  int64_t q_tok, q_head;
+  const void* k;
+  int64_t k_tok, k_head;
+  const void* v;
+  int64_t v_tok, v_head;
+  void* out;
+  int64_t o_tok, o_head;
+  float* lse;
+  int64_t T, q_heads, kv_heads, head_dim, dtype;
+  const int32_t* cu;
+  int64_t sequences, max_len, causal_chunk;
+  double scale;
+  void* scratch;
+  int64_t scratch_bytes;
+} qvggt_prompt_attention_args;
+int qvggt_prompt_attention(const qvggt_prompt_attention_args* args, void* stream);
+int qvggt_prompt_attention_scratch(int64_t T, int32_t q_heads, int32_t kv_heads, int32_t sequences, int64_t max_len,
+                                   int32_t head_dim, int64_t* bytes);
+
 /* ---------------------------------------------------------- patch embed */
 
 /* images fp16 [S, 3, H, W] (pixels in [0, 1]) -> patches fp16

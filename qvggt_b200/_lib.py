@@ -61,6 +61,11 @@ SIGNATURES = {
     "qvggt_kv_gather": [C.c_char_p, vp],
     "qvggt_cached_attention": [C.c_char_p, vp],
     "qvggt_cached_attention_scratch": [i64, i32, i32, i32, i32, i64, i32, i64p],
+    "qvggt_key_weights": [C.c_char_p, vp],
+    "qvggt_evict_plan": [C.c_char_p, vp],
+    "qvggt_kv_evict": [C.c_char_p, vp],
+    "qvggt_prompt_attention": [C.c_char_p, vp],
+    "qvggt_prompt_attention_scratch": [i64, i32, i32, i32, i64, i32, i64p],
     "qvggt_pose_encoding_to_extri_intri": [vp, i64, i32, i32, vp, vp, vp],
     "qvggt_unproject_depth": [vp, i64, i32, i32, vp, vp, vp, vp],
 }

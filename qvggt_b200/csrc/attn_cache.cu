@@ -36,6 +36,7 @@ struct RowLay {
 // The rows of an item, their keys in units.
 template <int D, int NT>
 struct RowBlock {
+  using Args = CacheAttnArgs;
   // A segment's start and merge cost about as much as two units on each warp;
   // a piece is not cut below four units for each (a join costs about that).
   static constexpr int START = 2 * RowLay<D, NT>::WARPS, MIN = START + 4 * RowLay<D, NT>::WARPS;

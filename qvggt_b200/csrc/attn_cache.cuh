@@ -149,7 +149,7 @@ struct __align__(16) Cut {
 // Running sums of the blocks' costs in shared memory, cum[0 .. THREADS]: entry
 // x starts at block x * g.  All THREADS threads call it; ends with a barrier.
 template <int THREADS, class Blk>
-__device__ __forceinline__ void scan_blocks(const CacheAttnArgs& a, long long* cum, int blocks, int g) {
+__device__ __forceinline__ void scan_blocks(const typename Blk::Args& a, long long* cum, int blocks, int g) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   long long sum = 0;
   for (int p = threadIdx.x * g; p < min(blocks, ((int)threadIdx.x + 1) * g); ++p)
@@ -187,12 +187,13 @@ __device__ __forceinline__ void scan_blocks(const CacheAttnArgs& a, long long* c
 // has at most one of each.
 template <int THREADS, class Blk>
 struct PieceWalk {
+  using Args = typename Blk::Args;
   long long W, begin, end, s;            // length of a piece, this one's ends, where block p starts
   int p, h, g;
   Blk blk;
   Cut cut;
 
-  __device__ __forceinline__ PieceWalk(const CacheAttnArgs& a, const long long* cum, int blocks, int g_) : g(g_) {
+  __device__ __forceinline__ PieceWalk(const Args& a, const long long* cum, int blocks, int g_) : g(g_) {
     const long long total = cum[THREADS] * a.hk;
     const int grid = gridDim.x;
     W = (total + grid - 1) / grid;
@@ -213,7 +214,7 @@ struct PieceWalk {
     else p = blocks;
   }
 
-  __device__ __forceinline__ void load(const CacheAttnArgs& a, int blocks) {
+  __device__ __forceinline__ void load(const Args& a, int blocks) {
     for (; p < blocks; ++p) {
       blk = Blk(a, p / a.row_blocks, p % a.row_blocks);
       if (blk.cost > 0 && s + blk.cost * a.hk > begin) {
@@ -225,7 +226,7 @@ struct PieceWalk {
   }
 
   // The next segment; false at the end of the piece.
-  __device__ __forceinline__ bool next(const CacheAttnArgs& a, int blocks, Segment& sg) {
+  __device__ __forceinline__ bool next(const Args& a, int blocks, Segment& sg) {
     const int grid = gridDim.x, x = blockIdx.x;
     while (p < blocks) {
       if (h == a.hk) {
@@ -263,8 +264,8 @@ struct PieceWalk {
 // Row `row` of a cut item, joined from its parts (rows_per_slot rows a slot) by
 // D / 4 threads, four columns each: the parts' normalised rows weighted by
 // their sums, in the pieces' order.
-template <bool BF16, int D>
-__device__ __forceinline__ void join_parts(const CacheAttnArgs& a, const Cut& cut, int rows_per_slot, int row, int col4,
+template <bool BF16, int D, class Args>
+__device__ __forceinline__ void join_parts(const Args& a, const Cut& cut, int rows_per_slot, int row, int col4,
                                            long long tok, int h) {
   auto at = [&](int k) { return (long long)(2 * k + (k == cut.first)) * rows_per_slot + row; };
   float mx = -INFINITY;

@@ -73,23 +73,6 @@ struct Lay {
   static constexpr int TOTAL = ROWS + 256 * 8 + 1024;
 };
 
-// One lane of a converged warp, the same one every time.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(p));
-  return p != 0;
-}
-
-// K-major or MN-major operand with 128-byte swizzle; lead: bytes between the
-// 64-element panels of an MN-major operand (unused by K-major ones).
-__device__ __forceinline__ uint64_t sdesc_panels(uint32_t saddr, uint32_t lead) {
-  return (sdesc_sw128(saddr) & ~(0x3fffull << 16)) | ((uint64_t)(lead >> 4) << 16);
-}
-
 // Constants of a 32-key chunk.
 struct Chunk {
   float ck, lv, inv_vs;
@@ -182,6 +165,7 @@ __device__ __forceinline__ bool exp_store(uint32_t (&s)[KT], const Chunk (&k)[KT
 // Q block `qb` of request b: its rows and keys.
 template <int KT>
 struct Block {
+  using Args = CacheAttnArgs;
   static constexpr int START = COST_START, MIN = COST_MIN;
   int q0, ql, n, tok0, nqt, tiles;
   long long cost;                        // of one kv head; 0: no such block

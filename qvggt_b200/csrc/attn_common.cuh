@@ -105,4 +105,21 @@ __device__ __forceinline__ void exp2_poly_pair(uint64_t x2, float& p0, float& p1
   p1 = __int_as_float(__float_as_int(q1) + (__float_as_int(t1) << 23));
 }
 
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
+}
+
+// K-major or MN-major operand with 128-byte swizzle; lead: bytes between the
+// 64-element panels of an MN-major operand (unused by K-major ones).
+__device__ __forceinline__ uint64_t sdesc_panels(uint32_t saddr, uint32_t lead) {
+  return (sdesc_sw128(saddr) & ~(0x3fffull << 16)) | ((uint64_t)(lead >> 4) << 16);
+}
+
 }  // namespace qv

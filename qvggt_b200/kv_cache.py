@@ -10,6 +10,10 @@ new queries attend to them without a dequantised copy.
 :func:`kv_append`         quantises new K/V rows into their blocks
 :func:`kv_gather`         reads rows back as fp16 / bf16 ``[k | v]``
 :func:`cached_attention`  attention over the cache, ragged requests, shared heads, block-causal mask
+:func:`prompt_attention`  attention over whole sequences packed one after another, before they enter the cache
+:func:`key_weights`       the attention weight that each cached key has gathered
+:func:`evict_plan`        which keys stay when a request has to shrink: those of largest weight
+:func:`kv_evict`          moves the keys that stay into the places of those that go
 :class:`PagedKVCache`     the buffers of several layers with one block table, and the calls in order
 
 Layout: codes int8 ``[num_blocks, kv_heads, block_size, head_dim]`` (K and V
@@ -36,7 +40,8 @@ from . import _lib
 from .awq_inference_engine import _Dev, _check_cuda, _check_dtype, _check_shape, _stream
 
 __all__ = ["rope_axes", "block_plan", "BlockPlan", "kv_append", "kv_gather", "cached_attention",
-           "attention_scratch_bytes", "PagedKVCache", "PLAN_STATUS"]
+           "attention_scratch_bytes", "prompt_attention", "prompt_scratch_bytes", "key_weights", "evict_plan", "EvictPlan",
+           "kv_evict", "PagedKVCache", "PLAN_STATUS"]
 
 _HALF = {torch.float16: 0, torch.bfloat16: 1}      # QVGGT_DTYPE_F16 / _BF16
 _LAYOUTS = {"axial": 0, "split": 1, "interleaved": 2}
@@ -54,6 +59,10 @@ _PLAN = struct.Struct("=16q").pack
 _APPEND = struct.Struct("=24q").pack
 _GATHER = struct.Struct("=14q").pack
 _ATTEND = struct.Struct("=27qd2q").pack
+_PROMPT = struct.Struct("=22qd2q").pack
+_WEIGHTS = struct.Struct("=25q2d").pack
+_EVICT_PLAN = struct.Struct("=17q").pack
+_EVICT = struct.Struct("=20q").pack
 
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _functions: dict = {}
@@ -350,14 +359,7 @@ def cached_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, cu_q, 
         so = (hq * d, d)
     else:
         so = _out3(name, out, q, dev, "out")
-    if lse is None:
-        lse_at = 0
-    else:
-        if lse.get_device() != dev:
-            _check_cuda(name, q, lse)
-        _check_shape(name, lse.dtype is _F32 and lse.is_contiguous() and lse.shape == (hq, T),
-                     f"lse must be contiguous float32 [{hq}, {T}]")
-        lse_at = lse.data_ptr()
+    lse_at = _lse_at(name, lse, q, dev, hq, T)
     nbytes = _scratch_bytes(dev, T, hq, hk, B, max_q, max_kv, d)
     scratch_at = scratch_len = 0
     if scratch is not None:
@@ -376,6 +378,239 @@ def cached_attention(q, k_cache, v_cache, k_scale, v_scale, block_tables, cu_q, 
                  block_tables.data_ptr(), wide, cu_q.data_ptr(), kv_lens.data_ptr(), B, max_q, max_kv, causal_chunk,
                  d ** -0.5 if scale is None else scale, scratch_at, scratch_len))
     return out
+
+
+# -------------------------------------------------------------------- prompts
+@functools.lru_cache(maxsize=1024)
+def _prompt_scratch(dev, *sizes):
+    nb = C.c_int64(0)
+    with torch.cuda.device(dev):
+        _lib.call("qvggt_prompt_attention_scratch", *sizes, C.byref(nb))
+    return int(nb.value)
+
+
+def prompt_scratch_bytes(tokens: int, q_heads: int, kv_heads: int, sequences: int, max_len: int, head_dim: int) -> int:
+    """Scratch :func:`prompt_attention` needs for these sizes on the current device."""
+    return _prompt_scratch(_current_device(), tokens, q_heads, kv_heads, sequences, max_len, head_dim)
+
+
+def prompt_attention(q, k, v, cu, max_len: int, causal_chunk: int = 0, scale: float | None = None, out=None, lse=None,
+                     scratch=None):
+    """``softmax(scale q k^T + mask) v`` within each of several sequences packed one after another.
+
+    q ``[tokens, Hq, head_dim]``, k and v ``[tokens, Hk, head_dim]`` fp16 /
+    bf16, any positive 16-byte aligned token and head strides (column ranges of
+    one projection's output, say), head_dim 64 or 128, ``Hq`` a multiple of
+    ``Hk`` (at most 128 times).  Sequence b is rows ``cu[b]`` to ``cu[b + 1]``
+    (int32 on the GPU), at most ``max_len`` of them; rows outside ``cu`` are
+    left as they are.  ``causal_chunk`` 0: every token sees its whole sequence;
+    1: causal; the tokens of a frame: its own and all earlier frames.  What a
+    token does not see adds nothing to it, be it NaN.  ``scale``: positive,
+    ``head_dim ** -0.5`` by default.  ``lse``: fp32 ``[Hq, tokens]`` to be
+    filled.  ``scratch``: uint8, at least :func:`prompt_scratch_bytes`
+    (allocated here if None).  Returns ``out`` ``[tokens, Hq, head_dim]``."""
+    name = "prompt_attention"
+    dev = q.get_device()
+    if dev < 0 or not dev == k.get_device() == v.get_device() == cu.get_device():
+        _check_cuda(name, q, k, v, cu)
+    dt = _half(name, q, "q")
+    sq, sk, sv = _rows3(name, q, "q"), _rows3(name, k, "k"), _rows3(name, v, "v")
+    _check_dtype(name, k, q.dtype)
+    _check_dtype(name, v, q.dtype)
+    T, hq, d = q.shape
+    shape = k.shape
+    if shape[0] != T or shape[2] != d or v.shape != shape:
+        raise ValueError(f"{name}: k {tuple(shape)} and v {tuple(v.shape)} must be [{T}, kv_heads, {d}]")
+    hk = shape[1]
+    _ints(name, cu, "cu")
+    B = cu.numel() - 1
+    if B < 0:
+        raise ValueError(f"{name}: cu must hold the running sums of the lengths, from 0 on")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        so = (hq * d, d)
+    else:
+        so = _out3(name, out, q, dev, "out")
+    lse_at = _lse_at(name, lse, q, dev, hq, T)
+    nbytes = _prompt_scratch(dev, T, hq, hk, B, max_len, d)
+    scratch_at = scratch_len = 0
+    if scratch is not None:
+        if scratch.get_device() != dev:
+            _check_cuda(name, q, scratch)
+        scratch_len = scratch.numel()
+        _check_shape(name, scratch.dtype is torch.uint8 and scratch.is_contiguous() and scratch_len >= nbytes,
+                     f"scratch must be a contiguous uint8 tensor of >= {nbytes} bytes")
+        scratch_at = scratch.data_ptr()
+    elif nbytes:
+        scratch = q.new_empty(nbytes, dtype=torch.uint8)
+        scratch_at, scratch_len = scratch.data_ptr(), nbytes
+    _run("qvggt_prompt_attention", dev, q,
+         _PROMPT(q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], out.data_ptr(), so[0],
+                 so[1], lse_at, T, hq, hk, d, dt, cu.data_ptr(), B, max_len, causal_chunk,
+                 d ** -0.5 if scale is None else scale, scratch_at, scratch_len))
+    return out
+
+
+def _lse_at(name, lse, q, dev, hq, T):
+    """Address of a log-sum-exp tensor, 0 for None."""
+    if lse is None:
+        return 0
+    if lse.get_device() != dev:
+        _check_cuda(name, q, lse)
+    _check_shape(name, lse.dtype is _F32 and lse.is_contiguous() and lse.shape == (hq, T),
+                 f"lse must be contiguous float32 [{hq}, {T}]")
+    return lse.data_ptr()
+
+
+# ------------------------------------------------------------------- eviction
+def key_weights(q, k_cache, k_scale, block_tables, cu_q, kv_lens, lse, weights, max_q: int, max_kv: int,
+                causal_chunk: int = 0, scale: float | None = None, fresh_from=None, decay: float = 1.0, out=None):
+    """What each cached key has gathered: ``out = decay * weights + sum of exp(scale q k - lse)`` over the queries that see it.
+
+    The arguments are :func:`cached_attention`'s, and ``lse`` fp32 ``[Hq,
+    tokens]`` is what it wrote for these queries (a row whose lse is not finite
+    counts for nothing).  ``weights`` and ``out`` fp32 ``[num_blocks, kv_heads,
+    block_size]`` stand in the cache's order; ``out`` is ``weights`` by default,
+    and places that hold no key of a request are left as they are.  Tokens from
+    ``fresh_from[b]`` on (int32 ``[requests]``: the lengths before the newest
+    tokens came; None: none) start from 0, whatever their places hold.
+    ``decay``: 0 to 1.  Requests must not share blocks.  Returns ``out``."""
+    name = "key_weights"
+    dev = q.get_device()
+    if dev < 0 or not (dev == k_cache.get_device() == k_scale.get_device() == block_tables.get_device()
+                       == cu_q.get_device() == kv_lens.get_device() == lse.get_device() == weights.get_device()):
+        _check_cuda(name, q, k_cache, k_scale, block_tables, cu_q, kv_lens, lse, weights)
+    shape, st = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or k_cache.dtype is not torch.int8:
+        raise TypeError(f"{name}: the cache must be int8 [num_blocks, kv_heads, block_size, head_dim]")
+    nb, hk, bs, d = shape
+    if st[1:] != (bs * d, d, 1):
+        raise ValueError(f"{name}: the cache must be dense inside a block")
+    if k_scale.dtype is not _F32 or k_scale.shape != (nb, hk) or not k_scale.is_contiguous():
+        raise ValueError(f"{name}: k_scale must be contiguous float32 [{nb}, {hk}]")
+    dt = _half(name, q, "q")
+    sq = _rows3(name, q, "q")
+    T, hq, dq = q.shape
+    if dq != d:
+        raise ValueError(f"{name}: q has head_dim {dq}, the cache {d}")
+    B = kv_lens.numel()
+    wide = _table(name, block_tables, B)
+    _ints(name, cu_q, "cu_q", (B + 1,))
+    _ints(name, kv_lens, "kv_lens")
+    lse_at = _lse_at(name, lse, q, dev, hq, T)
+    fresh_at = 0
+    if fresh_from is not None:
+        if fresh_from.get_device() != dev:
+            _check_cuda(name, q, fresh_from)
+        _ints(name, fresh_from, "fresh_from", (B,))
+        fresh_at = fresh_from.data_ptr()
+    if out is None:
+        out = weights
+    elif out.get_device() != dev:
+        _check_cuda(name, q, out)
+    for what, t in (("weights", weights), ("out", out)):
+        if t.dtype is not _F32 or t.shape != (nb, hk, bs) or not t.is_contiguous():
+            raise ValueError(f"{name}: {what} must be contiguous float32 [{nb}, {hk}, {bs}]")
+    _run("qvggt_key_weights", dev, q,
+         _WEIGHTS(k_cache.data_ptr(), st[0], k_scale.data_ptr(), nb, hk, bs, d, q.data_ptr(), sq[0], sq[1], T, hq, dt,
+                  lse_at, block_tables.data_ptr(), wide, cu_q.data_ptr(), kv_lens.data_ptr(), fresh_at, B, max_q, max_kv,
+                  causal_chunk, weights.data_ptr(), out.data_ptr(), d ** -0.5 if scale is None else scale, decay))
+    return out
+
+
+class EvictPlan(NamedTuple):
+    """What :func:`evict_plan` writes (all on the GPU)."""
+    src: torch.Tensor          # int32 [layers, requests, kv_heads, max_moves]: tokens that move, ascending, then -1
+    dst: torch.Tensor          # the same shape: the places they take, ascending, then -1
+    counts: torch.Tensor       # int32 [layers, requests, kv_heads]
+
+
+def _weights4(name, t):
+    """[layers, num_blocks, kv_heads, block_size] weights -> their shape."""
+    if t.dtype is not _F32 or t.dim() != 4 or not t.is_contiguous():
+        raise ValueError(f"{name}: weights must be contiguous float32 [layers, num_blocks, kv_heads, block_size]")
+    return t.shape
+
+
+def evict_plan(weights, block_tables, lens, keep, sink: int, recent: int, max_moves: int, max_len: int = 0) -> EvictPlan:
+    """Which tokens stay when the requests go from ``lens`` to ``keep`` tokens (int32 ``[requests]``), on the GPU.
+
+    For every layer and kv head apart: the first ``sink`` and the last
+    ``recent`` tokens as the cache holds them (as far as ``keep`` goes, the
+    first ones before the last), then those of largest weight, of equal ones
+    the earlier.  ``weights`` fp32 ``[layers, num_blocks, kv_heads,
+    block_size]`` as :func:`key_weights` gathers them; NaN counts as the lowest,
+    infinities as the largest finite ones.  A token that stays but stands at
+    ``keep`` or later takes the place of one that goes, so the others need not
+    move (and their codes are not rounded again).  ``keep >= lens``: nothing.
+    ``max_moves``: at least the largest ``min(keep, lens - keep)``; moves past it
+    are dropped and the status word says so.  ``max_len``: about the longest
+    length, if one shorter than the tables' is known.  :func:`kv_evict` carries the plan out, and a
+    :func:`block_plan` to ``keep`` tokens then gives the blocks back."""
+    name = "evict_plan"
+    dev = weights.get_device()
+    if dev < 0 or not dev == block_tables.get_device() == lens.get_device() == keep.get_device():
+        _check_cuda(name, weights, block_tables, lens, keep)
+    layers, nb, h, bs = _weights4(name, weights)
+    B = lens.numel()
+    wide = _table(name, block_tables, B)
+    _ints(name, lens, "lens")
+    _ints(name, keep, "keep", (B,))
+    if max_moves < 0:
+        raise ValueError(f"{name}: max_moves must not be negative")
+    rows = layers * B * h
+    # one allocation, the counts last
+    buf = lens.new_empty(rows * (2 * max_moves + 1))
+    src, dst, counts = buf.split_with_sizes([rows * max_moves, rows * max_moves, rows])
+    at = buf.data_ptr()
+    _run("qvggt_evict_plan", dev, buf,
+         _EVICT_PLAN(weights.data_ptr(), layers, nb, h, bs, block_tables.data_ptr(), wide, lens.data_ptr(), keep.data_ptr(),
+                     B, sink, recent, max_moves, max_len, at, at + 4 * rows * max_moves, at + 8 * rows * max_moves))
+    return EvictPlan(src.view(layers, B, h, max_moves), dst.view(layers, B, h, max_moves), counts.view(layers, B, h))
+
+
+def kv_evict(k_cache, v_cache, k_scale, v_scale, weights, block_tables, keep, plan: EvictPlan) -> None:
+    """Carries out the moves of :func:`evict_plan`: codes, scales and weights (or None) of each moved token, in place.
+
+    The caches int8 ``[layers, num_blocks, kv_heads, block_size, head_dim]``,
+    the scales fp32 ``[layers, num_blocks, kv_heads]``.  A block's scale grows
+    when the rows it receives need it, and its other codes are rounded to the
+    new scale, as in :func:`kv_append`."""
+    name = "kv_evict"
+    src, dst, counts = plan
+    dev = k_cache.get_device()
+    if dev < 0 or not (dev == v_cache.get_device() == k_scale.get_device() == v_scale.get_device()
+                       == block_tables.get_device() == keep.get_device() == src.get_device() == dst.get_device()
+                       == counts.get_device()):
+        _check_cuda(name, k_cache, v_cache, k_scale, v_scale, block_tables, keep, src, dst, counts)
+    shape, st = k_cache.shape, k_cache.stride()
+    if len(shape) != 5 or k_cache.dtype is not torch.int8 or v_cache.dtype is not torch.int8:
+        raise TypeError(f"{name}: the caches must be int8 [layers, num_blocks, kv_heads, block_size, head_dim]")
+    layers, nb, h, bs, d = shape
+    if v_cache.shape != shape or st[2:] != (bs * d, d, 1) or v_cache.stride() != st:
+        raise ValueError(f"{name}: K and V caches must have the same shape and strides, dense inside a block")
+    for t in (k_scale, v_scale):
+        if t.dtype is not _F32 or t.shape != (layers, nb, h) or not t.is_contiguous():
+            raise ValueError(f"{name}: k_scale and v_scale must be contiguous float32 [{layers}, {nb}, {h}]")
+    w_at = 0
+    if weights is not None:
+        if weights.get_device() != dev:
+            _check_cuda(name, k_cache, weights)
+        if _weights4(name, weights) != (layers, nb, h, bs):
+            raise ValueError(f"{name}: weights {tuple(weights.shape)} must be [{layers}, {nb}, {h}, {bs}]")
+        w_at = weights.data_ptr()
+    B = keep.numel()
+    wide = _table(name, block_tables, B)
+    _ints(name, keep, "keep")
+    _ints(name, counts, "counts", (layers, B, h))
+    if src.dim() != 4 or src.shape[:3] != (layers, B, h):
+        raise ValueError(f"{name}: src {tuple(src.shape)} must be [{layers}, {B}, {h}, max_moves]")
+    _ints(name, src, "src")
+    _ints(name, dst, "dst", src.shape)
+    _run("qvggt_kv_evict", dev, k_cache,
+         _EVICT(k_cache.data_ptr(), v_cache.data_ptr(), st[1], k_scale.data_ptr(), v_scale.data_ptr(), nb, h, bs, d, layers,
+                st[0], w_at, block_tables.data_ptr(), wide, keep.data_ptr(), B, src.data_ptr(), dst.data_ptr(),
+                counts.data_ptr(), src.shape[3]))
 
 
 class PagedKVCache:

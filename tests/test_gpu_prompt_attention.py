@@ -1,0 +1,258 @@
+"""GPU: attention over packed sequences against its 64-bit restatement.
+
+Bound, element by element: the output's rounding, the weights' rounding to the inputs' type (and 2^-13 for scores and
+exponentials) times sum w |v|, and for fp16 the weights' steps below its normal range: n keys, 2^-25 each of the largest |v|.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_evict as oe
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float16, torch.bfloat16]
+U = {t: torch.finfo(t).eps / 2 for t in DTYPES}
+TINY = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126}
+
+
+@pytest.fixture(scope="module")
+def kc():
+    from qvggt_b200 import _lib, kv_cache
+    _lib.device_status(clear=True)
+    yield kv_cache
+    assert _lib.device_status(clear=True) == 0
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def cu_of(lens, start=0):
+    return [start] + [start + int(x) for x in np.cumsum(lens)]
+
+
+def inputs(seed, T, hq, hk, D, dtype):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.randn(T, h, D, generator=g, device="cuda").to(dtype) for h in (hq, hk, hk)]
+
+
+def check(got, lse, ref, dtype, vmax, n):
+    out, want_lse, mag = ref
+    floor = n * 2.0 ** -25 * vmax if dtype is torch.float16 else 0.0
+    bound = U[dtype] * out.abs() * 1.01 + (U[dtype] + 2.0 ** -13) * mag + floor + TINY[dtype]
+    assert torch.isfinite(got).all()
+    off = (got.double() - out).abs()
+    assert (off <= bound).all(), float((off / bound).max())
+    assert ((lse.double() - want_lse).abs() <= 2e-4).all()
+
+
+CASES = [
+    # lens, hq, hk, D, chunk
+    ([1], 1, 1, 64, 0), ([1, 1, 1], 3, 1, 128, 1), ([5], 2, 2, 64, 1), ([60, 23, 1, 0, 7], 16, 16, 128, 1),
+    ([128], 2, 2, 64, 1), ([129], 2, 2, 64, 0), ([255, 256, 257], 4, 2, 64, 1), ([64, 65, 63], 2, 1, 128, 1),
+    ([700, 33], 14, 2, 128, 1), ([700, 33], 14, 2, 64, 5), ([300, 20, 411], 3, 1, 128, 7), ([274 * 3, 274], 2, 2, 64, 274),
+    ([1374], 2, 2, 64, 0), ([2049], 1, 1, 64, 1), ([2049], 1, 1, 128, 0), ([3000, 10, 1500], 2, 2, 64, 1),
+    ([2000, 1, 2748], 2, 1, 128, 1374), ([1] * 70, 4, 1, 64, 1), ([17 * i % 200 for i in range(40)], 4, 4, 64, 1),
+    ([40, 3], 128, 1, 64, 1), ([130], 100, 1, 128, 1), ([513, 1200], 5, 1, 64, 0)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,hq,hk,D,chunk", CASES)
+def test_prompt_attention(kc, dtype, lens, hq, hk, D, chunk):
+    T = sum(lens)
+    q, k, v = inputs(T + D, T, hq, hk, D, dtype)
+    lse = torch.full((hq, T), 7.0, device="cuda")
+    cu = cu_of(lens)
+    got = kc.prompt_attention(q, k, v, ints(cu), max(lens), chunk, lse=lse)
+    check(got, lse, oe.prompt_attention(q, k, v, cu, chunk), dtype, float(v.abs().max()), max(lens))
+    # again, and without lse: the same bits
+    assert torch.equal(kc.prompt_attention(q, k, v, ints(cu), max(lens), chunk), got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,hint,chunk", [([50], 100000, 1), ([3000, 20], 5000, 1), ([3000, 20], 3020, 64)])
+def test_length_hint_and_rows_outside(kc, dtype, lens, hint, chunk):
+    """max_len may be larger than needed; rows before and behind the sequences keep what they hold, and what they hold
+    (NaN) reaches nobody."""
+    T = 9 + sum(lens) + 300
+    q, k, v = inputs(1, T, 2, 2, 64, dtype)
+    cu = cu_of(lens, 9)
+    want = oe.prompt_attention(q, k, v, cu, chunk)
+    for t in (q, k, v):
+        t[:9], t[cu[-1]:] = math.nan, math.nan
+    out = torch.full_like(q, 3.0)
+    lse = torch.full((2, T), 7.0, device="cuda")
+    got = kc.prompt_attention(q, k, v, ints(cu), hint, chunk, out=out, lse=lse)
+    assert got is out and (out[:9] == 3).all() and (out[cu[-1]:] == 3).all()
+    assert (lse[:, :9] == 7).all() and (lse[:, cu[-1]:] == 7).all()
+    inside = slice(9, cu[-1])
+    check(got[inside], lse[:, inside], [want[0][inside], want[1][:, inside], want[2][inside]], dtype,
+          float(v[inside].abs().max()), max(lens))
+
+
+@pytest.mark.parametrize("D,hq,hk", [(64, 4, 2), (128, 2, 2), (64, 2, 1)])
+def test_strides_scale_and_scratch(kc, D, hq, hk):
+    lens, chunk, dtype = [1300, 77], 1, torch.bfloat16
+    T = sum(lens)
+    q, k, v = inputs(9, T, hq, hk, D, dtype)
+    cu = cu_of(lens)
+    qkv = torch.randn(T, hq + 2 * hk, D, device="cuda").to(dtype)
+    qs, ks, vs = qkv.split([hq, hk, hk], 1)
+    for a, b in zip((qs, ks, vs), (q, k, v)):
+        a.copy_(b)
+    wide = torch.zeros(hq, T, 2 * D, device="cuda").to(dtype)
+    out = wide.transpose(0, 1)[..., D:]
+    need = kc.prompt_scratch_bytes(T, hq, hk, 2, 1300, D)
+    scratch = torch.full((need + 64,), 255, dtype=torch.uint8, device="cuda")
+    lse = torch.empty(hq, T, device="cuda")
+    got = kc.prompt_attention(qs, ks, vs, ints(cu), 1300, chunk, scale=0.3, out=out, lse=lse, scratch=scratch)
+    assert got is out and (wide[..., :D] == 0).all()
+    check(got, lse, oe.prompt_attention(q, k, v, cu, chunk, 0.3), dtype, float(v.abs().max()), 1300)
+    # heads outermost
+    heads = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+    assert torch.equal(kc.prompt_attention(*heads, ints(cu), 1300, chunk, scale=0.3), got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,chunk,n,hq", [(64, 40, 200, 2), (128, 1, 150, 1), (64, 1374, 2748, 1), (64, 64, 1500, 4),
+                                          (128, 500, 1800, 2)])
+def test_what_a_token_does_not_see(kc, dtype, D, chunk, n, hq):
+    """NaN and infinities in later chunks and in the next sequence leave a token's bits as they are; the tokens that see
+    them get NaN and infinities where 64-bit arithmetic has them."""
+    lens = [n, 90]
+    q, k, v = inputs(4, sum(lens), hq, 1, D, dtype)
+    cu = ints(cu_of(lens))
+    base_lse, lse = (torch.empty(hq, sum(lens), device="cuda") for _ in range(2))
+    base = kc.prompt_attention(q, k, v, cu, n, chunk, lse=base_lse)
+    at = (n // 2 + 3) // chunk * chunk + chunk // 3          # a token of a middle chunk
+    first = at // chunk * chunk                              # whose chunk begins here
+    v2 = v.clone()
+    v2[at, 0, 3], v2[at, 0, D - 1], v2[at + 1, 0, 5] = math.nan, math.inf, -math.inf
+    v2[min(n - 1, at + 2 * chunk + 1), 0, D - 1] = -math.inf
+    v2[n:] = math.nan                                        # the next sequence
+    k2, q2 = k.clone(), q.clone()
+    k2[n:], q2[n:] = math.nan, math.nan
+    got = kc.prompt_attention(q2, k2, v2, cu, n, chunk, lse=lse)
+    assert torch.equal(got[:first], base[:first]) and torch.equal(lse[:, :n], base_lse[:, :n])
+    ref = oe.prompt_attention(q2[:n], k2[:n], v2[:n], [0, n], chunk)[0]
+    assert torch.equal(torch.isnan(got[:n]), torch.isnan(ref)) and torch.equal(torch.isinf(got[:n]), torch.isinf(ref))
+    inf = torch.isinf(ref)
+    assert torch.equal(got[:n][inf].double(), ref[inf])
+    plain = torch.isfinite(ref)
+    assert ((got[:n].double() - base[:n].double())[plain].abs() <= 2 * U[dtype] * base[:n].double()[plain].abs() + 2e-6).all()
+    assert torch.isnan(got[n:]).all()
+    # a key of NaN, one of infinities: rows that see it are NaN, the others as they were
+    for x in (math.nan, math.inf):
+        k3 = k.clone()
+        k3[at, 0, 7] = x
+        got = kc.prompt_attention(q, k3, v, cu, n, chunk, lse=lse)
+        assert torch.equal(got[:first], base[:first]) and torch.equal(got[n:], base[n:])
+        ref = oe.prompt_attention(q[:n], k3[:n], v[:n], [0, n], chunk)[0]
+        assert torch.equal(torch.isnan(got[:n]), torch.isnan(ref))
+
+
+def test_bad_sequences_are_skipped_and_reported(kc):
+    from qvggt_b200 import _lib
+    q, k, v = inputs(8, 300, 2, 2, 64, torch.float16)
+    good = kc.prompt_attention(q, k, v, ints([0, 100, 300]), 200, 1)
+    assert _lib.device_status() == 0
+    for cu, served in [([0, 100, 301], slice(0, 100)), ([-1, 100, 300], slice(100, 300)), ([100, 0, 200], None)]:
+        out = torch.full_like(q, 3.0)
+        kc.prompt_attention(q, k, v, ints(cu), 200, 1, out=out)
+        assert _lib.device_status(clear=True) == 0x202
+        if served is not None:
+            assert torch.equal(out[served], good[served])
+    out = torch.full_like(q, 3.0)
+    kc.prompt_attention(q, k, v, ints([0, 100, 300]), 150, 1, out=out)        # longer than max_len
+    assert _lib.device_status(clear=True) == 0x202
+    assert torch.equal(out[:100], good[:100]) and (out[100:] == 3).all()
+
+
+def test_rows_past_two_gib(kc):
+    """Rows that start beyond 2^31 elements, in every tensor."""
+    n, H, D = 600, 1, 64
+    stride = 2 ** 32 // n // 64 * 64
+    big = torch.zeros(n * stride, dtype=torch.float16, device="cuda")
+    q, k, v, out = (big[i * 64:].as_strided((n, H, D), (stride, D, 1)) for i in range(4))
+    small = inputs(3, n, H, H, D, torch.float16)
+    for a, b in zip((q, k, v), small):
+        a.copy_(b)
+    for chunk in (0, 1):
+        got = kc.prompt_attention(q, k, v, ints([0, n]), n, chunk, out=out)
+        assert torch.equal(got, kc.prompt_attention(*small, ints([0, n]), n, chunk))
+
+
+def test_streams_and_graphs(kc):
+    lens = [1100, 300]
+    T = sum(lens)
+    q, k, v = inputs(5, T, 4, 2, 64, torch.float16)
+    cu = ints(cu_of(lens))
+    want = kc.prompt_attention(q, k, v, cu, 1100, 1)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        late = torch.zeros_like(q)
+        a = torch.randn(4096, 4096, device="cuda")
+        for _ in range(8):
+            a = a @ a * 1e-3
+        late.copy_(q + (a[0, 0] * 0).half().nan_to_num())
+        got = kc.prompt_attention(late, k, v, cu, 1100, 1)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+    graphs, outs, qs = [], [], [torch.zeros_like(q) for _ in range(2)]
+    for x in qs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(kc.prompt_attention(x, k, v, cu, 1100, 1))
+        graphs.append(g)
+    qs[0].copy_(q)
+    qs[1].copy_(q.flip(0))
+    flipped = kc.prompt_attention(qs[1], k, v, cu, 1100, 1)
+    for g in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], flipped)
+
+
+def test_refusals(kc):
+    from qvggt_b200._lib import QvggtError
+    q, k, v = inputs(2, 10, 4, 2, 64, torch.float16)
+    cu = ints([0, 10])
+    call = kc.prompt_attention
+    with pytest.raises(TypeError, match="float16"):
+        call(q.float(), k, v, cu, 10)
+    with pytest.raises(TypeError):
+        call(q, k.bfloat16(), v, cu, 10)
+    with pytest.raises(ValueError, match="kv_heads"):
+        call(q, k[:9], v, cu, 10)
+    with pytest.raises(ValueError, match="kv_heads"):
+        call(q, k, v[:, :1], cu, 10)
+    with pytest.raises(QvggtError, match="share"):
+        call(q[:, :3].contiguous(), k, v, cu, 10)
+    with pytest.raises(QvggtError, match="head_dim"):
+        call(q[..., :32].contiguous(), k[..., :32].contiguous(), v[..., :32].contiguous(), cu, 10)
+    with pytest.raises(QvggtError, match="128 query heads"):
+        call(torch.zeros(10, 129, 64, device="cuda").half(), k[:, :1], v[:, :1], cu, 10)
+    with pytest.raises(TypeError, match="int32"):
+        call(q, k, v, cu.long(), 10)
+    with pytest.raises(ValueError, match="cu"):
+        call(q, k, v, cu[:0], 10)
+    with pytest.raises(QvggtError, match="aligned"):
+        call(torch.zeros(10 * 4 * 64 + 1, device="cuda").half()[1:].view(10, 4, 64), k, v, cu, 10)
+    with pytest.raises(QvggtError, match="strides"):
+        call(q, k[:1].expand(10, 2, 64), v, cu, 10)
+    with pytest.raises(QvggtError, match="scale"):
+        call(q, k, v, cu, 10, scale=0.0)
+    with pytest.raises(QvggtError, match="causal_chunk"):
+        call(q, k, v, cu, 10, -1)
+    with pytest.raises(ValueError, match="lse"):
+        call(q, k, v, cu, 10, lse=torch.empty(4, 9, device="cuda"))
+    with pytest.raises(ValueError, match="scratch"):
+        big = inputs(2, 4000, 4, 2, 64, torch.float16)
+        call(*big, ints([0, 4000]), 4000, scratch=torch.empty(1, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(ValueError, match="CUDA|devices"):
+        call(q, k, v, cu.cpu(), 10)
+    assert call(q[:0], k[:0], v[:0], ints([0]), 0).shape == (0, 4, 64)
