@@ -13,6 +13,7 @@ namespace {
 
 constexpr int UNIT = 32;                 // keys a warp takes at a time: never across two blocks
 constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int ROWS_MAX = 32;             // more rows of a key head go to key_weights_sm100.cu
 
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -215,6 +216,8 @@ extern "C" int qvggt_key_weights(const qvggt_key_weights_args* p, void* stream) 
   a.ctl = make_ctl();
   const bool bf16 = p->dtype == QVGGT_DTYPE_BF16;
   const long long rows = (long long)a.max_q * a.group, pairs = (long long)a.hk * a.B;
+  if (rows > ROWS_MAX && key_weight_tiles_can_read(a))
+    return launch_key_weight_tiles(a, (int)p->head_dim, bf16, static_cast<cudaStream_t>(stream));
   const long long units = std::max<long long>(1, (p->max_kv + UNIT - 1) / UNIT);
   // about eight CTAs per SM and at most eight units a warp before a CTA takes more
   const long long per = std::max<long long>(1, std::min<long long>(8, units * pairs / (32LL * device_info().num_sms)));
