@@ -15,6 +15,7 @@ struct KeyWeightArgs {
   float* out;
   long long q_tok, q_head, block_stride, Tq;
   int B, hq, hk, group, wide, num_blocks, bs_log2, chunk, max_q;
+  uint32_t chunk_mul, chunk_shift;       // division by chunk
   int row_blocks;                        // 1: a request is one entry of scan_blocks
   float scale_log2, decay;
   uint32_t wait_tries;                   // bound of every wait
