@@ -87,24 +87,42 @@ __global__ void __launch_bounds__(THREADS) key_weights_rows_kernel(KeyWeightArgs
         ks = a.ks[(long long)id * a.hk + kvh];
       }
     }
+    // the next unit's codes and old weight are on their way while one is used
+    uint4 w[2][2][KC], wn[2][2][KC];     // keys 16 mt + 8 half + g
+    float old = 0.f, old_n = 0.f;
+    auto fetch = [&](int i) {
+      const int blk = __shfl_sync(~0u, id, i);
+      if (i < 32 && blk >= 0) {
+        const int key0 = (u0 + i * stride) * UNIT;
+        const int8_t* kp = a.kc + blk * a.block_stride + ((long long)kvh * bs + (key0 & (bs - 1))) * D;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+              wn[mt][half][c] = __ldg(reinterpret_cast<const uint4*>(kp + (16 * mt + 8 * half + g) * D + 64 * c + 16 * t));
+        const int key = key0 + 16 * (t / 2) + 8 * (t % 2) + g;
+        old_n = key < n && key < fresh ? a.w[(((long long)blk * a.hk + kvh) << a.bs_log2) + (key & (bs - 1))] : 0.f;
+      }
+    };
+    fetch(0);
     for (int i = 0; i < 32 && u0 + i * stride < units; ++i) {
       const int blk = __shfl_sync(~0u, id, i);
       const float ck = __shfl_sync(~0u, ks, i) * a.scale_log2;
-      if (blk < 0) continue;
-      const int key0 = (u0 + i * stride) * UNIT;
-      const int8_t* kp = a.kc + blk * a.block_stride + ((long long)kvh * bs + (key0 & (bs - 1))) * D;
-      uint4 w[2][2][KC];                 // keys 16 mt + 8 half + g
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int c = 0; c < KC; ++c)
-            w[mt][half][c] = __ldg(reinterpret_cast<const uint4*>(kp + (16 * mt + 8 * half + g) * D + 64 * c + 16 * t));
+          for (int c = 0; c < KC; ++c) w[mt][half][c] = wn[mt][half][c];
+      old = old_n * a.decay;
+      fetch(i + 1);                      // (of unit 32 nothing: its lane is outside the batch)
+      if (blk < 0) continue;
+      const int key0 = (u0 + i * stride) * UNIT;
       // the place this lane writes: key 16 (t / 2) + 8 (t % 2) + g
       const int key = key0 + 16 * (t / 2) + 8 * (t % 2) + g;
       const long long place = (((long long)blk * a.hk + kvh) << a.bs_log2) + (key & (bs - 1));
-      const float old = key < n && key < fresh ? a.w[place] * a.decay : 0.f;
       float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
       for (int row0 = 0; row0 < rows; row0 += 8 * NT) {
         if (!once) load_rows(row0);

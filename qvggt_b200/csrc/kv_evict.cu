@@ -4,6 +4,8 @@
 // Keys may lie in any order in the cache (their positions are in the rotated
 // rows), so only survivors past the new length move, each into the place of an
 // evicted key below it; what stays where it is is not rounded again.
+#include <type_traits>
+
 #include "host.hpp"
 #include "kv_cache.cuh"
 
@@ -11,12 +13,13 @@ namespace qv {
 namespace {
 
 // ------------------------------------------------------------------- choice
-constexpr int CHOOSE_THREADS = 512, CHOOSE_WARPS = CHOOSE_THREADS / 32;
+constexpr int CHOOSE_THREADS = 1024, CHOOSE_WARPS = CHOOSE_THREADS / 32;
 constexpr int SPAN = 128;                // positions a warp takes at a time, four a lane
 // Digits of the 32-bit keys, from the top: 12, 10 and 10 bits.  The first one
 // holds the exponent and three bits more, which spreads weights of any size
 // over enough bins that few lanes meet in one.
 constexpr int BINS1 = 4096, BINS2 = 1024;
+static_assert(BINS1 == 4 * CHOOSE_THREADS && BINS2 == CHOOSE_THREADS, "a thread sums four bins, or one");
 
 struct ChooseArgs {
   const float* w;                        // [layers][num_blocks][heads][bs]
@@ -28,17 +31,22 @@ struct ChooseArgs {
 };
 
 // Weights as integers in their order: NaN and what is below every finite float
-// count as the lowest, infinity as the largest finite one, -0 as 0.
+// count as the lowest (the maximum takes its other operand), infinity as the
+// largest finite one, -0 as 0.
 __device__ __forceinline__ uint32_t order_of(float w) {
   const float big = 3.4028234663852886e38f;
-  const float x = (w != w ? -big : fminf(fmaxf(w, -big), big)) + 0.f;
-  const uint32_t u = __float_as_uint(x);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const int u = __float_as_int(fminf(fmaxf(w, -big), big) + 0.f);
+  return (uint32_t)u ^ (uint32_t)(u >> 31 | 0x80000000);
 }
 
 __device__ __forceinline__ uint4 ld_cluster_u4(uint32_t at) {
   uint4 v;
   asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
   return v;
 }
 __device__ __forceinline__ uint32_t cluster_size() {
@@ -47,7 +55,7 @@ __device__ __forceinline__ uint32_t cluster_size() {
   return n;
 }
 
-// One (layer, request, head) per cluster of up to eight CTAs.  The `keep`-th
+// One (layer, request, head) per cluster of one to four CTAs.  The `keep`-th
 // largest key is found digit by digit: each CTA counts its positions' digits in
 // shared memory, after a cluster barrier each adds up all CTAs' counts.  The
 // positions of a warp are consecutive, so ranks in order come from running sums
@@ -59,8 +67,9 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
   __shared__ __align__(16) uint32_t hist[BINS1 + 2 * BINS2];
   __shared__ uint32_t warp_sum[CHOOSE_WARPS];
   __shared__ uint32_t found[3];          // the digit, how many of its keys stay, how many there are
-  __shared__ int cnt[3][CHOOSE_WARPS];   // per warp: ties, holes, late survivors
-  __shared__ __align__(16) int total[4]; // of this CTA
+  __shared__ uint32_t cnt[CHOOSE_WARPS]; // per warp: ties, then holes
+  __shared__ uint32_t late_cnt[CHOOSE_WARPS];              // and late survivors
+  __shared__ uint32_t total[3];          // of this CTA: ties, holes, late survivors
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   for (int i = tid; i < BINS1 + 2 * BINS2; i += CHOOSE_THREADS) hist[i] = 0;
   pdl_wait();
@@ -84,7 +93,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
   }
   const int sink = min(a.sink, keep), recent = min(a.recent, keep - sink);
   const int middle = n - sink - recent;  // positions [sink, sink + middle) compete for the rest
-  int want = keep - sink - recent;
+  uint32_t want = keep - sink - recent;
   const int per_warp = (int)(((long long)n + C * CHOOSE_WARPS * SPAN - 1) / (C * CHOOSE_WARPS * SPAN)) * SPAN;
   const int start = (int)min((long long)n, (long long)(rank * CHOOSE_WARPS + warp) * per_warp);
   const int end = (int)min((long long)n, (long long)start + per_warp);
@@ -105,48 +114,38 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
   auto keys_of = [&](int i) {
     return held ? *reinterpret_cast<const uint4*>(keys + warp * per_warp + i - start) : fetch(i);
   };
-  // f(position, key, valid) for this warp's positions, four a lane, in their order
+  // f(base, position, keys) for this warp's positions, four a lane, in their order
   auto each = [&](auto load, auto f) {
 #pragma unroll 4
     for (int base = start; base < end; base += SPAN) {
       const int i = base + lane * 4;
       uint4 k = make_uint4(0, 0, 0, 0);
       if (i < end) k = load(i);
-      f(i, k);
+      f(base, i, k);
     }
   };
   auto competes = [&](int i) { return (unsigned)(i - sink) < (unsigned)middle; };
-  auto count = [&](uint32_t* bins, uint32_t bin, bool in) {
-    // a whole warp in one bin (weights that are all 0, say) adds once
-    const uint32_t first = __shfl_sync(~0u, bin, 0);
-    if (__all_sync(~0u, in && bin == first)) {
-      if (lane == 0) atomicAdd(&bins[first], 32u);
-    } else if (in) {
-      atomicAdd(&bins[bin], 1u);
-    }
-  };
-  // The bin that holds the `want`-th key from the top, over all CTAs.
-  auto find = [&](const uint32_t* bins, int size) {
+  // Spans that lie whole among the competing positions need no look at each one;
+  // the comparisons bound the kernel (its ALU pipe was 68 % busy with them all).
+  auto whole = [&](int base) { return base >= sink && base + SPAN <= min(end, sink + middle); };
+  // The bin that holds the `want`-th key from the top, over all CTAs.  PER: bins a thread sums.
+  auto find = [&](const uint32_t* bins, auto PER) {
     if (C > 1) cluster_sync();
     else __syncthreads();
-    const int mine = size / CHOOSE_THREADS;                // 8 or 2 bins a thread, from the top
-    const int lo = size - (tid + 1) * mine;
-    uint32_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int r = 0; r < C; ++r) {
-      const uint32_t at = mapa_shared(bins + (mine == 8 ? lo : lo & ~3), r);
-      const uint4 x = ld_cluster_u4(at);
-      if (mine == 8) {
-        const uint4 y = ld_cluster_u4(at + 16);
-        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+    const int lo = (CHOOSE_THREADS - 1 - tid) * PER;       // the first thread takes the top ones
+    uint4 v = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (r >= C) continue;
+      const uint32_t at = mapa_shared(bins + lo, r);
+      if constexpr (PER == 4) {
+        const uint4 x = ld_cluster_u4(at);
+        v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
       } else {
-        v[6] += lo & 2 ? x.z : x.x;
-        v[7] += lo & 2 ? x.w : x.y;
+        v.w += ld_cluster_u32(at);
       }
     }
-    uint32_t sum = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum += v[e];
+    const uint32_t sum = v.x + v.y + v.z + v.w;
     uint32_t inc = sum;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -155,82 +154,78 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
     }
     if (lane == 31) warp_sum[warp] = inc;
     __syncthreads();
-    uint32_t before = inc - sum;
-    for (int x = 0; x < warp; ++x) before += warp_sum[x];
-    if (before < (uint32_t)want && (uint32_t)want <= before + sum) {
-      uint32_t c = before;
+    const uint32_t others = lane < warp ? warp_sum[lane] : 0u;
+    uint32_t c = __reduce_add_sync(~0u, others) + inc - sum;
+    if (c < want && want <= c + sum) {
+      const uint32_t x[4] = {v.w, v.z, v.y, v.x};          // from the top
 #pragma unroll
-      for (int e = 7; e >= 0; --e) {                       // v[7] is the top one
-        if (c < (uint32_t)want && (uint32_t)want <= c + v[e]) {
-          found[0] = (uint32_t)(lo + e - (8 - mine));
-          found[1] = (uint32_t)want - c;
-          found[2] = v[e];
+      for (int e = 0; e < PER; ++e) {
+        if (c < want && want <= c + x[e]) {
+          found[0] = (uint32_t)(lo + PER - 1 - e);
+          found[1] = want - c;
+          found[2] = x[e];
         }
-        c += v[e];
+        c += x[e];
       }
     }
     __syncthreads();
   };
 
   uint32_t border = 0xffffffffu, ties = 0, ties_kept = 0;  // no key is above this border
-  if (held) {
-    each(fetch, [&](int i, uint4 k) {
-      if (i < end) *reinterpret_cast<uint4*>(keys + warp * per_warp + i - start) = k;
-    });
-    __syncwarp();
-  }
   __syncthreads();
+  // the first digit is counted as the keys come in
+  each(fetch, [&](int base, int i, uint4 k) {
+    if (held && i < end) *reinterpret_cast<uint4*>(keys + warp * per_warp + i - start) = k;
+    const uint32_t x[4] = {k.x >> 20, k.y >> 20, k.z >> 20, k.w >> 20};
+    if (whole(base)) {
+      // all in one bin (weights that are all 0, say) add once: else they would queue
+      const uint32_t first = __shfl_sync(~0u, x[0], 0);
+      if (__all_sync(~0u, ((x[0] ^ first) | (x[1] ^ first) | (x[2] ^ first) | (x[3] ^ first)) == 0)) {
+        if (lane == 0) atomicAdd(&hist[first], (uint32_t)SPAN);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) atomicAdd(&hist[x[e]], 1u);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i < end && competes(i + e)) atomicAdd(&hist[x[e]], 1u);
+    }
+  });
   if (want > 0) {
-    const uint32_t* k1 = hist;
-    each(keys_of, [&](int i, uint4 k) {
-      const uint32_t x[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) count(hist, x[e] >> 20, i < end && competes(i + e));
-    });
-    find(k1, BINS1);
+    find(hist, std::integral_constant<int, 4>());
     border = found[0] << 20;
-    want = (int)found[1];
+    want = found[1];
     __syncthreads();
-    each(keys_of, [&](int i, uint4 k) {
-      const uint32_t x[4] = {k.x, k.y, k.z, k.w};
+    // f(key) for the keys that compete
+    auto count = [&](uint32_t* bins, int above, int shift) {
+      each(keys_of, [&](int base, int i, uint4 k) {
+        const uint32_t x[4] = {k.x, k.y, k.z, k.w};
+        const bool all = whole(base);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (i < end && competes(i + e) && x[e] >> 20 == border >> 20) atomicAdd(&hist[BINS1 + (x[e] >> 10 & 1023)], 1u);
-    });
-    find(hist + BINS1, BINS2);
+        for (int e = 0; e < 4; ++e)
+          if ((x[e] ^ border) >> above == 0 && (all || (i < end && competes(i + e)))) atomicAdd(&bins[x[e] >> shift & 1023], 1u);
+      });
+    };
+    count(hist + BINS1, 20, 10);
+    find(hist + BINS1, std::integral_constant<int, 1>());
     border |= found[0] << 10;
-    want = (int)found[1];
+    want = found[1];
     __syncthreads();
-    each(keys_of, [&](int i, uint4 k) {
-      const uint32_t x[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (i < end && competes(i + e) && x[e] >> 10 == border >> 10) atomicAdd(&hist[BINS1 + BINS2 + (x[e] & 1023)], 1u);
-    });
-    find(hist + BINS1 + BINS2, BINS2);
+    count(hist + BINS1 + BINS2, 10, 0);
+    find(hist + BINS1 + BINS2, std::integral_constant<int, 1>());
     border |= found[0];
     ties_kept = found[1];
     ties = found[2];
   }
 
-  // Running sums over the CTAs and warps before this one of what `cnt[x]` holds.
-  auto before_this = [&](int x) {
-    __syncthreads();
-    int in_cta = 0, all = 0;
-    for (int y = 0; y < CHOOSE_WARPS; ++y) {
-      if (y == warp) in_cta = all;
-      all += cnt[x][y];
-    }
-    if (C == 1) return in_cta;
-    if (tid == 0) total[x] = all;
-    cluster_sync();
-    for (int r = 0; r < rank; ++r) {
-      int v;
-      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(&total[x], r)) : "memory");
-      in_cta += v;
-    }
-    return in_cta;
+  // The sum of the warps' counts before this one, and of all.
+  auto warps_before = [&](const uint32_t* c, uint32_t& all) {
+    const uint32_t v = c[lane];
+    all = __reduce_add_sync(~0u, v);
+    return __reduce_add_sync(~0u, lane < warp ? v : 0u);
   };
+  static_assert(CHOOSE_WARPS == 32, "a lane per warp");
   const unsigned below = (1u << lane) - 1;
   // how many marks in lanes before this one, and in all, of four flags a lane
   auto rank4 = [&](const bool (&f)[4], int& all) {
@@ -249,88 +244,108 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
   int tie0 = 0;
   if (some_ties) {
     int c = 0;
-    each(keys_of, [&](int i, uint4 k) {
+    each(keys_of, [&](int, int i, uint4 k) {
       const uint32_t x[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) c += i < end && competes(i + e) && x[e] == border;
     });
     c = __reduce_add_sync(~0u, c);
-    if (lane == 0) cnt[0][warp] = c;
-    tie0 = before_this(0);
+    if (lane == 0) cnt[warp] = c;
+    __syncthreads();
+    uint32_t all;
+    tie0 = warps_before(cnt, all);
+    if (tid == 0) total[0] = all;
+    if (C > 1) {
+      cluster_sync();
+      const uint32_t v = lane < rank ? ld_cluster_u32(mapa_shared(&total[0], lane)) : 0u;
+      tie0 += __reduce_add_sync(~0u, v);
+    }
+    __syncthreads();                     // everyone has read cnt
   }
-  // f(position, hole flags, late flags) in order
+  // f(position, flags of keys that go / stay, whether those are holes, late ones) in order
+  const uint32_t lowest = some_ties || ties == 0 ? border + (border != 0xffffffffu) : border;   // stays, ties apart
   auto marks = [&](auto f) {
     int tie = tie0;
-    each(keys_of, [&](int i, uint4 k) {
+    each(keys_of, [&](int base, int i, uint4 k) {
       const uint32_t x[4] = {k.x, k.y, k.z, k.w};
-      bool eq[4], hole[4], late[4];
+      bool flag[4];
+      if (!some_ties && whole(base) && (base + SPAN <= keep || base >= keep)) {
+        const bool hole = base < keep;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) flag[e] = (x[e] < lowest) == hole;
+        f(i, flag, hole, !hole);
+        return;
+      }
+      bool eq[4], late[4];
       int rank_eq = 0, all = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) eq[e] = i < end && competes(i + e) && x[e] == border;
+      for (int e = 0; e < 4; ++e) eq[e] = some_ties && i < end && competes(i + e) && x[e] == border;
       if (some_ties) rank_eq = tie + rank4(eq, all);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int p = i + e;
-        bool stays = !competes(p) || x[e] > border;
-        if (eq[e]) stays = !some_ties ? ties > 0 : rank_eq < (int)ties_kept;
+        bool stays = !competes(p) || x[e] >= lowest;
+        if (eq[e]) stays = rank_eq < (int)ties_kept;
         rank_eq += eq[e];
-        hole[e] = p < keep && !stays && i < end;
+        flag[e] = p < keep && !stays && i < end;
         late[e] = p >= keep && p < n && stays && i < end;
       }
       tie += all;
-      f(i, hole, late);
+      f(i, flag, true, false);
+      f(i, late, false, true);
     });
   };
   int holes = 0, lates = 0;
-  marks([&](int, const bool (&hole)[4], const bool (&late)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      holes += hole[e];
-      lates += late[e];
-    }
+  marks([&](int, const bool (&flag)[4], bool hole, bool late) {
+    const int c = flag[0] + flag[1] + flag[2] + flag[3];
+    if (hole) holes += c;
+    if (late) lates += c;
   });
   holes = __reduce_add_sync(~0u, holes);
   lates = __reduce_add_sync(~0u, lates);
   if (lane == 0) {
-    cnt[1][warp] = holes;
-    cnt[2][warp] = lates;
+    cnt[warp] = holes;
+    late_cnt[warp] = lates;
   }
-  int hole_at = before_this(1), late_at = before_this(2);
-  bool over = false;
-  marks([&](int i, const bool (&hole)[4], const bool (&late)[4]) {
-    int all_h, all_l;
-    int x = hole_at + rank4(hole, all_h), y = late_at + rank4(late, all_l);
-    hole_at += all_h;
-    late_at += all_l;
+  __syncthreads();
+  uint32_t all_holes, all_lates;
+  int hole_at = warps_before(cnt, all_holes), late_at = warps_before(late_cnt, all_lates);
+  int moves = (int)all_holes;
+  if (C > 1) {
+    if (tid == 0) {
+      total[1] = all_holes;
+      total[2] = all_lates;
+    }
+    cluster_sync();
+    const uint32_t vh = lane < C ? ld_cluster_u32(mapa_shared(&total[1], lane)) : 0u;
+    const uint32_t vl = lane < rank ? ld_cluster_u32(mapa_shared(&total[2], lane)) : 0u;
+    moves = __reduce_add_sync(~0u, vh);
+    hole_at += __reduce_add_sync(~0u, lane < rank ? vh : 0u);
+    late_at += __reduce_add_sync(~0u, vl);
+  }
+  marks([&](int i, const bool (&flag)[4], bool hole, bool) {
+    int32_t* to = hole ? dst : src;
+    int all, x = (hole ? hole_at : late_at) + rank4(flag, all);
+    if (hole) hole_at += all;
+    else late_at += all;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (hole[e]) {
-        if (x < a.max_moves) dst[x] = i + e;
-        else over = true;
-        ++x;
-      }
-      if (late[e]) {
-        if (y < a.max_moves) src[y] = i + e;
-        ++y;
-      }
+      if (flag[e] && x < a.max_moves) to[x] = i + e;
+      x += flag[e];
     }
   });
-  if (over) report_status(a.ctl, ST_BAD_LENGTH);
-  // the last warp's running sum is the number of moves; every CTA pads its share
-  if (rank == C - 1 && warp == CHOOSE_WARPS - 1 && lane == 0) total[3] = hole_at;
-  if (C > 1) cluster_sync();
-  else __syncthreads();
-  int moves;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(moves) : "r"(mapa_shared(&total[3], C - 1)) : "memory");
-  moves = min(moves, a.max_moves);
-  if (rank == 0 && tid == 0) a.counts[row] = moves;
+  if (rank == 0 && tid == 0) {
+    if (moves > a.max_moves) report_status(a.ctl, ST_BAD_LENGTH);
+    a.counts[row] = min(moves, a.max_moves);
+  }
   pad_from(moves);
   if (C > 1) cluster_sync();             // nobody leaves while others read its shared memory
 }
 
 // --------------------------------------------------------------------- move
 constexpr int MOVE_THREADS = 256, MOVE_WARPS = MOVE_THREADS / 32;
-constexpr int MOVE_BLOCKS = 256;         // blocks whose moves a CTA looks up at a time
+constexpr int MOVE_BLOCKS = 32;          // blocks of a CTA at most
+constexpr int MOVE_LOADS = 4;            // 16-byte pieces a lane has under way
 
 struct MoveArgs {
   int8_t* codes[2];
@@ -339,6 +354,7 @@ struct MoveArgs {
   const int32_t *table, *keep, *src, *dst, *counts;
   long long layer_stride, block_stride;
   int B, heads, wide, num_blocks, bs_log2, max_moves;
+  int parts, span;                       // CTAs of a (layer, request, head), blocks of each
   Ctl ctl;
 };
 
@@ -359,25 +375,59 @@ __device__ __forceinline__ int warp_lower_bound(const int32_t* a, int n, int x) 
   return lo;
 }
 
-// One (layer, request, head) per cluster; a warp takes K or V of one block that
-// receives rows: the rows' largest magnitude, the block's scale (it only grows,
-// as when rows are appended), the rows' codes, and, where the scale grew, the
-// block's other codes.  Rows leave places from the new length on and enter
-// places below it, so the only block that is both read for others and written
-// is the one that the new length falls into: it waits until the whole cluster
-// is done with the others.
-template <int D>
-__global__ void __launch_bounds__(MOVE_THREADS) kv_evict_kernel(MoveArgs a) {
+// Four codes c rounded anew: rint(c f g).  A byte with its sign bit flipped under
+// the exponent of 2^23 is the float 2^23 + 128 + c, and adding 1.5 * 2^23 rounds to
+// the nearest integer, ties to even, into the low byte: a conversion each way goes
+// through the 16-a-clock pipe, which then bounds the kernel.  (The products stay
+// between -128 and 127 because the scale covers them.)
+template <bool TWO>
+__device__ __forceinline__ uint32_t recode4(uint32_t c, float f, float g) {
+  const uint32_t u = c ^ 0x80808080u;
+  const uint64_t B = f2_pack(-8388736.f, -8388736.f), M = f2_pack(12582912.f, 12582912.f), F = f2_pack(f, f);
+  float y[4];
+#pragma unroll
+  for (int e = 0; e < 4; e += 2) {
+    uint64_t x = f2_add(f2_pack(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 | e)),
+                                __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441 | e))), B);
+    if (TWO) x = f2_mul(x, F);
+    // the last product alone: a paired one is compiled into one rounding with the addition
+    const float z = TWO ? g : f;
+    f2_unpack(x, y[e], y[e + 1]);
+    f2_unpack(f2_add(f2_pack(__fmul_rn(y[e], z), __fmul_rn(y[e + 1], z)), M), y[e], y[e + 1]);
+  }
+  return __byte_perm(__byte_perm(__float_as_uint(y[0]), __float_as_uint(y[1]), 0x0040),
+                     __byte_perm(__float_as_uint(y[2]), __float_as_uint(y[3]), 0x0040), 0x5410);
+}
+template <bool TWO>
+__device__ __forceinline__ uint4 recode16(uint4 c, float f, float g) {
+  return make_uint4(recode4<TWO>(c.x, f, g), recode4<TWO>(c.y, f, g), recode4<TWO>(c.z, f, g), recode4<TWO>(c.w, f, g));
+}
+// The largest magnitude of 16 codes.
+__device__ __forceinline__ float largest16(uint4 c) {
+  const uint32_t m = __vmaxu4(__vmaxu4(__vabs4(c.x), __vabs4(c.y)), __vmaxu4(__vabs4(c.z), __vabs4(c.w)));
+  return (float)max(max(m & 0xffu, m >> 8 & 0xffu), max(m >> 16 & 0xffu, m >> 24));
+}
+
+// A CTA takes up to MOVE_BLOCKS blocks of one (layer, request, head), a warp K or
+// V of one of them that receives rows: the rows' largest magnitude, the block's
+// scale (it only grows, as when rows are appended), the rows' codes, and, where
+// the scale grew, the block's other codes.  Rows leave places from the new length
+// on and enter places below it, so the only block that is both read for others
+// and written is the one that the new length falls into: a second launch (EDGE)
+// does that one, when all others are done.
+template <int D, bool EDGE>
+__global__ void __launch_bounds__(MOVE_THREADS, 4) kv_evict_kernel(MoveArgs a) {
   constexpr int PARTS = D / 16;          // 16-byte pieces of a row
+  constexpr int AT_ONCE = 32 * MOVE_LOADS;                 // pieces of a warp under way
   __shared__ int2 range[MOVE_BLOCKS];    // a block's moves
   __shared__ int bounds[2];
-  __shared__ int row_slot[MOVE_WARPS][128];                // where an incoming row is, -1: nowhere
-  __shared__ uint8_t row_dst[MOVE_WARPS][128];
+  __shared__ int2 row_from[MOVE_WARPS][128];               // where an incoming row is (-1: nowhere), its scale
+  __shared__ uint8_t row_to[MOVE_WARPS][128];
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const int C = (int)cluster_size(), rank = (int)cluster_ctarank();
-  const int row = blockIdx.x / C, h = row % a.heads, b = row / a.heads % a.B, layer = row / a.heads / a.B;
+  const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+  const int h = row % a.heads, b = row / a.heads % a.B, layer = row / a.heads / a.B;
   const int bs = 1 << a.bs_log2;
   const int keep = a.keep[b];
   int moves = a.counts[row];
@@ -399,6 +449,9 @@ __global__ void __launch_bounds__(MOVE_THREADS) kv_evict_kernel(MoveArgs a) {
       if (lane == 0) report_bad_block(a.ctl);
       return;
     }
+    int8_t* codes = (side ? a.codes[1] : a.codes[0]) + layer * a.layer_stride + ((long long)h << a.bs_log2) * D;
+    float* scales = side ? a.scales[1] : a.scales[0];
+    const float before = scales[cell(blk)];
     unsigned taken[4] = {0, 0, 0, 0};    // the block's rows that are written
     for (int r0 = 0; r0 < rows; r0 += 32) {
       const int r = r0 + lane;
@@ -408,94 +461,103 @@ __global__ void __launch_bounds__(MOVE_THREADS) kv_evict_kernel(MoveArgs a) {
         to = dst[m0 + r] - (j << a.bs_log2);
         const bool fits = s >= keep && s < (a.wide << a.bs_log2) && to >= 0 && to < bs && to + (j << a.bs_log2) < keep;
         const int from = fits ? table[s >> a.bs_log2] : 0;
-        if (fits && in_pool(from)) slot = (from << a.bs_log2) + (s & (bs - 1));
-        else report_status(a.ctl, fits ? ST_BAD_BLOCK : ST_BAD_LENGTH);
-        row_slot[warp][r] = slot;
-        row_dst[warp][r] = (uint8_t)to;
-        if (side == 0 && a.w && slot >= 0)
-          a.w[(cell(blk) << a.bs_log2) + to] = a.w[(cell(slot >> a.bs_log2) << a.bs_log2) + (slot & (bs - 1))];
+        float f = 0.f;
+        if (fits && in_pool(from)) {
+          slot = (from << a.bs_log2) + (s & (bs - 1));
+          f = scales[cell(from)];
+          if (side == 0 && a.w) a.w[(cell(blk) << a.bs_log2) + to] = a.w[(cell(from) << a.bs_log2) + (s & (bs - 1))];
+        } else {
+          report_status(a.ctl, fits ? ST_BAD_BLOCK : ST_BAD_LENGTH);
+        }
+        row_from[warp][r] = make_int2(slot, __float_as_int(f));
+        row_to[warp][r] = (uint8_t)to;
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x) taken[x] |= __reduce_or_sync(~0u, slot >= 0 && to / 32 == x ? 1u << (to & 31) : 0u);
     }
     __syncwarp();
-    int8_t* codes = (side ? a.codes[1] : a.codes[0]) + layer * a.layer_stride + ((long long)h << a.bs_log2) * D;
-    float* scales = side ? a.scales[1] : a.scales[0];
-    const float before = scales[cell(blk)];
     auto at = [&](int slot, int part) {
       return reinterpret_cast<uint4*>(codes + (long long)(slot >> a.bs_log2) * a.block_stride + (slot & (bs - 1)) * D + part * 16);
     };
+    uint4 c[MOVE_LOADS];
+    auto load = [&](int p0) {
+#pragma unroll
+      for (int x = 0; x < MOVE_LOADS; ++x) {
+        const int p = p0 + 32 * x + lane;
+        c[x] = make_uint4(0, 0, 0, 0);
+        if (p < rows * PARTS) {
+          const int slot = row_from[warp][p / PARTS].x;
+          if (slot >= 0) c[x] = *at(slot, p % PARTS);
+        }
+      }
+    };
+    // where all rows fit the registers (`once`) they are read once, else again for their codes
+    const bool once = rows * PARTS <= AT_ONCE;
     float most = 0.f;
-    for (int p = lane; p < rows * PARTS; p += 32) {
-      const int slot = row_slot[warp][p / PARTS];
-      if (slot < 0) continue;
-      const uint4 c = *at(slot, p % PARTS);
-      const uint32_t m = __vmaxu4(__vmaxu4(__vabs4(c.x), __vabs4(c.y)), __vmaxu4(__vabs4(c.z), __vabs4(c.w)));
-      const uint32_t m1 = max(max(m & 0xffu, m >> 8 & 0xffu), max(m >> 16 & 0xffu, m >> 24));
-      most = fmaxf(most, __fmul_rn((float)m1, scales[cell(slot >> a.bs_log2)]));
+    for (int p0 = 0; p0 < rows * PARTS; p0 += AT_ONCE) {
+      load(p0);
+#pragma unroll
+      for (int x = 0; x < MOVE_LOADS; ++x) {
+        const int p = p0 + 32 * x + lane;
+        if (p < rows * PARTS) most = fmaxf(most, __fmul_rn(largest16(c[x]), __int_as_float(row_from[warp][p / PARTS].y)));
+      }
     }
     most = warp_max(most);
     const float s = fmaxf(fmaxf(before, __fdiv_rn(most, 127.f)), KV_SCALE_MIN);
     const float inv = __frcp_rn(s);
-    auto round4 = [&](uint32_t c, float f, float g) {      // codes of c f g
-      auto one = [&](int x) { return (uint32_t)(uint8_t)kv_code(__fmul_rn(__fmul_rn((float)x, f), g)); };
-      return one((int8_t)c) | one((int8_t)(c >> 8)) << 8 | one((int8_t)(c >> 16)) << 16 | one((int8_t)(c >> 24)) << 24;
-    };
-    for (int p = lane; p < rows * PARTS; p += 32) {
-      const int slot = row_slot[warp][p / PARTS];
-      if (slot < 0) continue;
-      const uint4 c = *at(slot, p % PARTS);
-      const float f = scales[cell(slot >> a.bs_log2)];
-      *at((blk << a.bs_log2) + row_dst[warp][p / PARTS], p % PARTS) =
-          make_uint4(round4(c.x, f, inv), round4(c.y, f, inv), round4(c.z, f, inv), round4(c.w, f, inv));
+    for (int p0 = 0; p0 < rows * PARTS; p0 += AT_ONCE) {
+      if (!once) load(p0);
+#pragma unroll
+      for (int x = 0; x < MOVE_LOADS; ++x) {
+        const int p = p0 + 32 * x + lane;
+        if (p >= rows * PARTS) continue;
+        const int2 from = row_from[warp][p / PARTS];
+        if (from.x >= 0)
+          *at((blk << a.bs_log2) + row_to[warp][p / PARTS], p % PARTS) = recode16<true>(c[x], __int_as_float(from.y), inv);
+      }
     }
     __syncwarp();
     if (s == before) return;
     const float f = __fmul_rn(before, inv);
-    for (int p = lane; p < bs * PARTS; p += 32) {
-      const int to = p / PARTS;
-      const unsigned word = to < 64 ? (to < 32 ? taken[0] : taken[1]) : (to < 96 ? taken[2] : taken[3]);
-      if (word >> (to & 31) & 1) continue;
-      uint4* q = at((blk << a.bs_log2) + to, p % PARTS);
-      const uint4 c = *q;
-      *q = make_uint4(round4(c.x, f, 1.f), round4(c.y, f, 1.f), round4(c.z, f, 1.f), round4(c.w, f, 1.f));
+    uint4* all = at(blk << a.bs_log2, 0);
+    for (int p0 = 0; p0 < bs * PARTS; p0 += AT_ONCE) {
+      auto stays = [&](int x) {
+        const int to = (p0 + 32 * x + lane) / PARTS;
+        const unsigned word = to < 64 ? (to < 32 ? taken[0] : taken[1]) : (to < 96 ? taken[2] : taken[3]);
+        return to < bs && !(word >> (to & 31) & 1);
+      };
+#pragma unroll
+      for (int x = 0; x < MOVE_LOADS; ++x)
+        if (stays(x)) c[x] = all[p0 + 32 * x + lane];
+#pragma unroll
+      for (int x = 0; x < MOVE_LOADS; ++x)
+        if (stays(x)) all[p0 + 32 * x + lane] = recode16<false>(c[x], f, 0.f);
     }
     if (lane == 0) scales[cell(blk)] = s;
   };
 
   const int blocks = (int)(((long long)keep + bs - 1) >> a.bs_log2);
   const int edge = keep & (bs - 1) ? keep >> a.bs_log2 : -1;
-  const int per = (blocks + C - 1) / C, last = min(blocks, (rank + 1) * per);
-  int2 at_edge = make_int2(0, 0);
-  if (moves > 0) {                       // (the same for the whole cluster)
-    for (int j0 = rank * per; j0 < last; j0 += MOVE_BLOCKS) {
-      const int j1 = min(last, j0 + MOVE_BLOCKS);
-      __syncthreads();
-      for (int j = tid; j < j1 - j0; j += MOVE_THREADS) range[j] = make_int2(0, 0);
-      if (warp < 2) {
-        const int x = warp_lower_bound(dst, moves, (warp == 0 ? j0 : j1) << a.bs_log2);
-        if (lane == 0) bounds[warp] = x;
-      }
-      __syncthreads();
-      // `dst` ascends: a block's moves are consecutive
-      for (int i = bounds[0] + tid; i < bounds[1]; i += MOVE_THREADS) {
-        const int j = dst[i] >> a.bs_log2;
-        if (j < j0 || j >= j1) continue;
-        if (i == bounds[0] || dst[i - 1] >> a.bs_log2 != j) range[j - j0].x = i;
-        if (i + 1 == bounds[1] || dst[i + 1] >> a.bs_log2 != j) range[j - j0].y = i + 1;
-      }
-      __syncthreads();
-      for (int u = warp; u < 2 * (j1 - j0); u += MOVE_WARPS) {
-        const int j = j0 + u / 2;
-        const int2 m = range[u / 2];
-        if (m.x >= m.y) continue;
-        if (j != edge) receive(j, m.x, m.y, u & 1);
-      }
-      if (edge >= j0 && edge < j1) at_edge = range[edge - j0];
-    }
-    if (C > 1) cluster_sync();
-    else __syncthreads();
-    if (at_edge.x < at_edge.y && warp < 2) receive(edge, at_edge.x, at_edge.y, warp);
+  const int j0 = EDGE ? edge : part * a.span, j1 = EDGE ? edge + 1 : min(blocks, j0 + a.span);
+  if (moves == 0 || j0 < 0 || j0 >= j1) return;
+  if (tid < MOVE_BLOCKS) range[tid] = make_int2(0, 0);
+  if (warp < 2) {
+    const int x = warp_lower_bound(dst, moves, (warp == 0 ? j0 : j1) << a.bs_log2);
+    if (lane == 0) bounds[warp] = x;
+  }
+  __syncthreads();
+  // `dst` ascends: a block's moves are consecutive
+  for (int i = bounds[0] + tid; i < bounds[1]; i += blockDim.x) {
+    const int j = dst[i] >> a.bs_log2;
+    if (j < j0 || j >= j1) continue;
+    if (i == bounds[0] || dst[i - 1] >> a.bs_log2 != j) range[j - j0].x = i;
+    if (i + 1 == bounds[1] || dst[i + 1] >> a.bs_log2 != j) range[j - j0].y = i + 1;
+  }
+  __syncthreads();
+  for (int u = warp; u < 2 * (j1 - j0); u += MOVE_WARPS) {
+    const int j = j0 + u / 2;
+    const int2 m = range[u / 2];
+    if (m.x < m.y && (EDGE || j != edge)) receive(j, m.x, m.y, u & 1);
   }
 }
 
@@ -527,7 +589,11 @@ extern "C" int qvggt_evict_plan(const qvggt_evict_plan_args* p, void* stream) {
   const int64_t rows = p->layers * p->requests * p->kv_heads;
   const int64_t longest = p->max_len ? std::min(p->max_len, p->max_blocks * p->block_size) : p->max_blocks * p->block_size;
   int C = 1;
-  while (C < 8 && rows * C < 2 * device_info().num_sms && longest > 2048LL * C) C *= 2;
+  // Clusters where the rows alone leave SMs idle and each CTA still has 8192 keys:
+  // a cluster's barriers cost about 8 us (16 rows of 44,000 keys: 45 us as one CTA
+  // each, 21 as four; 128 rows of 8,000: 11.5 and 24).  Eight CTAs to a cluster
+  // only halve how many run at once (16 rows: 40 us).
+  while (C < 4 && 2 * rows * C <= device_info().num_sms && longest > 8192LL * C) C *= 2;
   const int64_t part = (longest + C * CHOOSE_WARPS * SPAN - 1) / (C * CHOOSE_WARPS * SPAN) * (CHOOSE_WARPS * SPAN);
   constexpr int ROOM_MAX = 48 * 1024;    // 192 KB of keys beside 25 KB of counts
   const int room = part <= ROOM_MAX ? (int)part : 0;
@@ -561,16 +627,24 @@ extern "C" int qvggt_kv_evict(const qvggt_kv_evict_args* p, void* stream) {
   if (p->layer_stride % 16) return set_error(QVGGT_ERR_ALIGN, "%s: the layers must be 16-byte aligned", name);
   if (p->layers > 1 && p->layer_stride < (c.num_blocks - 1) * c.block_stride + c.kv_heads * c.block_size * c.head_dim)
     return set_error(QVGGT_ERR_INVALID, "%s: layer stride smaller than a layer", name);
+  const int64_t rows = p->layers * p->requests * c.kv_heads;
+  // as many blocks a CTA as leave every SM a few dozen CTAs, up to four for each warp
+  const int64_t span = std::max<int64_t>(4, std::min<int64_t>(MOVE_BLOCKS, rows * p->max_blocks / (32 * device_info().num_sms)));
+  const int64_t parts = std::max<int64_t>(1, (p->max_blocks + span - 1) / span);
+  if (rows * parts > 2147483647LL) return set_error(QVGGT_ERR_UNSUPPORTED, "%s: too many blocks", name);
   MoveArgs a{{c.k_cache, c.v_cache}, {c.k_scale, c.v_scale}, p->weights, p->block_tables, p->keep, p->src, p->dst,
              p->counts, p->layer_stride, c.block_stride, (int)p->requests, (int)c.kv_heads, (int)p->max_blocks,
-             (int)c.num_blocks, log2_of(c.block_size), (int)p->max_moves, make_ctl()};
-  const int64_t rows = p->layers * p->requests * c.kv_heads;
-  int C = 1;
-  while (C < 8 && rows * C < 8 * device_info().num_sms && p->max_blocks > 4LL * C) C *= 2;
-  const auto fn = c.head_dim == 64 ? kv_evict_kernel<64> : kv_evict_kernel<128>;
-  int rc = check_cuda(launch_pdl(fn, dim3((unsigned)(rows * C)), dim3(MOVE_THREADS), 0, static_cast<cudaStream_t>(stream),
-                                 (unsigned)C, a),
-                      "kv_evict launch");
-  if (!rc) count_launch(1);
-  return rc;
+             (int)c.num_blocks, log2_of(c.block_size), (int)p->max_moves, (int)parts, (int)span, make_ctl()};
+  using Kfn = void (*)(MoveArgs);
+  static const Kfn fns[2][2] = {{kv_evict_kernel<64, false>, kv_evict_kernel<64, true>},
+                                {kv_evict_kernel<128, false>, kv_evict_kernel<128, true>}};
+  for (int edge = 0; edge < 2; ++edge) {
+    if (edge) a.parts = 1;
+    if (int rc = check_cuda(launch_pdl(fns[c.head_dim == 128][edge], dim3((unsigned)(rows * a.parts)),
+                                       dim3(edge ? 64 : MOVE_THREADS), 0, static_cast<cudaStream_t>(stream), 1u, a),
+                            "kv_evict launch"))
+      return rc;
+    count_launch(1);
+  }
+  return QVGGT_OK;
 }
