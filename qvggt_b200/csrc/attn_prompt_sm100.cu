@@ -10,10 +10,10 @@
 // Per key tile of KT keys (128 for head_dim 64, 64 for 128):
 //   warp 0         TMA of K, V and Q tiles, K and V through rings of KV stages
 //   warp 1         S_i = Q_i K^T        warp 3   O_i += P_i V
-//   warps 4..7     clean V tiles that some row of the block does not see whole
-//   warps 8..15    softmax, one thread per row of Q tile i = 0, 1
 //   warp 2         the segments (an item, or the part of it that falls to this
-//                  CTA), a few ahead; every other role reads them from a ring
+//                  CTA), two ahead, read by every role from a ring; cleans V tiles
+//                  that some row of the block does not see whole
+//   warps 4..11    softmax, one thread per row of Q tile i = 0, 1
 // The running maximum is raised lazily (2^8).  All waits are bounded; on expiry
 // every role leaves and the status word is set.
 //
@@ -31,10 +31,10 @@
 namespace qv {
 namespace {
 
-constexpr int THREADS = 512;
+constexpr int THREADS = 384;
 constexpr int KV = 4;           // stages of K and of V
 constexpr int SEGS = 4;         // segments handed out ahead
-constexpr int SEG_READERS = 15; // producer, two issuers, 4 + 8 warps
+constexpr int SEG_READERS = 12; // producer, two issuers, the V tiles' warp, 8 warps
 constexpr int Q_ROWS = 256;     // rows of an item
 // Cost of an item on the line, in tenths of a tile with two Q tiles: a start-up
 // (loads, first products, epilogue) and its key tiles.
@@ -191,24 +191,24 @@ struct Block {
   }
 };
 
-// Whether one of a word's two halves is an infinity or NaN.
+// Bits 15 and 31: whether the word's halves are infinities or NaN (adding one to
+// the exponent carries into the sign's place only then).
 template <bool BF16>
-__device__ __forceinline__ bool odd2(uint32_t w) {
-  constexpr uint32_t E = BF16 ? 0x7f80u : 0x7c00u;
-  return (w & E) == E || (w >> 16 & E) == E;
+__device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
+  return (w & 0x7fff7fffu) + (BF16 ? 0x00800080u : 0x04000400u);
 }
 
 // Adds what was taken out of the V tiles to columns cc.. of a row that sees
 // keys [from, to): elements that are not finite.  Any weight of theirs gives
 // the same sum, an infinity or NaN.
 template <bool BF16, int W>
-__device__ __noinline__ void add_odd(const PromptArgs& a, uint32_t* acc, int q0, int kvh, int cc, int from, int to) {
+__device__ __forceinline__ void add_odd(const PromptArgs& a, uint32_t (&acc)[W], int q0, int kvh, int cc, int from, int to) {
 #pragma unroll 1
   for (int j = from; j < to; ++j) {
     const uint16_t* p = a.v + (long long)(q0 + j) * a.v_tok + (long long)kvh * a.v_head + cc;
-#pragma unroll 1
+#pragma unroll
     for (int e = 0; e < W; ++e)
-      if (odd2<BF16>(p[e])) acc[e] = __float_as_uint(__uint_as_float(acc[e]) + half_bits_to_f32<BF16>(p[e]));
+      if (odd_bits<BF16>(p[e]) & 0x8000u) acc[e] = __float_as_uint(__uint_as_float(acc[e]) + half_bits_to_f32<BF16>(p[e]));
   }
 }
 
@@ -251,8 +251,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_clean[s], 4);
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&v_clean[s], 1);
+      mbar_init(&v_empty[s], 2);     // the product, and the warp that has seen to the tile
     }
     for (int s = 0; s < SEGS; ++s) {
       mbar_init(&seg_full[s], 1);
@@ -286,34 +286,106 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tmem = *tmem_slot;
   const int tpt = 128 / a.group;                           // tokens of a Q tile
 
-  // Registers: launched at 128 each; 128 (56 + 56 + 2 * 200) = 128 * 512.
+  // Registers: launched at 168 each; 128 (64 + 2 * 216) <= 168 * 384.
   // Every warp of a warpgroup runs the same setmaxnreg.
   if (warp < 4) {
-    regs_dec<56>();
+    regs_dec<64>();
     if (warp == 2) {
-      // ---------------------------------------------------------- segments
-      if (lane == 0) {
-        PieceWalk<THREADS, Block<KT>> walk(a, cum, blocks, g);
+      // ------------------------------------------------- segments and V tiles
+      PieceWalk<THREADS, Block<KT>> walk(a, cum, blocks, g);               // (lane 0's is used)
+      auto publish = [&](int seg) {            // lane 0; whether there was room in time, and one to hand out
+        const int st = seg % SEGS;
         Segment sg;
-        for (int seg = 0;; ++seg) {
-          const bool more = walk.next(a, blocks, sg);
-          const int st = seg % SEGS;
-          if (!wait(&seg_empty[st], ((seg / SEGS) & 1) ^ 1, tries)) break;
-          segs[st].b = sg.b;
-          segs[st].kvh = sg.kvh;
-          segs[st].tok0 = sg.tok0;
-          segs[st].q0 = sg.q0;
-          segs[st].ql = sg.ql;
-          segs[st].nqt = sg.nqt;
-          segs[st].t0 = sg.t0;
-          segs[st].nt = more ? sg.nt : -1;
-          segs[st].slot = sg.slot;
-          segs[st].pad[0] = 0;
-          mbar_arrive(&seg_full[st]);
-          if (!more) break;
+        const bool more = walk.next(a, blocks, sg);
+        if (!wait(&seg_empty[st], ((seg / SEGS) & 1) ^ 1, tries)) return -1;
+        segs[st].b = sg.b;
+        segs[st].kvh = sg.kvh;
+        segs[st].tok0 = sg.tok0;
+        segs[st].q0 = sg.q0;
+        segs[st].ql = sg.ql;
+        segs[st].nqt = sg.nqt;
+        segs[st].t0 = sg.t0;
+        segs[st].nt = more ? sg.nt : -1;
+        segs[st].slot = sg.slot;
+        segs[st].pad[0] = 0;
+        mbar_arrive(&seg_full[st]);
+        return more ? 1 : 0;
+      };
+      int left = 2;                            // 1: the last segment is out, 0: its end mark too, -1: gave up
+      auto hand_out = [&](int seg) {
+        int more = 0;
+        if (lane == 0) more = publish(seg);
+        return __shfl_sync(~0u, more, 0);
+      };
+      int jg = 0, ahead = 0;                   // tiles so far; segments handed out
+      for (; left > 0 && ahead < 2; ++ahead) left = hand_out(ahead);
+      for (int seg = 0; left >= 0; ++seg) {
+        if (left > 0) {
+          left = hand_out(ahead);
+          ++ahead;
+          if (left < 0) break;
         }
-        if (a.can_split) reinterpret_cast<Cut*>(a.part_lse + 2LL * gridDim.x * Q_ROWS)[blockIdx.x] = walk.cut;
+        const int ss = seg % SEGS;
+        __syncwarp();
+        const int nt = segs[ss].nt, t0 = segs[ss].t0, n = segs[ss].ql, tok0 = segs[ss].tok0;
+        if (nt < 0) {
+          if (lane == 0) mbar_arrive(&seg_empty[ss]);
+          break;
+        }
+        const int seen = key_limit(tok0, n, n, a.chunk);   // keys that every row sees
+        bool ok = true;
+        for (int j = 0; j < nt; ++j, ++jg) {
+          const int st = jg % KV, key0 = (t0 + j) * KT;
+          ok = warp_wait(&v_full[st], (jg / KV) & 1, tries);
+          if (!ok) break;
+          if (key0 + KT > seen) {
+            // 16-byte pieces (the swizzle moves them within their row only): is there
+            // an odd one?  This warp looks after two Q tiles' softmax, so it looks fast
+            // first and works only on what it found.
+            const int first = max(0, seen - key0);         // the tile's first row that some row does not see
+            uint32_t any = 0;
+#pragma unroll 1
+            for (int panel = 0; panel < L::PANELS; ++panel) {
+              const uint32_t at = sbase + L::V + st * OP_BYTES + panel * KT * 128;
+#pragma unroll 8
+              for (int p = first * 8 + lane; p < KT * 8; p += 32) {
+                uint32_t w[4];
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at + p * 16) : "memory");
+#pragma unroll
+                for (int e = 0; e < 4; ++e) any |= odd_bits<BF16>(w[e]);
+              }
+            }
+            if (__any_sync(~0u, (any & 0x80008000u) != 0)) {
+              bool odd = false;
+#pragma unroll 1
+              for (int p = lane; p < OP_BYTES / 16; p += 32) {
+                const int key = key0 + p / 8 % KT;
+                const uint32_t at = sbase + L::V + st * OP_BYTES + p * 16;
+                if (key < seen) continue;
+                uint32_t w[4];
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t o = odd_bits<BF16>(w[e]);
+                  odd |= key < n && (o & 0x80008000u);
+                  if (key >= n || o & 0x8000u) w[e] &= 0xffff0000u;
+                  if (key >= n || o & 0x80000000u) w[e] &= 0xffffu;
+                }
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+              }
+              if (odd) segs[ss].pad[0] = 1;
+            }
+            fence_proxy_async_smem();          // these stores before the product's reads
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_clean[st]);
+          }
+          if (lane == 0) mbar_arrive(&v_empty[st]);
+        }
+        if (!ok) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&seg_empty[ss]);
       }
+      if (lane == 0 && a.can_split) reinterpret_cast<Cut*>(a.part_lse + 2LL * gridDim.x * Q_ROWS)[blockIdx.x] = walk.cut;
     } else if (warp == 0) {
       // ---------------------------------------------------------- producer
       bool ok = true;
@@ -426,17 +498,22 @@ __global__ void __launch_bounds__(THREADS, 1)
       constexpr uint32_t idesc = idesc_f16(128, D, false, true, BF16);
       uint32_t cp[2] = {0, 0};                             // PV_i products issued so far
       int jg = 0;
+      uint32_t cleaned = 0;                                // bit st: phase of v_clean[st], completed by cleaned tiles alone
       bool ok = true;
       for (int seg = 0; ok; ++seg) {
         const int ss = seg % SEGS;
         if (!warp_wait(&seg_full[ss], (seg / SEGS) & 1, tries)) { ok = false; break; }
-        const int nt = segs[ss].nt, nqt = segs[ss].nqt;
+        const int nt = segs[ss].nt, nqt = segs[ss].nqt, t0 = segs[ss].t0, n = segs[ss].ql;
+        const int seen = nt < 0 ? 0 : key_limit(segs[ss].tok0, n, n, a.chunk);
         __syncwarp();
         if (lane == 0) mbar_arrive(&seg_empty[ss]);
         if (nt < 0) break;
         for (int j = 0; j < nt; ++j, ++jg) {
           const int st = jg % KV;
-          if (!warp_wait(&v_clean[st], (jg / KV) & 1, tries)) { ok = false; break; }
+          if ((t0 + j + 1) * KT > seen) {
+            if (!warp_wait(&v_clean[st], cleaned >> st & 1, tries)) { ok = false; break; }
+            cleaned ^= 1u << st;
+          } else if (!warp_wait(&v_full[st], (jg / KV) & 1, tries)) { ok = false; break; }
           for (int i = 0; i < nqt; ++i) {
             if (!warp_wait(&p_full[i], cp[i] & 1, tries)) { ok = false; break; }
             ++cp[i];
@@ -463,58 +540,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       __syncwarp();
     }
-  } else if (warp < 8) {
-    // ------------------------------------------------------------ V tiles
-    regs_dec<56>();
-    const int th = threadIdx.x - 128;                      // 0..127
-    bool ok = true;
-    int jg = 0;
-    for (int seg = 0; ok; ++seg) {
-      const int ss = seg % SEGS;
-      if (!warp_wait(&seg_full[ss], (seg / SEGS) & 1, tries)) { ok = false; break; }
-      const int nt = segs[ss].nt, t0 = segs[ss].t0, n = segs[ss].ql;
-      const int seen = nt < 0 ? 0 : key_limit(segs[ss].tok0, n, n, a.chunk);       // keys that every row sees
-      for (int j = 0; j < nt; ++j, ++jg) {
-        const int st = jg % KV, key0 = (t0 + j) * KT;
-        if (!warp_wait(&v_full[st], (jg / KV) & 1, tries)) { ok = false; break; }
-        if (key0 + KT > seen) {
-          bool odd = false;
-          // 16-byte pieces; the swizzle moves pieces within their row only
-          for (int p = th; p < OP_BYTES / 16; p += 128) {
-            const int key = key0 + p / 8 % KT;
-            const uint32_t at = sbase + L::V + st * OP_BYTES + p * 16;
-            if (key < seen) continue;
-            uint32_t w[4];
-            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-            bool clean = key < n;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (key >= n) {
-                w[e] = 0;
-              } else if (odd2<BF16>(w[e])) {
-                clean = false;
-                odd = true;
-                if (odd2<BF16>(w[e] & 0xffffu)) w[e] &= 0xffff0000u;
-                if (odd2<BF16>(w[e] >> 16)) w[e] &= 0xffffu;
-              }
-            }
-            if (!clean)
-              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-          }
-          if (odd) segs[ss].pad[0] = 1;
-          fence_proxy_async_smem();                        // these stores before the product's reads
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_clean[st]);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&seg_empty[ss]);
-      if (nt < 0) break;
-    }
   } else {
     // ------------------------------------------------------------ softmax of Q tile i
-    regs_inc<200>();
-    const int i = (warp - 8) / 4;
+    regs_inc<216>();
+    const int i = (warp - 4) / 4;
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
@@ -527,7 +556,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // the row's token in the block (past any block's for a row that holds none)
     // and head in the group: kept in shared memory, as registers held through
     // the tile loop push scores to local memory
-    volatile int2* row_at = reinterpret_cast<volatile int2*>(smem + L::ROWS) + (threadIdx.x - 256);
+    volatile int2* row_at = reinterpret_cast<volatile int2*>(smem + L::ROWS) + (threadIdx.x - 128);
     row_at->x = r < tpt * a.group ? i * tpt + r / a.group : 1 << 30;
     row_at->y = r % a.group;
     bool ok = true;
@@ -628,12 +657,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             // keys of the tiles that were cleaned: from what every row sees to what this one does
             const int ql = segs[ss].ql, t0 = segs[ss].t0 * KT;
             const int from = max(t0, key_limit(segs[ss].tok0, ql, ql, a.chunk));
-            uint32_t u[W];
-#pragma unroll
-            for (int e = 0; e < W; ++e) u[e] = v[e];
-            add_odd<BF16, W>(a, u, segs[ss].q0, segs[ss].kvh, cc, from, min(t0 + nt * KT, t0 + left));
-#pragma unroll
-            for (int e = 0; e < W; ++e) v[e] = u[e];
+            add_odd<BF16, W>(a, v, segs[ss].q0, segs[ss].kvh, cc, from, min(t0 + nt * KT, t0 + left));
           }
 #pragma unroll
           for (int e = 0; e < W; ++e) v[e] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(v[e]) * inv);
