@@ -625,14 +625,16 @@ class PagedKVCache:
             o = cache.attend(layer, q, plan, max_q, max_kv, causal_chunk)
         cache.commit(plan)                             # the plan's lengths become the cache's
 
-    Nothing waits for the GPU; :meth:`check` does, and raises if the plan
+    With ``weights`` the cache also holds what each key has gathered
+    (:meth:`weigh`, after a layer's :meth:`attend`), and :meth:`evict` makes
+    room between two steps.  Nothing waits for the GPU; :meth:`check` does, and raises if the plan
     could not be served (its tokens then have no place: :meth:`append` writes
     nothing and :meth:`attend` leaves its output as allocated).  One stream at
     a time.  :meth:`commit` takes the plan's tensors for the cache's, so a step
     captured in a CUDA graph would start from the same lengths at each replay."""
 
     def __init__(self, layers: int, num_blocks: int, kv_heads: int, head_dim: int, requests: int, max_len: int,
-                 block_size: int = 64, device="cuda"):
+                 block_size: int = 64, device="cuda", weights: bool = False):
         if block_size not in (32, 64, 128) or head_dim not in (64, 128):
             raise ValueError("PagedKVCache: block_size must be 32, 64 or 128 and head_dim 64 or 128")
         dev = torch.device(device)
@@ -642,6 +644,7 @@ class PagedKVCache:
         self.v = torch.zeros(shape, dtype=torch.int8, device=dev)
         self.k_scale = torch.ones(shape[:3], dtype=torch.float32, device=dev)
         self.v_scale = torch.ones(shape[:3], dtype=torch.float32, device=dev)
+        self.weights = torch.zeros(shape[:4], dtype=torch.float32, device=dev) if weights else None
         self.block_tables = torch.full((requests, -(-max_len // block_size)), -1, dtype=torch.int32, device=dev)
         self.lens = torch.zeros(requests, dtype=torch.int32, device=dev)
         self.free_ring = torch.arange(num_blocks, dtype=torch.int32, device=dev)
@@ -658,15 +661,37 @@ class PagedKVCache:
         kv_append(k, v, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer], self.block_tables,
                   self.lens, plan.cu_new, plan.cu_blocks)
 
-    def attend(self, layer: int, q, plan: BlockPlan, max_q: int, max_kv: int, causal_chunk: int = 0, out=None):
+    def attend(self, layer: int, q, plan: BlockPlan, max_q: int, max_kv: int, causal_chunk: int = 0, out=None, lse=None):
         """The new tokens' queries over everything the layer holds, the new tokens among it."""
         need = attention_scratch_bytes(q.shape[0], q.shape[1], self.k.shape[2], self.lens.numel(), max_q, max_kv,
                                        self.k.shape[4])
         if need and (self._scratch is None or self._scratch.numel() < need):
             self._scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
         return cached_attention(q, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer],
-                                self.block_tables, plan.cu_new, plan.lens, max_q, max_kv, causal_chunk, out=out,
+                                self.block_tables, plan.cu_new, plan.lens, max_q, max_kv, causal_chunk, out=out, lse=lse,
                                 scratch=self._scratch if need else None)
+
+    def weigh(self, layer: int, q, plan: BlockPlan, lse, max_q: int, max_kv: int, causal_chunk: int = 0,
+              decay: float = 1.0) -> None:
+        """Adds what the new tokens' queries give each key of the layer to its weight (see :func:`key_weights`), after
+        :meth:`append` and with the ``lse`` of :meth:`attend`; the new tokens' own weights start here."""
+        self._has_weights("weigh")
+        key_weights(q, self.k[layer], self.k_scale[layer], self.block_tables, plan.cu_new, plan.lens, lse,
+                    self.weights[layer], max_q, max_kv, causal_chunk, fresh_from=self.lens, decay=decay)
+
+    def evict(self, keep, max_moves: int, sink: int = 0, recent: int = 0) -> EvictPlan:
+        """Takes the requests down to ``keep`` tokens (int32 ``[requests]`` on the GPU; one that holds no more stays as it
+        is), in every layer and head those of largest weight (see :func:`evict_plan`), and gives the surplus blocks back.
+        Between steps: a plan made before does not survive it."""
+        self._has_weights("evict")
+        plan = evict_plan(self.weights, self.block_tables, self.lens, keep, sink, recent, max_moves)
+        kv_evict(self.k, self.v, self.k_scale, self.v_scale, self.weights, self.block_tables, keep, plan)
+        self.commit(self.plan(torch.minimum(keep, self.lens), 0))
+        return plan
+
+    def _has_weights(self, what):
+        if self.weights is None:
+            raise ValueError(f"PagedKVCache.{what}: the cache was made without weights")
 
     def gather(self, layer: int, slots, dtype=torch.float16):
         """Rows of one layer back as ``[k | v]`` (see :func:`kv_gather`)."""
