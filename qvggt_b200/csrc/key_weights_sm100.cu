@@ -540,14 +540,14 @@ int launch_key_weight_tiles(KeyWeightArgs& a, int D, bool bf16, cudaStream_t str
                            dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   a.row_blocks = 1;
+  // a try_wait that fails takes about 1.4 us
+  a.wait_tries = (uint32_t)std::min<unsigned long long>(1u << 26, a.ctl.timeout_ns / 1024 + 1);
   // p / chunk = (p mul) >> (31 + s) for p < 2^31: mul = 2^(31 + s) / chunk, rounded
   // up, with 2^s >= chunk (a chunk of 1 needs none of it)
   int s = 1;
   while (1LL << s < a.chunk) ++s;
   a.chunk_shift = s - 1;
   a.chunk_mul = a.chunk > 1 ? (uint32_t)((1ull << (31 + s)) / (unsigned)a.chunk + 1) : 0;
-  // a try_wait that fails takes about 1.4 us
-  a.wait_tries = (uint32_t)std::min<unsigned long long>(1u << 26, a.ctl.timeout_ns / 1024 + 1);
   const long long most = (long long)a.B * (((long long)a.wide << a.bs_log2) + KEYS - 1) / KEYS * a.hk;
   const int grid = (int)std::min<long long>(std::max<long long>(1, most), device_info().num_sms);
   using Kfn = void (*)(CUtensorMap, KeyWeightArgs);

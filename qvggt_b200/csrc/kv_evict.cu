@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
   };
   // f(base, position, keys) for this warp's positions, four a lane, in their order
   auto each = [&](auto load, auto f) {
-#pragma unroll 4
+#pragma unroll 2
     for (int base = start; base < end; base += SPAN) {
       const int i = base + lane * 4;
       uint4 k = make_uint4(0, 0, 0, 0);
@@ -345,7 +345,9 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
 // --------------------------------------------------------------------- move
 constexpr int MOVE_THREADS = 256, MOVE_WARPS = MOVE_THREADS / 32;
 constexpr int MOVE_BLOCKS = 32;          // blocks of a CTA at most
-constexpr int MOVE_LOADS = 4;            // 16-byte pieces a lane has under way
+constexpr int MOVE_ROWS = 1024;          // rows they have at most
+constexpr uint32_t NOWHERE = 0xffffffffu;
+constexpr int MOVE_LOADS = 8;            // 16-byte pieces a lane has under way
 
 struct MoveArgs {
   int8_t* codes[2];
@@ -408,21 +410,26 @@ __device__ __forceinline__ float largest16(uint4 c) {
   return (float)max(max(m & 0xffu, m >> 8 & 0xffu), max(m >> 16 & 0xffu, m >> 24));
 }
 
-// A CTA takes up to MOVE_BLOCKS blocks of one (layer, request, head), a warp K or
-// V of one of them that receives rows: the rows' largest magnitude, the block's
+// A CTA takes up to MOVE_BLOCKS blocks of one (layer, request, head).  It looks up
+// where all their incoming rows are and at what scales (a chain of four loads that
+// each block would wait for alone), and moves their weights.  Then a warp takes K
+// or V of one block that receives rows: the rows' largest magnitude, the block's
 // scale (it only grows, as when rows are appended), the rows' codes, and, where
 // the scale grew, the block's other codes.  Rows leave places from the new length
 // on and enter places below it, so the only block that is both read for others
 // and written is the one that the new length falls into: a second launch (EDGE)
 // does that one, when all others are done.
 template <int D, bool EDGE>
-__global__ void __launch_bounds__(MOVE_THREADS, 4) kv_evict_kernel(MoveArgs a) {
+__global__ void __launch_bounds__(MOVE_THREADS, 3) kv_evict_kernel(MoveArgs a) {
   constexpr int PARTS = D / 16;          // 16-byte pieces of a row
   constexpr int AT_ONCE = 32 * MOVE_LOADS;                 // pieces of a warp under way
-  __shared__ int2 range[MOVE_BLOCKS];    // a block's moves
+  __shared__ int2 range[MOVE_BLOCKS];    // a block's moves, from the CTA's first on
+  __shared__ int block_id[MOVE_BLOCKS];  // -1: outside the cache
+  __shared__ float block_scale[2][MOVE_BLOCKS];
   __shared__ int bounds[2];
-  __shared__ int2 row_from[MOVE_WARPS][128];               // where an incoming row is (-1: nowhere), its scale
-  __shared__ uint8_t row_to[MOVE_WARPS][128];
+  __shared__ uint32_t row_at[MOVE_ROWS];   // where an incoming row's codes are, in 16-byte pieces, NOWHERE: nowhere
+  __shared__ float row_scale[2][MOVE_ROWS];
+  __shared__ uint8_t row_to[MOVE_ROWS];
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
@@ -430,134 +437,126 @@ __global__ void __launch_bounds__(MOVE_THREADS, 4) kv_evict_kernel(MoveArgs a) {
   const int h = row % a.heads, b = row / a.heads % a.B, layer = row / a.heads / a.B;
   const int bs = 1 << a.bs_log2;
   const int keep = a.keep[b];
-  int moves = a.counts[row];
+  const int moves = a.counts[row];
   if (keep < 0 || keep > (a.wide << a.bs_log2) || moves < 0 || moves > a.max_moves) {
     if (tid == 0) report_status(a.ctl, ST_BAD_LENGTH);
-    moves = 0;
+    return;
   }
+  const int blocks = (int)(((long long)keep + bs - 1) >> a.bs_log2);
+  const int edge = keep & (bs - 1) ? keep >> a.bs_log2 : -1;
+  const int j0 = EDGE ? edge : part * a.span, j1 = EDGE ? edge + 1 : min(blocks, j0 + a.span);
+  if (moves == 0 || j0 < 0 || j0 >= j1) return;
   const int32_t* src = a.src + (long long)row * a.max_moves;
   const int32_t* dst = a.dst + (long long)row * a.max_moves;
   const int32_t* table = a.table + (long long)b * a.wide;
   const long long cell0 = (long long)layer * a.num_blocks * a.heads + h;
   auto cell = [&](int blk) { return cell0 + (long long)blk * a.heads; };
   auto in_pool = [&](int blk) { return blk >= 0 && blk < a.num_blocks; };
+  auto piece_of = [&](int blk) { return (uint32_t)(blk * (a.block_stride / 16)) + (uint32_t)(h << a.bs_log2) * PARTS; };
 
-  // K (side 0) or V of block j, which receives moves [m0, m1)
-  auto receive = [&](int j, int m0, int m1, int side) {
-    const int blk = table[j], rows = min(m1 - m0, bs);
-    if (!in_pool(blk)) {
-      if (lane == 0) report_bad_block(a.ctl);
-      return;
+  if (tid < j1 - j0) {
+    const int blk = table[j0 + tid];
+    range[tid] = make_int2(0, 0);
+    block_id[tid] = in_pool(blk) ? blk : -1;
+    if (in_pool(blk)) {
+      block_scale[0][tid] = a.scales[0][cell(blk)];
+      block_scale[1][tid] = a.scales[1][cell(blk)];
     }
-    int8_t* codes = (side ? a.codes[1] : a.codes[0]) + layer * a.layer_stride + ((long long)h << a.bs_log2) * D;
-    float* scales = side ? a.scales[1] : a.scales[0];
-    const float before = scales[cell(blk)];
-    unsigned taken[4] = {0, 0, 0, 0};    // the block's rows that are written
-    for (int r0 = 0; r0 < rows; r0 += 32) {
-      const int r = r0 + lane;
-      int slot = -1, to = 0;
-      if (r < rows) {
-        const int s = src[m0 + r];
-        to = dst[m0 + r] - (j << a.bs_log2);
-        const bool fits = s >= keep && s < (a.wide << a.bs_log2) && to >= 0 && to < bs && to + (j << a.bs_log2) < keep;
-        const int from = fits ? table[s >> a.bs_log2] : 0;
-        float f = 0.f;
-        if (fits && in_pool(from)) {
-          slot = (from << a.bs_log2) + (s & (bs - 1));
-          f = scales[cell(from)];
-          if (side == 0 && a.w) a.w[(cell(blk) << a.bs_log2) + to] = a.w[(cell(from) << a.bs_log2) + (s & (bs - 1))];
-        } else {
-          report_status(a.ctl, fits ? ST_BAD_BLOCK : ST_BAD_LENGTH);
-        }
-        row_from[warp][r] = make_int2(slot, __float_as_int(f));
-        row_to[warp][r] = (uint8_t)to;
-      }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) taken[x] |= __reduce_or_sync(~0u, slot >= 0 && to / 32 == x ? 1u << (to & 31) : 0u);
+  }
+  if (warp < 2) {
+    const int x = warp_lower_bound(dst, moves, (warp == 0 ? j0 : j1) << a.bs_log2);
+    if (lane == 0) bounds[warp] = x;
+  }
+  __syncthreads();
+  // `dst` ascends: a block's moves are consecutive, and no more than its rows
+  const int m0 = bounds[0], m1 = min(bounds[1], m0 + MOVE_ROWS);
+  for (int m = m0 + tid; m < m1; m += blockDim.x) {
+    const int to = dst[m], s = src[m], j = to >> a.bs_log2;
+    row_at[m - m0] = NOWHERE;
+    if (j < j0 || j >= j1) continue;
+    if (m == m0 || dst[m - 1] >> a.bs_log2 != j) range[j - j0].x = m - m0;
+    if (m + 1 == m1 || dst[m + 1] >> a.bs_log2 != j) range[j - j0].y = m + 1 - m0;
+    if (!EDGE && j == edge) continue;    // the second launch's
+    const bool fits = s >= keep && s < (a.wide << a.bs_log2) && to < keep;
+    const int from = fits ? table[s >> a.bs_log2] : -1, at = block_id[j - j0];
+    if (in_pool(from) && at >= 0) {
+      row_at[m - m0] = piece_of(from) + (s & (bs - 1)) * PARTS;
+      row_to[m - m0] = (uint8_t)(to & (bs - 1));
+      row_scale[0][m - m0] = a.scales[0][cell(from)];
+      row_scale[1][m - m0] = a.scales[1][cell(from)];
+      if (a.w) a.w[(cell(at) << a.bs_log2) + (to & (bs - 1))] = a.w[(cell(from) << a.bs_log2) + (s & (bs - 1))];
+    } else {
+      report_status(a.ctl, fits ? ST_BAD_BLOCK : ST_BAD_LENGTH);
     }
-    __syncwarp();
-    auto at = [&](int slot, int part) {
-      return reinterpret_cast<uint4*>(codes + (long long)(slot >> a.bs_log2) * a.block_stride + (slot & (bs - 1)) * D + part * 16);
-    };
+  }
+  __syncthreads();
+
+  for (int u = warp; u < 2 * (j1 - j0); u += MOVE_WARPS) {
+    const int j = u / 2, side = u & 1, blk = block_id[j];
+    const int2 m = range[j];
+    const int rows = min(m.y - m.x, bs);
+    if (rows <= 0 || blk < 0 || (!EDGE && j0 + j == edge)) continue;
+    const uint32_t* from = row_at + m.x;
+    const float* from_scale = row_scale[side] + m.x;
+    const uint8_t* to = row_to + m.x;
+    uint4* codes = reinterpret_cast<uint4*>((side ? a.codes[1] : a.codes[0]) + layer * a.layer_stride);
+    uint4* mine = codes + piece_of(blk);
+    const float before = block_scale[side][j];
+    const int pieces = rows * PARTS;
     uint4 c[MOVE_LOADS];
     auto load = [&](int p0) {
 #pragma unroll
       for (int x = 0; x < MOVE_LOADS; ++x) {
         const int p = p0 + 32 * x + lane;
         c[x] = make_uint4(0, 0, 0, 0);
-        if (p < rows * PARTS) {
-          const int slot = row_from[warp][p / PARTS].x;
-          if (slot >= 0) c[x] = *at(slot, p % PARTS);
-        }
+        if (p < pieces && from[p / PARTS] != NOWHERE) c[x] = codes[from[p / PARTS] + p % PARTS];
       }
     };
     // where all rows fit the registers (`once`) they are read once, else again for their codes
-    const bool once = rows * PARTS <= AT_ONCE;
+    const bool once = pieces <= AT_ONCE;
     float most = 0.f;
-    for (int p0 = 0; p0 < rows * PARTS; p0 += AT_ONCE) {
+    for (int p0 = 0; p0 < pieces; p0 += AT_ONCE) {
       load(p0);
 #pragma unroll
       for (int x = 0; x < MOVE_LOADS; ++x) {
         const int p = p0 + 32 * x + lane;
-        if (p < rows * PARTS) most = fmaxf(most, __fmul_rn(largest16(c[x]), __int_as_float(row_from[warp][p / PARTS].y)));
+        if (p < pieces && from[p / PARTS] != NOWHERE) most = fmaxf(most, __fmul_rn(largest16(c[x]), from_scale[p / PARTS]));
       }
     }
     most = warp_max(most);
     const float s = fmaxf(fmaxf(before, __fdiv_rn(most, 127.f)), KV_SCALE_MIN);
     const float inv = __frcp_rn(s);
-    for (int p0 = 0; p0 < rows * PARTS; p0 += AT_ONCE) {
+    for (int p0 = 0; p0 < pieces; p0 += AT_ONCE) {
       if (!once) load(p0);
 #pragma unroll
       for (int x = 0; x < MOVE_LOADS; ++x) {
-        const int p = p0 + 32 * x + lane;
-        if (p >= rows * PARTS) continue;
-        const int2 from = row_from[warp][p / PARTS];
-        if (from.x >= 0)
-          *at((blk << a.bs_log2) + row_to[warp][p / PARTS], p % PARTS) = recode16<true>(c[x], __int_as_float(from.y), inv);
+        const int p = p0 + 32 * x + lane, r = p / PARTS;
+        if (p < pieces && from[r] != NOWHERE) mine[to[r] * PARTS + p % PARTS] = recode16<true>(c[x], from_scale[r], inv);
       }
     }
-    __syncwarp();
-    if (s == before) return;
+    if (s == before) continue;
+    unsigned taken[4] = {0, 0, 0, 0};    // the block's rows that were written
+    for (int r0 = 0; r0 < rows; r0 += 32) {
+      const int r = r0 + lane;
+      const int at = r < rows && from[r] != NOWHERE ? to[r] : 128;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) taken[x] |= __reduce_or_sync(~0u, at / 32 == x ? 1u << (at & 31) : 0u);
+    }
     const float f = __fmul_rn(before, inv);
-    uint4* all = at(blk << a.bs_log2, 0);
     for (int p0 = 0; p0 < bs * PARTS; p0 += AT_ONCE) {
       auto stays = [&](int x) {
-        const int to = (p0 + 32 * x + lane) / PARTS;
-        const unsigned word = to < 64 ? (to < 32 ? taken[0] : taken[1]) : (to < 96 ? taken[2] : taken[3]);
-        return to < bs && !(word >> (to & 31) & 1);
+        const int r = (p0 + 32 * x + lane) / PARTS;
+        const unsigned word = r < 64 ? (r < 32 ? taken[0] : taken[1]) : (r < 96 ? taken[2] : taken[3]);
+        return r < bs && !(word >> (r & 31) & 1);
       };
 #pragma unroll
       for (int x = 0; x < MOVE_LOADS; ++x)
-        if (stays(x)) c[x] = all[p0 + 32 * x + lane];
+        if (stays(x)) c[x] = mine[p0 + 32 * x + lane];
 #pragma unroll
       for (int x = 0; x < MOVE_LOADS; ++x)
-        if (stays(x)) all[p0 + 32 * x + lane] = recode16<false>(c[x], f, 0.f);
+        if (stays(x)) mine[p0 + 32 * x + lane] = recode16<false>(c[x], f, 0.f);
     }
-    if (lane == 0) scales[cell(blk)] = s;
-  };
-
-  const int blocks = (int)(((long long)keep + bs - 1) >> a.bs_log2);
-  const int edge = keep & (bs - 1) ? keep >> a.bs_log2 : -1;
-  const int j0 = EDGE ? edge : part * a.span, j1 = EDGE ? edge + 1 : min(blocks, j0 + a.span);
-  if (moves == 0 || j0 < 0 || j0 >= j1) return;
-  if (tid < MOVE_BLOCKS) range[tid] = make_int2(0, 0);
-  if (warp < 2) {
-    const int x = warp_lower_bound(dst, moves, (warp == 0 ? j0 : j1) << a.bs_log2);
-    if (lane == 0) bounds[warp] = x;
-  }
-  __syncthreads();
-  // `dst` ascends: a block's moves are consecutive
-  for (int i = bounds[0] + tid; i < bounds[1]; i += blockDim.x) {
-    const int j = dst[i] >> a.bs_log2;
-    if (j < j0 || j >= j1) continue;
-    if (i == bounds[0] || dst[i - 1] >> a.bs_log2 != j) range[j - j0].x = i;
-    if (i + 1 == bounds[1] || dst[i + 1] >> a.bs_log2 != j) range[j - j0].y = i + 1;
-  }
-  __syncthreads();
-  for (int u = warp; u < 2 * (j1 - j0); u += MOVE_WARPS) {
-    const int j = j0 + u / 2;
-    const int2 m = range[u / 2];
-    if (m.x < m.y && (EDGE || j != edge)) receive(j, m.x, m.y, u & 1);
+    if (lane == 0) (side ? a.scales[1] : a.scales[0])[cell(blk)] = s;
   }
 }
 
@@ -624,12 +623,16 @@ extern "C" int qvggt_kv_evict(const qvggt_kv_evict_args* p, void* stream) {
     return set_error(QVGGT_ERR_UNSUPPORTED, "%s: too many layers, requests and heads", name);
   if (!p->block_tables || !p->keep || !p->src || !p->dst || !p->counts)
     return set_error(QVGGT_ERR_INVALID, "%s: null tensor", name);
+  // (places are 32-bit numbers of 16-byte pieces)
+  if (c.num_blocks * c.block_stride / 16 >= NOWHERE)
+    return set_error(QVGGT_ERR_UNSUPPORTED, "%s: a layer of more than 2^36 bytes", name);
   if (p->layer_stride % 16) return set_error(QVGGT_ERR_ALIGN, "%s: the layers must be 16-byte aligned", name);
   if (p->layers > 1 && p->layer_stride < (c.num_blocks - 1) * c.block_stride + c.kv_heads * c.block_size * c.head_dim)
     return set_error(QVGGT_ERR_INVALID, "%s: layer stride smaller than a layer", name);
   const int64_t rows = p->layers * p->requests * c.kv_heads;
-  // as many blocks a CTA as leave every SM a few dozen CTAs, up to four for each warp
-  const int64_t span = std::max<int64_t>(4, std::min<int64_t>(MOVE_BLOCKS, rows * p->max_blocks / (32 * device_info().num_sms)));
+  // as many blocks a CTA as leave every SM some CTAs, and as its lists hold
+  const int64_t most = std::min<int64_t>(MOVE_BLOCKS, MOVE_ROWS / c.block_size);
+  const int64_t span = std::max<int64_t>(4, std::min<int64_t>(most, rows * p->max_blocks / (32 * device_info().num_sms)));
   const int64_t parts = std::max<int64_t>(1, (p->max_blocks + span - 1) / span);
   if (rows * parts > 2147483647LL) return set_error(QVGGT_ERR_UNSUPPORTED, "%s: too many blocks", name);
   MoveArgs a{{c.k_cache, c.v_cache}, {c.k_scale, c.v_scale}, p->weights, p->block_tables, p->keep, p->src, p->dst,
