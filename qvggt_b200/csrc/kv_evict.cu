@@ -343,9 +343,16 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
 }
 
 // --------------------------------------------------------------------- move
+// --------------------------------------------------------------------- move
+#ifndef TRIG
+#define TRIG 1
+#endif
+#ifndef SPANF
+#define SPANF 16
+#endif
 constexpr int MOVE_THREADS = 256, MOVE_WARPS = MOVE_THREADS / 32;
-constexpr int MOVE_BLOCKS = 32;          // blocks of a CTA at most
-constexpr int MOVE_ROWS = 1024;          // rows they have at most
+constexpr int MOVE_BLOCKS = 256;         // blocks of a CTA at most
+constexpr int MOVE_ROWS = 2048;          // rows they receive at most
 constexpr uint32_t NOWHERE = 0xffffffffu;
 constexpr int MOVE_LOADS = 8;            // 16-byte pieces a lane has under way
 
@@ -422,7 +429,6 @@ __device__ __forceinline__ float largest16(uint4 c) {
 template <int D, bool EDGE>
 __global__ void __launch_bounds__(MOVE_THREADS, 3) kv_evict_kernel(MoveArgs a) {
   constexpr int PARTS = D / 16;          // 16-byte pieces of a row
-  constexpr int AT_ONCE = 32 * MOVE_LOADS;                 // pieces of a warp under way
   __shared__ int2 range[MOVE_BLOCKS];    // a block's moves, from the CTA's first on
   __shared__ int block_id[MOVE_BLOCKS];  // -1: outside the cache
   __shared__ float block_scale[2][MOVE_BLOCKS];
@@ -431,7 +437,6 @@ __global__ void __launch_bounds__(MOVE_THREADS, 3) kv_evict_kernel(MoveArgs a) {
   __shared__ float row_scale[2][MOVE_ROWS];
   __shared__ uint8_t row_to[MOVE_ROWS];
   pdl_wait();
-  pdl_trigger();
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const int h = row % a.heads, b = row / a.heads % a.B, layer = row / a.heads / a.B;
@@ -454,13 +459,13 @@ __global__ void __launch_bounds__(MOVE_THREADS, 3) kv_evict_kernel(MoveArgs a) {
   auto in_pool = [&](int blk) { return blk >= 0 && blk < a.num_blocks; };
   auto piece_of = [&](int blk) { return (uint32_t)(blk * (a.block_stride / 16)) + (uint32_t)(h << a.bs_log2) * PARTS; };
 
-  if (tid < j1 - j0) {
-    const int blk = table[j0 + tid];
-    range[tid] = make_int2(0, 0);
-    block_id[tid] = in_pool(blk) ? blk : -1;
+  for (int j = tid; j < j1 - j0; j += blockDim.x) {
+    const int blk = table[j0 + j];
+    range[j] = make_int2(0, 0);
+    block_id[j] = in_pool(blk) ? blk : -1;
     if (in_pool(blk)) {
-      block_scale[0][tid] = a.scales[0][cell(blk)];
-      block_scale[1][tid] = a.scales[1][cell(blk)];
+      block_scale[0][j] = a.scales[0][cell(blk)];
+      block_scale[1][j] = a.scales[1][cell(blk)];
     }
   }
   if (warp < 2) {
@@ -490,74 +495,87 @@ __global__ void __launch_bounds__(MOVE_THREADS, 3) kv_evict_kernel(MoveArgs a) {
     }
   }
   __syncthreads();
-
-  for (int u = warp; u < 2 * (j1 - j0); u += MOVE_WARPS) {
-    const int j = u / 2, side = u & 1, blk = block_id[j];
-    const int2 m = range[j];
-    const int rows = min(m.y - m.x, bs);
-    if (rows <= 0 || blk < 0 || (!EDGE && j0 + j == edge)) continue;
-    const uint32_t* from = row_at + m.x;
-    const float* from_scale = row_scale[side] + m.x;
-    const uint8_t* to = row_to + m.x;
-    uint4* codes = reinterpret_cast<uint4*>((side ? a.codes[1] : a.codes[0]) + layer * a.layer_stride);
-    uint4* mine = codes + piece_of(blk);
-    const float before = block_scale[side][j];
-    const int pieces = rows * PARTS;
-    uint4 c[MOVE_LOADS];
-    auto load = [&](int p0) {
+  // A group of lanes for each side of a block: a warp, or eight lanes where the
+  // blocks receive few rows (a step that makes room for one frame in 32 moves two
+  // rows into a block: 368 us with a warp each, 24 layers of 43,968 keys).
+  const auto units = [&](auto GROUP) {
+    constexpr int G = GROUP, AT_ONCE = G * MOVE_LOADS;     // pieces under way
+    const int gl = tid % G;
+    const unsigned mask = G == 32 ? ~0u : ((1u << (G & 31)) - 1) << (lane & ~(G - 1));
+    for (int u = tid / G; u < 2 * (j1 - j0); u += blockDim.x / G) {
+      const int j = u / 2, side = u & 1, blk = block_id[j];
+      const int2 m = range[j];
+      const int rows = min(m.y - m.x, bs);
+      if (rows <= 0 || blk < 0 || (!EDGE && j0 + j == edge)) continue;
+      const uint32_t* from = row_at + m.x;
+      const float* from_scale = row_scale[side] + m.x;
+      const uint8_t* to = row_to + m.x;
+      uint4* codes = reinterpret_cast<uint4*>((side ? a.codes[1] : a.codes[0]) + layer * a.layer_stride);
+      uint4* mine = codes + piece_of(blk);
+      const float before = block_scale[side][j];
+      const int pieces = rows * PARTS;
+      uint4 c[MOVE_LOADS];
+      auto load = [&](int p0) {
 #pragma unroll
-      for (int x = 0; x < MOVE_LOADS; ++x) {
-        const int p = p0 + 32 * x + lane;
-        c[x] = make_uint4(0, 0, 0, 0);
-        if (p < pieces && from[p / PARTS] != NOWHERE) c[x] = codes[from[p / PARTS] + p % PARTS];
-      }
-    };
-    // where all rows fit the registers (`once`) they are read once, else again for their codes
-    const bool once = pieces <= AT_ONCE;
-    float most = 0.f;
-    for (int p0 = 0; p0 < pieces; p0 += AT_ONCE) {
-      load(p0);
-#pragma unroll
-      for (int x = 0; x < MOVE_LOADS; ++x) {
-        const int p = p0 + 32 * x + lane;
-        if (p < pieces && from[p / PARTS] != NOWHERE) most = fmaxf(most, __fmul_rn(largest16(c[x]), from_scale[p / PARTS]));
-      }
-    }
-    most = warp_max(most);
-    const float s = fmaxf(fmaxf(before, __fdiv_rn(most, 127.f)), KV_SCALE_MIN);
-    const float inv = __frcp_rn(s);
-    for (int p0 = 0; p0 < pieces; p0 += AT_ONCE) {
-      if (!once) load(p0);
-#pragma unroll
-      for (int x = 0; x < MOVE_LOADS; ++x) {
-        const int p = p0 + 32 * x + lane, r = p / PARTS;
-        if (p < pieces && from[r] != NOWHERE) mine[to[r] * PARTS + p % PARTS] = recode16<true>(c[x], from_scale[r], inv);
-      }
-    }
-    if (s == before) continue;
-    unsigned taken[4] = {0, 0, 0, 0};    // the block's rows that were written
-    for (int r0 = 0; r0 < rows; r0 += 32) {
-      const int r = r0 + lane;
-      const int at = r < rows && from[r] != NOWHERE ? to[r] : 128;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) taken[x] |= __reduce_or_sync(~0u, at / 32 == x ? 1u << (at & 31) : 0u);
-    }
-    const float f = __fmul_rn(before, inv);
-    for (int p0 = 0; p0 < bs * PARTS; p0 += AT_ONCE) {
-      auto stays = [&](int x) {
-        const int r = (p0 + 32 * x + lane) / PARTS;
-        const unsigned word = r < 64 ? (r < 32 ? taken[0] : taken[1]) : (r < 96 ? taken[2] : taken[3]);
-        return r < bs && !(word >> (r & 31) & 1);
+        for (int x = 0; x < MOVE_LOADS; ++x) {
+          const int p = p0 + G * x + gl;
+          c[x] = make_uint4(0, 0, 0, 0);
+          if (p < pieces && from[p / PARTS] != NOWHERE) c[x] = codes[from[p / PARTS] + p % PARTS];
+        }
       };
+      // where all rows fit the registers (`once`) they are read once, else again for their codes
+      const bool once = pieces <= AT_ONCE;
+      float most = 0.f;
+      for (int p0 = 0; p0 < pieces; p0 += AT_ONCE) {
+        load(p0);
 #pragma unroll
-      for (int x = 0; x < MOVE_LOADS; ++x)
-        if (stays(x)) c[x] = mine[p0 + 32 * x + lane];
+        for (int x = 0; x < MOVE_LOADS; ++x) {
+          const int p = p0 + G * x + gl;
+          if (p < pieces && from[p / PARTS] != NOWHERE) most = fmaxf(most, __fmul_rn(largest16(c[x]), from_scale[p / PARTS]));
+        }
+      }
 #pragma unroll
-      for (int x = 0; x < MOVE_LOADS; ++x)
-        if (stays(x)) mine[p0 + 32 * x + lane] = recode16<false>(c[x], f, 0.f);
+      for (int d = G / 2; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(mask, most, d));
+      const float s = fmaxf(fmaxf(before, __fdiv_rn(most, 127.f)), KV_SCALE_MIN);
+      const float inv = __frcp_rn(s);
+      for (int p0 = 0; p0 < pieces; p0 += AT_ONCE) {
+        if (!once) load(p0);
+#pragma unroll
+        for (int x = 0; x < MOVE_LOADS; ++x) {
+          const int p = p0 + G * x + gl, r = p / PARTS;
+          if (p < pieces && from[r] != NOWHERE) mine[to[r] * PARTS + p % PARTS] = recode16<true>(c[x], from_scale[r], inv);
+        }
+      }
+      if (s == before) continue;
+      unsigned taken[4] = {0, 0, 0, 0};  // the block's rows that were written
+      for (int r0 = 0; r0 < rows; r0 += G) {
+        const int r = r0 + gl;
+        const int at = r < rows && from[r] != NOWHERE ? to[r] : 128;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) taken[x] |= __reduce_or_sync(mask, at / 32 == x ? 1u << (at & 31) : 0u);
+      }
+      const float f = __fmul_rn(before, inv);
+      for (int p0 = 0; p0 < bs * PARTS; p0 += AT_ONCE) {
+        auto stays = [&](int x) {
+          const int r = (p0 + G * x + gl) / PARTS;
+          const unsigned word = r < 64 ? (r < 32 ? taken[0] : taken[1]) : (r < 96 ? taken[2] : taken[3]);
+          return r < bs && !(word >> (r & 31) & 1);
+        };
+#pragma unroll
+        for (int x = 0; x < MOVE_LOADS; ++x)
+          if (stays(x)) c[x] = mine[p0 + G * x + gl];
+#pragma unroll
+        for (int x = 0; x < MOVE_LOADS; ++x)
+          if (stays(x)) mine[p0 + G * x + gl] = recode16<false>(c[x], f, 0.f);
+      }
+      if (gl == 0) (side ? a.scales[1] : a.scales[0])[cell(blk)] = s;
     }
-    if (lane == 0) (side ? a.scales[1] : a.scales[0])[cell(blk)] = s;
-  }
+  };
+  if (EDGE || (m1 - m0) * PARTS > 32 * (j1 - j0)) units(std::integral_constant<int, 32>());
+  else units(std::integral_constant<int, 8>());
+  // at the end: CTAs of the next kernel that wait beside this one's slow it (four
+  // layers and their reading: 213 us with the call at the start, 198 here)
+  pdl_trigger();
 }
 
 int log2_of(int64_t bs) { return bs == 32 ? 5 : bs == 64 ? 6 : 7; }
@@ -630,9 +648,10 @@ extern "C" int qvggt_kv_evict(const qvggt_kv_evict_args* p, void* stream) {
   if (p->layers > 1 && p->layer_stride < (c.num_blocks - 1) * c.block_stride + c.kv_heads * c.block_size * c.head_dim)
     return set_error(QVGGT_ERR_INVALID, "%s: layer stride smaller than a layer", name);
   const int64_t rows = p->layers * p->requests * c.kv_heads;
-  // as many blocks a CTA as leave every SM some CTAs, and as its lists hold
-  const int64_t most = std::min<int64_t>(MOVE_BLOCKS, MOVE_ROWS / c.block_size);
-  const int64_t span = std::max<int64_t>(4, std::min<int64_t>(most, rows * p->max_blocks / (32 * device_info().num_sms)));
+  // as many blocks a CTA as leave every SM some CTAs, and as its lists hold: all rows
+  // of the blocks, or all moves there can be
+  const int64_t most = p->max_moves <= MOVE_ROWS ? MOVE_BLOCKS : std::min<int64_t>(MOVE_BLOCKS, MOVE_ROWS / c.block_size);
+  const int64_t span = std::max<int64_t>(4, std::min<int64_t>(most, rows * p->max_blocks / (16 * device_info().num_sms)));
   const int64_t parts = std::max<int64_t>(1, (p->max_blocks + span - 1) / span);
   if (rows * parts > 2147483647LL) return set_error(QVGGT_ERR_UNSUPPORTED, "%s: too many blocks", name);
   MoveArgs a{{c.k_cache, c.v_cache}, {c.k_scale, c.v_scale}, p->weights, p->block_tables, p->keep, p->src, p->dst,
