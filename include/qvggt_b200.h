@@ -544,7 +544,7 @@ int qvggt_kv_evict(const qvggt_kv_evict_args* args, void* stream);
  * mask) v within each.
  * q, out [T, q_heads, head_dim], k, v [T, kv_heads, head_dim], fp16 or bf16,
  * element strides of token and head (positive multiples of 8 where there is more
- * than one; out's may not overlap), unit stride inside, 16-byte aligned;
+ * than one), unit stride inside, 16-byte aligned, out apart from k and v;
  * head_dim 64 or 128; query head h reads key head h / (q_heads / kv_heads), at
  * most 128 query heads to a key head.  Sequence b is rows [cu[b], cu[b + 1]), at
  * most max_len of them.

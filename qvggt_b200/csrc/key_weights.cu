@@ -13,7 +13,10 @@ namespace {
 
 constexpr int UNIT = 32;                 // keys a warp takes at a time: never across two blocks
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int ROWS_MAX = 32;             // more rows of a key head go to key_weights_sm100.cu
+// More rows of a key head than this go to key_weights_sm100.cu: eight streams of
+// 8,000 keys take 62 us there at 40 rows (mostly padding of its 128), here 71 at
+// 32 rows of 20,000 keys and twice that at 33, when the codes are read twice.
+constexpr int ROWS_MAX = 32;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -279,7 +282,7 @@ extern "C" int qvggt_key_weights(const qvggt_key_weights_args* p, void* stream) 
     return set_error(QVGGT_ERR_ALIGN, "%s: cache codes and their block stride must be 16-byte aligned", name);
   if (p->block_stride < p->kv_heads * p->block_size * p->head_dim)
     return set_error(QVGGT_ERR_INVALID, "%s: block stride smaller than a block", name);
-  if (!aligned16(p->q) || p->q_tok % 8 || p->q_head % 8)
+  if (!aligned16(p->q) || (p->Tq > 1 && p->q_tok % 8) || (p->q_heads > 1 && p->q_head % 8))
     return set_error(QVGGT_ERR_ALIGN, "%s: q rows must be 16-byte aligned", name);
   KeyWeightArgs a{};
   a.kc = p->k_cache;
@@ -310,7 +313,7 @@ extern "C" int qvggt_key_weights(const qvggt_key_weights_args* p, void* stream) 
   a.ctl = make_ctl();
   const bool bf16 = p->dtype == QVGGT_DTYPE_BF16;
   const long long rows = (long long)a.max_q * a.group, pairs = (long long)a.hk * a.B;
-  if (rows > ROWS_MAX && key_weight_tiles_can_read(a))
+  if (rows > ROWS_MAX && a.Tq > 0 && key_weight_tiles_can_read(a))
     return launch_key_weight_tiles(a, (int)p->head_dim, bf16, static_cast<cudaStream_t>(stream));
   const long long units = std::max<long long>(1, (p->max_kv + UNIT - 1) / UNIT);
   // Units of a warp: up to 16, and fewer where there would be less than about six

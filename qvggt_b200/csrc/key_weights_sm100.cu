@@ -142,11 +142,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   if (warp == 0 && lane == 0) tma_prefetch_desc(&tmQ);
   pdl_wait();
-  pdl_trigger();
   const int g = (a.B + THREADS - 1) / THREADS;
   tc_fence_before();
   scan_blocks<THREADS, Request>(a, cum, a.B, g);
   tc_fence_after();
+  pdl_trigger();                                           // (this CTA has its TMEM by now)
   const uint32_t tmem = *tmem_slot;
   const int tpt = 128 / a.group;                           // tokens of a Q tile
 

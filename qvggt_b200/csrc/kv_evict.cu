@@ -644,7 +644,7 @@ extern "C" int qvggt_kv_evict(const qvggt_kv_evict_args* p, void* stream) {
   // (places are 32-bit numbers of 16-byte pieces)
   if (c.num_blocks * c.block_stride / 16 >= NOWHERE)
     return set_error(QVGGT_ERR_UNSUPPORTED, "%s: a layer of more than 2^36 bytes", name);
-  if (p->layer_stride % 16) return set_error(QVGGT_ERR_ALIGN, "%s: the layers must be 16-byte aligned", name);
+  if (p->layers > 1 && p->layer_stride % 16) return set_error(QVGGT_ERR_ALIGN, "%s: the layers must be 16-byte aligned", name);
   if (p->layers > 1 && p->layer_stride < (c.num_blocks - 1) * c.block_stride + c.kv_heads * c.block_size * c.head_dim)
     return set_error(QVGGT_ERR_INVALID, "%s: layer stride smaller than a layer", name);
   const int64_t rows = p->layers * p->requests * c.kv_heads;
@@ -655,7 +655,7 @@ extern "C" int qvggt_kv_evict(const qvggt_kv_evict_args* p, void* stream) {
   const int64_t parts = std::max<int64_t>(1, (p->max_blocks + span - 1) / span);
   if (rows * parts > 2147483647LL) return set_error(QVGGT_ERR_UNSUPPORTED, "%s: too many blocks", name);
   MoveArgs a{{c.k_cache, c.v_cache}, {c.k_scale, c.v_scale}, p->weights, p->block_tables, p->keep, p->src, p->dst,
-             p->counts, p->layer_stride, c.block_stride, (int)p->requests, (int)c.kv_heads, (int)p->max_blocks,
+             p->counts, p->layers > 1 ? p->layer_stride : 0, c.block_stride, (int)p->requests, (int)c.kv_heads, (int)p->max_blocks,
              (int)c.num_blocks, log2_of(c.block_size), (int)p->max_moves, (int)parts, (int)span, make_ctl()};
   using Kfn = void (*)(MoveArgs);
   static const Kfn fns[2][2] = {{kv_evict_kernel<64, false>, kv_evict_kernel<64, true>},

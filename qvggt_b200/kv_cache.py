@@ -408,7 +408,8 @@ def prompt_attention(q, k, v, cu, max_len: int, causal_chunk: int = 0, scale: fl
     token does not see adds nothing to it, be it NaN.  ``scale``: positive,
     ``head_dim ** -0.5`` by default.  ``lse``: fp32 ``[Hq, tokens]`` to be
     filled.  ``scratch``: uint8, at least :func:`prompt_scratch_bytes`
-    (allocated here if None).  Returns ``out`` ``[tokens, Hq, head_dim]``."""
+    (allocated here if None).  Returns ``out`` ``[tokens, Hq, head_dim]``, which
+    must not overlap k or v."""
     name = "prompt_attention"
     dev = q.get_device()
     if dev < 0 or not dev == k.get_device() == v.get_device() == cu.get_device():

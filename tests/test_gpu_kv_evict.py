@@ -95,6 +95,15 @@ def test_key_weights(kc, dtype, ql, kl, hq, hk, D, bs, chunk):
     assert torch.equal(first, second)
 
 
+@pytest.mark.parametrize("ql,kl", [([40, 0, 130], [70, 700, 131]), ([0, 0, 300], [10, 0, 2000]), ([0, 0], [300, 40])])
+def test_key_weights_of_requests_without_queries(kc, ql, kl):
+    """Their keys only age; so do all, where there is no query at all, whatever max_q says."""
+    *args, w = weigh_inputs(6, ql, kl, 4, 2, 64, 64, torch.float16, 1)
+    for most in (max(ql), 500):
+        got = kc.key_weights(*args, w, most, max(kl), 1, decay=0.5, out=w.clone())
+        check_weights(got, oe.key_weights(*args, w, 1, None, None, 0.5))
+
+
 @pytest.mark.parametrize("ql,hint", [(2, 1), (2, 300000), (200, 1), (200, 300000)])
 def test_key_weights_length_hint_is_only_a_hint(kc, ql, hint):
     *args, w = weigh_inputs(3, [ql], [3000], 2, 2, 64, 64, torch.float16, 1)

@@ -154,6 +154,18 @@ def test_what_a_token_does_not_see(kc, dtype, D, chunk, n, hq):
         assert torch.equal(torch.isnan(got[:n]), torch.isnan(ref))
 
 
+def test_one_token_of_any_stride_and_out_in_place_of_q(kc):
+    """The stride of an axis of length one means nothing; the result may take the queries' place."""
+    for T, hq, hk in ((1, 4, 2), (1, 1, 1), (300, 1, 1)):
+        q, k, v = inputs(6, T, hq, hk, 64, torch.float16)
+        want = kc.prompt_attention(q, k, v, ints([0, T]), T, 1)
+        odd = [t.as_strided(t.shape, (t.stride(0) if T > 1 else 3, t.stride(1) if t.shape[1] > 1 else 5, 1)) for t in (q, k, v)]
+        assert torch.equal(kc.prompt_attention(*odd, ints([0, T]), T, 1), want)
+    q, k, v = inputs(7, 3000, 4, 2, 64, torch.float16)
+    want = kc.prompt_attention(q, k, v, ints([0, 2900, 3000]), 2900, 1)
+    assert kc.prompt_attention(q, k, v, ints([0, 2900, 3000]), 2900, 1, out=q) is q and torch.equal(q, want)
+
+
 def test_bad_sequences_are_skipped_and_reported(kc):
     from qvggt_b200 import _lib
     q, k, v = inputs(8, 300, 2, 2, 64, torch.float16)

@@ -65,6 +65,25 @@ def test_steps_after_a_prompt_match_all_at_once(time_axis):
         assert (dx - dw).norm() <= 3e-2 * dw.norm()
 
 
+@pytest.mark.parametrize("kind", ["w4", "w8"])
+def test_prompt_and_step_of_either_weight_format(kind):
+    """int8 blocks take the same path: their first frames at once are their first frames one after another, but for the
+    cache's 8 bits (3e-2 of the updates) and the activations' (a code more or less: 1e-2)."""
+    from qvggt_b200.streaming import StreamingRunner
+    from tests.test_gpu_streaming_frames import _blocks as blocks_of
+    dev = torch.device("cuda", 0)
+    cfg = _config()
+    blocks = blocks_of(cfg, dev, kind)
+    x = _tokens(cfg, 3, 9)
+    outs = []
+    for first in (0, 2):
+        run = StreamingRunner(cfg, *blocks, 1, 3, dev, block_size=32, sink_frames=0)
+        got = [run.prompt(x[:2].clone(), [2])[-1][1]] if first else []
+        got += [run.step(x[i:i + 1].clone())[-1][1] for i in range(first, 3)]
+        outs.append(torch.cat([t.view(-1, cfg.dim) for t in got]).double() - x.view(-1, cfg.dim).double())
+    assert (outs[0] - outs[1]).norm() <= 4e-2 * outs[0].norm()
+
+
 def _snapshot(cache):
     return [t.cpu().numpy().copy() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.weights,
                                              cache.block_tables, cache.lens)]
