@@ -13,9 +13,10 @@ namespace {
 
 constexpr int UNIT = 32;                 // keys a warp takes at a time: never across two blocks
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-// More rows of a key head than this go to key_weights_sm100.cu: eight streams of
-// 8,000 keys take 62 us there at 40 rows (mostly padding of its 128), here 71 at
-// 32 rows of 20,000 keys and twice that at 33, when the codes are read twice.
+// More rows of a key head than this go to key_weights_sm100.cu.  Eight streams, 16
+// heads, us here / there: head_dim 64 over 10,000 to 20,000 keys at 28 rows 62 / 127,
+// at 40 (the codes unpacked twice) 158 / 127; head_dim 128 96 / 187 and 231 / 187;
+// over 500 to 1,000 keys at 28 rows 15 / 15 and 20 / 18.
 constexpr int ROWS_MAX = 32;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {

@@ -32,6 +32,9 @@ namespace {
 constexpr int THREADS = 768;
 constexpr int KEYS = 256;       // keys of an item
 constexpr int ITEMS = 4;        // items handed out ahead
+// Sums being put together: a warp opens item x + 4 only when all have opened x
+// (the items' ring), so it writes its sums of x + 5 after all others' of x are read.
+constexpr int PARTS = ITEMS + 1;
 constexpr int ITEM_READERS = 3 + 4 + 16;   // issuers and rows, keys, sums
 constexpr uint32_t TMEM_COLS = 512;
 
@@ -40,7 +43,7 @@ struct __align__(16) Item {
   int b, kvh, key0, n;
   int q0, ql, t0, t1;
   int nkt;                               // key tiles; -1: no more items
-  int pad[3];
+  int fresh, pad[2];
 };
 
 template <int D>
@@ -53,12 +56,12 @@ struct Lay {
   static constexpr int KEY = K + 2 * 2 * PANELS * PANEL;   // [item % 2][256]: factor of the exponent, place
   static constexpr int ROW = KEY + 2 * KEYS * 8;           // [stage][128]: -lse log2e
   static constexpr int LIM = ROW + QS * 128 * 4;           // [stage][128]: keys the row sees
-  static constexpr int LOW = LIM + QS * 128 * 4;           // [stage]: the fewest any row sees
-  static constexpr int PART = LOW + QS * 16;               // [item % 2][warpgroup][256]: sums of its rows
-  static constexpr int BAR = PART + 2 * 4 * KEYS * 4;
+  static constexpr int SEEN = LIM + QS * 128 * 4;          // [stage][warpgroup]: the fewest and the most keys its rows see
+  static constexpr int PART = SEEN + QS * 32;              // [item % PARTS][warpgroup][256]: sums of its rows
+  static constexpr int BAR = PART + PARTS * 4 * KEYS * 4;
   // q_full[QS], q_empty[QS], k_full[2], k_empty[2], item_full[ITEMS], item_empty[ITEMS],
-  // s_full[2], s_free[2], part_full[2], drain[2]
-  static constexpr int NUM_BARS = 2 * QS + 4 + 2 * ITEMS + 8;
+  // s_full[2], s_free[2], part_full[PARTS], drain[2]
+  static constexpr int NUM_BARS = 2 * QS + 4 + 2 * ITEMS + 6 + PARTS;
   static constexpr int MISC = BAR + (NUM_BARS + 1) / 2 * 16;
   static constexpr int ITEM = MISC + 16;
   static constexpr int CUM = ITEM + ITEMS * (int)sizeof(Item);   // long long [THREADS + 1]
@@ -103,14 +106,14 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* s_full = item_empty + ITEMS;       // [Q tile % 2]
   uint64_t* s_free = s_full + 2;
   uint64_t* part_full = s_free + 2;
-  uint64_t* drain = part_full + 2;
+  uint64_t* drain = part_full + PARTS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::MISC);
   volatile Item* items = reinterpret_cast<volatile Item*>(smem + L::ITEM);
   float* key_ck = reinterpret_cast<float*>(smem + L::KEY);         // [item % 2][256]
   int* key_at = reinterpret_cast<int*>(key_ck + 2 * KEYS);         // block * block_size + offset, -1: none
   float* row_nl = reinterpret_cast<float*>(smem + L::ROW);
   int* row_lim = reinterpret_cast<int*>(smem + L::LIM);
-  int* low = reinterpret_cast<int*>(smem + L::LOW);
+  int2* row_seen = reinterpret_cast<int2*>(smem + L::SEEN);
   float* part = reinterpret_cast<float*>(smem + L::PART);
   long long* cum = reinterpret_cast<long long*>(smem + L::CUM);
   const uint32_t tries = a.wait_tries;
@@ -124,7 +127,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int s = 0; s < 2; ++s) {
       mbar_init(&k_full[s], 4);
       mbar_init(&k_empty[s], 2 + 16);
-      mbar_init(&part_full[s], 16);
       mbar_init(&s_full[s], 4);
       mbar_init(&s_free[s], 16);
     }
@@ -132,6 +134,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&item_full[s], 1);
       mbar_init(&item_empty[s], ITEM_READERS);
     }
+    for (int s = 0; s < PARTS; ++s) mbar_init(&part_full[s], 16);
     mbar_init(&drain[0], 1);
     mbar_init(&drain[1], 1);
     fence_mbar_init();
@@ -193,6 +196,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           items[st].ql = rql;
           items[st].t0 = first <= 0 ? 0 : first >= rql ? t1 : (int)first / tpt;
           items[st].t1 = t1;
+          items[st].fresh = a.fresh ? a.fresh[b] : rn;
           items[st].nkt = rn - key0 > 128 ? 2 : 1;
         }
         mbar_arrive(&item_full[st]);
@@ -312,7 +316,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int t = t0; t < t1; ++t, ++tg) {
           const int st = tg % QS;
           float nl[4];
-          int lim[4], fewest = n;
+          int lim[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             nl[x] = -l[x] * LOG2E;
@@ -324,17 +328,17 @@ __global__ void __launch_bounds__(THREADS, 1)
               seen = pos < 0 ? 0 : (int)min((long long)n, (long long)(c + 1) * a.chunk);
             }
             lim[x] = isfinite(l[x]) ? seen : 0;
-            if (lane + 32 * x < most) fewest = min(fewest, lim[x]);
           }
           fetch(t + 1);
-          fewest = __reduce_min_sync(~0u, fewest);
           if (!warp_wait(&q_empty[st], ((tg / QS) & 1) ^ 1, tries)) { ok = false; break; }
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             row_nl[st * 128 + lane + 32 * x] = nl[x];
             row_lim[st * 128 + lane + 32 * x] = lim[x];
+            // (rows that no token has score 0 and weigh 0: they are no reason to look at each)
+            const int fewest = __reduce_min_sync(~0u, lane + 32 * x < most ? lim[x] : n), largest = __reduce_max_sync(~0u, lim[x]);
+            if (lane == 0) row_seen[st * 4 + x] = make_int2(fewest, largest);
           }
-          if (lane == 0) low[st] = fewest;
           __syncwarp();
           if (lane == 0) mbar_arrive(&q_full[st]);
         }
@@ -349,52 +353,71 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (p / 8 % 128 >= tpt * a.group)
           asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(sbase + L::Q + p * 16), "r"(0) : "memory");
     constexpr int LOADS = 4;                   // 16-byte pieces a lane has under way: 32 keys with head_dim 64, 16 with 128
-    bool ok = true, bad = false;
-    for (int it = 0; ok; ++it) {
-      const int is = it % ITEMS, kb = it & 1;
-      if (!warp_wait(&item_full[is], (it / ITEMS) & 1, tries)) { ok = false; break; }
-      const int nkt = items[is].nkt, kvh = items[is].kvh, key0 = items[is].key0, n = items[is].n, b = items[is].b;
+    constexpr int STEPS = D / 64;              // of a key tile
+    bool bad = false;
+    // An item, and the blocks and scales of this warp's keys in its key tiles.
+    struct Keys {
+      int nkt, kvh, key0, n, id[2];
+      float ks[2];
+    };
+    auto open = [&](int it, Keys& x) {
+      const int is = it % ITEMS;
+      if (!warp_wait(&item_full[is], (it / ITEMS) & 1, tries)) return false;
+      x.nkt = items[is].nkt;
+      x.kvh = items[is].kvh;
+      x.key0 = items[is].key0 + 32 * (warp - 4);
+      x.n = items[is].n;
+      const int b = items[is].b;
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[is]);
-      if (nkt < 0) break;
-      int id[2];
-      float ks[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int k = key0 + 128 * i + 32 * (warp - 4);    // this warp's first key
-        id[i] = -1;
-        ks[i] = 0.f;
-        if (k < n) {
-          id[i] = a.table[(long long)b * a.wide + (k >> a.bs_log2)];
-          if (id[i] >= 0 && id[i] < a.num_blocks) {
-            ks[i] = a.ks[(long long)id[i] * a.hk + kvh];
+        const int k = x.key0 + 128 * i;        // this warp's first key
+        x.id[i] = -1;
+        x.ks[i] = 0.f;
+        if (i < x.nkt && k < x.n) {
+          x.id[i] = a.table[(long long)b * a.wide + (k >> a.bs_log2)];
+          if (x.id[i] >= 0 && x.id[i] < a.num_blocks) {
+            x.ks[i] = a.ks[(long long)x.id[i] * a.hk + x.kvh];
           } else {
-            id[i] = -1;
+            x.id[i] = -1;
             bad = true;
           }
         }
       }
-      bool room = it < 2;
-      for (int u = 0; u < nkt * (D / 64); ++u) {
-        const int i = u / (D / 64), half = u % (D / 64);
-        const int k = key0 + 128 * i + 32 * (warp - 4), blk = i ? id[1] : id[0];
-        const int8_t* kp = a.kc + blk * a.block_stride + ((long long)kvh * bs + (k & (bs - 1))) * D;
-        uint4 w[LOADS];
+      return true;
+    };
+    auto load = [&](const Keys& x, int u, uint4 (&w)[LOADS]) {
+      const int i = u / STEPS, part = u % STEPS, blk = i ? x.id[1] : x.id[0];
+      const int8_t* kp = a.kc + blk * a.block_stride + ((long long)x.kvh * bs + ((x.key0 + 128 * i) & (bs - 1))) * D;
+#pragma unroll
+      for (int y = 0; y < LOADS; ++y) {
+        w[y] = make_uint4(0, 0, 0, 0);
+        if (blk >= 0) w[y] = __ldg(reinterpret_cast<const uint4*>(kp) + (part * LOADS + y) * 32 + lane);
+      }
+    };
+    Keys cur, next;
+    uint4 w[LOADS], ahead[LOADS];
+    bool ok = open(0, cur);
+    if (ok && cur.nkt > 0) load(cur, 0, w);
+    for (int it = 0; ok && cur.nkt > 0; ++it) {
+      const int kb = it & 1;
+      ok = open(it + 1, next);
+      for (int u = 0; ok && u < cur.nkt * STEPS; ++u) {
+        // the next step's codes are on their way while these are unpacked
+        if (u + 1 < cur.nkt * STEPS) load(cur, u + 1, ahead);
+        else if (next.nkt > 0) load(next, 0, ahead);
+        if (u == 0 && it >= 2 && !warp_wait(&k_empty[kb], ((it - 2) / 2) & 1, tries)) { ok = false; break; }
+        const int i = u / STEPS, part = u % STEPS;
+        if (part == 0) {
+          const int blk = i ? cur.id[1] : cur.id[0];
+          const int key = cur.key0 + 128 * i + lane, at = kb * KEYS + 128 * i + 32 * (warp - 4) + lane;
+          key_ck[at] = (i ? cur.ks[1] : cur.ks[0]) * a.scale_log2;
+          key_at[at] = blk < 0 || key >= cur.n ? -1 : (blk << a.bs_log2) + (key & (bs - 1));
+        }
 #pragma unroll
         for (int x = 0; x < LOADS; ++x) {
-          w[x] = make_uint4(0, 0, 0, 0);
-          if (blk >= 0) w[x] = __ldg(reinterpret_cast<const uint4*>(kp) + (half * LOADS + x) * 32 + lane);
-        }
-        if (!room && !warp_wait(&k_empty[kb], ((it - 2) / 2) & 1, tries)) { ok = false; break; }
-        room = true;
-        if (half == 0) {
-          const int key = k + lane, at = kb * KEYS + 128 * i + 32 * (warp - 4) + lane;
-          key_ck[at] = (i ? ks[1] : ks[0]) * a.scale_log2;
-          key_at[at] = blk < 0 || key >= n ? -1 : (blk << a.bs_log2) + (key & (bs - 1));
-        }
-#pragma unroll
-        for (int x = 0; x < LOADS; ++x) {
-          const int p = (half * LOADS + x) * 32 + lane;    // piece p % (D / 16) of row p / (D / 16)
+          const int p = (part * LOADS + x) * 32 + lane;    // piece p % (D / 16) of row p / (D / 16)
           const int piece = p % (D / 16), r = 32 * (warp - 4) + p / (D / 16), panel = piece / 4;
           const uint32_t c[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
           uint32_t y[8];
@@ -409,11 +432,14 @@ __global__ void __launch_bounds__(THREADS, 1)
           asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + c0), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]) : "memory");
           asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(line + c1), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7]) : "memory");
         }
+#pragma unroll
+        for (int x = 0; x < LOADS; ++x) w[x] = ahead[x];
       }
       if (!ok) break;
       fence_proxy_async_smem();                // these stores before the products' reads
       __syncwarp();
       if (lane == 0) mbar_arrive(&k_full[kb]);
+      cur = next;
     }
     if (bad && lane == 0) report_bad_block(a.ctl);
   } else {
@@ -423,10 +449,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t tg = 0;                           // Q tiles so far
     bool ok = true;
     for (int it = 0; ok; ++it) {
-      const int is = it % ITEMS, kb = it & 1;
+      const int is = it % ITEMS, kb = it & 1, pb = it % PARTS;
       if (!warp_wait(&item_full[is], (it / ITEMS) & 1, tries)) { ok = false; break; }
       const int nkt = items[is].nkt, nt = items[is].t1 - items[is].t0, kvh = items[is].kvh, key0 = items[is].key0;
-      const int fresh = nkt < 0 || !a.fresh ? 0x7fffffff : a.fresh[items[is].b];
+      const int fresh = items[is].fresh;
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[is]);
       if (nkt < 0) break;
@@ -434,6 +460,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       // this thread's keys, and the one whose sums it puts together (two warpgroups do)
       const float ck0 = key_ck[kb * KEYS + r], ck1 = nkt > 1 ? key_ck[kb * KEYS + 128 + r] : 0.f;
       const int at = wg < nkt ? key_at[kb * KEYS + 128 * wg + r] : -1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&k_empty[kb]);            // (the products arrive too)
       const long long place = (((long long)(at >> a.bs_log2) * a.hk + kvh) << a.bs_log2) + (at & ((1 << a.bs_log2) - 1));
       float old = 0.f;
       if (at >= 0 && key0 + 128 * wg + r < fresh) old = a.w[place];
@@ -443,8 +471,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int st = tg % QS, x = tg & 1;
         if (!__all_sync(~0u, ready) && !warp_wait(&s_full[x], (tg >> 1) & 1, tries)) { ok = false; break; }
         tc_fence_after();
-        // every row sees every key of the item
-        const bool all = low[st] >= key0 + 128 * nkt;
+        // whether every row sees every key of the item, and whether one sees any
+        const int2 seen = row_seen[st * 4 + wg];
+        const bool all = seen.x >= key0 + 128 * nkt, none = seen.y <= key0;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t v0[16], v1[16];
@@ -462,6 +491,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             // asked ahead: an answer takes a while
             ready = t + 1 < nt && test(smem_u32(&s_full[x ^ 1]), ((tg + 1) >> 1) & 1);
           }
+          if (none) continue;
           if (all) {
             const uint64_t c0 = f2_pack(ck0, ck0), c1 = f2_pack(ck1, ck1);
 #pragma unroll
@@ -497,18 +527,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       // the warpgroups' sums join in their order
       float lo, hi;
       f2_unpack(s0, lo, hi);
-      part[(kb * 4 + wg) * KEYS + r] = lo + hi;
+      part[(pb * 4 + wg) * KEYS + r] = lo + hi;
       f2_unpack(s1, lo, hi);
-      part[(kb * 4 + wg) * KEYS + 128 + r] = lo + hi;
+      part[(pb * 4 + wg) * KEYS + 128 + r] = lo + hi;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&part_full[kb]);
+      if (lane == 0) mbar_arrive(&part_full[pb]);
       if (wg < 2) {
-        if (!warp_wait(&part_full[kb], (it / 2) & 1, tries)) { ok = false; break; }
-        const float* p = part + kb * 4 * KEYS + 128 * wg + r;
+        if (!warp_wait(&part_full[pb], (it / PARTS) & 1, tries)) { ok = false; break; }
+        const float* p = part + pb * 4 * KEYS + 128 * wg + r;
         if (at >= 0) a.out[place] = fmaf(old, a.decay, (p[0] + p[KEYS]) + (p[2 * KEYS] + p[3 * KEYS]));
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&k_empty[kb]);            // (the products arrive too)
     }
     if (!ok && lane == 0) report_status(a.ctl, ST_TIMEOUT_SOFTMAX);
   }
