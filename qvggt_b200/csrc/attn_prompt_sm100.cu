@@ -38,7 +38,7 @@ constexpr int SEG_READERS = 12; // producer, two issuers, the V tiles' warp, 8 w
 constexpr int Q_ROWS = 256;     // rows of an item
 // Cost of an item on the line, in tenths of a tile with two Q tiles: a start-up
 // (loads, first products, epilogue) and its key tiles.  (A start of 30 costs four
-// streams of one to six frames 1 % more, 20 costs them 2 % and causal sequences
+// streams of one to six frames 1 % more, 20 costs them 3 % and causal sequences
 // of 400 to 4,099 tokens 10 %.)
 constexpr int COST_START = 50, COST_TILE2 = 10, COST_TILE1 = 9;
 // No piece is cut shorter than this (8 tiles): a join costs about as much.

@@ -343,13 +343,6 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
 }
 
 // --------------------------------------------------------------------- move
-// --------------------------------------------------------------------- move
-#ifndef TRIG
-#define TRIG 1
-#endif
-#ifndef SPANF
-#define SPANF 16
-#endif
 constexpr int MOVE_THREADS = 256, MOVE_WARPS = MOVE_THREADS / 32;
 constexpr int MOVE_BLOCKS = 256;         // blocks of a CTA at most
 constexpr int MOVE_ROWS = 2048;          // rows they receive at most
@@ -443,6 +436,7 @@ __global__ void __launch_bounds__(MOVE_THREADS, 3) kv_evict_kernel(MoveArgs a) {
   const int bs = 1 << a.bs_log2;
   const int keep = a.keep[b];
   const int moves = a.counts[row];
+  if (moves == 0) return;                // whatever `keep` says: a request that holds no more stays
   if (keep < 0 || keep > (a.wide << a.bs_log2) || moves < 0 || moves > a.max_moves) {
     if (tid == 0) report_status(a.ctl, ST_BAD_LENGTH);
     return;
@@ -450,9 +444,11 @@ __global__ void __launch_bounds__(MOVE_THREADS, 3) kv_evict_kernel(MoveArgs a) {
   const int blocks = (int)(((long long)keep + bs - 1) >> a.bs_log2);
   const int edge = keep & (bs - 1) ? keep >> a.bs_log2 : -1;
   const int j0 = EDGE ? edge : part * a.span, j1 = EDGE ? edge + 1 : min(blocks, j0 + a.span);
-  if (moves == 0 || j0 < 0 || j0 >= j1) return;
   const int32_t* src = a.src + (long long)row * a.max_moves;
   const int32_t* dst = a.dst + (long long)row * a.max_moves;
+  // (places that lie in no block below `keep`, at either end as they ascend, come to no CTA's list)
+  if (!EDGE && part == 0 && tid == 0 && (dst[0] < 0 || dst[moves - 1] >= keep)) report_status(a.ctl, ST_BAD_LENGTH);
+  if (j0 < 0 || j0 >= j1) return;
   const int32_t* table = a.table + (long long)b * a.wide;
   const long long cell0 = (long long)layer * a.num_blocks * a.heads + h;
   auto cell = [&](int blk) { return cell0 + (long long)blk * a.heads; };

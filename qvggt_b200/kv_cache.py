@@ -538,8 +538,9 @@ def evict_plan(weights, block_tables, lens, keep, sink: int, recent: int, max_mo
 
     For every layer and kv head apart: the first ``sink`` and the last
     ``recent`` tokens as the cache holds them (as far as ``keep`` goes, the
-    first ones before the last), then those of largest weight, of equal ones
-    the earlier.  ``weights`` fp32 ``[layers, num_blocks, kv_heads,
+    first ones before the last; those that move lose their place, so the last
+    are the newest only among tokens added since the eviction before), then
+    those of largest weight, of equal ones the earlier.  ``weights`` fp32 ``[layers, num_blocks, kv_heads,
     block_size]`` as :func:`key_weights` gathers them; NaN counts as the lowest,
     infinities as the largest finite ones.  A token that stays but stands at
     ``keep`` or later takes the place of one that goes, so the others need not

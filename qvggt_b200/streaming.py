@@ -22,7 +22,7 @@ for the steps that follow.
 then also gathers how much attention each cached key has got
 (:func:`~qvggt_b200.kv_cache.key_weights`), and before a step that would not
 fit, every layer and head drops the keys that got least, except those of the
-first ``sink_frames`` frames and the last ``recent_frames`` that came.
+first ``sink_frames`` frames and the last ``recent_frames`` of the newest step.
 
 With ``time_axis`` q and k of the global blocks turn by (time, height, width)
 positions (:func:`~qvggt_b200.kv_cache.rope_axes`) in place of the model's
@@ -51,7 +51,8 @@ class StreamingRunner(AggregatorRunner):
     each per step; the cache holds ``max_frames`` frames of each.  With
     ``sink_frames`` (0 or more) a stream that has filled it drops the tokens
     that got least attention, never those of its first ``sink_frames`` frames
-    nor of the last ``recent_frames`` of the cache; ``weight_decay`` ages what
+    nor of the last ``recent_frames`` (at most ``frames``: tokens of earlier
+    steps have no fixed place in the cache); ``weight_decay`` (0 to 1) ages what
     they have got, once a step.  One GPU."""
 
     def __init__(self, cfg: AggConfig, frame_blocks, global_blocks, frames: int, max_frames: int, device,
@@ -62,10 +63,15 @@ class StreamingRunner(AggregatorRunner):
             raise ValueError(f"StreamingRunner: heads of 64 dims, got {cfg.dim} / {cfg.heads}")
         P = cfg.tokens_per_frame
         per_stream = -(-max_frames * P // block_size)
-        if sink_frames is not None and (frames > max_frames or
-                                        not 0 <= sink_frames + recent_frames <= max_frames - frames):
-            raise ValueError(f"StreamingRunner: {sink_frames} + {recent_frames} frames that stay and {frames} new ones do "
-                             f"not fit {max_frames}")
+        if sink_frames is not None:
+            if frames > max_frames or min(sink_frames, recent_frames) < 0 or sink_frames + recent_frames > max_frames - frames:
+                raise ValueError(f"StreamingRunner: {sink_frames} + {recent_frames} frames that stay and {frames} new ones "
+                                 f"do not fit {max_frames}")
+            if recent_frames > frames:
+                raise ValueError(f"StreamingRunner: recent_frames {recent_frames} must not pass a step's {frames}: the "
+                                 f"tokens of earlier steps have no fixed place in the cache")
+            if not 0 <= weight_decay <= 1:
+                raise ValueError(f"StreamingRunner: weight_decay must be 0 to 1, got {weight_decay}")
         self.frames, self.streams, self.max_frames = frames, streams, max_frames
         self.sink_frames, self.recent_frames, self.weight_decay = sink_frames, recent_frames, weight_decay
         self._seen, self._held = [0] * streams, [0] * streams        # frames of each stream: so far, in the cache

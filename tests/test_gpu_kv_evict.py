@@ -242,7 +242,7 @@ def test_evict_plan(kc, layers, H, bs, lens, part, sink, recent, hint):
 
 
 def test_evict_plan_longer_than_shared_memory(kc):
-    """More keys than eight CTAs hold: they are read again for each digit."""
+    """More keys than four CTAs hold: they are read again for each digit."""
     rng = np.random.default_rng(1)
     n, bs = 500000, 128
     table, num = random_table(rng, [n], bs)
@@ -379,6 +379,47 @@ def test_kv_evict_skips_and_reports_bad_moves(kc):
         assert _lib.device_status(clear=True) == (0x201 if change == "block" else 0x202)
         mine = table[0][table[0] >= 0]
         assert all((a[:, mine] == b[:, mine]).all() for a, b in zip(got, [*codes, *scales, w]))
+
+
+def test_kv_evict_reports_places_outside_and_takes_any_keep_without_moves(kc):
+    """Destinations at or past the new length and before 0 are skipped and reported, also where they lie in no block below
+    it or nothing stays; a request that holds no more than `keep` has no moves, however large `keep` is."""
+    from qvggt_b200 import _lib
+    rng = np.random.default_rng(6)
+    lens, bs = [300, 200], 32
+    for keep, ends in (([150, 100], [(0, -1)]), ([160, 100], [(-1, 290)]), ([150, 100], [(-1, 155)]),
+                       ([160, 100], [(0, -1), (-1, 160)])):
+        table, codes, scales, w, plan = move_case(rng, 1, 2, 64, bs, lens, keep, 150)
+        spoiled, left = [x.copy() for x in plan], [x.copy() for x in plan]
+        n = plan[2][0, 0, 1]
+        lo, hi = 0, n
+        for end, place in ends:
+            spoiled[1][0, 0, 1, end % n] = place
+            lo, hi = (1, hi) if end == 0 else (lo, n - 1)
+        for x in left[:2]:
+            x[0, 0, 1, :hi - lo] = x[0, 0, 1, lo:hi].copy()
+        left[2][0, 0, 1] = hi - lo
+        got = run_move(kc, table, codes, scales, w, spoiled, keep)
+        assert _lib.device_status(clear=True) == 0x202
+        for c, s in zip(codes, scales):
+            oe.kv_evict(c, s, table, *left)
+        oe.evict_weights(w, table, *left)
+        for a, b in zip(got, [*codes, *scales, w]):
+            assert (a == b).all()
+    # nothing stays, but moves are asked for
+    table, codes, scales, w, plan = move_case(rng, 1, 2, 64, bs, lens, [150, 100], 150)
+    got = run_move(kc, table, codes, scales, w, plan, [0, 0])
+    assert _lib.device_status(clear=True) == 0x202
+    assert all((a == b).all() for a, b in zip(got, [*codes, *scales, w]))
+    # far more than the tables hold: nothing moves, nothing is wrong
+    keep = [2 ** 31 - 1, 100]
+    table, codes, scales, w, plan = move_case(rng, 1, 2, 64, bs, lens, keep, 100)
+    got = run_move(kc, table, codes, scales, w, plan, keep)
+    assert _lib.device_status(clear=True) == 0
+    for c, s in zip(codes, scales):
+        oe.kv_evict(c, s, table, *plan)
+    oe.evict_weights(w, table, *plan)
+    assert all((a == b).all() for a, b in zip(got, [*codes, *scales, w]))
 
 
 # --------------------------------------------------------------- streams, graphs

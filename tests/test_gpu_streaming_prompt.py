@@ -198,6 +198,19 @@ def test_streaming_aggregator_prompt_is_the_models():
     assert (both[:1374].double() - got).norm() <= 1e-3 * got.norm()      # the first frame does not see the second
 
 
+@pytest.mark.parametrize("per_step,hold,sink,recent,decay,match", [
+    (1, 4, 0, 2, 1.0, "recent_frames"), (1, 4, -1, 1, 1.0, "fit"), (1, 4, 2, -1, 1.0, "fit"), (2, 5, 2, 2, 1.0, "fit"),
+    (3, 2, 0, 0, 1.0, "fit"), (1, 4, 1, 1, 1.5, "decay"), (1, 4, 1, 1, float("nan"), "decay")])
+def test_windows_that_cannot_be_kept_are_refused(per_step, hold, sink, recent, decay, match):
+    """A recent window that reaches back past a step would pin what stands there, not the newest."""
+    from qvggt_b200.streaming import StreamingRunner
+    dev = torch.device("cuda", 0)
+    cfg = _config()
+    with pytest.raises(ValueError, match=match):
+        StreamingRunner(cfg, *_blocks(cfg, dev), per_step, hold, dev, block_size=32, sink_frames=sink, recent_frames=recent,
+                        weight_decay=decay)
+
+
 def test_command_line(capsys):
     from qvggt_b200 import streaming
     streaming.main(["--frames", "5", "--depth", "1", "--prompt", "2", "--hold", "3", "--time-axis"])
