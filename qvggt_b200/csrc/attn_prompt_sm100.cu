@@ -7,7 +7,7 @@
 // gives late blocks many times the keys of early ones: the items' key tiles are
 // laid out as one line of cost and cut into equal pieces, one per SM
 // (attn_cache.cuh); what a cut separates is joined by a second launch.
-// Per key tile of KT keys (128 for head_dim 64, 64 for 128):
+// Per key tile of KT keys (128; 64 where no sequence is longer):
 //   warp 0         TMA of K, V and Q tiles, K and V through rings of KV stages
 //   warp 1         S_i = Q_i K^T        warp 3   O_i += P_i V
 //   warp 2         the segments (an item, or the part of it that falls to this
@@ -23,7 +23,12 @@
 // sequence become 0 and elements that are not finite become 0; where one was,
 // the rows that do see it add it at the end (add_odd).
 //
-// TMEM columns: S_i at i KT, P_i at 2 KT + i KT / 2, O_i at 512 - (2 - i) D.
+// TMEM columns: S_i at i KT, P_i at 2 KT + i KT / 2, O_i at 512 - (2 - i) D.  With
+// head_dim 128 and 128-key tiles that is 128 columns too many: S_0 and S_1 take
+// turns at column 0 (a score tile is read into registers at once, so its place is
+// free again long before the exponentials are done), and P_i is at KT + i KT / 2.
+// 64-key tiles with places of their own cost half as many waits and TMEM reads
+// again for each key: 1,234 us against 1,020 (two sequences of 8,192, 16 heads).
 #include "attn_cache.cuh"
 #include "attn_common.cuh"
 #include "host.hpp"
@@ -32,7 +37,6 @@ namespace qv {
 namespace {
 
 constexpr int THREADS = 384;
-constexpr int KV = 4;           // stages of K and of V
 constexpr int SEGS = 4;         // segments handed out ahead
 constexpr int SEG_READERS = 12; // producer, two issuers, the V tiles' warp, 8 warps
 constexpr int Q_ROWS = 256;     // rows of an item
@@ -43,7 +47,6 @@ constexpr int Q_ROWS = 256;     // rows of an item
 constexpr int COST_START = 50, COST_TILE2 = 10, COST_TILE1 = 9;
 // No piece is cut shorter than this (8 tiles): a join costs about as much.
 constexpr int COST_MIN = COST_START + 8 * COST_TILE2;
-constexpr int OP_BYTES = 16384; // K or V of a tile
 constexpr uint32_t TMEM_COLS = 512;
 
 struct PromptArgs {
@@ -61,9 +64,10 @@ struct PromptArgs {
   Ctl ctl;
 };
 
-template <int D>
+template <int D, int KT>
 struct Lay {
-  static constexpr int KT = D == 64 ? 128 : 64;
+  static constexpr int OP_BYTES = KT * D * 2;              // K or V of a tile
+  static constexpr int KV = OP_BYTES > 16384 ? 2 : 4;      // stages of each
   static constexpr int PANELS = D / 64;                    // 64-dim (128-byte) panels of Q and K / V rows
   static constexpr int Q_PANEL = 128 * 128;                // bytes: 128 rows x 64 dims
   static constexpr int Q = 0;                              // [tile][panel]
@@ -214,13 +218,14 @@ __device__ __forceinline__ void add_odd(const PromptArgs& a, uint32_t (&acc)[W],
   }
 }
 
-template <bool BF16, int D>
+template <bool BF16, int D, int KT>
 __global__ void __launch_bounds__(THREADS, 1)
     prompt_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                             const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PromptArgs a) {
-  using L = Lay<D>;
-  constexpr int KT = L::KT;
-  constexpr uint32_t COL_S = 0, COL_P = 2 * KT, COL_O = 512 - 2 * D;
+  using L = Lay<D, KT>;
+  constexpr int KV = L::KV, OP_BYTES = L::OP_BYTES;
+  constexpr bool ONE_S = 3 * KT + 2 * D > 512;           // both Q tiles' scores take turns in one place
+  constexpr uint32_t COL_S = 0, COL_P = ONE_S ? KT : 2 * KT, COL_O = 512 - 2 * D;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
@@ -450,7 +455,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // group of MMAs: from inside a one-lane branch the same MMAs issue a
       // third slower (their descriptors are then not warp-uniform).
       constexpr uint32_t idesc = idesc_f16(128, KT, false, false, BF16);
-      uint32_t cs[2] = {0, 0};                             // S_i products issued so far
+      uint32_t cs[2] = {0, 0};                             // products issued so far into each place of scores
       int jg = 0, it = 0;
       bool ok = true;
       for (int seg = 0; ok; ++seg) {
@@ -466,15 +471,16 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int st = jg % KV;
           if (!warp_wait(&k_full[st], (jg / KV) & 1, tries)) { ok = false; break; }
           for (int i = 0; i < nqt; ++i) {
-            if (cs[i] > 0 && !warp_wait(&s_free[i], (cs[i] - 1) & 1, tries)) { ok = false; break; }
-            ++cs[i];
+            const int x = ONE_S ? 0 : i;
+            if (cs[x] > 0 && !warp_wait(&s_free[x], (cs[x] - 1) & 1, tries)) { ok = false; break; }
+            ++cs[x];
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
               for (int p = 0; p < L::PANELS; ++p)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  mma_f16_ss(tmem + COL_S + i * KT,
+                  mma_f16_ss(tmem + COL_S + x * KT,
                              sdesc_sw128(sbase + L::Q + (i * L::PANELS + p) * L::Q_PANEL + k * 32),
                              sdesc_sw128(sbase + L::K + st * OP_BYTES + p * KT * 128 + k * 32), idesc,
                              (p | k) ? 1u : 0u);
@@ -549,11 +555,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tS = tmem + lane_base + COL_S + i * KT;
+    const uint32_t tS = tmem + lane_base + COL_S + (ONE_S ? 0 : i * KT);
     const uint32_t tP = tmem + lane_base + COL_P + i * (KT / 2);
     const uint32_t tO = tmem + lane_base + COL_O + i * D;
     const uint32_t bar_s_full = smem_u32(&s_full[i]);
-    const uint32_t bar_s_free = bar_s_full + 16, bar_p_full = bar_s_full + 32, bar_o_done = bar_s_full + 48;
+    const uint32_t bar_s_free = ONE_S ? smem_u32(s_free) : bar_s_full + 16, bar_p_full = bar_s_full + 32, bar_o_done = bar_s_full + 48;
     const float c = a.scale_log2;
     // the row's token in the block (past any block's for a row that holds none)
     // and head in the group: kept in shared memory, as registers held through
@@ -607,8 +613,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
         float lj = 0.f;
-        // (the previous item's epilogue has waited for its last PV product)
-        if (!exp_store<BF16, 1>(s, c, neg_m, lj, tP, j == 0, bar_o_done, (cnt - 1) & 1, tries)) { ok = false; break; }
+        // (the previous item's epilogue has waited for its last PV product.)  Two of 16
+        // exponentials on the FMA pipe with head_dim 64, whose limit the others are; with
+        // 128 none (two sequences of 8,192: 955 us, 990 with two)
+        if (!exp_store<BF16, D == 64 ? 1 : 0>(s, c, neg_m, lj, tP, j == 0, bar_o_done, (cnt - 1) & 1, tries)) { ok = false; break; }
         ready = j + 1 < ntr && test(bar_s_full, (cnt + 1) & 1);
         l = l * alpha + lj;
         if (rescale) {
@@ -646,7 +654,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const bool odd = segs[ss].pad[0] != 0;
         // 16 columns at a time where the score row is 128 wide: more would cost
         // the tile loop registers
-        constexpr int W = D == 64 ? 16 : 32;
+        constexpr int W = KT == 128 ? 16 : 32;
 #pragma unroll 1
         for (int cc = 0; cc < D; cc += W) {
           uint32_t v[W];
@@ -717,21 +725,27 @@ __global__ void __launch_bounds__(256) prompt_attention_join_kernel(PromptArgs a
 }
 
 // Whether items may be cut (a rule on the longest length alone: the join is launched by it).
-bool can_cut(long long max_len, int D) { return max_len > 8 * (D == 64 ? 128 : 64); }
+bool can_cut(long long max_len) { return max_len > 8 * 128; }
+
+// 64-key tiles where one holds the longest sequence (400 sequences of 20 to 40
+// causal tokens, 16 heads x 128: 143 us, 203 with 128-key tiles; five: 9.5 and
+// 11.4), else 128 (80 of 100 to 200 tokens: 87, 85 with 64-key tiles; five of up to
+// 256: 17 and 21).
+int tile_keys(long long max_len) { return max_len <= 64 ? 64 : 128; }
 
 // One CTA per SM at most, and no more than there can be pieces.
-int grid_of(long long items, long long max_len, int D) {
-  const int kt = D == 64 ? 128 : 64;
+int grid_of(long long items, long long max_len) {
+  const int kt = tile_keys(max_len);
   const long long cost = items * (COST_START + (max_len + kt - 1) / kt * COST_TILE2);
-  const long long pieces = can_cut(max_len, D) ? (cost + COST_MIN - 1) / COST_MIN : items;
+  const long long pieces = can_cut(max_len) ? (cost + COST_MIN - 1) / COST_MIN : items;
   return (int)std::max<long long>(1, std::min<long long>(pieces, device_info().num_sms));
 }
 
 int64_t row_blocks_of(int64_t max_len, int group) { return (max_len + 2 * (128 / group) - 1) / (2 * (128 / group)); }
 
 int64_t scratch_of(long long items, long long max_len, int D) {
-  if (!can_cut(max_len, D)) return 0;
-  const int64_t grid = grid_of(items, max_len, D);
+  if (!can_cut(max_len)) return 0;
+  const int64_t grid = grid_of(items, max_len);
   return grid > 1 ? grid * (2 * Q_ROWS * (D + 1) * (int64_t)sizeof(float) + (int64_t)sizeof(Cut)) : 0;
 }
 
@@ -824,30 +838,34 @@ extern "C" int qvggt_prompt_attention(const qvggt_prompt_attention_args* p, void
   if (need && (!p->scratch || p->scratch_bytes < need || !aligned16(p->scratch)))
     return set_error(QVGGT_ERR_INVALID, "%s: needs %lld bytes of 16-byte aligned scratch, got %lld", name, (long long)need,
                      (long long)p->scratch_bytes);
-  const int smem = D == 64 ? Lay<64>::TOTAL : Lay<128>::TOTAL;
+  const int kt = tile_keys(max_len);
+  const int smem = D == 64 ? (kt == 64 ? Lay<64, 64>::TOTAL : Lay<64, 128>::TOTAL)
+                           : (kt == 64 ? Lay<128, 64>::TOTAL : Lay<128, 128>::TOTAL);
   if (smem > device_info().max_smem_optin)
     return set_error(QVGGT_ERR_UNSUPPORTED, "%s: shared memory %d > %d", name, smem, device_info().max_smem_optin);
   const bool bf16 = p->dtype == QVGGT_DTYPE_BF16;
-  const uint32_t kt = D == 64 ? Lay<64>::KT : Lay<128>::KT;
   CUtensorMap tmQ, tmK, tmV;
   if (int rc = rows_map(&tmQ, bf16, p->q, D, a.hq, T, p->q_head, p->q_tok, (uint32_t)a.group, (uint32_t)(128 / a.group)))
     return rc;
-  if (int rc = rows_map(&tmK, bf16, p->k, D, a.hk, T, p->k_head, p->k_tok, 1, kt)) return rc;
-  if (int rc = rows_map(&tmV, bf16, p->v, D, a.hk, T, p->v_head, p->v_tok, 1, kt)) return rc;
-  const int grid = grid_of(items, max_len, (int)D);
+  if (int rc = rows_map(&tmK, bf16, p->k, D, a.hk, T, p->k_head, p->k_tok, 1, (uint32_t)kt)) return rc;
+  if (int rc = rows_map(&tmV, bf16, p->v, D, a.hk, T, p->v_head, p->v_tok, 1, (uint32_t)kt)) return rc;
+  const int grid = grid_of(items, max_len);
   a.can_split = need > 0;
   a.part_o = static_cast<float*>(p->scratch);
   a.part_lse = a.can_split ? a.part_o + 2LL * grid * Q_ROWS * D : nullptr;
   using Kfn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, PromptArgs);
-  static const Kfn fns[2][2] = {{prompt_attention_kernel<false, 64>, prompt_attention_kernel<false, 128>},
-                                {prompt_attention_kernel<true, 64>, prompt_attention_kernel<true, 128>}};
+  static const Kfn fns[2][2][2] = {
+      {{prompt_attention_kernel<false, 64, 64>, prompt_attention_kernel<false, 64, 128>},
+       {prompt_attention_kernel<false, 128, 64>, prompt_attention_kernel<false, 128, 128>}},
+      {{prompt_attention_kernel<true, 64, 64>, prompt_attention_kernel<true, 64, 128>},
+       {prompt_attention_kernel<true, 128, 64>, prompt_attention_kernel<true, 128, 128>}}};
   using Jfn = void (*)(PromptArgs, int);
   static const Jfn joins[2][2] = {{prompt_attention_join_kernel<false, 64>, prompt_attention_join_kernel<false, 128>},
                                   {prompt_attention_join_kernel<true, 64>, prompt_attention_join_kernel<true, 128>}};
-  static DeviceFlags attr[2][2];
-  const Kfn fn = fns[bf16][D == 128];
+  static DeviceFlags attr[2][2][2];
+  const Kfn fn = fns[bf16][D == 128][kt == 128];
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int rc = ensure_smem(attr[bf16][D == 128], fn, smem, "cudaFuncSetAttribute(prompt_attention)")) return rc;
+  if (int rc = ensure_smem(attr[bf16][D == 128][kt == 128], fn, smem, "cudaFuncSetAttribute(prompt_attention)")) return rc;
   if (int rc = check_cuda(launch_pdl(fn, dim3((unsigned)grid), dim3(THREADS), smem, st, 1u, tmQ, tmK, tmV, a),
                           "prompt_attention launch"))
     return rc;
