@@ -204,6 +204,15 @@ __device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
   return (w & 0x7fff7fffu) + (BF16 ? 0x00800080u : 0x04000400u);
 }
 
+// 0 w + sum in both halves: NaN once w was an infinity or NaN, else +-0.
+template <bool BF16>
+__device__ __forceinline__ uint32_t add_zero_times(uint32_t w, uint32_t sum) {
+  uint32_t r;
+  if (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0), "r"(sum));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0), "r"(sum));
+  return r;
+}
+
 // Adds what was taken out of the V tiles to columns cc.. of a row that sees
 // keys [from, to): elements that are not finite.  Any weight of theirs gives
 // the same sum, an infinity or NaN.
@@ -347,22 +356,23 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (!ok) break;
           if (key0 + KT > seen) {
             // 16-byte pieces (the swizzle moves them within their row only): is there
-            // an odd one?  This warp looks after two Q tiles' softmax, so it looks fast
-            // first and works only on what it found.
+            // an odd one?  P V may wait for this, so one product per word looks first
+            // (222 causal sequences of 256, 16 heads x 128: 232 us; 258 with a test of
+            // the exponents, 196 with no look at all), and the rest works on what is found.
             const int first = max(0, seen - key0);         // the tile's first row that some row does not see
-            uint32_t any = 0;
+            uint32_t sum[4] = {0, 0, 0, 0};                // of 0 times each: 0, or NaN
 #pragma unroll 1
             for (int panel = 0; panel < L::PANELS; ++panel) {
               const uint32_t at = sbase + L::V + st * OP_BYTES + panel * KT * 128;
-#pragma unroll 8
+#pragma unroll 4
               for (int p = first * 8 + lane; p < KT * 8; p += 32) {
                 uint32_t w[4];
                 asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at + p * 16) : "memory");
 #pragma unroll
-                for (int e = 0; e < 4; ++e) any |= odd_bits<BF16>(w[e]);
+                for (int e = 0; e < 4; ++e) sum[e] = add_zero_times<BF16>(w[e], sum[e]);
               }
             }
-            if (__any_sync(~0u, (any & 0x80008000u) != 0)) {
+            if (__any_sync(~0u, ((sum[0] | sum[1] | sum[2] | sum[3]) & 0x7fff7fffu) != 0)) {
               bool odd = false;
 #pragma unroll 1
               for (int p = lane; p < OP_BYTES / 16; p += 32) {
