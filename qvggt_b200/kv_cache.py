@@ -458,8 +458,8 @@ def _lse_at(name, lse, q, dev, hq, T):
         return 0
     if lse.get_device() != dev:
         _check_cuda(name, q, lse)
-    _check_shape(name, lse.dtype is _F32 and lse.is_contiguous() and lse.shape == (hq, T),
-                 f"lse must be contiguous float32 [{hq}, {T}]")
+    if lse.dtype is not _F32 or lse.shape != (hq, T) or not lse.is_contiguous():
+        raise ValueError(f"{name}: lse must be contiguous float32 [{hq}, {T}]")
     return lse.data_ptr()
 
 
@@ -505,13 +505,15 @@ def key_weights(q, k_cache, k_scale, block_tables, cu_q, kv_lens, lse, weights, 
             _check_cuda(name, q, fresh_from)
         _ints(name, fresh_from, "fresh_from", (B,))
         fresh_at = fresh_from.data_ptr()
+    if weights.dtype is not _F32 or weights.shape != (nb, hk, bs) or not weights.is_contiguous():
+        raise ValueError(f"{name}: weights must be contiguous float32 [{nb}, {hk}, {bs}]")
     if out is None:
         out = weights
-    elif out.get_device() != dev:
-        _check_cuda(name, q, out)
-    for what, t in (("weights", weights), ("out", out)):
-        if t.dtype is not _F32 or t.shape != (nb, hk, bs) or not t.is_contiguous():
-            raise ValueError(f"{name}: {what} must be contiguous float32 [{nb}, {hk}, {bs}]")
+    elif out is not weights:
+        if out.get_device() != dev:
+            _check_cuda(name, q, out)
+        if out.dtype is not _F32 or out.shape != (nb, hk, bs) or not out.is_contiguous():
+            raise ValueError(f"{name}: out must be contiguous float32 [{nb}, {hk}, {bs}]")
     _run("qvggt_key_weights", dev, q,
          _WEIGHTS(k_cache.data_ptr(), st[0], k_scale.data_ptr(), nb, hk, bs, d, q.data_ptr(), sq[0], sq[1], T, hq, dt,
                   lse_at, block_tables.data_ptr(), wide, cu_q.data_ptr(), kv_lens.data_ptr(), fresh_at, B, max_q, max_kv,
@@ -560,15 +562,13 @@ def evict_plan(weights, block_tables, lens, keep, sink: int, recent: int, max_mo
     _ints(name, keep, "keep", (B,))
     if max_moves < 0:
         raise ValueError(f"{name}: max_moves must not be negative")
-    rows = layers * B * h
-    # one allocation, the counts last
-    buf = lens.new_empty(rows * (2 * max_moves + 1))
-    src, dst, counts = buf.split_with_sizes([rows * max_moves, rows * max_moves, rows])
-    at = buf.data_ptr()
-    _run("qvggt_evict_plan", dev, buf,
+    # (three allocations cost the host 5 us, parts of one 8)
+    src = lens.new_empty((layers, B, h, max_moves))
+    dst, counts = torch.empty_like(src), lens.new_empty((layers, B, h))
+    _run("qvggt_evict_plan", dev, weights,
          _EVICT_PLAN(weights.data_ptr(), layers, nb, h, bs, block_tables.data_ptr(), wide, lens.data_ptr(), keep.data_ptr(),
-                     B, sink, recent, max_moves, max_len, at, at + 4 * rows * max_moves, at + 8 * rows * max_moves))
-    return EvictPlan(src.view(layers, B, h, max_moves), dst.view(layers, B, h, max_moves), counts.view(layers, B, h))
+                     B, sink, recent, max_moves, max_len, src.data_ptr(), dst.data_ptr(), counts.data_ptr()))
+    return EvictPlan(src, dst, counts)
 
 
 def kv_evict(k_cache, v_cache, k_scale, v_scale, weights, block_tables, keep, plan: EvictPlan) -> None:
