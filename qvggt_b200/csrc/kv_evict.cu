@@ -15,6 +15,7 @@ namespace {
 // ------------------------------------------------------------------- choice
 constexpr int CHOOSE_THREADS = 1024, CHOOSE_WARPS = CHOOSE_THREADS / 32;
 constexpr int SPAN = 128;                // positions a warp takes at a time, four a lane
+constexpr int ROOM_MAX = 48 * 1024;      // keys a CTA holds: 192 KB beside 25 KB of counts
 // Digits of the 32-bit keys, from the top: 12, 10 and 10 bits.  The first one
 // holds the exponent and three bits more, which spreads weights of any size
 // over enough bins that few lanes meet in one.
@@ -53,6 +54,14 @@ __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t n;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
   return n;
+}
+
+// How many times four positions a thread has, of n over C CTAs with room for
+// `room` keys each.  A multiple of four would put eight lanes' 16-byte reads into
+// at most half of the banks: one more then, where it fits.
+__host__ __device__ inline int quads_of(long long n, int C, int room) {
+  const int q = (int)((n + 4LL * C * CHOOSE_THREADS - 1) / (4LL * C * CHOOSE_THREADS));
+  return q % 4 == 0 && (q + 1) * 4LL * CHOOSE_THREADS <= room ? q + 1 : q;
 }
 
 // One (layer, request, head) per cluster of one to four CTAs.  The `keep`-th
@@ -94,7 +103,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
   const int sink = min(a.sink, keep), recent = min(a.recent, keep - sink);
   const int middle = n - sink - recent;  // positions [sink, sink + middle) compete for the rest
   uint32_t want = keep - sink - recent;
-  const int per_warp = (int)(((long long)n + C * CHOOSE_WARPS * SPAN - 1) / (C * CHOOSE_WARPS * SPAN)) * SPAN;
+  const int run = 4 * quads_of(n, C, a.room), per_warp = 32 * run;
   const int start = (int)min((long long)n, (long long)(rank * CHOOSE_WARPS + warp) * per_warp);
   const int end = (int)min((long long)n, (long long)start + per_warp);
   const bool held = (long long)per_warp * CHOOSE_WARPS <= a.room;
@@ -114,20 +123,24 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
   auto keys_of = [&](int i) {
     return held ? *reinterpret_cast<const uint4*>(keys + warp * per_warp + i - start) : fetch(i);
   };
-  // f(base, position, keys) for this warp's positions, four a lane, in their order
-  auto each = [&](auto load, auto f) {
+  auto competes = [&](int i) { return (unsigned)(i - sink) < (unsigned)middle; };
+  // From the second pass on a lane looks at `run` positions in a row, which gives
+  // ranks by sums alone (with four of each 128 it took votes: 83 us against XXX,
+  // 24 layers of 43,968).  Where all of a warp's runs lie among the competing
+  // positions none is looked at alone.
+  const int my = min((long long)n, (long long)start + lane * run), my_end = min((long long)n, (long long)my + run);
+  const bool inside = __all_sync(~0u, my >= sink && my_end == my + run && my_end <= sink + middle);
+  // f(position, key) of this lane's in their order
+  auto own = [&](auto f) {
 #pragma unroll 2
-    for (int base = start; base < end; base += SPAN) {
-      const int i = base + lane * 4;
-      uint4 k = make_uint4(0, 0, 0, 0);
-      if (i < end) k = load(i);
-      f(base, i, k);
+    for (int i = my; i < my_end; i += 4) {
+      const uint4 k = keys_of(i);
+      f(i, k.x);
+      f(i + 1, k.y);
+      f(i + 2, k.z);
+      f(i + 3, k.w);
     }
   };
-  auto competes = [&](int i) { return (unsigned)(i - sink) < (unsigned)middle; };
-  // Spans that lie whole among the competing positions need no look at each one;
-  // the comparisons bound the kernel (its ALU pipe was 68 % busy with them all).
-  auto whole = [&](int base) { return base >= sink && base + SPAN <= min(end, sink + middle); };
   // The bin that holds the `want`-th key from the top, over all CTAs.  PER: bins a thread sums.
   auto find = [&](const uint32_t* bins, auto PER) {
     if (C > 1) cluster_sync();
@@ -174,10 +187,14 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
   uint32_t border = 0xffffffffu, ties = 0, ties_kept = 0;  // no key is above this border
   __syncthreads();
   // the first digit is counted as the keys come in
-  each(fetch, [&](int base, int i, uint4 k) {
+#pragma unroll 2
+  for (int base = start; base < end; base += SPAN) {
+    const int i = base + lane * 4;
+    uint4 k = make_uint4(0, 0, 0, 0);
+    if (i < end) k = fetch(i);
     if (held && i < end) *reinterpret_cast<uint4*>(keys + warp * per_warp + i - start) = k;
     const uint32_t x[4] = {k.x >> 20, k.y >> 20, k.z >> 20, k.w >> 20};
-    if (whole(base)) {
+    if (base >= sink && base + SPAN <= min(end, sink + middle)) {
       // all in one bin (weights that are all 0, say) add once: else they would queue
       const uint32_t first = __shfl_sync(~0u, x[0], 0);
       if (__all_sync(~0u, ((x[0] ^ first) | (x[1] ^ first) | (x[2] ^ first) | (x[3] ^ first)) == 0)) {
@@ -191,29 +208,42 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
       for (int e = 0; e < 4; ++e)
         if (i < end && competes(i + e)) atomicAdd(&hist[x[e]], 1u);
     }
-  });
+  }
+  __syncwarp();                          // the lanes read each other's keys from here on
   if (want > 0) {
     find(hist, std::integral_constant<int, 4>());
     border = found[0] << 20;
     want = found[1];
     __syncthreads();
-    // f(key) for the keys that compete
-    auto count = [&](uint32_t* bins, int above, int shift) {
-      each(keys_of, [&](int base, int i, uint4 k) {
-        const uint32_t x[4] = {k.x, k.y, k.z, k.w};
-        const bool all = whole(base);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if ((x[e] ^ border) >> above == 0 && (all || (i < end && competes(i + e)))) atomicAdd(&bins[x[e] >> shift & 1023], 1u);
-      });
-    };
-    count(hist + BINS1, 20, 10);
-    find(hist + BINS1, std::integral_constant<int, 1>());
+    uint32_t* bins = hist + BINS1;
+    own([&](int p, uint32_t x) {
+      const uint32_t d = x - border;
+      if (d < 1u << 20 && (inside || competes(p))) atomicAdd(&bins[d >> 10], 1u);
+    });
+    find(bins, std::integral_constant<int, 1>());
     border |= found[0] << 10;
     want = found[1];
     __syncthreads();
-    count(hist + BINS1 + BINS2, 10, 0);
-    find(hist + BINS1 + BINS2, std::integral_constant<int, 1>());
+    bins += BINS2;
+    if (inside) {
+      // few keys have the border's first two digits: one branch for four
+#pragma unroll 2
+      for (int i = my; i < my_end; i += 4) {
+        const uint4 k = keys_of(i);
+        const uint32_t d[4] = {k.x - border, k.y - border, k.z - border, k.w - border};
+        if (min(min(d[0], d[1]), min(d[2], d[3])) < 1024) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d[e] < 1024) atomicAdd(&bins[d[e]], 1u);
+        }
+      }
+    } else {
+      own([&](int p, uint32_t x) {
+        const uint32_t d = x - border;
+        if (d < 1024 && competes(p)) atomicAdd(&bins[d], 1u);
+      });
+    }
+    find(bins, std::integral_constant<int, 1>());
     border |= found[0];
     ties_kept = found[1];
     ties = found[2];
@@ -226,34 +256,28 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
     return __reduce_add_sync(~0u, lane < warp ? v : 0u);
   };
   static_assert(CHOOSE_WARPS == 32, "a lane per warp");
-  const unsigned below = (1u << lane) - 1;
-  // how many marks in lanes before this one, and in all, of four flags a lane
-  auto rank4 = [&](const bool (&f)[4], int& all) {
-    int mine = 0;
-    all = 0;
+  // The sum over the lanes before this one.
+  auto lanes_before = [&](int v) {
+    int inc = v;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const unsigned m = __ballot_sync(~0u, f[e]);
-      mine += __popc(m & below);
-      all += __popc(m);
+    for (int d = 1; d < 32; d *= 2) {
+      const int o = __shfl_up_sync(~0u, inc, d);
+      if (lane >= d) inc += o;
     }
-    return mine;
+    return inc - v;
   };
   // Of keys equal to the border the first `ties_kept` stay.
   const bool some_ties = ties != ties_kept;
   int tie0 = 0;
   if (some_ties) {
     int c = 0;
-    each(keys_of, [&](int, int i, uint4 k) {
-      const uint32_t x[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c += i < end && competes(i + e) && x[e] == border;
-    });
+    own([&](int p, uint32_t x) { c += x == border && competes(p); });
+    tie0 = lanes_before(c);
     c = __reduce_add_sync(~0u, c);
     if (lane == 0) cnt[warp] = c;
     __syncthreads();
     uint32_t all;
-    tie0 = warps_before(cnt, all);
+    tie0 += warps_before(cnt, all);
     if (tid == 0) total[0] = all;
     if (C > 1) {
       cluster_sync();
@@ -262,54 +286,64 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
     }
     __syncthreads();                     // everyone has read cnt
   }
-  // f(position, flags of keys that go / stay, whether those are holes, late ones) in order
-  const uint32_t lowest = some_ties || ties == 0 ? border + (border != 0xffffffffu) : border;   // stays, ties apart
-  auto marks = [&](auto f) {
-    int tie = tie0;
-    each(keys_of, [&](int base, int i, uint4 k) {
-      const uint32_t x[4] = {k.x, k.y, k.z, k.w};
-      bool flag[4];
-      if (!some_ties && whole(base) && (base + SPAN <= keep || base >= keep)) {
-        const bool hole = base < keep;
+  // Marks among the competing positions: below `keep` what goes (a hole), from there on
+  // what stays (a late survivor), which has to move.  The last `tail` positions, which
+  // all stay, are the last to move.
+  const int tail = min(recent, n - keep);
+  const bool among = my >= sink && my_end <= sink + middle, apart = my_end <= sink || my >= sink + middle;
+  const bool plain = __all_sync(~0u, apart || (among && !some_ties && (my_end <= keep || my >= keep) && my_end % 4 == 0));
+  const int last = apart ? my : my_end;
+  // marks of positions i .. i + 3, the first one's in bit 3
+  auto marks = [&](int i, int& tie, auto PLAIN) {
+    const uint4 k = keys_of(i);
+    const bool alike = PLAIN || (!some_ties && competes(i) && competes(i + 3) && (i >= keep) == (i + 3 >= keep));
+    if (alike) {
+      const uint32_t stay = (k.x >= border ? 8 : 0) | (k.y >= border ? 4 : 0) | (k.z >= border ? 2 : 0) | (k.w >= border ? 1 : 0);
+      return stay ^ ((PLAIN ? my : i) >= keep ? 0u : 15u);
+    }
+    const uint32_t x[4] = {k.x, k.y, k.z, k.w};
+    uint32_t bits = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) flag[e] = (x[e] < lowest) == hole;
-        f(i, flag, hole, !hole);
-        return;
-      }
-      bool eq[4], late[4];
-      int rank_eq = 0, all = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) eq[e] = some_ties && i < end && competes(i + e) && x[e] == border;
-      if (some_ties) rank_eq = tie + rank4(eq, all);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int p = i + e;
-        bool stays = !competes(p) || x[e] >= lowest;
-        if (eq[e]) stays = rank_eq < (int)ties_kept;
-        rank_eq += eq[e];
-        flag[e] = p < keep && !stays && i < end;
-        late[e] = p >= keep && p < n && stays && i < end;
-      }
-      tie += all;
-      f(i, flag, true, false);
-      f(i, late, false, true);
-    });
+    for (int e = 0; e < 4; ++e) {
+      const int p = i + e;
+      const bool in = competes(p), stays = x[e] > border || (x[e] == border && in && (!some_ties || tie++ < (int)ties_kept));
+      if (in && stays == (p >= keep)) bits |= 8 >> e;
+    }
+    return bits;
   };
-  int holes = 0, lates = 0;
-  marks([&](int, const bool (&flag)[4], bool hole, bool late) {
-    const int c = flag[0] + flag[1] + flag[2] + flag[3];
-    if (hole) holes += c;
-    if (late) lates += c;
-  });
-  holes = __reduce_add_sync(~0u, holes);
-  lates = __reduce_add_sync(~0u, lates);
+  const std::true_type PLAIN;
+  const std::false_type MIXED;
+  int holes = 0, lates = 0, tie = tie0;
+  uint64_t mark = 0;                     // of this lane's positions, the first one's in the highest bit
+  static_assert(ROOM_MAX / CHOOSE_THREADS <= 64, "a mask of a lane's positions");
+  if (held) {
+    if (plain) {
+#pragma unroll 2
+      for (int i = my; i < last; i += 4) mark = mark << 4 | marks(i, tie, PLAIN);
+    } else {
+#pragma unroll 1
+      for (int i = my; i < last; i += 4) mark = mark << 4 | marks(i, tie, MIXED);
+    }
+    if (last > my) mark <<= 64 - (last - my + 3) / 4 * 4;
+    const int before_keep = max(0, keep - my);             // positions, 0 to all
+    holes = __popcll(before_keep >= 64 ? mark : mark & ~(~0ull >> before_keep));
+    lates = __popcll(mark) - holes;
+  } else {
+    for (int i = my; i < last; i += 4) {
+      const uint32_t b = marks(i, tie, MIXED), h = i >= keep ? 0 : keep - i >= 4 ? b : b & ~(15u >> (keep - i));
+      holes += __popc(h);
+      lates += __popc(b ^ h);
+    }
+  }
+  const int holes0 = lanes_before(holes), lates0 = lanes_before(lates);
+  const int warp_holes = __reduce_add_sync(~0u, holes), warp_lates = __reduce_add_sync(~0u, lates);
   if (lane == 0) {
-    cnt[warp] = holes;
-    late_cnt[warp] = lates;
+    cnt[warp] = warp_holes;
+    late_cnt[warp] = warp_lates;
   }
   __syncthreads();
   uint32_t all_holes, all_lates;
-  int hole_at = warps_before(cnt, all_holes), late_at = warps_before(late_cnt, all_lates);
+  int hole_at = warps_before(cnt, all_holes), late_at = warps_before(late_cnt, all_lates);    // of this warp
   int moves = (int)all_holes;
   if (C > 1) {
     if (tid == 0) {
@@ -323,17 +357,41 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
     hole_at += __reduce_add_sync(~0u, lane < rank ? vh : 0u);
     late_at += __reduce_add_sync(~0u, vl);
   }
-  marks([&](int i, const bool (&flag)[4], bool hole, bool) {
-    int32_t* to = hole ? dst : src;
-    int all, x = (hole ? hole_at : late_at) + rank4(flag, all);
-    if (hole) hole_at += all;
-    else late_at += all;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (flag[e] && x < a.max_moves) to[x] = i + e;
-      x += flag[e];
+  if (held) {
+    // through shared memory, in the place of this warp's keys: each lane's own are
+    // scattered (16 % slower with 60,000 keys)
+    int32_t* list = reinterpret_cast<int32_t*>(keys + warp * per_warp);
+    const int to_late = warp_holes + lates0 - holes;       // a lane's holes come before its late survivors
+    int c = 0;
+    __syncwarp();
+    for (uint64_t m = mark; m; ++c) {
+      const int x = __clzll((long long)m);
+      list[c + (c < holes ? holes0 : to_late)] = my + x;
+      m &= ~(1ull << 63 >> x);
     }
-  });
+    __syncwarp();
+    for (int x = lane; x < warp_holes; x += 32)
+      if (hole_at + x < a.max_moves) dst[hole_at + x] = list[x];
+    for (int x = lane; x < warp_lates; x += 32)
+      if (late_at + x < a.max_moves) src[late_at + x] = list[warp_holes + x];
+  } else {
+    hole_at += holes0;
+    late_at += lates0;
+    tie = tie0;
+    for (int i = my; i < last; i += 4) {
+      const uint32_t b = marks(i, tie, MIXED);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool on = b >> (3 - e) & 1, late = i + e >= keep;
+        const int at = late ? late_at : hole_at;
+        if (on && at < a.max_moves) (late ? src : dst)[at] = i + e;
+        late_at += late && on;
+        hole_at += !late && on;
+      }
+    }
+  }
+  for (int x = rank * CHOOSE_THREADS + tid; x < tail; x += C * CHOOSE_THREADS)
+    if (moves - tail + x < a.max_moves) src[moves - tail + x] = n - tail + x;
   if (rank == 0 && tid == 0) {
     if (moves > a.max_moves) report_status(a.ctl, ST_BAD_LENGTH);
     a.counts[row] = min(moves, a.max_moves);
@@ -607,8 +665,7 @@ extern "C" int qvggt_evict_plan(const qvggt_evict_plan_args* p, void* stream) {
   // each, 21 as four; 128 rows of 8,000: 11.5 and 24).  Eight CTAs to a cluster
   // only halve how many run at once (16 rows: 40 us).
   while (C < 4 && 2 * rows * C <= device_info().num_sms && longest > 8192LL * C) C *= 2;
-  const int64_t part = (longest + C * CHOOSE_WARPS * SPAN - 1) / (C * CHOOSE_WARPS * SPAN) * (CHOOSE_WARPS * SPAN);
-  constexpr int ROOM_MAX = 48 * 1024;    // 192 KB of keys beside 25 KB of counts
+  const int64_t part = quads_of(longest, C, ROOM_MAX) * 4LL * CHOOSE_THREADS;
   const int room = part <= ROOM_MAX ? (int)part : 0;
   ChooseArgs a{p->weights, p->block_tables, p->lens, p->keep, p->src, p->dst, p->counts, (int)p->requests,
                (int)p->kv_heads, (int)p->max_blocks, (int)p->num_blocks, log2_of(p->block_size),
