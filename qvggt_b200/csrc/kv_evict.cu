@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
   };
   auto competes = [&](int i) { return (unsigned)(i - sink) < (unsigned)middle; };
   // From the second pass on a lane looks at `run` positions in a row, which gives
-  // ranks by sums alone (with four of each 128 it took votes: 83 us against XXX,
+  // ranks by sums alone (with four of each 128 it took votes: 83 us against 57,
   // 24 layers of 43,968).  Where all of a warp's runs lie among the competing
   // positions none is looked at alone.
   const int my = min((long long)n, (long long)start + lane * run), my_end = min((long long)n, (long long)my + run);

@@ -416,23 +416,22 @@ def prompt_attention(q, k, v, cu, max_len: int, causal_chunk: int = 0, scale: fl
         _check_cuda(name, q, k, v, cu)
     dt = _half(name, q, "q")
     sq, sk, sv = _rows3(name, q, "q"), _rows3(name, k, "k"), _rows3(name, v, "v")
-    _check_dtype(name, k, q.dtype)
-    _check_dtype(name, v, q.dtype)
+    if not q.dtype is k.dtype is v.dtype:
+        raise TypeError(f"{name}: q, k and v must have one type, got {q.dtype}, {k.dtype} and {v.dtype}")
     T, hq, d = q.shape
-    shape = k.shape
-    if shape[0] != T or shape[2] != d or v.shape != shape:
+    Tk, hk, dk = shape = k.shape
+    if Tk != T or dk != d or v.shape != shape:
         raise ValueError(f"{name}: k {tuple(shape)} and v {tuple(v.shape)} must be [{T}, kv_heads, {d}]")
-    hk = shape[1]
     _ints(name, cu, "cu")
     B = cu.numel() - 1
     if B < 0:
         raise ValueError(f"{name}: cu must hold the running sums of the lengths, from 0 on")
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = q.new_empty((T, hq, d))
         so = (hq * d, d)
     else:
         so = _out3(name, out, q, dev, "out")
-    lse_at = _lse_at(name, lse, q, dev, hq, T)
+    lse_at = 0 if lse is None else _lse_at(name, lse, q, dev, hq, T)
     nbytes = _prompt_scratch(dev, T, hq, hk, B, max_len, d)
     scratch_at = scratch_len = 0
     if scratch is not None:
