@@ -43,6 +43,7 @@ struct RowBlock {
   int q0, ql, n, tok0, nqt, tiles;       // tok0: first row (token * group + head)
   long long cost;
   __device__ __forceinline__ int tile_cost() const { return 1; }
+  __device__ __forceinline__ int start() const { return START; }
   __device__ __forceinline__ RowBlock() {}
   __device__ __forceinline__ RowBlock(const CacheAttnArgs& a, int b, int qb) {
     q0 = a.cu_q[b];

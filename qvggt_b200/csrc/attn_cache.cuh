@@ -235,7 +235,7 @@ struct PieceWalk {
         load(a, blocks);
         continue;
       }
-      const long long s0 = s + h * blk.cost, k0 = s0 + Blk::START;        // the item, its first tile
+      const long long s0 = s + h * blk.cost, k0 = s0 + blk.start();      // the item, its first tile
       if (s0 >= end) return false;
       const int head = h++;
       const int c = blk.tile_cost();

@@ -170,6 +170,7 @@ struct Block {
   int q0, ql, n, tok0, nqt, tiles;
   long long cost;                        // of one kv head; 0: no such block
   __device__ __forceinline__ int tile_cost() const { return nqt == 2 ? COST_TILE2 : COST_TILE1; }
+  __device__ __forceinline__ int start() const { return START; }
   __device__ __forceinline__ Block() {}
   __device__ __forceinline__ Block(const CacheAttnArgs& a, int b, int qb) {
     q0 = a.cu_q[b];

@@ -41,10 +41,12 @@ constexpr int SEGS = 4;         // segments handed out ahead
 constexpr int SEG_READERS = 12; // producer, two issuers, the V tiles' warp, 8 warps
 constexpr int Q_ROWS = 256;     // rows of an item
 // Cost of an item on the line, in tenths of a tile with two Q tiles: a start-up
-// (loads, first products, epilogue) and its key tiles.  (A start of 30 costs four
-// streams of one to six frames 1 % more, 20 costs them 3 % and causal sequences
-// of 400 to 4,099 tokens 10 %.)
-constexpr int COST_START = 50, COST_TILE2 = 10, COST_TILE1 = 9;
+// (loads, first products, epilogue), its key tiles, and again those that its first
+// row does not see to their end (their V is looked through, their scores hidden).
+// By fits of equal items: 2 to 2.5 tiles, and 0.5 to 1 for each such tile.  Against a
+// start of 50 for all items: nine causal sequences to 4,099, 32 / 8 heads x 128 540 ->
+// 525 us, four streams of one to six frames, 16 x 128 666 -> 632, 16 x 64 the same.
+constexpr int COST_START = 20, COST_TILE2 = 10, COST_TILE1 = 9, COST_MASKED = 10;
 // No piece is cut shorter than this (8 tiles): a join costs about as much.
 constexpr int COST_MIN = COST_START + 8 * COST_TILE2;
 constexpr uint32_t TMEM_COLS = 512;
@@ -177,10 +179,11 @@ __device__ __forceinline__ bool sequence_ok(const PromptArgs& a, int q0, int ql)
 template <int KT>
 struct Block {
   using Args = PromptArgs;
-  static constexpr int START = COST_START, MIN = COST_MIN;
-  int q0, ql, n, tok0, nqt, tiles;
+  static constexpr int MIN = COST_MIN;
+  int q0, ql, n, tok0, nqt, tiles, masked;
   long long cost;                        // of one kv head; 0: no such block
   __device__ __forceinline__ int tile_cost() const { return nqt == 2 ? COST_TILE2 : COST_TILE1; }
+  __device__ __forceinline__ int start() const { return COST_START + masked * COST_MASKED; }
   __device__ __forceinline__ Block() {}
   __device__ __forceinline__ Block(const PromptArgs& a, int b, int qb) {
     q0 = a.cu[b];
@@ -188,12 +191,13 @@ struct Block {
     const int tpt = 128 / a.group;       // tokens of a Q tile
     tok0 = qb * 2 * tpt;
     nqt = tok0 + tpt < ql ? 2 : 1;
-    tiles = 0;
+    tiles = masked = 0;
     cost = 0;
     // (a negative length is for sequence_ok to report)
     if ((ql >= 0 && tok0 >= ql) || !sequence_ok(a, q0, ql)) return;
     tiles = (key_limit(min(ql, tok0 + 2 * tpt) - 1, ql, n, a.chunk) + KT - 1) / KT;
-    cost = COST_START + (long long)tiles * tile_cost();
+    masked = tiles - key_limit(tok0, ql, n, a.chunk) / KT;
+    cost = start() + (long long)tiles * tile_cost();
   }
 };
 
