@@ -241,6 +241,23 @@ def test_evict_plan(kc, layers, H, bs, lens, part, sink, recent, hint):
     check_choice(kc, odd, table, lens, keep, sink, recent, hint=hint)
 
 
+@pytest.mark.parametrize("n,bs", [(1, 32), (3, 32), (4095, 32), (4097, 64), (16383, 128), (16384, 32), (16387, 64), (45056, 128),
+                                  (45059, 32), (49152, 64), (49153, 64), (65541, 128)])
+def test_evict_plan_borders_between_lanes(kc, n, bs):
+    """Lengths about a multiple of what a thread, a CTA or its shared memory takes, with `sink`, `recent` and `keep` that end
+    inside a quad of positions, on its edge, and past one another; weights all different, and of five values."""
+    rng = np.random.default_rng(n)
+    table, num = random_table(rng, [n], bs)
+    w = rng.permutation(num * bs).astype(np.float32).reshape(1, num, 1, bs) - num
+    few = rng.integers(0, 5, w.shape).astype(np.float32)
+    for sink, recent, keep in ((0, 0, n // 2), (5, 7, n - 1), (n // 3 + 1, n // 4, n * 3 // 4), (n // 2, n, n - n // 5),
+                               (1, 1, min(n, 2)), (2, 1, min(n - 1, 6)), (0, n // 2, n // 3), (n, 0, n // 7 + 1)):
+        if keep >= n:
+            continue
+        check_choice(kc, w, table, [n], [keep], sink, recent)
+        check_choice(kc, few, table, [n], [keep], sink, recent)
+
+
 def test_evict_plan_longer_than_shared_memory(kc):
     """More keys than four CTAs hold: they are read again for each digit."""
     rng = np.random.default_rng(1)

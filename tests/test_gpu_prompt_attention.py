@@ -117,6 +117,32 @@ def test_strides_scale_and_scratch(kc, D, hq, hk):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,hq,hk", [(64, 2, 2), (64, 8, 2), (128, 2, 2), (128, 12, 4)])
+@pytest.mark.parametrize("longest", [63, 64, 65, 128, 129])
+def test_lengths_about_one_tile(kc, dtype, D, hq, hk, longest):
+    """Tiles of 64 and of 128 keys, full and not, with NaN where a token does not look; both paths of the same rows."""
+    lens = [longest, 1, longest // 2, longest - 1]
+    T = sum(lens)
+    q, k, v = inputs(longest + hq, T, hq, hk, D, dtype)
+    cu = cu_of(lens)
+    for chunk in (0, 1, 16):
+        lse = torch.empty(hq, T, device="cuda")
+        got = kc.prompt_attention(q, k, v, ints(cu), longest, chunk, lse=lse)
+        want = oe.prompt_attention(q, k, v, cu, chunk)
+        check(got, lse, want, dtype, float(v.abs().max()), longest)
+        # a hint that asks for 128-key tiles
+        check(kc.prompt_attention(q, k, v, ints(cu), 200, chunk, lse=lse), lse, want, dtype, float(v.abs().max()), longest)
+        if chunk == 0:
+            continue
+        at = longest // 2 // chunk * chunk
+        k2, v2 = k.clone(), v.clone()
+        k2[at:longest], v2[at:longest] = math.nan, math.nan
+        bad = kc.prompt_attention(q, k2, v2, ints(cu), longest, chunk)
+        assert torch.equal(bad[:at], got[:at]) and torch.equal(bad[longest:], got[longest:])
+        assert torch.isnan(bad[at:longest]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D,chunk,n,hq", [(64, 40, 200, 2), (128, 1, 150, 1), (64, 1374, 2748, 1), (64, 64, 1500, 4),
                                           (128, 500, 1800, 2)])
 def test_what_a_token_does_not_see(kc, dtype, D, chunk, n, hq):
