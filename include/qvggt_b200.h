@@ -551,10 +551,13 @@ int qvggt_kv_evict(const qvggt_kv_evict_args* args, void* stream);
  * Mask: causal_chunk 0: every token sees its whole sequence; c > 0: token i sees
  * tokens j < (i / c + 1) * c (1: causal; the tokens of a frame: its own and all
  * earlier frames).  What a token does not see adds nothing to it, NaN and
- * infinities among it.  Rows outside cu are left as they are.  lse (fp32
- * [q_heads][T], may be NULL): ln sum_j exp(scale q.k_j).
+ * infinities and the largest finite values among it.  Rows outside cu are left as
+ * they are.  lse (fp32 [q_heads][T], may be NULL): ln sum_j exp(scale q.k_j).
  * scale: above 1e-30, at most 1e30.  Sums, maxima and products are held in fp32;
- * the weights are rounded to the inputs' type for the product with V.
+ * the weights are rounded to the inputs' type for the product with V, and one
+ * under 2^-125 of the row's largest counts as 0.  The product is divided by the
+ * sum of the weights last, which are up to 2^8 each: bf16 values near fp32's
+ * largest, seen with such weights, can overflow it.
  * scratch: qvggt_prompt_attention_scratch() bytes (0 for some shapes), 16-byte
  * aligned; calls that may overlap on the GPU may not share it.  A sequence
  * outside [0, T) or longer than max_len is skipped and sets the device status

@@ -81,8 +81,11 @@ __device__ __forceinline__ void reg_fence(uint32_t (&s)[N]) {
 // x = n + f, n = round(x), f in [-1/2, 1/2]; 2^f by a degree-3 polynomial
 // fitted to minimise the relative error on [-1/2, 1/2] (max 7.5e-5, well under
 // the fp16 rounding P gets afterwards); 2^n added into the exponent field).
-// Arguments are clamped at -125 so 2^n stays a normal float; those values
-// round to 0 in fp16 anyway.
+// Arguments are clamped at -125 so 2^n stays a normal float: what is under it,
+// -inf among it, gives 2^-125.  That rounds to 0 in fp16, but not in bf16, where a
+// hidden key (-inf) would weigh 2^-125 of V's up to 2^128: ZERO gives 0 there, and
+// whoever rounds to more than fp16's exponents has to ask for it.
+template <bool ZERO = false>
 __device__ __forceinline__ void exp2_poly_pair(uint64_t x2, float& p0, float& p1) {
   const uint64_t MAGIC = f2_pack(12582912.0f, 12582912.0f);        // 1.5 * 2^23: rounds to an integer
   const uint64_t NEG_MAGIC = f2_pack(-12582912.0f, -12582912.0f);
@@ -103,6 +106,10 @@ __device__ __forceinline__ void exp2_poly_pair(uint64_t x2, float& p0, float& p1
   f2_unpack(t, t0, t1);
   p0 = __int_as_float(__float_as_int(q0) + (__float_as_int(t0) << 23));
   p1 = __int_as_float(__float_as_int(q1) + (__float_as_int(t1) << 23));
+  if (ZERO) {
+    p0 = x0 < -125.f ? 0.f : p0;
+    p1 = x1 < -125.f ? 0.f : p1;
+  }
 }
 
 // One lane of a converged warp, the same one every time.

@@ -17,11 +17,12 @@
 // The running maximum is raised lazily (2^8).  All waits are bounded; on expiry
 // every role leaves and the status word is set.
 //
-// What a row does not see must not reach it.  Its scores become -inf, its
-// weights 0, but 0 times an infinity or NaN of V would still be NaN.  So in the
-// tiles that the block's first row does not see to their end, rows of V past the
-// sequence become 0 and elements that are not finite become 0; where one was,
-// the rows that do see it add it at the end (add_odd).
+// What a row does not see must not reach it.  Its scores become -inf and its
+// weights exactly 0, which is all that keeps finite V out, the next sequence's in
+// the last tile among it.  But 0 times an infinity or NaN of V would still be NaN.
+// So the tiles that the block's first row does not see to their end are looked
+// through, and where one holds such an element, these and its rows past the
+// sequence become 0; the rows that do see the element add it at the end (add_odd).
 //
 // TMEM columns: S_i at i KT, P_i at 2 KT + i KT / 2, O_i at 512 - (2 - i) D.  With
 // head_dim 128 and 128-key tiles that is 128 columns too many: S_0 and S_1 take
@@ -126,7 +127,7 @@ __device__ __forceinline__ void exp_chunk(uint32_t (&s)[KT], uint64_t c2, uint64
     const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), c2, nm2);
     float p0, p1;
     if ((e & 7) < POLY) {
-      exp2_poly_pair(x2, p0, p1);
+      exp2_poly_pair<BF16>(x2, p0, p1);                    // (bf16 holds the 2^-125 of hidden keys)
     } else {
       float x0, x1;
       f2_unpack(x2, x0, x1);
@@ -629,7 +630,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         float lj = 0.f;
         // (the previous item's epilogue has waited for its last PV product.)  Two of 16
         // exponentials on the FMA pipe with head_dim 64, whose limit the others are; with
-        // 128 none (two sequences of 8,192: 955 us, 990 with two)
+        // 128 none (two sequences of 8,192: 955 us, 990 with two).  With bf16 they pay for
+        // the select to 0 too (four streams of one to six frames, 16 x 64: 483 us, 491
+        // with none, 470 with fp16, which needs no select)
         if (!exp_store<BF16, D == 64 ? 1 : 0>(s, c, neg_m, lj, tP, j == 0, bar_o_done, (cnt - 1) & 1, tries)) { ok = false; break; }
         ready = j + 1 < ntr && test(bar_s_full, (cnt + 1) & 1);
         l = l * alpha + lj;

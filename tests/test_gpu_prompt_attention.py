@@ -180,6 +180,42 @@ def test_what_a_token_does_not_see(kc, dtype, D, chunk, n, hq):
         assert torch.equal(torch.isnan(got[:n]), torch.isnan(ref))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,hq,chunk", [([40, 17], 1, 1), ([60, 3], 2, 16), ([100, 100, 100], 1, 1), ([200, 90], 4, 40),
+                                           ([700, 60], 1, 274), ([1500, 90], 1, 64), ([2100, 700], 2, 1)])
+def test_the_largest_values_that_a_token_does_not_see(kc, dtype, D, lens, hq, chunk):
+    """The largest finite values of V in later chunks, in the next sequence and behind the last one leave a token's bits as
+    they are: 2^-125 of them would be 8."""
+    T, n = sum(lens), lens[0]
+    q, k, v = inputs(T + D, T + 50, hq, 1, D, dtype)
+    cu, big = ints(cu_of(lens)), torch.finfo(dtype).max
+    base_lse, lse = (torch.zeros(hq, T + 50, device="cuda") for _ in range(2))
+    base = kc.prompt_attention(q, k, v, cu, max(lens), chunk, out=torch.zeros_like(q), lse=base_lse)
+    for at, end in ((T, T + 50), (n, T + 50), (n // 2 // chunk * chunk, n), (0, n)):
+        v2 = v.clone()
+        v2[at:end, :, ::2], v2[at:end, :, 1::2] = big, -big
+        got = kc.prompt_attention(q, k, v2, cu, max(lens), chunk, out=torch.zeros_like(q), lse=lse)
+        assert torch.equal(got[:at], base[:at]) and torch.equal(got[end:], base[end:]) and torch.equal(lse, base_lse)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,chunk", [(60, 0), (60, 1), (200, 0), (200, 1), (1300, 16)])
+def test_weights_too_small_to_count(kc, dtype, D, n, chunk):
+    """Keys that a token sees with weights under 2^-500, and the largest finite values of V: 0 in 64 bits too.  (They take
+    no part in the bound's steps below fp16's normal range: what is under half such a step is 0.)"""
+    q, k, v = inputs(n + D, n, 1, 1, D, dtype)
+    q[..., 0], k[..., 0] = 8, 0
+    most = float(v.abs().max())
+    far, big = slice(5, None, 7), torch.finfo(dtype).max
+    k[far, :, 0] = -600                  # times 8 log2(e) / sqrt(head_dim): -612 at least, the other dims give some +-10
+    v[far, :, ::2], v[far, :, 1::2] = big, -big
+    lse = torch.empty(1, n, device="cuda")
+    got = kc.prompt_attention(q, k, v, ints([0, n]), n, chunk, lse=lse)
+    check(got, lse, oe.prompt_attention(q, k, v, [0, n], chunk), dtype, most, n)
+
+
 def test_one_token_of_any_stride_and_out_in_place_of_q(kc):
     """The stride of an axis of length one means nothing; the result may take the queries' place."""
     for T, hq, hk in ((1, 4, 2), (1, 1, 1), (300, 1, 1)):
