@@ -553,8 +553,10 @@ int qvggt_kv_evict(const qvggt_kv_evict_args* args, void* stream);
  * earlier frames).  What a token does not see adds nothing to it, NaN and
  * infinities and the largest finite values among it.  Rows outside cu are left as
  * they are.  lse (fp32 [q_heads][T], may be NULL): ln sum_j exp(scale q.k_j).
- * scale: above 1e-30, at most 1e30.  Sums, maxima and products are held in fp32;
- * the weights are rounded to the inputs' type for the product with V, and one
+ * scale: above 1e-30, at most 1e30.  Sums, maxima and products are held in fp32:
+ * a row that sees a score of NaN or, scaled and times log2 e, above 2^27 (fp16) or
+ * 2^31 (bf16) is NaN, and its largest should not be under the negatives of these.
+ * The weights are rounded to the inputs' type for the product with V, and one
  * under 2^-125 of the row's largest counts as 0.  The product is divided by the
  * sum of the weights last, which are up to 2^8 each: bf16 values near fp32's
  * largest, seen with such weights, can overflow it.

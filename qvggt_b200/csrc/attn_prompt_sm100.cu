@@ -612,11 +612,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (lane == 0) arrive(bar_s_free);
         const int valid = left - j * KT;                   // keys of the tile that the row sees (may be <= 0)
         if (__any_sync(~0u, valid < KT)) hide_keys(s, valid);
-        const float top = tile_max(s);
-        // a score that is NaN or +inf makes the row NaN (the exponentials alone
-        // would not: the polynomial's clamp drops NaN)
-        if (!(top <= 3.4028234663852886e38f)) l = __int_as_float(0x7fffffff);
-        const float mx = fmaxf(m_used, top * c);
+        const float top = tile_max(s) * c;
+        // A score that is NaN makes the row NaN (the exponentials alone would not: the
+        // polynomial's clamp drops NaN).  So does one past 2^27 or 2^31: the maximum m is
+        // rounded, so x - m of the largest score is off by up to m 2^-25, and 2^4 beside
+        // the lazy maximum's 2^8, or 2^64, is what P's type holds either way (past that
+        // a row would become 0 in silence).
+        if (!(top <= (BF16 ? 2147483648.f : 134217728.f))) l = __int_as_float(0x7fffffff);
+        const float mx = fmaxf(m_used, top);
         const bool need = mx > m_used + 8.0f;
         float alpha = 1.f;
         bool rescale = false;

@@ -216,6 +216,40 @@ def test_weights_too_small_to_count(kc, dtype, D, n, chunk):
     check(got, lse, oe.prompt_attention(q, k, v, [0, n], chunk), dtype, most, n)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,lens", [(64, [50, 40]), (128, [50, 40]), (64, [200, 90]), (128, [200, 90]), (64, [1500, 90])])
+def test_scores_of_any_size(kc, dtype, D, lens):
+    """A row with scaled scores up to 2^27 (fp16) and 2^31 (bf16) is a mean of what it sees; above, where the weights' type
+    may hold none of them, it is NaN, not 0.  Either way the other rows keep theirs."""
+    T, n = sum(lens), lens[0]
+    q, k, v = inputs(T, T, 1, 1, D, dtype)
+    at, cu = n // 2, [0, n, T]
+    want = kc.prompt_attention(q, k, v, ints(cu), max(lens), 1)
+    for x, ok in ((2048 if dtype is torch.float16 else 8192, True), (60000, False)):
+        # 64 2048^2 log2(e) / 8 = 2^25.5, 64 8192^2 log2(e) / 8 = 2^29.5, half a power more with 128; 60000: over 2^35
+        q[at:n], k[at:n] = x, x
+        lse = torch.zeros(1, T, device="cuda")
+        got = kc.prompt_attention(q, k, v, ints(cu), max(lens), 1, lse=lse)
+        assert torch.equal(got[:at], want[:at]) and torch.equal(got[n:], want[n:]) and torch.isfinite(got[:at]).all()
+        if not ok:
+            assert torch.isnan(got[at:n]).all() and torch.isnan(lse[0, at:n]).all()
+            continue
+        ref = oe.prompt_attention(q, k, v, cu, 1)
+        # log-sum-exps of some 10^7 to 10^9: five roundings (scale, maximum, sum, ln 2 and the product), 2^-24 each
+        lse, far = lse.double(), ref[1][0, at:n]
+        assert ((lse[0, at:n] - far).abs() <= 2.0 ** -21 * far.abs()).all()
+        lse[0, at:n] = far
+        near = got.clone()
+        if n > 1024:
+            # Items are cut, and the parts joined by log-sum-exps that fp32 holds to 2 and more at this size: any mean of
+            # what a row sees among the large scores, whose rows weigh the same, may be the result.
+            low, high = (f(v[at:n], 0).values for f in (torch.cummin, torch.cummax))
+            step = 2 * U[dtype] * v.abs().max()
+            assert (got[at:n] >= low - step).all() and (got[at:n] <= high + step).all()
+            near[at:n] = ref[0][at:n].to(dtype)
+        check(near, lse, ref, dtype, float(v.abs().max()), n)
+
+
 def test_one_token_of_any_stride_and_out_in_place_of_q(kc):
     """The stride of an axis of length one means nothing; the result may take the queries' place."""
     for T, hq, hk in ((1, 4, 2), (1, 1, 1), (300, 1, 1)):
