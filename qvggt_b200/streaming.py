@@ -96,8 +96,13 @@ class StreamingRunner(AggregatorRunner):
 
     @property
     def seen(self) -> int:
-        """Frames so far, of the stream that has most."""
+        """Frames so far, of the stream that has most.  Assigned, it holds for every stream, and for what the cache holds."""
         return max(self._seen)
+
+    @seen.setter
+    def seen(self, frames: int) -> None:
+        self._seen = [frames] * self.streams
+        self._held = [min(frames, self.max_frames)] * self.streams
 
     def _positions(self, counts):
         """(time, height, width) of the tokens of `counts` frames of each stream, times from 0 on."""

@@ -222,3 +222,24 @@ def test_python_refuses_cpu_tensors_and_bad_streams():
     for counts, match in [([2], "streams"), ([2, -1], "streams"), ([4, 0], "streams"), ([0, 0], "streams"), ([2, 1], "tokens")]:
         with pytest.raises(ValueError, match=match):
             run.prompt(x, counts)
+
+
+def test_the_frames_so_far_can_be_set():
+    """`seen` is read and assigned, as by a program that restores or clears the cache itself; it counts for the room left."""
+    from qvggt_b200.aggregator import AggConfig
+    from qvggt_b200.streaming import StreamingRunner
+    cfg = AggConfig(depth=0, tokens_per_frame=25, grid_w=5)
+    run = StreamingRunner(cfg, [], [], 1, 3, "cpu", streams=2)
+    assert run.seen == 0
+    run.seen = 3
+    assert run.seen == 3
+    x = torch.zeros(2, 25, cfg.dim).half()
+    with pytest.raises(ValueError, match="3 are in it"):
+        run.step(x)
+    with pytest.raises(ValueError, match="3 frames were before it"):
+        run.prompt(x, [1, 1])
+    run.seen = 0
+    assert run.seen == 0
+    run = StreamingRunner(cfg, [], [], 1, 3, "cpu", sink_frames=1)
+    run.seen = 7                         # frames that have gone since are not in the cache
+    assert run.seen == 7 and run._held == [3]
