@@ -207,12 +207,14 @@ class StreamingAggregator(VGGTAggregator):
 
     Takes :class:`VGGTAggregator`'s arguments (the weights and configuration
     are the same) plus ``max_frames``, ``time_axis`` and, to go on when the cache
-    is full, ``sink_frames`` and ``recent_frames`` (see
+    is full, ``sink_frames``, ``recent_frames`` and ``weight_decay`` (see
     :class:`StreamingRunner`); one GPU, one stream."""
 
     def __init__(self, cfg, pe, agg_specials, frame_blocks, global_blocks, frames: int, device, max_frames: int,
-                 time_axis: bool = False, img_hw=(518, 518), sink_frames: int | None = None, recent_frames: int = 0):
-        self._stream_args = dict(time_axis=time_axis, sink_frames=sink_frames, recent_frames=recent_frames)
+                 time_axis: bool = False, img_hw=(518, 518), sink_frames: int | None = None, recent_frames: int = 0,
+                 weight_decay: float = 1.0):
+        self._stream_args = dict(time_axis=time_axis, sink_frames=sink_frames, recent_frames=recent_frames,
+                                 weight_decay=weight_decay)
         self._max_frames = max_frames
         super().__init__(cfg, pe, agg_specials, frame_blocks, global_blocks, frames, device, img_hw=img_hw)
 

@@ -243,3 +243,21 @@ def test_the_frames_so_far_can_be_set():
     run = StreamingRunner(cfg, [], [], 1, 3, "cpu", sink_frames=1)
     run.seen = 7                         # frames that have gone since are not in the cache
     assert run.seen == 7 and run._held == [3]
+
+
+def test_streaming_aggregator_passes_the_runners_arguments(monkeypatch):
+    """Windows and decay reach the runner."""
+    from qvggt_b200.aggregator import AggConfig, VGGTAggregator
+    from qvggt_b200.streaming import StreamingAggregator
+
+    def init(self, cfg, pe, specials, frame_blocks, global_blocks, frames, device, img_hw):
+        self.runner = self._make_runner(cfg, frame_blocks, global_blocks, frames, device, None, 1, 0)
+
+    monkeypatch.setattr(VGGTAggregator, "__init__", init)
+    cfg = AggConfig(depth=0, tokens_per_frame=25, grid_w=5)
+    run = StreamingAggregator(cfg, None, None, [], [], 1, "cpu", max_frames=4, sink_frames=2, recent_frames=1,
+                              weight_decay=0.9).runner
+    assert (run.max_frames, run.sink_frames, run.recent_frames, run.weight_decay) == (4, 2, 1, 0.9)
+    assert StreamingAggregator(cfg, None, None, [], [], 1, "cpu", max_frames=4).runner.weight_decay == 1
+    with pytest.raises(ValueError, match="weight_decay"):
+        StreamingAggregator(cfg, None, None, [], [], 1, "cpu", max_frames=4, sink_frames=2, weight_decay=2.0)
