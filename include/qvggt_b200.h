@@ -463,7 +463,9 @@ int qvggt_cached_attention_scratch(int64_t Tq, int32_t q_heads, int32_t kv_heads
  * may hold anything.
  * weights, out fp32 [num_blocks][kv_heads][block_size], the cache's order, and
  * may be the same; places that hold no key of a request are left as they are.
- * lse fp32 [q_heads][Tq] as the attention over the same keys gives it; a row
+ * lse fp32 [q_heads][Tq] as the attention over the same keys gives it (a row then
+ * hands out 1 in all; over the keys before they were rounded to codes, e^d times
+ * more or less at most, d being what the rounding may change a score by); a row
  * whose lse is not finite (no key, or NaN) counts for nothing.  q, cu_q, kv_lens,
  * block_tables, max_q, max_kv, causal_chunk, scale as in qvggt_cached_attention;
  * requests have their own blocks.  decay: 0 to 1.  Sums are held in fp32 and

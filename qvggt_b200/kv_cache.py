@@ -468,8 +468,10 @@ def key_weights(q, k_cache, k_scale, block_tables, cu_q, kv_lens, lse, weights, 
     """What each cached key has gathered: ``out = decay * weights + sum of exp(scale q k - lse)`` over the queries that see it.
 
     The arguments are :func:`cached_attention`'s, and ``lse`` fp32 ``[Hq,
-    tokens]`` is what it wrote for these queries (a row whose lse is not finite
-    counts for nothing).  ``weights`` and ``out`` fp32 ``[num_blocks, kv_heads,
+    tokens]`` is what it wrote for these queries: a row then hands out 1 in all
+    (with :func:`prompt_attention`'s, over the keys before they were rounded to
+    8 bits, up to e^d times more or less, where d is what the rounding may
+    change a score by).  A row whose lse is not finite counts for nothing.  ``weights`` and ``out`` fp32 ``[num_blocks, kv_heads,
     block_size]`` stand in the cache's order; ``out`` is ``weights`` by default,
     and places that hold no key of a request are left as they are.  Tokens from
     ``fresh_from[b]`` on (int32 ``[requests]``: the lengths before the newest
@@ -675,7 +677,8 @@ class PagedKVCache:
     def weigh(self, layer: int, q, plan: BlockPlan, lse, max_q: int, max_kv: int, causal_chunk: int = 0,
               decay: float = 1.0) -> None:
         """Adds what the new tokens' queries give each key of the layer to its weight (see :func:`key_weights`), after
-        :meth:`append` and with the ``lse`` of :meth:`attend`; the new tokens' own weights start here."""
+        :meth:`append` and with the ``lse`` of :meth:`attend` (or of :func:`prompt_attention` over the same rows); the new
+        tokens' own weights start here."""
         self._has_weights("weigh")
         key_weights(q, self.k[layer], self.k_scale[layer], self.block_tables, plan.cu_new, plan.lens, lse,
                     self.weights[layer], max_q, max_kv, causal_chunk, fresh_from=self.lens, decay=decay)

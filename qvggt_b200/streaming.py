@@ -171,7 +171,8 @@ class StreamingRunner(AggregatorRunner):
     def prompt(self, tokens: torch.Tensor, counts, keep: tuple[int, ...] = ()) -> dict:
         """The first ``counts[s]`` frames of each stream s at once (0 to ``max_frames``), tokens ``[sum(counts), P, C]``
         fp16, stream after stream (modified in place); returns :meth:`AggregatorRunner.forward`'s outputs for them.
-        Their global attention reads their K / V rows as they are, not the cache's 8 bits."""
+        Their global attention reads their K / V rows as they are, not the cache's 8 bits (and what the cache's keys gather
+        is by its log-sum-exps: see :func:`~qvggt_b200.kv_cache.key_weights`)."""
         P, counts = self.cfg.tokens_per_frame, [int(n) for n in counts]
         if len(counts) != self.streams or min(counts) < 0 or max(counts) > self.max_frames or max(counts) == 0:
             raise ValueError(f"StreamingRunner: {counts} frames for {self.streams} streams of up to {self.max_frames}")

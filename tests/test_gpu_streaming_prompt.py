@@ -138,6 +138,39 @@ def test_streams_go_on_when_the_cache_is_full(per_step, hold, sink, recent):
     assert run.cache.lens.tolist() == [0, 0]
 
 
+def test_weights_after_a_prompt():
+    """A prompt's log-sum-exps are over its own fp16 keys, its weights over the cache's 8-bit ones: the weights are the
+    operator's for these inputs, and a row hands out 1 times at most e^d, at least e^-d, where d is what rounding the keys may
+    change a score by: scale |q|_1 times half a step (and the log-sum-exp's error of 2e-4)."""
+    from qvggt_b200.streaming import StreamingRunner
+    dev = torch.device("cuda", 0)
+    cfg = _config()
+    P, H, counts = cfg.tokens_per_frame, cfg.heads, [3, 0, 1]
+    run = StreamingRunner(cfg, *_blocks(cfg, dev), 1, 4, dev, streams=3, block_size=32, sink_frames=0)
+    cache, weigh, calls = run.cache, run.cache.weigh, []
+
+    def kept(layer, q, plan, lse, *args, **kwargs):
+        calls.append((layer, q.clone(), lse.clone()))
+        weigh(layer, q, plan, lse, *args, **kwargs)
+
+    cache.weigh = kept
+    run.prompt(_tokens(cfg, 4, 11), counts)
+    assert [c[0] for c in calls] == list(range(cfg.depth))
+    cu = torch.tensor([0, 3 * P, 3 * P, 4 * P])
+    for layer, q, lse in calls:
+        want, err = oe.key_weights(q, cache.k[layer], cache.k_scale[layer], cache.block_tables, cu, cache.lens, lse,
+                                   torch.zeros_like(cache.weights[layer]), P, None, [0, 0, 0])
+        assert ((cache.weights[layer].double() - want).abs() <= err).all()
+        for b, n in enumerate(counts):
+            ids = cache.block_tables[b, :-(-n * P // 32)].long()
+            got = cache.weights[layer, ids].double().sum((0, 2))             # a block is one stream's
+            rows = q[int(cu[b]):int(cu[b + 1])].double().abs().sum(-1)       # [tokens, heads]
+            half = 0.5 * cache.k_scale[layer, ids].double().amax(0) if n else torch.zeros(H, device=dev).double()
+            d = rows * half / 8 + 2e-4
+            assert (got <= d.exp().sum(0)).all() and (got >= (-d).exp().sum(0)).all()
+            assert n == 0 or float(d.max()) < 0.5
+
+
 def test_evicting_what_nobody_looks_at_changes_little():
     """A third of the keys point away from every query; a cache that drops just as many drops those, and the attention
     over what is left is the attention over all (the lost weights, 40 keys of e^-16 each, and one rounding of moved rows)."""
