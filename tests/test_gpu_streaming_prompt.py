@@ -209,6 +209,50 @@ def test_evicting_what_nobody_looks_at_changes_little():
     assert (got.float() - want.float()).abs().max() <= 2 * score * float(v.abs().max()) + step + 40 * math.exp(-16) + 2e-3
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,bs,ql", [(64, 32, 3), (64, 64, 90), (128, 128, 3), (128, 32, 90)])
+def test_attention_over_what_an_eviction_leaves(dtype, D, bs, ql):
+    """Append, attend, weigh and evict.  Each place then holds its survivor, to half a step of the block's scale (1e-5 for the
+    step itself), and new queries get the attention in 64 bits over the codes, scales and tables that are there, within the
+    attention's own bound, which is far under its results."""
+    from qvggt_b200 import kv_cache
+    from tests.test_gpu_kv_cache import _check_attention
+    H, hq, lens, keep = 2, 4, [300, 0, 135], [170, 5, 130]
+    g = torch.Generator(device="cuda").manual_seed(D + ql)
+    cache = kv_cache.PagedKVCache(1, 20, H, D, 3, 400, bs, weights=True)
+    T, most = sum(lens), max(lens)
+    q = torch.randn(T, hq, D, generator=g, device="cuda").to(dtype)
+    k, v = (torch.randn(T, H, D, generator=g, device="cuda").to(dtype) for _ in range(2))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    plan = cache.plan(ints(lens), T)
+    cache.append(0, k, v, plan)
+    lse = torch.empty(hq, T, device="cuda")
+    cache.attend(0, q, plan, most, most, lse=lse)          # (no mask: with one the first tokens gather most, and stay)
+    cache.weigh(0, q, plan, lse, most, most)
+    cache.commit(plan)
+    state = lambda: [t[0].clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    before, table = state(), cache.block_tables.clone()
+    moved = cache.evict(ints(keep), 130, sink=3)
+    assert cache.lens.tolist() == [170, 0, 130] and int(moved.counts.min(-1).values[0, 0]) > 20
+    after = state()
+    for r, n in ((0, 170), (2, 130)):
+        for h in range(H):
+            here = torch.arange(n, device="cuda")
+            at, m = here.clone(), int(moved.counts[0, r, h])
+            at[moved.dst[0, r, h, :m].long()] = moved.src[0, r, h, :m].long()
+            old, new = table[r, at // bs].long(), cache.block_tables[r, here // bs].long()
+            for side in range(2):
+                x = before[side][old, h, at % bs].double() * before[2 + side][old, h, None].double()
+                y = after[side][new, h, here % bs].double() * after[2 + side][new, h, None].double()
+                assert ((x - y).abs() <= (0.5 + 1e-5) * after[2 + side][new, h, None].double()).all()
+    x = torch.randn(2 * ql, hq, D, generator=g, device="cuda").to(dtype)
+    cu, lse = ints([0, ql, ql, 2 * ql]), torch.empty(hq, 2 * ql, device="cuda")
+    got = kv_cache.cached_attention(x, *after, cache.block_tables, cu, cache.lens, ql, 170, 0, lse=lse)
+    ref = ok.cached_attention(x, *after, cache.block_tables, cu, cache.lens, 0)
+    _check_attention(got, lse, ref, dtype, float(after[3].max() * 128), 170)
+    assert ref[0].abs().max() > 0.2      # (the bound is some 2e-3, bf16's output rounding beside it)
+
+
 def test_streaming_aggregator_prompt_is_the_models():
     """One frame at once, nothing cached: the model itself; then the next frame arrives."""
     from qvggt_b200.aggregator import AggConfig
