@@ -601,6 +601,8 @@ __global__ void __launch_bounds__(MOVE_THREADS, 3) kv_evict_kernel(MoveArgs a) {
         }
       }
       if (s == before) continue;
+      // (in the block that the new length falls into these rows are incoming ones' sources too: all lanes' reads first)
+      __syncwarp(mask);
       unsigned taken[4] = {0, 0, 0, 0};  // the block's rows that were written
       for (int r0 = 0; r0 < rows; r0 += G) {
         const int r = r0 + gl;
