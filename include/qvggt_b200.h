@@ -526,9 +526,9 @@ int qvggt_evict_plan(const qvggt_evict_plan_args* args, void* stream);
  * 127, 2^-60), incoming values x become rint(x * (1 / s)), and if s grew all
  * other codes c of the block rint(c * (s_old * (1 / s))).  Blocks that receive
  * nothing are left as they are, and so is what stands at keep[b] or later, but
- * for the rest of the block that keep[b] falls into.  Places outside [0,
- * keep[b]) in dst, or before keep[b] in src, and block ids outside the cache are
- * skipped and reported (0x202, 0x201).  New entry point. */
+ * for the rest of the block that keep[b] falls into.  Requests have their own
+ * blocks.  Places outside [0, keep[b]) in dst, or before keep[b] in src, and block
+ * ids outside the cache are skipped and reported (0x202, 0x201).  New entry point. */
 typedef struct {
   qvggt_kv_cache cache;
   int64_t layers, layer_stride;

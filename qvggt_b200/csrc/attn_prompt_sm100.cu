@@ -29,7 +29,8 @@
 // turns at column 0 (a score tile is read into registers at once, so its place is
 // free again long before the exponentials are done), and P_i is at KT + i KT / 2.
 // 64-key tiles with places of their own cost half as many waits and TMEM reads
-// again for each key: 1,234 us against 1,020 (two sequences of 8,192, 16 heads).
+// again for each key: 1,234 us against 1,020 when this was chosen (two sequences of
+// 8,192, 16 heads; 940 to 980 now).
 #include "attn_cache.cuh"
 #include "attn_common.cuh"
 #include "host.hpp"
@@ -45,8 +46,9 @@ constexpr int Q_ROWS = 256;     // rows of an item
 // (loads, first products, epilogue), its key tiles, and again those that its first
 // row does not see to their end (their V is looked through, their scores hidden).
 // By fits of equal items: 2 to 2.5 tiles, and 0.5 to 1 for each such tile.  Against a
-// start of 50 for all items: nine causal sequences to 4,099, 32 / 8 heads x 128 540 ->
-// 525 us, four streams of one to six frames, 16 x 128 666 -> 632, 16 x 64 the same.
+// start of 50 for all items, in short runs at full clock: nine causal sequences to
+// 4,099, 32 / 8 heads x 128 540 -> 525 us, four streams of one to six frames, 16 x 128
+// 666 -> 632, 16 x 64 the same.
 constexpr int COST_START = 20, COST_TILE2 = 10, COST_TILE1 = 9, COST_MASKED = 10;
 // No piece is cut shorter than this (8 tiles): a join costs about as much.
 constexpr int COST_MIN = COST_START + 8 * COST_TILE2;

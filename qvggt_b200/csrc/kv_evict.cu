@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) evict_plan_kernel(ChooseArgs a
 }
 
 // --------------------------------------------------------------------- move
-constexpr int MOVE_THREADS = 256, MOVE_WARPS = MOVE_THREADS / 32;
+constexpr int MOVE_THREADS = 256;
 constexpr int MOVE_BLOCKS = 256;         // blocks of a CTA at most
 constexpr int MOVE_ROWS = 2048;          // rows they receive at most
 constexpr uint32_t NOWHERE = 0xffffffffu;
@@ -550,8 +550,10 @@ __global__ void __launch_bounds__(MOVE_THREADS, 3) kv_evict_kernel(MoveArgs a) {
   }
   __syncthreads();
   // A group of lanes for each side of a block: a warp, or eight lanes where the
-  // blocks receive few rows (a step that makes room for one frame in 32 moves two
-  // rows into a block: 368 us with a warp each, 24 layers of 43,968 keys).
+  // blocks receive few rows.  A step that makes room for one frame in 32 moves two
+  // rows into a block: 24 layers of 43,968 keys, scales that hold what comes in, 124
+  // us, 368 with a warp each.  (464 the first time, when the scales of a quarter of
+  // all blocks grow and their other rows are rounded anew, by eight lanes a block.)
   const auto units = [&](auto GROUP) {
     constexpr int G = GROUP, AT_ONCE = G * MOVE_LOADS;     // pieces under way
     const int gl = tid % G;
@@ -630,7 +632,7 @@ __global__ void __launch_bounds__(MOVE_THREADS, 3) kv_evict_kernel(MoveArgs a) {
   if (EDGE || (m1 - m0) * PARTS > 32 * (j1 - j0)) units(std::integral_constant<int, 32>());
   else units(std::integral_constant<int, 8>());
   // at the end: CTAs of the next kernel that wait beside this one's slow it (four
-  // layers and their reading: 213 us with the call at the start, 198 here)
+  // layers and their reading, no scale grows: 213 us with the call at the start, 198 here)
   pdl_trigger();
 }
 
@@ -665,7 +667,11 @@ extern "C" int qvggt_evict_plan(const qvggt_evict_plan_args* p, void* stream) {
   // Clusters where the rows alone leave SMs idle and each CTA still has 8192 keys:
   // a cluster's barriers cost about 8 us (16 rows of 44,000 keys: 45 us as one CTA
   // each, 21 as four; 128 rows of 8,000: 11.5 and 24).  Eight CTAs to a cluster
-  // only halve how many run at once (16 rows: 40 us).
+  // only halve how many run at once (16 rows: 40 us).  The rule looks at the rows
+  // alone.  Where the longest passes ROOM_MAX nothing is held with one CTA a row, and
+  // two CTAs for each row, which hold it, would take 107 us against 145 (384 rows of
+  // 49,464 keys), 161 against 211 (of 60,456), 43 against 64 (128 of 49,464); for one
+  // such row of 24 beside short ones (16 heads) 66 against 55.
   while (C < 4 && 2 * rows * C <= device_info().num_sms && longest > 8192LL * C) C *= 2;
   const int64_t part = quads_of(longest, C, ROOM_MAX) * 4LL * CHOOSE_THREADS;
   const int room = part <= ROOM_MAX ? (int)part : 0;

@@ -578,7 +578,7 @@ def kv_evict(k_cache, v_cache, k_scale, v_scale, weights, block_tables, keep, pl
     The caches int8 ``[layers, num_blocks, kv_heads, block_size, head_dim]``,
     the scales fp32 ``[layers, num_blocks, kv_heads]``.  A block's scale grows
     when the rows it receives need it, and its other codes are rounded to the
-    new scale, as in :func:`kv_append`."""
+    new scale, as in :func:`kv_append`.  Requests must not share blocks."""
     name = "kv_evict"
     src, dst, counts = plan
     dev = k_cache.get_device()
@@ -685,8 +685,9 @@ class PagedKVCache:
 
     def evict(self, keep, max_moves: int, sink: int = 0, recent: int = 0) -> EvictPlan:
         """Takes the requests down to ``keep`` tokens (int32 ``[requests]`` on the GPU; one that holds no more stays as it
-        is), in every layer and head those of largest weight (see :func:`evict_plan`), and gives the surplus blocks back.
-        Between steps: a plan made before does not survive it."""
+        is), in every layer and head those of largest weight (see :func:`evict_plan`, whose ``max_moves``, ``sink`` and
+        ``recent`` these are: with a ``max_moves`` that is too small survivors are lost, and the status word says so), and
+        gives the surplus blocks back.  Between steps: a plan made before does not survive it."""
         self._has_weights("evict")
         plan = evict_plan(self.weights, self.block_tables, self.lens, keep, sink, recent, max_moves)
         kv_evict(self.k, self.v, self.k_scale, self.v_scale, self.weights, self.block_tables, keep, plan)
